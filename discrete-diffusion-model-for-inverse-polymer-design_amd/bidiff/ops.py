@@ -1,0 +1,475 @@
+"""Stand-alone operators for denoisers built from this package's parts, each with its gradient.
+
+``rotary`` turns query and key heads by their positions (beside the learned position table of ``DiffusionBackbone``),
+``differential_attention`` is the difference of two softmax maps over one set of values (beside the attention of
+``MultiHeadAttention``), and ``linear_cross_entropy`` is the masked cross entropy of the vocabulary head without its
+logits (beside ``training.autograd.masked_cross_entropy``). All run on the current stream of their operands' device, take
+their scratch memory from torch's allocator, repeat bit for bit, and may be captured into a HIP graph (packed rows:
+with ``max_seqlen`` given). Operands on a CPU raise ``RuntimeError``: there is no other execution path.
+"""
+import ctypes as C
+import math
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_DTYPES = {torch.bfloat16: 0, torch.float32: 1}
+_S3 = C.c_longlong * 3
+# beyond this many keys the forward of a training step leaves each map's output in fp32 for the backward (16 * head_dim
+# bytes a row and head); up to here the backward walks the keys once more instead
+_MAPS_KEYS = 128
+
+
+class _On:
+    """The operands' device made current for the launches inside (nothing to do in the usual case)."""
+
+    def __init__(self, device):
+        self.ctx = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.ctx is not None:
+            self.ctx.__enter__()
+        return _lib.stream_handle()
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+        return False
+
+
+def _same_device(what, first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"bidiff {what}: operands on {first.device} and {t.device}; all must be on one device")
+
+
+def _strides(t, n):
+    """The leading strides of ``t`` as three values (batch, row, head), 0 where the axis has one entry; a tensor
+    without a batch axis gets batch stride 0."""
+    st = [0 if size == 1 else stride for size, stride in zip(t.shape, t.stride())][:n]
+    return [0] * (3 - len(st)) + st
+
+
+def _rows_of_16_bytes(t, n):
+    """``t`` or a copy of it whose rows the kernels can read in 16-byte pieces."""
+    per = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 for s in _strides(t, n)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+# ------------------------------------------------------------------------------------------------ rotary positions
+def rotary_table(dim: int, max_positions: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
+                 original_positions: Optional[int] = None, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 device=None) -> torch.Tensor:
+    """Table of (cos, sin) for ``rotary``: fp32 [max_positions, dim / 2, 2], from angles evaluated in 64 bits.
+
+    ``scaling`` stretches the positions for contexts longer than those trained on by ``factor``: None; ``"linear"``
+    (positions divided by it); ``"ntk"`` (the base raised so that the slowest pair is stretched by the factor and the
+    fastest not at all); ``"yarn"`` (pairs that turn at least ``beta_fast`` times within ``original_positions`` are kept,
+    those below ``beta_slow`` turns are stretched, a linear ramp over the pair's index between; cos and sin times 0.1 ln(factor) + 1)."""
+    if dim <= 0 or dim % 2:
+        raise ValueError(f"rotary_table: dim must be positive and even, got {dim}")
+    if max_positions <= 0 or not base > 0.0 or not factor > 0.0:
+        raise ValueError("rotary_table: max_positions, base and factor must be positive")
+    i = torch.arange(dim // 2, dtype=torch.float64)
+    freq = base ** (-2.0 * i / dim)
+    scale = 1.0
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "ntk":
+        if dim == 2:
+            raise ValueError("rotary_table: ntk scaling needs more than one pair")
+        freq = (base * factor ** (dim / (dim - 2))) ** (-2.0 * i / dim)
+    elif scaling == "yarn":
+        if not original_positions or original_positions <= 0 or not beta_fast > beta_slow > 0.0:
+            raise ValueError("rotary_table: yarn scaling needs original_positions > 0 and beta_fast > beta_slow > 0")
+        if not base > 1.0:
+            raise ValueError("rotary_table: yarn scaling needs a base above 1")
+
+        def pair_of(turns):      # the (fractional) pair that turns this often within the original positions
+            return dim * math.log(original_positions / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+        low, high = max(math.floor(pair_of(beta_fast)), 0), min(math.ceil(pair_of(beta_slow)), dim - 1)
+        stretched = ((i - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        freq = freq / factor * stretched + freq * (1.0 - stretched)
+        scale = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    elif scaling is not None:
+        raise ValueError(f"rotary_table: unknown scaling {scaling!r}")
+    angle = torch.arange(max_positions, dtype=torch.float64)[:, None] * freq
+    return (torch.stack([angle.cos(), angle.sin()], -1) * scale).float().to(device if device is not None else "cpu")
+
+
+def _rotary_launch(pairs, table, positions, interleaved, inverse):
+    """pairs: one or two (source, destination) of [B, L, heads, D] (or [rows, heads, D])."""
+    src = pairs[0][0]
+    B, L = (1, src.shape[0]) if src.dim() == 3 else src.shape[:2]
+    arr = (_lib.RotaryTensor * len(pairs))()
+    for a, (s, d) in zip(arr, pairs):
+        a.src, a.dst, a.n_heads = s.data_ptr(), d.data_ptr(), s.shape[-2]
+        a.src_stride, a.dst_stride = _S3(*_strides(s, s.dim() - 1)), _S3(*_strides(d, d.dim() - 1))
+    pos_stride = 0 if positions is None or positions.dim() == 1 else positions.stride(0)
+    with _On(src.device) as stream:
+        _lib.check(_lib.lib().bd_rotary(arr, len(pairs), _lib.ptr(table), table.shape[0], _lib.ptr(positions), pos_stride, B, L,
+                                        src.shape[-1], 2 * table.shape[1], int(interleaved), int(inverse), _DTYPES[src.dtype],
+                                        stream), "bd_rotary")
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, positions, interleaved, *xs):
+        ctx.save_for_backward(table, positions)
+        ctx.interleaved, ctx.n = interleaved, len(xs)
+        out = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
+        _rotary_launch(list(zip(xs, out)), table, positions, interleaved, False)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        table, positions = ctx.saved_tensors
+        wanted = [i for i in range(ctx.n) if ctx.needs_input_grad[3 + i]]
+        dx = [None] * ctx.n
+        pairs = []
+        for i in wanted:
+            g = grads[i] if grads[i].stride(-1) == 1 else grads[i].contiguous()
+            dx[i] = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+            pairs.append((g, dx[i]))
+        if pairs:
+            _rotary_launch(pairs, table, positions, ctx.interleaved, True)
+        return (None, None, None, *dx)
+
+
+def _rotary_check(xs, table, positions):
+    q = xs[0]
+    _same_device("rotary", q, *xs[1:], table, positions)
+    if q.dim() not in (3, 4):
+        raise ValueError(f"rotary: expected [batch, tokens, heads, head_dim] or [rows, heads, head_dim], got {tuple(q.shape)}")
+    for x in xs:
+        if x.dtype not in _DTYPES:
+            raise TypeError(f"rotary: bf16 or fp32 heads expected, got {x.dtype}")
+        if x.dtype != q.dtype or x.shape[:-2] != q.shape[:-2] or x.shape[-1] != q.shape[-1]:
+            raise ValueError("rotary: q and k must agree in dtype, tokens and head size")
+    if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2 or not table.is_contiguous() or not table.numel():
+        raise ValueError("rotary: table must be a contiguous fp32 [positions, rotary_dim / 2, 2] tensor (rotary_table makes one)")
+    if 2 * table.shape[1] > q.shape[-1]:
+        raise ValueError(f"rotary: the table turns {2 * table.shape[1]} values, a head has {q.shape[-1]}")
+    if table.requires_grad:
+        raise NotImplementedError("rotary: the table has no gradient")
+    lead = tuple(q.shape[:-2])
+    if positions is not None:
+        if positions.dtype != torch.long:
+            raise TypeError(f"rotary: positions must be int64, got {positions.dtype}")
+        if tuple(positions.shape) != lead and tuple(positions.shape) != lead[-1:]:
+            raise ValueError(f"rotary: positions must be {list(lead)} or {list(lead[-1:])}, got {tuple(positions.shape)}")
+        if positions.stride(-1) != 1 and positions.shape[-1] > 1:
+            positions = positions.contiguous()
+    return positions
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, positions: Optional[torch.Tensor] = None,
+           interleaved: bool = False):
+    """(q, k) with their heads turned by the tokens' positions; differentiable. q [B, L, heads, D] and k [B, L, key heads, D]
+    (or packed rows [rows, heads, D]; k may be None, and None comes back), bf16 or fp32, any strides with a contiguous last
+    axis. The first ``2 * table.shape[1]`` values of a head turn, the others are copied. ``positions`` int64 [B, L] or [L]
+    (default: 0, 1, ...); a token whose position the table does not hold comes out NaN. ``interleaved``: pairs (2 i, 2 i + 1)
+    instead of (i, i + half)."""
+    xs = [q] if k is None else [q, k]
+    positions = _rotary_check(xs, table, positions)
+    _lib.require_device(q, "rotary")
+    xs = [x if x.stride(-1) == 1 else x.contiguous() for x in xs]
+    if q.numel() == 0 or (k is not None and k.numel() == 0):
+        if q.shape[:-2].numel() == 0:
+            return q.clone(), None if k is None else k.clone()
+        raise ValueError("rotary: q and k need at least one head")
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        out = _Rotary.apply(table, positions, bool(interleaved), *xs)
+    else:
+        out = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
+        _rotary_launch(list(zip(xs, out)), table, positions, interleaved, False)
+    return out[0], out[1] if k is not None else None
+
+
+def rotary_(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, positions: Optional[torch.Tensor] = None,
+            interleaved: bool = False, inverse: bool = False):
+    """``rotary`` in place, for inference and for kernels' own buffers (no gradient is recorded). ``inverse`` turns back."""
+    xs = [q] if k is None else [q, k]
+    positions = _rotary_check(xs, table, positions)
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        raise RuntimeError("rotary_: in place on a tensor that requires grad; use rotary")
+    for x in xs:
+        if x.numel() and x.stride(-1) != 1:
+            raise ValueError("rotary_: the last axis must be contiguous")
+        if any(s == 0 and n > 1 for s, n in zip(x.stride(), x.shape)):
+            raise ValueError("rotary_: in place on an expanded tensor")
+    _lib.require_device(q, "rotary_")
+    if all(x.numel() for x in xs):
+        _rotary_launch([(x, x) for x in xs], table, positions, interleaved, inverse)
+    elif q.shape[:-2].numel():
+        raise ValueError("rotary_: q and k need at least one head")
+    return q, k
+
+
+# ------------------------------------------------------------------------------------------------ differential attention
+def _attention_args(q, k, v, lam, key_mask, cu, longest, scale):
+    a = _lib.DiffAttnArgs()
+    a.q, a.k, a.v, a.lam = q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr()
+    n = q.dim() - 1
+    a.q_stride, a.k_stride, a.v_stride = _S3(*_strides(q, n)), _S3(*_strides(k, n)), _S3(*_strides(v, n))
+    a.lam_stride = _S3(*_strides(lam, n))
+    a.lam_dtype = _DTYPES[lam.dtype]
+    if key_mask is not None:
+        a.key_mask, a.key_mask_stride = key_mask.data_ptr(), key_mask.stride(0)
+    if cu is not None:
+        a.cu_seqlens, a.total_rows, a.B, a.Lq, a.Lk = cu.data_ptr(), q.shape[0], cu.numel() - 1, longest, longest
+    else:
+        a.B, a.Lq, a.Lk = q.shape[0], q.shape[1], k.shape[1]
+    a.H, a.Hkv, a.head_dim = v.shape[-2] * (q.shape[-2] // k.shape[-2]), v.shape[-2], q.shape[-1]
+    a.scale = scale
+    return a
+
+
+def _workspace(a, backward, device):
+    need = _lib.lib().bd_diff_attention_workspace_bytes(C.byref(a), int(backward))
+    if need < 0:
+        _lib.check(-1, "bd_diff_attention_workspace_bytes")
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    a.workspace, a.workspace_bytes = (ws.data_ptr() if need else None), need
+    return ws
+
+
+def _attention_forward(q, k, v, lam, key_mask, cu, longest, scale, training):
+    H, E = q.shape[-2] // 2, v.shape[-1]
+    a = _attention_args(q, k, v, lam, key_mask, cu, longest, scale)
+    out = torch.empty(*q.shape[:-2], H, E, dtype=q.dtype, device=q.device)
+    a.out, a.out_stride = out.data_ptr(), _S3(*_strides(out, out.dim() - 1))
+    lse = maps = None
+    if training:
+        rows = q.shape[:-2].numel()
+        lse = torch.empty(rows, H, 2, dtype=torch.float32, device=q.device)
+        a.lse = lse.data_ptr()
+        if a.Lk > _MAPS_KEYS:
+            maps = torch.empty(rows, H, 2, E, dtype=torch.float32, device=q.device)
+            a.maps = maps.data_ptr()
+    with _On(q.device) as stream:
+        ws = _workspace(a, False, q.device)
+        _lib.check(_lib.lib().bd_diff_attention_fwd(C.byref(a), stream), "bd_diff_attention_fwd")
+        del ws
+    return out, lse, maps
+
+
+class _DiffAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, key_mask, cu, longest, scale):
+        full = lam.expand(*q.shape[:-2], q.shape[-2] // 2)
+        out, lse, maps = _attention_forward(q, k, v, full, key_mask, cu, longest, scale, True)
+        ctx.save_for_backward(q, k, v, lam, key_mask, cu, lse, maps)
+        ctx.longest, ctx.scale = longest, scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, lam, key_mask, cu, lse, maps = ctx.saved_tensors
+        H = q.shape[-2] // 2
+        dout = _rows_of_16_bytes(dout, dout.dim() - 1)
+        a = _attention_args(q, k, v, lam.expand(*q.shape[:-2], H), key_mask, cu, ctx.longest, ctx.scale)
+        n = q.dim() - 1
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        rows = q.shape[:-2].numel()
+        dlam = torch.empty(rows, H, dtype=torch.float32, device=q.device)
+        a.dout, a.dout_stride = dout.data_ptr(), _S3(*_strides(dout, n))
+        a.lse, a.maps = lse.data_ptr(), (None if maps is None else maps.data_ptr())
+        a.dq, a.dk, a.dv, a.dlam = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr()
+        a.dq_stride, a.dk_stride, a.dv_stride = _S3(*_strides(dq, n)), _S3(*_strides(dk, n)), _S3(*_strides(dv, n))
+        with _On(q.device) as stream:
+            ws = _workspace(a, True, q.device)
+            _lib.check(_lib.lib().bd_diff_attention_bwd(C.byref(a), stream), "bd_diff_attention_bwd")
+            del ws
+            dl = None
+            if ctx.needs_input_grad[3]:
+                lead = (1,) * (3 - q.dim() + 1) + tuple(q.shape[:-2])                  # (batch, rows)
+                shape = (1,) * (3 - lam.dim()) + tuple(lam.shape)
+                dl = torch.empty(lam.shape, dtype=lam.dtype, device=lam.device)
+                _lib.check(_lib.lib().bd_diff_attention_dlam(
+                    _lib.ptr(dlam), _lib.ptr(dl), _DTYPES[lam.dtype], lead[0], lead[1], H, int(shape[0] == lead[0]),
+                    int(shape[1] == lead[1]), int(shape[2] == H), stream), "bd_diff_attention_dlam")
+        return dq, dk, dv, dl, None, None, None, None
+
+
+def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,
+                           key_mask: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None,
+                           max_seqlen: Optional[int] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """sum_j (softmax(q1 k1) - lam softmax(q2 k2))_ij v_j, every query against every visible key of its sequence.
+
+    bf16: q [B, Lq, 2 H, D] (heads 2 h and 2 h + 1 are the two maps of head h), k [B, Lk, 2 Hkv, D], v [B, Lk, Hkv, 2 D],
+    D = 32, 64 or 128, H a multiple of Hkv; returns [B, Lq, H, 2 D]. ``lam`` (bf16 or fp32) broadcasts to [B, Lq, H]: a
+    weight per head, or one for each row. ``key_mask`` [B, Lk]: non-zero = visible; a query without a visible key gives
+    zeros, and what masked keys and values hold reaches nothing (their gradients are zeros). Packed rows: the same tensors
+    without the batch axis, ``cu_seqlens`` int [sequences + 1] (rows cu[b] .. cu[b + 1] - 1 belong to sequence b, rows
+    behind the last come out zero), ``max_seqlen`` the longest (None: read back from the device; rows of a longer sequence
+    come out NaN), ``key_mask`` [sequences, max_seqlen]. ``scale`` defaults to 1 / sqrt(D)."""
+    _same_device("differential_attention", q, k, v, lam, key_mask, cu_seqlens)
+    packed = cu_seqlens is not None
+    dims = 3 if packed else 4
+    if q.dim() != dims or k.dim() != dims or v.dim() != dims:
+        raise ValueError(f"differential_attention: q, k and v need {dims} axes"
+                         f"{' (packed rows have no batch axis)' if packed else ''}, got {q.dim()}, {k.dim()} and {v.dim()}")
+    for t in (q, k, v):
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"differential_attention: q, k and v must be bf16, got {t.dtype}")
+    if lam.dtype not in _DTYPES:
+        raise TypeError(f"differential_attention: lam must be bf16 or fp32, got {lam.dtype}")
+    D, Hkv = q.shape[-1], v.shape[-2]
+    if D not in (32, 64, 128):
+        raise NotImplementedError(f"differential_attention: head sizes 32, 64 and 128 are supported, got {D}")
+    if k.shape[-1] != D or v.shape[-1] != 2 * D or k.shape[-2] != 2 * Hkv or q.shape[-2] % 2 or Hkv == 0 or q.shape[-2] == 0:
+        raise ValueError(f"differential_attention: heads do not fit: q {tuple(q.shape[-2:])}, k {tuple(k.shape[-2:])}, "
+                         f"v {tuple(v.shape[-2:])} (two maps a head, values twice as wide)")
+    H = q.shape[-2] // 2
+    if H % Hkv:
+        raise ValueError(f"differential_attention: {H} heads cannot share {Hkv} key heads evenly")
+    if k.shape[:-2] != v.shape[:-2] or (packed and q.shape[0] != k.shape[0]) or (not packed and q.shape[0] != k.shape[0]):
+        raise ValueError("differential_attention: q, k and v disagree in batch or rows")
+    lead = tuple(q.shape[:-2])
+    try:
+        fits = torch.broadcast_shapes(tuple(lam.shape), lead + (H,)) == torch.Size(lead + (H,))
+    except RuntimeError:
+        fits = False
+    if not fits:
+        raise ValueError(f"differential_attention: lam {tuple(lam.shape)} does not broadcast to {lead + (H,)}")
+    if lam.dim() == 0:
+        lam = lam.reshape(1)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"differential_attention: scale must be positive and finite, got {scale}")
+    longest = None
+    if packed and max_seqlen is None:
+        _lib.require_device(q, "differential_attention")
+    if packed:
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.dtype not in (torch.int32, torch.int64):
+            raise ValueError("differential_attention: cu_seqlens must be an int32 or int64 vector of sequences + 1 offsets")
+        if cu_seqlens.dtype != torch.int32 or not cu_seqlens.is_contiguous():
+            cu_seqlens = cu_seqlens.to(torch.int32).contiguous()
+        longest = int((cu_seqlens[1:] - cu_seqlens[:-1]).max()) if max_seqlen is None else int(max_seqlen)
+        if longest < 0 or (max_seqlen is not None and longest == 0 and q.shape[0]):
+            raise ValueError(f"differential_attention: max_seqlen must be positive, got {longest}")
+        longest = max(longest, 1)
+    elif max_seqlen is not None:
+        raise ValueError("differential_attention: max_seqlen goes with cu_seqlens")
+    if key_mask is not None:
+        want = (cu_seqlens.numel() - 1, longest) if packed else tuple(k.shape[:2])
+        if tuple(key_mask.shape) != want:
+            raise ValueError(f"differential_attention: key_mask must be {want}, got {tuple(key_mask.shape)}")
+        if key_mask.dtype not in (torch.bool, torch.uint8):
+            key_mask = key_mask != 0
+        if key_mask.stride(1) != 1 and key_mask.shape[1] > 1:
+            key_mask = key_mask.contiguous()
+        if key_mask.dtype == torch.bool:
+            key_mask = key_mask.view(torch.uint8)
+    _lib.require_device(q, "differential_attention")
+    if q.numel() == 0 or k.numel() == 0:         # nothing to attend with or to: zeros that stay attached to the graph
+        return q.new_zeros(*lead, H, 2 * D) + sum(t.reshape(-1)[:0].sum() for t in (q, k, v, lam)).to(q.dtype)
+    n = dims - 1
+    q, k, v = (_rows_of_16_bytes(t, n) for t in (q, k, v))
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam)):
+        return _DiffAttention.apply(q, k, v, lam, key_mask, cu_seqlens, longest, scale)
+    return _attention_forward(q, k, v, lam.expand(*lead, H), key_mask, cu_seqlens, longest, scale, False)[0]
+
+
+# ------------------------------------------------------------------------------------------------ vocabulary head
+def _to_bf16(x, stream):
+    if x.dtype == torch.bfloat16:
+        return x.contiguous()
+    x = x.contiguous()
+    y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+    _lib.check(_lib.lib().bd_cast_f32_to_bf16(_lib.ptr(x), _lib.ptr(y), x.numel(), stream), "bd_cast_f32_to_bf16")
+    return y
+
+
+class _LinearCE(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, indicator, attention_mask):
+        dev = hidden.device
+        V, d = weight.shape
+        M = targets.numel()
+        L_ = _lib.lib()
+        with _On(dev) as stream:
+            h, w = _to_bf16(hidden, stream), _to_bf16(weight, stream)
+            loss = torch.empty((), dtype=torch.float32, device=dev)
+            state = torch.empty(L_.bd_linear_ce_state_bytes(M, d), dtype=torch.uint8, device=dev)
+            ws = torch.empty(L_.bd_linear_ce_workspace_bytes(M, d, V, 0), dtype=torch.uint8, device=dev)
+            _lib.check(L_.bd_linear_ce_fwd(_lib.ptr(h), _lib.ptr(w), _lib.ptr(targets), _lib.ptr(indicator),
+                                           _lib.ptr(attention_mask), _lib.ptr(loss), M, d, V, _lib.ptr(state), state.numel(),
+                                           _lib.ptr(ws), ws.numel(), stream), "bd_linear_ce_fwd")
+        if any(ctx.needs_input_grad[:2]):
+            # (the weighted rows are in the state; of the head the bf16 copy is kept where one was made)
+            ctx.save_for_backward(weight if w is weight else None, None if w is weight else w, state)
+            ctx.like = (hidden.shape, hidden.dtype, weight.dtype)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout):
+        weight, copy, state = ctx.saved_tensors
+        w = weight if copy is None else copy
+        shape, hidden_dtype, weight_dtype = ctx.like
+        V, d = w.shape
+        M = shape[:-1].numel()
+        L_ = _lib.lib()
+        dev = w.device
+        with _On(dev) as stream:
+            g = gout.reshape(1).float().contiguous()
+            dh = torch.empty(shape, dtype=torch.bfloat16, device=dev) if ctx.needs_input_grad[0] else None
+            dw = None
+            if ctx.needs_input_grad[1]:      # fp32 gradients are accumulated into, bf16 ones written
+                dw = (torch.zeros if weight_dtype == torch.float32 else torch.empty)(V, d, dtype=weight_dtype, device=dev)
+            ws = torch.empty(L_.bd_linear_ce_workspace_bytes(M, d, V, 1), dtype=torch.uint8, device=dev)
+            _lib.check(L_.bd_linear_ce_bwd(_lib.ptr(w), _lib.ptr(g), _lib.ptr(dh), _lib.ptr(dw), _DTYPES[weight_dtype], M, d, V,
+                                           _lib.ptr(state), state.numel(), _lib.ptr(ws), ws.numel(), stream), "bd_linear_ce_bwd")
+        return (dh.to(hidden_dtype) if dh is not None else None), dw, None, None, None
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                         mask_indicator: Optional[torch.Tensor] = None,
+                         attention_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``masked_cross_entropy(hidden @ weight.T, targets, mask_indicator, attention_mask)`` without the logits: the mean
+    cross entropy (fp32) over the rows that are marked and attended, an exact zero when there is none.
+
+    hidden [..., d] (the rows behind the final norm) and weight [V, d] in bf16 or fp32 (fp32 operands are rounded to bf16
+    once, as the head's product does), d a multiple of 64, any V; targets int64 [...]; ``mask_indicator`` [...] (non-zero =
+    counts) and ``attention_mask`` [...] (the row's weight) may be None. Rows that do not count are never read and get
+    zero gradients; a counted row whose target lies outside the vocabulary makes the loss NaN. Gradients come in their
+    operand's dtype, that of an fp32 weight accumulated in fp32."""
+    _same_device("linear_cross_entropy", hidden, weight, targets, mask_indicator, attention_mask)
+    for t, name in ((hidden, "hidden"), (weight, "weight")):
+        if t.dtype not in _DTYPES:
+            raise TypeError(f"linear_cross_entropy: {name} must be bf16 or fp32, got {t.dtype}")
+    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1] or weight.shape[0] == 0:
+        raise ValueError(f"linear_cross_entropy: hidden {tuple(hidden.shape)} does not meet weight {tuple(weight.shape)}")
+    lead = hidden.shape[:-1]
+    if weight.shape[1] == 0 or weight.shape[1] % 64:
+        raise NotImplementedError(f"linear_cross_entropy: the hidden size must be a multiple of 64, got {weight.shape[1]}")
+    if targets.dtype != torch.long:
+        raise TypeError(f"linear_cross_entropy: targets must be int64, got {targets.dtype}")
+    for t, name in ((targets, "targets"), (mask_indicator, "mask_indicator"), (attention_mask, "attention_mask")):
+        if t is not None and t.shape != lead:
+            raise ValueError(f"linear_cross_entropy: {name} must be {list(lead)}, got {tuple(t.shape)}")
+    _lib.require_device(hidden, "linear_cross_entropy")
+    if targets.numel() == 0:                     # no row at all: a zero that stays attached to the graph
+        return (hidden.reshape(-1)[:0].sum() + weight.reshape(-1)[:0].sum()).float()
+    if mask_indicator is not None:
+        if mask_indicator.dtype not in (torch.bool, torch.uint8):
+            mask_indicator = mask_indicator != 0
+        mask_indicator = mask_indicator.contiguous()
+        if mask_indicator.dtype == torch.bool:
+            mask_indicator = mask_indicator.view(torch.uint8)
+    if attention_mask is not None:
+        attention_mask = attention_mask.to(torch.long).contiguous()
+    if hidden.data_ptr() % 16:
+        hidden = hidden.clone(memory_format=torch.contiguous_format)
+    if weight.data_ptr() % 16:
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    return _LinearCE.apply(hidden, weight, targets.contiguous(), mask_indicator, attention_mask)

@@ -1,0 +1,626 @@
+// Cross entropy of the vocabulary head without keeping its logits (gfx950, bf16 MFMA).
+//
+//   z = h W^T,  loss = sum_i w_i (lse_i - z_{i, t_i}) / sum_i w_i,  lse_i = log sum_v exp z_iv
+//   dz_iv = (g / sum w) w_i (exp(z_iv - lse_i) - [v = t_i]),   dh = dz W,  dW = dz^T h
+//
+// for hidden rows h [M, d] and head weights W [V, d]. Only rows with a weight (masked by the corruption and attended)
+// are computed: they are first gathered, in order, into a compact matrix whose row count stays on the device.
+//   forward:  tiles of z = Hc W^T reduce each row's maximum and sum of exponentials over 64 columns in registers; one
+//             wave per row joins these pairs, adds the target's score (a dot product of its own) and the loss follows
+//             in a fixed order: two runs give the same bits.
+//   backward: piece by piece of the vocabulary, the tiles are computed again and leave w (p - onehot) in bf16 (values of
+//             [-w, w], the common factor g / sum w is applied in fp32 where the products end), then
+//             dh += dz W and dW = dz^T Hc. The last two read their operands along the summed axis through the
+//             transposing LDS read, so that no transposed copy of anything is written. Sums over splits of a long axis
+//             go to slabs of their own and are added in order.
+// Bound by the matrix cores: 2 N V d flops forward and 6 N V d backward for N weighted rows.
+#include "bd_common.h"
+#include "bd_prof.h"
+#include "bidiff.h"
+
+namespace {
+
+constexpr float VL_LOG2E = 1.44269504088896f, VL_LN2 = 0.69314718055995f;
+constexpr int SCAN = 64;              // rows per workgroup of the gathering kernels
+
+enum { VL_STATS = 0, VL_DLOG = 1, VL_SLAB = 2, VL_DW = 3 };
+
+struct VlState {                      // what the forward leaves for the backward (device memory of the caller)
+  int* head;                          // [0] weighted rows, [1] sum of weights (float bits)
+  int *idx, *pos, *tgt;               // compact row -> row; row -> compact row or -1; target of a compact row
+  float *w, *lse;                     // weight and log2-sum-exp2 of z * log2(e) of a compact row
+  unsigned short* hc;                 // [m_pad, d] compact rows, zeros behind the last
+  long long bytes;
+};
+
+__host__ __device__ inline long long vl_up(long long x, long long m) { return (x + m - 1) / m * m; }
+
+VlState vl_state(void* base, long long M, int d) {
+  char* p = (char*)base;
+  const long long mp = vl_up(M, 256), r4 = vl_up(mp * 4, 256);
+  VlState s;
+  s.head = (int*)p; p += 256;
+  s.idx = (int*)p; p += r4;
+  s.pos = (int*)p; p += r4;
+  s.tgt = (int*)p; p += r4;
+  s.w = (float*)p; p += r4;
+  s.lse = (float*)p; p += r4;
+  s.hc = (unsigned short*)p; p += mp * d * 2;
+  s.bytes = p - (char*)base;
+  return s;
+}
+
+__device__ __forceinline__ float vl_weight(const unsigned char* ind, const long long* attn, long long m) {
+  if (ind && !ind[m]) return 0.f;
+  return attn ? (float)attn[m] : 1.f;
+}
+
+// weighted rows and sum of weights of each group of SCAN rows: one wave per group
+__global__ __launch_bounds__(256) void vl_count_kernel(const unsigned char* __restrict__ ind, const long long* __restrict__ attn,
+                                                       int* __restrict__ counts, float* __restrict__ sums, int M) {
+  const int grp = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if ((long long)grp * SCAN >= M) return;
+  const int row = grp * SCAN + lane;
+  const float w = row < M ? vl_weight(ind, attn, row) : 0.f;
+  const unsigned long long live = __ballot(w != 0.f);
+  const float s = bd_wave_sum(w);
+  if (lane == 0) { counts[grp] = __popcll(live); sums[grp] = s; }
+}
+
+// the group's weighted rows to their places: the counts of the groups before it are added up first (in order)
+__global__ __launch_bounds__(256) void vl_gather_kernel(const unsigned short* __restrict__ hidden, const long long* __restrict__ targets,
+                                                        const unsigned char* __restrict__ ind, const long long* __restrict__ attn,
+                                                        const int* __restrict__ counts, const float* __restrict__ sums, VlState st,
+                                                        int M, int d, int V) {
+  __shared__ int before[4], all[4], src[SCAN];
+  __shared__ float wsum[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int groups = (M + SCAN - 1) / SCAN, grp = blockIdx.x;
+  int nb = 0, na = 0;
+  float ws = 0.f;
+  for (int i = tid; i < groups; i += 256) {
+    const int n = counts[i];
+    na += n;
+    if (i < grp) nb += n;
+    ws += sums[i];
+  }
+  nb = bd_wave_sum_i(nb); na = bd_wave_sum_i(na); ws = bd_wave_sum(ws);
+  if (lane == 0) { before[wave] = nb; all[wave] = na; wsum[wave] = ws; }
+  __syncthreads();
+  const int first = before[0] + before[1] + before[2] + before[3], total = all[0] + all[1] + all[2] + all[3];
+  if (wave == 0) {
+    const int row = grp * SCAN + lane;
+    const float w = row < M ? vl_weight(ind, attn, row) : 0.f;
+    const unsigned long long live = __ballot(w != 0.f);
+    const int at = __popcll(live & ((1ull << lane) - 1ull));
+    if (row < M) st.pos[row] = w != 0.f ? first + at : -1;
+    if (w != 0.f) {
+      src[at] = row;
+      st.idx[first + at] = row;
+      st.w[first + at] = w;
+      const long long t = targets[row];
+      st.tgt[first + at] = t >= 0 && t < V ? (int)t : -1;      // outside the vocabulary: the row's loss is NaN
+    }
+    if (lane == 0) before[0] = __popcll(live);
+    if (grp == 0 && lane == 0) {
+      st.head[0] = total;
+      ((float*)st.head)[1] = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
+    }
+  }
+  __syncthreads();
+  const int n = before[0], per = d / 8;
+  for (int i = tid; i < n * per; i += 256) {
+    const int r = i / per, ch = i - r * per;
+    *(u32x4*)(st.hc + (long long)(first + r) * d + 8 * ch) = *(const u32x4*)(hidden + (long long)src[r] * d + 8 * ch);
+  }
+  if (grp == groups - 1) {           // zeros behind the last row, to the end of its 256-row tile
+    const int end = (int)vl_up(total, 256);
+    for (long long i = tid; i < (long long)(end - total) * per; i += 256)
+      *(u32x4*)(st.hc + (long long)total * d + 8 * i) = (u32x4){0u, 0u, 0u, 0u};
+  }
+}
+
+// =====================================================================================
+// C[m, n] = sum_k A(m, k) B(n, k) on BM x BN tiles. AKC / BKC: the operand is stored along k (rows of K values) or, if
+// not, along its own axis (row k holds the values of all m / n). MFMA operand order: n is the A side and m the B side,
+// with n permuted inside 64 columns, so that a lane ends up with 16 consecutive n of one row m.
+// K is staged 64 at a time by LDS-DMA, two stages in turn.
+// =====================================================================================
+struct VlGemm {
+  const unsigned short *A, *B;
+  long long lda, ldb;
+  const int* head;                    // weighted rows on the device
+  int M, N, K;                        // capacities; m_live / k_live: M / K is the device's row count instead
+  int n_rows;                         // rows of B that exist (BKC): columns behind them re-read the last one
+  int m_live, k_live, n_split;
+  int v0, V;                          // VL_STATS, VL_DLOG: n is vocabulary column v0 + n, valid below V. VL_DW: m is
+  const float *w, *lse;               // VL_DLOG
+  const int* tgt;
+  f32x2* pairs;                       // VL_STATS: [64-column block][M] (maximum, sum) in base 2
+  unsigned short* dlog;               // VL_DLOG: [M, ldo]
+  float* slab;                        // VL_SLAB: [split][M][N]
+  long long slab_stride, ldo;
+  int add;                            // VL_SLAB: add to what the slab holds
+  const float* gout;                  // VL_DW
+  void* dw;                           // [V, N]: bf16, or fp32 that is added to
+  int dw_f32;
+};
+
+typedef __attribute__((address_space(3))) void vl_lds;
+
+template <int R> __device__ __forceinline__ int vl_kc(int row, int ch) { return R * row + 16 * (ch ^ ((row >> 1) & 7)); }
+template <int R, bool NSIDE> __device__ __forceinline__ int vl_mc(int row, int ch) {
+  return R * row + 16 * (ch ^ (NSIDE ? (((row & 1) << 3) | ((row >> 1) & 1)) : ((row & 3) << 2)));
+}
+__device__ __forceinline__ s16x4 vl_read_tr(const unsigned char* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+}
+__device__ __forceinline__ bf16x8 vl_join(s16x4 a, s16x4 b) {
+  union { struct { s16x4 a, b; } s; bf16x8 v; } u;
+  u.s.a = a; u.s.b = b;
+  return u.v;
+}
+
+template <int BM, int BN, bool AKC, bool BKC, int EPI>
+__global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGemm p) {
+  constexpr int WM = 2, WN = BN / 64, NW = WM * WN, TM = BM / WM / 16, TN = 4;
+  constexpr int SA = BM * 128, SB = BN * 128, STAGE = SA + SB;      // bytes of a 64-deep stage, either layout
+  extern __shared__ __attribute__((aligned(1024))) unsigned char vl_smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int g = lane >> 4, c = lane & 15, q4 = c >> 2, p4 = c & 3;
+  const int live = p.head[0];
+  const int M = p.m_live ? min(live, p.M) : p.M, K = p.k_live ? min((live + 63) & ~63, p.K) : p.K;      // (whole stages of rows: zeros behind the last)
+  // tile list: groups of 8 tile rows, column by column inside a group; each XCD takes one contiguous part
+  const int tiles_m = (M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN, n_all = tiles_m * tiles_n * p.n_split;
+  int tile;
+  {
+    const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, q = n_all >> 3, rr = n_all & 7;
+    if (j >= q + (xcd < rr ? 1 : 0)) return;
+    tile = (xcd < rr ? xcd * (q + 1) : rr * (q + 1) + (xcd - rr) * q) + j;
+  }
+  const int split = tile / (tiles_m * tiles_n);
+  tile -= split * tiles_m * tiles_n;
+  const int group = tile / (8 * tiles_n), rows_here = min(tiles_m - 8 * group, 8), in_group = tile - group * 8 * tiles_n;
+  const int m0 = (8 * group + in_group % rows_here) * BM, n0 = (in_group / rows_here) * BN;
+  const int kt_all = (K + 63) >> 6, kt_per = (kt_all + p.n_split - 1) / p.n_split;
+  const int kt_beg = min(split * kt_per, kt_all), kt_end = min(kt_beg + kt_per, kt_all);
+
+  // ---- staging: wave w sends pieces w, w + NW, ...; a lane's offset inside a stage's source is fixed but in a last
+  //      stage that ends inside (summed axis along the rows), where rows past the end re-read the last one
+  constexpr int PA = SA / 1024 / NW, PB = SB / 1024 / NW;
+  auto off_a = [&](int j, int k0) -> unsigned {
+    const int at = (wave + NW * j) * 1024 + lane * 16;
+    if (AKC) {
+      const int row = at >> 7, ch = ((at >> 4) & 7) ^ ((row >> 1) & 7);
+      return (unsigned)(((long long)(min(m0 + row, p.M - 1) - m0) * p.lda + 8 * ch) * 2);
+    }
+    constexpr int R = 2 * BM;
+    const int row = at / R, ch = (vl_mc<R, false>(row, (at % R) >> 4) - R * row) >> 4;
+    return (unsigned)(((long long)min(row, K - 1 - k0) * p.lda + min(m0 + 8 * ch, p.M - 8) - m0) * 2);
+  };
+  auto off_b = [&](int j, int k0) -> unsigned {
+    const int at = (wave + NW * j) * 1024 + lane * 16;
+    if (BKC) {
+      const int rx = at >> 7, ch = ((at >> 4) & 7) ^ ((rx >> 1) & 7);
+      const int i = rx & 15, n = 64 * (rx >> 6) + 16 * (i >> 2) + 4 * ((rx >> 4) & 3) + (i & 3);     // permuted: see above
+      return (unsigned)(((long long)(min(n0 + n, p.n_rows - 1) - n0) * p.ldb + 8 * ch) * 2);
+    }
+    constexpr int R = 2 * BN;
+    const int row = at / R, ch = (vl_mc<R, true>(row, (at % R) >> 4) - R * row) >> 4;
+    return (unsigned)(((long long)min(row, K - 1 - k0) * p.ldb + min(n0 + 8 * ch, p.N - 8) - n0) * 2);
+  };
+  unsigned va[PA], vb[PB];
+#pragma unroll
+  for (int j = 0; j < PA; ++j) va[j] = off_a(j, 0);
+#pragma unroll
+  for (int j = 0; j < PB; ++j) vb[j] = off_b(j, 0);
+  const unsigned lds0 = (unsigned)(size_t)(vl_lds*)vl_smem;
+  auto glds = [&](const unsigned char* src, unsigned vo, unsigned dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(vo), "s"(src) : "memory", "m0");
+  };
+  auto issue = [&](int kt, int buf) {
+    const unsigned base = lds0 + buf * STAGE;
+    const unsigned char* sa = (const unsigned char*)(AKC ? p.A + (long long)m0 * p.lda + 64ll * kt : p.A + 64ll * kt * p.lda + m0);
+    const unsigned char* sb = (const unsigned char*)(BKC ? p.B + (long long)n0 * p.ldb + 64ll * kt : p.B + 64ll * kt * p.ldb + n0);
+    const bool ragged = 64 * kt + 64 > K;
+#pragma unroll
+    for (int j = 0; j < PA; ++j) glds(sa, !AKC && ragged ? off_a(j, 64 * kt) : va[j], base + (wave + NW * j) * 1024);
+#pragma unroll
+    for (int j = 0; j < PB; ++j) glds(sb, !BKC && ragged ? off_b(j, 64 * kt) : vb[j], base + SA + (wave + NW * j) * 1024);
+  };
+
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  if (kt_beg < kt_end) issue(kt_beg, 0);
+  int buf = 0;
+  for (int kt = kt_beg; kt < kt_end; ++kt, buf ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (kt + 1 < kt_end) issue(kt + 1, buf ^ 1);
+    const unsigned char* const As = vl_smem + buf * STAGE;
+    const unsigned char* const Bs = As + SA;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      bf16x8 x[TN];
+#pragma unroll
+      for (int tn = 0; tn < TN; ++tn) {
+        if (BKC) {
+          x[tn] = *(const bf16x8*)(Bs + vl_kc<128>(64 * wn + 16 * tn + c, 4 * kk + g));
+        } else {
+          constexpr int R = 2 * BN;
+          const int r0 = 32 * kk + 8 * g + q4, ch = 8 * wn + 2 * p4 + (tn >> 1);
+          x[tn] = vl_join(vl_read_tr(Bs + vl_mc<R, true>(r0, ch) + 8 * (tn & 1)), vl_read_tr(Bs + vl_mc<R, true>(r0 + 4, ch) + 8 * (tn & 1)));
+        }
+      }
+#pragma unroll
+      for (int tm = 0; tm < TM; ++tm) {
+        bf16x8 y;
+        if (AKC) {
+          y = *(const bf16x8*)(As + vl_kc<128>(16 * TM * wm + 16 * tm + c, 4 * kk + g));
+        } else {
+          constexpr int R = 2 * BM;
+          const int r0 = 32 * kk + 8 * g + q4, ch = 2 * (TM * wm + tm) + (p4 >> 1);
+          y = vl_join(vl_read_tr(As + vl_mc<R, false>(r0, ch) + 8 * (p4 & 1)), vl_read_tr(As + vl_mc<R, false>(r0 + 4, ch) + 8 * (p4 & 1)));
+        }
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn) acc[tm][tn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[tn], y, acc[tm][tn], 0, 0, 0);
+      }
+    }
+  }
+
+  // ---- lane: row m0 + 16 (TM wm + tm) + c, columns nb + 4 tn + j
+  const int nb = n0 + 64 * wn + 16 * g;
+  float coef = 0.f;
+  if (EPI == VL_DW) {
+    const float sw = ((const float*)p.head)[1];
+    coef = sw > 0.f ? p.gout[0] / sw : 0.f;
+  }
+#pragma unroll
+  for (int tm = 0; tm < TM; ++tm) {
+    const int m = m0 + 16 * (TM * wm + tm) + c;
+    if (EPI == VL_STATS) {
+      float mx = -INFINITY, se = 0.f;
+#pragma unroll
+      for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[tm][tn][j] = p.v0 + nb + 4 * tn + j < p.V ? acc[tm][tn][j] * VL_LOG2E : -INFINITY;
+          mx = fmaxf(mx, acc[tm][tn][j]);
+        }
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+      for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) se += __builtin_amdgcn_exp2f(acc[tm][tn][j] - ref);
+      se += __shfl_xor(se, 16, 64);
+      se += __shfl_xor(se, 32, 64);
+      if (g == 0 && m < M && n0 + 64 * wn < p.N) p.pairs[(long long)((n0 >> 6) + wn) * p.M + m] = (f32x2){mx, se};
+    } else if (EPI == VL_DLOG) {
+      // (rows behind the last weighted one: zeros, they are summed over by dW's product)
+      const bool in = m < M;
+      const int tcol = in ? p.tgt[m] - p.v0 - nb : -1;
+      const float lse = in ? p.lse[m] : 0.f, w = in ? p.w[m] : 0.f;
+      float v[16];
+#pragma unroll
+      for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int col = 4 * tn + j;
+          const float pr = __builtin_amdgcn_exp2f(acc[tm][tn][j] * VL_LOG2E - lse);
+          v[col] = in && p.v0 + nb + col < p.V ? w * (pr - (col == tcol ? 1.f : 0.f)) : 0.f;
+        }
+      if (nb < p.N) {
+        u32x4 lo, hi;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { lo[i] = bd_pack_bf16x2(v[2 * i], v[2 * i + 1]); hi[i] = bd_pack_bf16x2(v[8 + 2 * i], v[9 + 2 * i]); }
+        unsigned short* o = p.dlog + (long long)m * p.ldo + nb;
+        *(u32x4*)o = lo;
+        *(u32x4*)(o + 8) = hi;
+      }
+    } else if (EPI == VL_SLAB) {
+      if (m < M && nb < p.N) {
+        float* o = p.slab + split * p.slab_stride + (long long)m * p.ldo + nb;
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn) {
+          f32x4 x = acc[tm][tn];
+          if (p.add) {
+            const f32x4 y = *(const f32x4*)(o + 4 * tn);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] += y[j];
+          }
+          *(f32x4*)(o + 4 * tn) = x;
+        }
+      }
+    } else {
+      if (p.v0 + m < p.V && nb < p.N) {
+        const long long at = (long long)(p.v0 + m) * p.ldo + nb;
+        if (p.dw_f32) {
+          float* o = (float*)p.dw + at;
+#pragma unroll
+          for (int tn = 0; tn < TN; ++tn) {
+            f32x4 y = *(const f32x4*)(o + 4 * tn);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] += coef * acc[tm][tn][j];
+            *(f32x4*)(o + 4 * tn) = y;
+          }
+        } else {
+          u32x4 lo, hi;
+          lo[0] = bd_pack_bf16x2(coef * acc[tm][0][0], coef * acc[tm][0][1]); lo[1] = bd_pack_bf16x2(coef * acc[tm][0][2], coef * acc[tm][0][3]);
+          lo[2] = bd_pack_bf16x2(coef * acc[tm][1][0], coef * acc[tm][1][1]); lo[3] = bd_pack_bf16x2(coef * acc[tm][1][2], coef * acc[tm][1][3]);
+          hi[0] = bd_pack_bf16x2(coef * acc[tm][2][0], coef * acc[tm][2][1]); hi[1] = bd_pack_bf16x2(coef * acc[tm][2][2], coef * acc[tm][2][3]);
+          hi[2] = bd_pack_bf16x2(coef * acc[tm][3][0], coef * acc[tm][3][1]); hi[3] = bd_pack_bf16x2(coef * acc[tm][3][2], coef * acc[tm][3][3]);
+          unsigned short* o = (unsigned short*)p.dw + at;
+          *(u32x4*)o = lo;
+          *(u32x4*)(o + 8) = hi;
+        }
+      }
+    }
+  }
+}
+
+// one wave per weighted row: joins the row's pairs and computes the target's score; rowloss[r] = w (lse - z_t)
+__global__ __launch_bounds__(256) void vl_join_kernel(VlState st, const unsigned short* __restrict__ weight, const f32x2* __restrict__ pairs,
+                                                      float* __restrict__ rowloss, int cap, int blocks, int d) {
+  const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= st.head[0]) return;
+  float m = -INFINITY, s = 0.f;
+  for (int i = lane; i < blocks; i += 64) {
+    const f32x2 x = pairs[(long long)i * cap + row];
+    const float mn = fmaxf(m, x[0]);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    s = s * __builtin_amdgcn_exp2f(m - ref) + x[1] * __builtin_amdgcn_exp2f(x[0] - ref);
+    m = mn;
+  }
+  const float mm = bd_wave_max(m);
+  const float ref = mm == -INFINITY ? 0.f : mm;
+  s = bd_wave_sum(s * __builtin_amdgcn_exp2f(m - ref));
+  const float lse = ref + __log2f(s);
+  const int t = st.tgt[row];
+  float z = 0.f;
+  if (t >= 0) {
+    const unsigned short *x = st.hc + (long long)row * d, *y = weight + (long long)t * d;
+    for (int i = 8 * lane; i < d; i += 512) {
+      const bf16x8 a = *(const bf16x8*)(x + i), b = *(const bf16x8*)(y + i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z += (float)a[e] * (float)b[e];
+    }
+  }
+  z = bd_wave_sum(z);
+  if (lane == 0) {
+    st.lse[row] = lse;
+    rowloss[row] = t >= 0 ? st.w[row] * (lse * VL_LN2 - z) : __uint_as_float(0x7fc00000u);
+  }
+}
+
+// loss = sum rowloss / sum w, in a fixed order; an exact zero without a weighted row
+__global__ __launch_bounds__(1024) void vl_finish_kernel(VlState st, const float* __restrict__ rowloss, float* __restrict__ loss) {
+  __shared__ float part[16];
+  const int n = st.head[0];
+  float s = 0.f;
+  for (int i = threadIdx.x; i < n; i += 1024) s += rowloss[i];
+  s = bd_wave_sum(s);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float t = 0.f;
+    for (int i = 0; i < 16; ++i) t += part[i];
+    const float sw = ((const float*)st.head)[1];
+    loss[0] = sw > 0.f ? t / sw : 0.f;
+  }
+}
+
+// dhidden rows from the slabs (added in order), zeros at rows without a weight
+__global__ __launch_bounds__(256) void vl_dh_kernel(VlState st, const float* __restrict__ slab, long long slab_stride, int n_slab,
+                                                    const float* __restrict__ gout, unsigned short* __restrict__ dh, int M, int d) {
+  const int per = d / 8;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long long)M * per) return;
+  const int row = (int)(i / per), ch = (int)(i - (long long)row * per);
+  const int at = st.pos[row];
+  u32x4 o = {0u, 0u, 0u, 0u};
+  if (at >= 0) {
+    const float sw = ((const float*)st.head)[1];
+    const float coef = sw > 0.f ? gout[0] / sw : 0.f;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < n_slab; ++s) {
+      const float* p = slab + s * slab_stride + (long long)at * d + 8 * ch;
+      const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { v[e] += a[e]; v[4 + e] += b[e]; }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = bd_pack_bf16x2(coef * v[2 * e], coef * v[2 * e + 1]);
+  }
+  *(u32x4*)(dh + (long long)row * d + 8 * ch) = o;
+}
+
+// dW rows v0 .. v0 + rows from the slabs of their splits
+__global__ __launch_bounds__(256) void vl_dw_kernel(VlState st, const float* __restrict__ slab, long long slab_stride, int n_slab,
+                                                    const float* __restrict__ gout, void* __restrict__ dw, int dw_f32, int v0, int rows, int d) {
+  const int per = d / 8;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long long)rows * per) return;
+  const float sw = ((const float*)st.head)[1];
+  const float coef = sw > 0.f ? gout[0] / sw : 0.f;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < n_slab; ++s) {
+    const float* p = slab + s * slab_stride + 8 * i;
+    const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { v[e] += a[e]; v[4 + e] += b[e]; }
+  }
+  const long long at = (long long)v0 * d + 8 * i;
+  if (dw_f32) {
+    float* o = (float*)dw + at;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] += coef * v[e];
+  } else {
+    u32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = bd_pack_bf16x2(coef * v[2 * e], coef * v[2 * e + 1]);
+    *(u32x4*)((unsigned short*)dw + at) = o;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+struct VlPlan {
+  long long m_pad;
+  int piece, n_pieces;                // vocabulary columns per backward piece
+  int big;                            // 256 x 256 tiles
+  int split_h, split_w;               // splits of dh's product over the piece, of dW's over the rows
+  long long slab_h, slab_w;           // floats of one slab
+  long long fwd_bytes, bwd_bytes;
+};
+
+constexpr long long VL_PIECE_BYTES = 256ll << 20;      // dz of one piece: what stays near the card's last-level cache
+
+int vl_splits(long long tiles, long long k_tiles) {
+  // one workgroup per CU and more where the axis is long enough for four stages each
+  long long n = tiles >= 256 ? 1 : (256 + tiles - 1) / tiles;
+  if (n > k_tiles / 4) n = k_tiles / 4;
+  return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+}
+
+VlPlan vl_plan(long long M, int d, int V) {
+  VlPlan p;
+  p.m_pad = vl_up(M, 256);
+  p.big = (p.m_pad / 256) * ((V + 255) / 256) >= 256;
+  const int bt = p.big ? 256 : 128;
+  long long piece = VL_PIECE_BYTES / 2 / p.m_pad / 256 * 256;
+  if (piece < 256) piece = 256;
+  const long long v_pad = vl_up(V, 256);
+  if (piece > v_pad) piece = v_pad;
+  p.n_pieces = (int)((v_pad + piece - 1) / piece);
+  p.piece = (int)vl_up((v_pad + p.n_pieces - 1) / p.n_pieces, 256);
+  p.split_h = vl_splits(vl_up(M, bt) / bt * (vl_up(d, bt) / bt), p.piece / 64);
+  p.split_w = vl_splits(vl_up(p.piece, bt) / bt * (vl_up(d, bt) / bt), p.m_pad / 64);
+  p.slab_h = p.m_pad * d;
+  p.slab_w = (long long)p.piece * d;
+  const long long groups = (M + SCAN - 1) / SCAN;
+  p.fwd_bytes = vl_up(groups * 4, 256) * 2 + vl_up(p.m_pad * 4, 256) + (v_pad / 64) * p.m_pad * 8;
+  p.bwd_bytes = p.m_pad * p.piece * 2 + (p.split_h * p.slab_h + (p.split_w > 1 ? p.split_w * p.slab_w : 0)) * 4;
+  return p;
+}
+
+template <bool AKC, bool BKC, int EPI>
+void vl_launch(const VlPlan& pl, const VlGemm& p, hipStream_t s) {
+  const int bt = pl.big ? 256 : 128;
+  const long long n = vl_up(p.M, bt) / bt * (vl_up(p.N, bt) / bt) * p.n_split;
+  const dim3 grid((unsigned)vl_up(n, 8));
+  if (pl.big) {
+    BD_SET_MAX_LDS((vl_gemm_kernel<256, 256, AKC, BKC, EPI>), 131072);
+    hipLaunchKernelGGL((vl_gemm_kernel<256, 256, AKC, BKC, EPI>), grid, dim3(512), 131072, s, p);
+  } else {
+    hipLaunchKernelGGL((vl_gemm_kernel<128, 128, AKC, BKC, EPI>), grid, dim3(256), 65536, s, p);
+  }
+}
+
+int vl_check(long long M, int d, int V, const char* what) {
+  BD_REQUIRE(M > 0 && V > 0 && d > 0, "%s: empty shape", what);
+  BD_REQUIRE(d % 64 == 0, "%s: the hidden size %d must be a multiple of 64", what, d);
+  BD_REQUIRE(M < (1ll << 24) && V < (1 << 28) && d <= 65536, "%s: too many rows, columns or classes", what);
+  return BD_OK;
+}
+
+}  // namespace
+
+extern "C" long long bd_linear_ce_state_bytes(long long M, int d) { return M > 0 && d > 0 ? vl_state(nullptr, M, d).bytes : -1; }
+
+extern "C" long long bd_linear_ce_workspace_bytes(long long M, int d, int V, int backward) {
+  if (M <= 0 || d <= 0 || V <= 0) return -1;
+  const VlPlan p = vl_plan(M, d, V);
+  return backward ? p.bwd_bytes : p.fwd_bytes;
+}
+
+extern "C" int bd_linear_ce_fwd(const void* hidden, const void* weight, const long long* targets, const unsigned char* indicator,
+                                const long long* attention_mask, float* loss, long long M, int d, int V, void* state, long long state_bytes,
+                                void* workspace, long long workspace_bytes, void* stream) {
+  const int rc = vl_check(M, d, V, "bd_linear_ce_fwd");
+  if (rc != BD_OK) return rc;
+  BD_REQUIRE(hidden && weight && targets && loss && state && workspace, "bd_linear_ce_fwd: null operand");
+  BD_REQUIRE((((uintptr_t)hidden | (uintptr_t)weight | (uintptr_t)state | (uintptr_t)workspace) & 15) == 0,
+             "bd_linear_ce_fwd: operands must be 16-byte aligned");
+  const VlPlan pl = vl_plan(M, d, V);
+  BD_REQUIRE(state_bytes >= bd_linear_ce_state_bytes(M, d), "bd_linear_ce_fwd: the state must hold %lld bytes", bd_linear_ce_state_bytes(M, d));
+  BD_REQUIRE(workspace_bytes >= pl.fwd_bytes, "bd_linear_ce_fwd: the workspace must hold %lld bytes", pl.fwd_bytes);
+  hipStream_t s = (hipStream_t)stream;
+  const VlState st = vl_state(state, M, d);
+  const int groups = (int)((M + SCAN - 1) / SCAN);
+  char* w = (char*)workspace;
+  int* counts = (int*)w; w += vl_up(groups * 4ll, 256);
+  float* sums = (float*)w; w += vl_up(groups * 4ll, 256);
+  float* rowloss = (float*)w; w += vl_up(pl.m_pad * 4, 256);
+  f32x2* pairs = (f32x2*)w;
+  bd_prof_scope prof(stream, 2.0 * M * (double)V * d, BD_PROF_GEMM);
+  hipLaunchKernelGGL(vl_count_kernel, dim3((groups + 3) / 4), dim3(256), 0, s, indicator, attention_mask, counts, sums, (int)M);
+  hipLaunchKernelGGL(vl_gather_kernel, dim3(groups), dim3(256), 0, s, (const unsigned short*)hidden, targets, indicator, attention_mask, counts,
+                     sums, st, (int)M, d, V);
+  VlGemm p = {};
+  p.A = st.hc; p.lda = d; p.B = (const unsigned short*)weight; p.ldb = d; p.head = st.head;
+  p.M = (int)pl.m_pad; p.N = V; p.n_rows = V; p.K = d; p.m_live = 1; p.n_split = 1; p.V = V; p.pairs = pairs;
+  vl_launch<true, true, VL_STATS>(pl, p, s);
+  hipLaunchKernelGGL(vl_join_kernel, dim3((unsigned)((M + 3) / 4)), dim3(256), 0, s, st, (const unsigned short*)weight, pairs, rowloss,
+                     (int)pl.m_pad, (V + 63) / 64, d);
+  hipLaunchKernelGGL(vl_finish_kernel, dim3(1), dim3(1024), 0, s, st, rowloss, loss);
+  return bd_check_launch("bd_linear_ce_fwd");
+}
+
+extern "C" int bd_linear_ce_bwd(const void* weight, const float* grad_out, void* dhidden, void* dweight, int dweight_dtype, long long M, int d,
+                                int V, const void* state, long long state_bytes, void* workspace, long long workspace_bytes, void* stream) {
+  const int rc = vl_check(M, d, V, "bd_linear_ce_bwd");
+  if (rc != BD_OK) return rc;
+  BD_REQUIRE(weight && grad_out && (dhidden || dweight) && state && workspace, "bd_linear_ce_bwd: null operand");
+  BD_REQUIRE((((uintptr_t)weight | (uintptr_t)dhidden | (uintptr_t)dweight | (uintptr_t)state | (uintptr_t)workspace) & 15) == 0,
+             "bd_linear_ce_bwd: operands must be 16-byte aligned");
+  BD_REQUIRE(dweight_dtype == BD_DTYPE_BF16 || dweight_dtype == BD_DTYPE_F32, "bd_linear_ce_bwd: dweight is neither bf16 nor fp32");
+  const VlPlan pl = vl_plan(M, d, V);
+  BD_REQUIRE(state_bytes >= bd_linear_ce_state_bytes(M, d), "bd_linear_ce_bwd: the state must hold %lld bytes", bd_linear_ce_state_bytes(M, d));
+  BD_REQUIRE(workspace_bytes >= pl.bwd_bytes, "bd_linear_ce_bwd: the workspace must hold %lld bytes", pl.bwd_bytes);
+  hipStream_t s = (hipStream_t)stream;
+  const VlState st = vl_state((void*)state, M, d);
+  unsigned short* dlog = (unsigned short*)workspace;
+  float* slab_h = (float*)((char*)workspace + pl.m_pad * pl.piece * 2);
+  float* slab_w = slab_h + pl.split_h * pl.slab_h;
+  bd_prof_scope prof(stream, 6.0 * M * (double)V * d, BD_PROF_GEMM);
+  for (int i = 0; i < pl.n_pieces; ++i) {
+    const int v0 = i * pl.piece, n = min(pl.piece, (int)vl_up(V - v0, 64));       // columns of the piece, whole 64s
+    if (v0 >= V) break;
+    const unsigned short* wp = (const unsigned short*)weight + (long long)v0 * d;
+    VlGemm p = {};
+    p.A = st.hc; p.lda = d; p.B = wp; p.ldb = d; p.head = st.head; p.M = (int)pl.m_pad; p.N = n; p.n_rows = min(n, V - v0); p.K = d; p.m_live = 1; p.n_split = 1;
+    p.v0 = v0; p.V = V; p.w = st.w; p.lse = st.lse; p.tgt = st.tgt; p.dlog = dlog; p.ldo = pl.piece;
+    vl_launch<true, true, VL_DLOG>(pl, p, s);
+    if (dhidden) {
+      p = VlGemm();
+      p.A = dlog; p.lda = pl.piece; p.B = wp; p.ldb = d; p.head = st.head; p.M = (int)pl.m_pad; p.N = d; p.K = min(n, V - v0); p.m_live = 1;
+      p.n_split = pl.split_h; p.slab = slab_h; p.slab_stride = pl.slab_h; p.ldo = d; p.add = i > 0;
+      vl_launch<true, false, VL_SLAB>(pl, p, s);
+    }
+    if (dweight) {
+      p = VlGemm();
+      p.A = dlog; p.lda = pl.piece; p.B = st.hc; p.ldb = d; p.head = st.head; p.M = n; p.N = d; p.K = (int)pl.m_pad; p.k_live = 1;
+      p.n_split = pl.split_w; p.v0 = v0; p.V = V; p.ldo = d;
+      if (pl.split_w > 1) {
+        p.slab = slab_w; p.slab_stride = pl.slab_w;
+        vl_launch<false, false, VL_SLAB>(pl, p, s);
+        const int rows = min(n, V - v0);
+        const long long items = (long long)rows * (d / 8);
+        hipLaunchKernelGGL(vl_dw_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, st, slab_w, pl.slab_w, pl.split_w, grad_out,
+                           dweight, dweight_dtype == BD_DTYPE_F32, v0, rows, d);
+      } else {
+        p.gout = grad_out; p.dw = dweight; p.dw_f32 = dweight_dtype == BD_DTYPE_F32;
+        vl_launch<false, false, VL_DW>(pl, p, s);
+      }
+    }
+  }
+  if (dhidden)
+    hipLaunchKernelGGL(vl_dh_kernel, dim3((unsigned)((M * (d / 8) + 255) / 256)), dim3(256), 0, s, st, slab_h, pl.slab_h, pl.split_h, grad_out,
+                       (unsigned short*)dhidden, (int)M, d);
+  return bd_check_launch("bd_linear_ce_bwd");
+}

@@ -761,6 +761,88 @@ int bd_gemm_bf16_tile256(const void* A, const void* W, const float* bias, void* 
  * slower kernel. stamps = null (the initial state) turns the stamps off; process-wide, not thread-safe. */
 int bd_clock_stamps_set(unsigned long long* stamps, int n_workgroups);
 
+/* ---------------------------------------------------------------- stand-alone operators */
+
+#define BD_DTYPE_BF16 0
+#define BD_DTYPE_F32 1
+
+/* Rotary positions: in every head the first rotary_dim values are turned pair by pair,
+ *   y_a = x_a cos - x_b sin, y_b = x_a sin + x_b cos
+ * with (a, b) = (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when interleaved; the others are copied. table
+ * [table_rows, rotary_dim / 2, 2] fp32 holds (cos, sin) of every position; positions [b * position_stride + l] (int64),
+ * or null for position l. A position outside the table reads nothing and makes the turned values of that token NaN.
+ * inverse: the sine's sign turned, i.e. the gradient. One launch serves one or two tensors (queries and keys) of one
+ * dtype (BD_DTYPE_*) and head size; strides are in elements (batch, token, head), the last axis is contiguous.
+ * dst may be src (same strides). Stands beside bd_embed's table of learned positions. */
+typedef struct {
+  const void* src;
+  void* dst;
+  long long src_stride[3], dst_stride[3];
+  int n_heads;
+} bd_rotary_tensor;
+int bd_rotary(const bd_rotary_tensor* tensors, int n_tensors, const float* table, int table_rows, const long long* positions,
+              long long position_stride, int B, int L, int head_dim, int rotary_dim, int interleaved, int inverse, int dtype,
+              void* stream);
+
+/* Differential attention, the difference of two softmax maps:
+ *   out_i = sum_j (P1_ij - lam_i P2_ij) v_j,  Pm_ij = softmax_j(scale q_im . k_jm) over the visible keys j,
+ * bf16, every query sees every visible key of its sequence; a query without one yields a zero row. H heads: head h's
+ * maps are query heads 2 h and 2 h + 1 (head_dim 32, 64 or 128) against key heads 2 hk and 2 hk + 1 and value head hk
+ * (width 2 head_dim), hk = h / (H / Hkv). lam: one weight per (row, head), bf16 or fp32 (BD_DTYPE_*).
+ * Padded batches: B sequences of Lq queries and Lk keys; key_mask (non-zero = visible) or null. Packed rows: cu_seqlens
+ * [B + 1] (int32, device), sequence b = rows cu[b] .. cu[b + 1] - 1 of all operands, Lq = Lk = the longest sequence,
+ * total_rows rows in all (batch strides are not used; rows behind cu[B] become zero in every output, rows of a sequence
+ * behind Lq become NaN in out). What masked keys hold never reaches a result. Strides are in elements (batch, row,
+ * head), multiples of 8 but for lam's (0 = shared), the last axis is contiguous; operands are 16-byte aligned.
+ * Training: lse [rows, H, 2] fp32 (base-2 log-sum-exp of the scaled scores; rows counted through the batch) and, beyond
+ * short sequences, maps [rows, H, 2, 2 head_dim] fp32 (each map's own output) are written by the forward and read by
+ * the backward (maps may be null in both: the backward then walks the keys once more). Backward: dq, dk, dv bf16 and
+ * dlam [rows, H] fp32 are overwritten. Workspaces of bd_diff_attention_workspace_bytes(args, backward) bytes; equal
+ * calls give equal bits. Stands beside bd_attention_fwd / bd_attention_bwd. */
+typedef struct {
+  const void *q, *k, *v, *lam;
+  long long q_stride[3], k_stride[3], v_stride[3], lam_stride[3], out_stride[3];
+  int lam_dtype;
+  const unsigned char* key_mask;
+  long long key_mask_stride;
+  const int* cu_seqlens;
+  int total_rows;
+  int B, Lq, Lk, H, Hkv, head_dim;
+  float scale;
+  void* out;
+  float *lse, *maps;
+  void* workspace;
+  long long workspace_bytes;
+  const void* dout;
+  void *dq, *dk, *dv;
+  float* dlam;
+  long long dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} bd_diff_attn_args;
+long long bd_diff_attention_workspace_bytes(const bd_diff_attn_args* args, int backward);
+int bd_diff_attention_fwd(const bd_diff_attn_args* args, void* stream);
+int bd_diff_attention_bwd(const bd_diff_attn_args* args, void* stream);
+/* dlam [B, L, H] fp32 as the backward leaves it, summed over the axes along which lam was broadcast (keep_* = 0), in
+ * out_dtype (BD_DTYPE_*), kept axes in order (packed rows: B = 1). */
+int bd_diff_attention_dlam(const float* dlam, void* out, int out_dtype, int B, int L, int H, int keep_b, int keep_l, int keep_h,
+                           void* stream);
+
+/* Masked cross-entropy of the vocabulary head, logits = hidden weight^T never stored: hidden [M, d] and weight [V, d]
+ * bf16 (contiguous, d a multiple of 64), weights of the rows as in bd_masked_ce_fwd (indicator * attention_mask, either
+ * may be null = ones). loss[0] = sum(w * ce) / sum(w), exactly 0 when no row carries weight. Rows without weight are
+ * never read; a weighted row whose target lies outside [0, V) makes the loss NaN. The forward leaves what the backward
+ * needs (the weighted rows, their targets, weights and log-sum-exps) in state (bd_linear_ce_state_bytes(M, d) bytes);
+ * workspaces of bd_linear_ce_workspace_bytes(M, d, V, backward) bytes are scratch. Backward, times grad_out[0]:
+ * dhidden [M, d] bf16 (overwritten; zeros at rows without weight) and dweight [V, d], bf16 overwritten or fp32 ADDED to
+ * (as the weight-gradient products of this library do); either may be null. Equal calls give equal bits.
+ * Stands beside bd_masked_ce_fwd / bd_masked_ce_bwd, which read the logits from memory. */
+long long bd_linear_ce_state_bytes(long long M, int d);
+long long bd_linear_ce_workspace_bytes(long long M, int d, int V, int backward);
+int bd_linear_ce_fwd(const void* hidden, const void* weight, const long long* targets, const unsigned char* indicator,
+                     const long long* attention_mask, float* loss, long long M, int d, int V, void* state, long long state_bytes,
+                     void* workspace, long long workspace_bytes, void* stream);
+int bd_linear_ce_bwd(const void* weight, const float* grad_out, void* dhidden, void* dweight, int dweight_dtype, long long M, int d,
+                     int V, const void* state, long long state_bytes, void* workspace, long long workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
