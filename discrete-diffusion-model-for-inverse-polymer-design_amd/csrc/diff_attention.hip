@@ -22,6 +22,8 @@
 #include "bd_prof.h"
 #include "bidiff.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int KT = 64;         // keys (or query slots) per staged tile
@@ -36,6 +38,7 @@ struct DaArgs {
   const int* cu;
   long long qs[3], ks[3], vs[3], ls[3], os[3], dos[3], dqs[3], dks[3], dvs[3], mask_stride;
   int B, Lq, Lk, H, Hkv, share, total, lam_f32, n_blk, n_split;
+  int small_strides;             // 64 rows of every operand lie within 4 GiB: staged by 32-bit offsets
   float scale;
 };
 
@@ -43,9 +46,9 @@ __device__ __attribute__((aligned(64))) const unsigned int bd_da_zero[16] = {};
 
 typedef __attribute__((address_space(3))) void da_lds;
 
-// Byte offset of 16-byte chunk ch of row `row` in a tile of R-byte rows. The XOR spreads what is read at a time over the
-// banks: eight rows 0-3 / 8-11 (or 4-7 / 12-15) at one chunk by ds_read_b128, four neighbouring rows of 32 bytes by the
-// transposing read.
+// A staged tile has rows of R bytes; 16-byte chunk ch of row `row` sits at chunk ch ^ f(row). The XOR spreads what is read
+// at a time over the banks: eight rows 0-3 / 8-11 (or 4-7 / 12-15) at one chunk by ds_read_b128, four neighbouring rows of
+// 32 bytes by the transposing read.
 template <int R>
 __device__ __forceinline__ int da_off(int row, int ch) {
   const int f = R >= 256 ? (((row & 3) << 2) | ((row >> 2) & 3))
@@ -54,40 +57,114 @@ __device__ __forceinline__ int da_off(int row, int ch) {
   return R * row + 16 * (ch ^ f);
 }
 
-__device__ __forceinline__ s16x4 da_read_tr(const unsigned char* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
-}
+typedef __attribute__((address_space(3))) const bf16x8 da_lds_b128;
+typedef __attribute__((address_space(3))) s16x4 da_lds_b64;
 
-// 16 (key) x 8 operand of a transposed product: rows r0 .. r0 + 3 and r0 + 4 .. r0 + 7 of the tile, columns 16 dt ..
+// Operand reads. Both take one per-lane base (with the tile's address added) and reach every fragment of the tile by an
+// XOR and a constant offset: row bits that enter f beside the lane's own (the 4 that tells the halves of 8 rows apart)
+// flip one bit, chunk bits above the lane's own flip theirs. One register instead of one per fragment.
+// natural rows: lane (g, c) reads row 32 h2 + 8 (c >> 2) + 4 half + (c & 3), chunk 4 ks + g
 template <int R>
-__device__ __forceinline__ bf16x8 da_frag_tr(const unsigned char* tile, int r0, int dt, int p4) {
-  const int ch = 2 * dt + (p4 >> 1);
+__device__ __forceinline__ unsigned da_nat_base(int g, int c) { return (unsigned)da_off<R>(8 * (c >> 2) + (c & 3), g); }
+template <int R>
+__device__ __forceinline__ bf16x8 da_nat(unsigned base, int h2, int half, int ks) {
+  const unsigned flip = (R >= 128 && half ? 16u : 0u) | (64u * (unsigned)(ks & (R >= 256 ? 3 : 1)));
+  const unsigned add = (32 * h2 + 4 * half) * R + (R == 512 ? 256 * (ks >> 2) : 0);
+  return *(da_lds_b128*)(size_t)((base ^ flip) + add);
+}
+// transposed: 8 rows (32 h2 + 8 g ..) x 16 columns (16 dt ..) as an operand whose summed axis runs along the rows
+template <int R>
+__device__ __forceinline__ unsigned da_tr_base(int g, int c) {
+  return (unsigned)(da_off<R>(8 * g + (c >> 2), (c & 3) >> 1) + 8 * (c & 1));
+}
+template <int R>
+__device__ __forceinline__ bf16x8 da_tr(unsigned base, int h2, int dt) {
+  const unsigned flip = 32u * (unsigned)(dt & (R >= 256 ? 7 : R == 128 ? 3 : 1));
+  const unsigned add = 32 * h2 * R + (R == 512 ? 256 * (dt >> 3) : 0);
   union { struct { s16x4 a, b; } s; bf16x8 v; } u;
-  u.s.a = da_read_tr(tile + da_off<R>(r0, ch) + 8 * (p4 & 1));
-  u.s.b = da_read_tr(tile + da_off<R>(r0 + 4, ch) + 8 * (p4 & 1));
+  u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_lds_b64*)(size_t)((base ^ flip) + add));
+  u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_lds_b64*)(size_t)((base ^ (flip | (R >= 128 ? 16u : 0u))) + add + 4 * R));
   return u.v;
 }
 
 __device__ __forceinline__ void da_dma16(const void* src, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
 }
+// (every lane holds the same pointer; the compiler does not always see that)
+__device__ __forceinline__ const unsigned char* da_uniform(const unsigned char* p) {
+  const unsigned long long x = (unsigned long long)p;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)x), hi = __builtin_amdgcn_readfirstlane((unsigned)(x >> 32));
+  return (const unsigned char*)(((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ void da_dma16s(const void* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
 
-// A tile of KT rows of R bytes to LDS in 1-KiB pieces, dealt to NW waves. row_ptr(row) = the row's first byte, or null
-// for a row that is to be zeros.
+// Staging of KT rows of R bytes in 1-KiB pieces dealt to NW waves: where in the tile a lane's 16 bytes of piece j land
+template <int R, int NW>
+struct DaPieces {
+  static constexpr int ALL = KT * R / 1024, N = (ALL + NW - 1) / NW;
+  static __device__ __forceinline__ int row(int wave, int lane, int j) { return ((wave + NW * j) * 1024 + lane * 16) / R; }
+  static __device__ __forceinline__ int chunk(int wave, int lane, int j) {
+    const int r = row(wave, lane, j), slot = ((wave + NW * j) * 64 + lane) % (R / 16);
+    return (da_off<R>(r, slot) - R * r) >> 4;              // the XOR is its own inverse
+  }
+  static __device__ __forceinline__ bool any(int wave, int j) { return ALL % NW == 0 || wave + NW * j < ALL; }
+};
+
+// rows at base + off[j] (a whole tile inside the tensor, the same offsets tile after tile)
+template <int R, int NW>
+__device__ __forceinline__ void da_stage_fast(unsigned lds, int wave, const unsigned char* base, const unsigned (&off)[DaPieces<R, NW>::N]) {
+  const unsigned char* const from = da_uniform(base);
+#pragma unroll
+  for (int j = 0; j < DaPieces<R, NW>::N; ++j)
+    if (DaPieces<R, NW>::any(wave, j)) da_dma16s(from, off[j], lds + (wave + NW * j) * 1024);
+}
+// row_ptr(row) = the row's first byte, or null for a row that is to be zeros
 template <int R, int NW, typename F>
 __device__ __forceinline__ void da_stage(unsigned lds, int wave, int lane, F row_ptr) {
-  constexpr int PIECES = KT * R / 1024, CPR = R / 16;
 #pragma unroll
-  for (int j = 0; j < (PIECES + NW - 1) / NW; ++j) {
-    const int piece = wave + NW * j;
-    if (PIECES % NW != 0 && piece >= PIECES) break;
-    const int at = piece * 1024 + lane * 16, row = at / R, slot = (at / 16) % CPR;
-    const int ch = ((da_off<R>(row, slot) - R * row) >> 4);       // the XOR is its own inverse
-    const unsigned char* p = row_ptr(row);
-    const unsigned char* src = p ? p + 16 * ch : (const unsigned char*)bd_da_zero;
-    da_dma16(src, lds + piece * 1024);
+  for (int j = 0; j < DaPieces<R, NW>::N; ++j) {
+    if (!DaPieces<R, NW>::any(wave, j)) break;
+    const unsigned char* p = row_ptr(DaPieces<R, NW>::row(wave, lane, j));
+    da_dma16(p ? p + 16 * DaPieces<R, NW>::chunk(wave, lane, j) : (const unsigned char*)bd_da_zero, lds + (wave + NW * j) * 1024);
   }
 }
+
+// Key tiles of one key head: both maps' keys and the values
+template <int D, int NW>
+struct DaKeyStage {
+  static constexpr int RK = 2 * D, RV = 4 * D;
+  const unsigned char *k0, *k1, *v;
+  long long ks, vs;                                        // row strides in bytes
+  unsigned ko[DaPieces<RK, NW>::N], vo[DaPieces<RV, NW>::N];
+  __device__ __forceinline__ void init(const DaArgs& a, long long bq, long long first, int hk, int wave, int lane) {
+    k0 = (const unsigned char*)(a.k + bq * a.ks[0] + first * a.ks[1] + (long long)(2 * hk) * a.ks[2]);
+    k1 = k0 + 2 * a.ks[2];
+    v = (const unsigned char*)(a.v + bq * a.vs[0] + first * a.vs[1] + (long long)hk * a.vs[2]);
+    ks = 2 * a.ks[1]; vs = 2 * a.vs[1];
+#pragma unroll
+    for (int j = 0; j < DaPieces<RK, NW>::N; ++j)
+      ko[j] = (unsigned)ks * DaPieces<RK, NW>::row(wave, lane, j) + 16 * DaPieces<RK, NW>::chunk(wave, lane, j);
+#pragma unroll
+    for (int j = 0; j < DaPieces<RV, NW>::N; ++j)
+      vo[j] = (unsigned)vs * DaPieces<RV, NW>::row(wave, lane, j) + 16 * DaPieces<RV, NW>::chunk(wave, lane, j);
+  }
+  __device__ __forceinline__ void run(const DaArgs& a, unsigned base, int kt0, unsigned long long vis, int wave, int lane) const {
+    if (vis == ~0ull && a.small_strides) {
+      da_stage_fast<RK, NW>(base, wave, k0 + ks * kt0, ko);
+      da_stage_fast<RK, NW>(base + KT * RK, wave, k1 + ks * kt0, ko);
+      da_stage_fast<RV, NW>(base + 2 * KT * RK, wave, v + vs * kt0, vo);
+      return;
+    }
+    auto at = [&](const unsigned char* p, long long st) {
+      return [=](int r) { return ((vis >> r) & 1ull) ? p + st * (kt0 + r) : (const unsigned char*)nullptr; };
+    };
+    da_stage<RK, NW>(base, wave, lane, at(k0, ks));
+    da_stage<RK, NW>(base + KT * RK, wave, lane, at(k1, ks));
+    da_stage<RV, NW>(base + 2 * KT * RK, wave, lane, at(v, vs));
+  }
+};
 
 struct DaSpan {          // one sequence: first row of queries / keys, their counts, the batch index for strides
   long long q0, k0;
@@ -116,6 +193,17 @@ __device__ __forceinline__ int da_visible_end(const DaArgs& a, int b, int Lk, in
   if (!a.mask) return Lk;
   const unsigned char* m = a.mask + b * a.mask_stride;
   int last = 0;
+  if (Lk <= 512) {                                         // every wave by itself: eight loads in flight, no barrier
+    unsigned char x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 64 * i + (tid & 63) < Lk ? m[64 * i + (tid & 63)] : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned long long v = __ballot(x[i] != 0);
+      last = v ? 64 * i + 64 - __builtin_clzll(v) : last;
+    }
+    return last;
+  }
   for (int j = tid; j < Lk; j += NT) last = m[j] ? j + 1 : last;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) last = max(last, __shfl_xor(last, o, 64));
@@ -134,16 +222,28 @@ __device__ __forceinline__ unsigned da_mask_byte(const DaArgs& a, int b, int key
   return *(const volatile unsigned char*)(a.mask + b * a.mask_stride + key);
 }
 
-// block -> (query block or key block, key head, sequence): each XCD works through one contiguous part of the list, so
-// that the blocks of one sequence and head find its rows in their XCD's L2
-__device__ __forceinline__ void da_block(int n_blk, int n_heads, int& blk, int& hk, int& b) {
-  const int n_all = gridDim.x, xcd = blockIdx.x & 7, q = n_all >> 3, rr = n_all & 7;
-  const int lin = (xcd < rr ? xcd * (q + 1) : rr * (q + 1) + (xcd - rr) * q) + (blockIdx.x >> 3);
-  blk = lin % n_blk;
-  const int t = lin / n_blk;
-  hk = t % n_heads;
-  b = t / n_heads;
+// Workgroups are handed to the 8 XCDs in turn (blockIdx & 7). The blocks of one (sequence, key head) group share an XCD, so
+// that they find the group's rows in its L2. Many groups: dealt to the XCDs one by one (ragged sequences then load all XCDs
+// alike); few: the list of all blocks is cut into eight contiguous parts. False: no work for this workgroup.
+__device__ __forceinline__ bool da_block(int n_blk, int n_heads, int seqs, int& blk, int& hk, int& b) {
+  const int groups = n_heads * seqs, xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
+  int grp;
+  if (groups % 8 == 0 || groups >= 64) {
+    grp = (j / n_blk) * 8 + xcd;
+    blk = j % n_blk;
+    if (grp >= groups) return false;
+  } else {
+    const int n_all = groups * n_blk, q = n_all >> 3, rr = n_all & 7;
+    if (j >= q + (xcd < rr ? 1 : 0)) return false;
+    const int lin = (xcd < rr ? xcd * (q + 1) : rr * (q + 1) + (xcd - rr) * q) + j;
+    blk = lin % n_blk;
+    grp = lin / n_blk;
+  }
+  hk = grp % n_heads;
+  b = grp / n_heads;
+  return true;
 }
+inline long long da_grid(long long n_blk, long long groups) { return n_blk * ((groups + 7) / 8) * 8; }
 
 // packed rows that belong to no sequence (behind cu[B]): zeros, heads hk * share .. of width W
 __device__ __forceinline__ void da_zero_tail(unsigned short* p, const long long* st, int first, int end, int head0, int heads,
@@ -159,8 +259,8 @@ __device__ __forceinline__ void da_zero_tail(unsigned short* p, const long long*
 // Forward. Waves work in pairs: wave 2 w + m holds map m of the 16 QB slots of query group w (NQG groups in a
 // workgroup). Split over keys (n_split > 1): each split leaves its unnormalised sums, maximum and normaliser.
 // =====================================================================================
-template <int D, int QB, int NQG>
-__global__ __launch_bounds__(128 * NQG, 2) void da_fwd_kernel(DaArgs a) {
+template <int D, int QB, int NQG, int OCC>
+__global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
   constexpr int E = 2 * D, KS = D / 32, DT = E / 16, NW = 2 * NQG, RK = 2 * D, RV = 2 * E;
   constexpr int TILE = KT * (2 * RK + RV), SLOTS = 16 * QB * NQG;
   extern __shared__ __attribute__((aligned(1024))) unsigned char da_smem[];
@@ -168,9 +268,9 @@ __global__ __launch_bounds__(128 * NQG, 2) void da_fwd_kernel(DaArgs a) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int map = wave & 1, grp = wave >> 1;
-  const int g = lane >> 4, c = lane & 15, q4 = c >> 2, p4 = c & 3;
+  const int g = lane >> 4, c = lane & 15;
   int blk, hk, b;
-  da_block(a.n_blk * a.n_split, a.Hkv, blk, hk, b);
+  if (!da_block(a.n_blk * a.n_split, a.Hkv, a.B + (a.cu ? 1 : 0), blk, hk, b)) return;
   const int split = blk % a.n_split;
   blk /= a.n_split;
   if (a.cu && b == a.B) {                                  // (packed: one more sequence, the rows behind the last one)
@@ -222,44 +322,33 @@ __global__ __launch_bounds__(128 * NQG, 2) void da_fwd_kernel(DaArgs a) {
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[qb][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  const float scale2 = a.scale * LOG2E;
+  const float scale2 = a.scale * LOG2E, slack = 8.f / scale2;
 
-  const unsigned char* const kb0 = (const unsigned char*)(a.k + bq * a.ks[0] + sp.k0 * a.ks[1] + (long long)(2 * hk) * a.ks[2]);
-  const unsigned char* const kb1 = kb0 + 2 * a.ks[2];
-  const unsigned char* const vb = (const unsigned char*)(a.v + bq * a.vs[0] + sp.k0 * a.vs[1] + (long long)hk * a.vs[2]);
+  DaKeyStage<D, NW> keys;
+  keys.init(a, bq, sp.k0, hk, wave, lane);
   const unsigned lds0 = (unsigned)(size_t)(da_lds*)da_smem;
-  auto stage = [&](int kt0, unsigned long long vis, int buf) {
-    const unsigned base = lds0 + buf * TILE;
-    auto at = [&](const unsigned char* p, long long st) {
-      return [=](int r) { return ((vis >> r) & 1ull) ? p + 2 * st * (kt0 + r) : (const unsigned char*)nullptr; };
-    };
-    da_stage<RK, NW>(base, wave, lane, at(kb0, a.ks[1]));
-    da_stage<RK, NW>(base + KT * RK, wave, lane, at(kb1, a.ks[1]));
-    da_stage<RV, NW>(base + 2 * KT * RK, wave, lane, at(vb, a.vs[1]));
-  };
+  const unsigned kbase = da_nat_base<RK>(g, c) + map * KT * RK, vbase = da_tr_base<RV>(g, c) + 2 * KT * RK;
   unsigned mb = da_mask_byte(a, b, kbeg + lane, kend);
   unsigned long long vis = __ballot(mb != 0u);
-  if (kbeg < kend) stage(kbeg, vis, 0);
+  if (kbeg < kend) keys.run(a, lds0, kbeg, vis, wave, lane);
   mb = da_mask_byte(a, b, kbeg + KT + lane, kend);
-  int buf = 0;
-  for (int kt0 = kbeg; kt0 < kend; kt0 += KT, buf ^= 1) {
+  unsigned cur = lds0, other = lds0 + TILE;
+  for (int kt0 = kbeg; kt0 < kend; kt0 += KT) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // this tile is there, nobody reads the other buffer
     const unsigned long long vis_next = __ballot(mb != 0u);
     mb = da_mask_byte(a, b, kt0 + 2 * KT + lane, kend);
-    if (kt0 + KT < kend) stage(kt0 + KT, vis_next, buf ^ 1);
-    const unsigned char* const Ks = da_smem + buf * TILE + map * KT * RK;
-    const unsigned char* const Vs = da_smem + buf * TILE + 2 * KT * RK;
+    if (kt0 + KT < kend) keys.run(a, other, kt0 + KT, vis_next, wave, lane);
+    const unsigned kb = cur + kbase, vb = cur + vbase;
 
     // S^T: s[qb][t][r] <-> key 32 (t >> 1) + 8 g + 4 (t & 1) + r of the tile, slot c of block qb
     f32x4 s[QB][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int krow = 32 * (t >> 1) + 8 * q4 + 4 * (t & 1) + p4;
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) s[qb][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        const bf16x8 kf = *(const bf16x8*)(Ks + da_off<RK>(krow, 4 * ks + g));
+        const bf16x8 kf = da_nat<RK>(kb, t >> 1, t & 1, ks);
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) s[qb][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[qb][ks], s[qb][t], 0, 0, 0);
       }
@@ -279,13 +368,16 @@ __global__ __launch_bounds__(128 * NQG, 2) void da_fwd_kernel(DaArgs a) {
       float mloc = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 4; ++t) mloc = fmaxf(fmaxf(mloc, fmaxf(s[qb][t][0], s[qb][t][1])), fmaxf(s[qb][t][2], s[qb][t][3]));
-      mloc = fmaxf(mloc, __shfl_xor(mloc, 16, 64));
-      mloc = fmaxf(mloc, __shfl_xor(mloc, 32, 64));
-      if (__any(mloc > m_run[qb])) {                       // some slot's maximum rises: rescale what was summed
+      // The reference of the exponentials follows the maximum only when a score passes it by 2^8: weights then reach 2^8 at
+      // most (no less exact in bf16 and fp32), and almost every tile goes without the exchange between a slot's four lanes
+      // and without rescaling.
+      if (__any(mloc > m_run[qb] + slack)) {
+        mloc = fmaxf(mloc, __shfl_xor(mloc, 16, 64));
+        mloc = fmaxf(mloc, __shfl_xor(mloc, 32, 64));
         const float m_new = fmaxf(m_run[qb], mloc);
         const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run[qb] - m_new) * scale2);
-        l_run[qb] *= alpha;
         m_run[qb] = m_new;
+        l_run[qb] *= alpha;
 #pragma unroll
         for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -298,7 +390,7 @@ __global__ __launch_bounds__(128 * NQG, 2) void da_fwd_kernel(DaArgs a) {
         for (int r = 0; r < 4; ++r) {
           const float p = __builtin_amdgcn_exp2f(s[qb][t][r] * scale2 - msc);
           l_run[qb] += p;                                  // the lane's own keys; the four lanes of a slot are added up at the end
-          // weights to bf16 for the second product (half a step: 2^-9 of each weight; the normaliser keeps them in fp32)
+          // weights to bf16 for the second product (half a step: 2^-8 of each weight; the normaliser keeps them in fp32)
           pf[qb][t >> 1][4 * (t & 1) + r] = (__bf16)p;
         }
     }
@@ -307,11 +399,12 @@ __global__ __launch_bounds__(128 * NQG, 2) void da_fwd_kernel(DaArgs a) {
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int h2 = 0; h2 < 2; ++h2) {
-        const bf16x8 vf = da_frag_tr<RV>(Vs, 32 * h2 + 8 * g + q4, dt, p4);
+        const bf16x8 vf = da_tr<RV>(vb, h2, dt);
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) o[qb][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qb][h2], o[qb][dt], 0, 0, 0);
       }
     vis = vis_next;
+    const unsigned sw = cur; cur = other; other = sw;
   }
   // lane holds O[slot c of block qb][16 dt + 4 g + r] of its map
 #pragma unroll
@@ -334,14 +427,16 @@ __global__ __launch_bounds__(128 * NQG, 2) void da_fwd_kernel(DaArgs a) {
   }
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    const float inv = l_run[qb] > 0.f || l_run[qb] != l_run[qb] ? 1.0f / l_run[qb] : 0.f;
+    const float l = l_run[qb];
+    const bool any = l > 0.f || l != l;
+    const float inv = any ? 1.0f / l : 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[qb][dt][r] *= inv;
     const long long rh = (bq * a.Lq + sp.q0 + row[qb]) * a.H + head[qb];       // row and head, counted through the batch
     if (ok[qb] && a.lse && g == 0)         // base 2, for the scaled scores; +inf: no visible key, every weight 2^-inf = 0
-      a.lse[2 * rh + map] = l_run[qb] > 0.f || l_run[qb] != l_run[qb] ? m_run[qb] * scale2 + __log2f(l_run[qb]) : INFINITY;
+      a.lse[2 * rh + map] = any ? m_run[qb] * scale2 + __log2f(l) : INFINITY;
     if (ok[qb] && a.maps) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *(f32x4*)(a.maps + (2 * rh + map) * E + 16 * dt + 4 * g) = o[qb][dt];
@@ -375,37 +470,68 @@ __global__ __launch_bounds__(128 * NQG, 2) void da_fwd_kernel(DaArgs a) {
   }
 }
 
-// joins the key splits of one slot: a workgroup of E threads, thread = value column
+// Joins the key splits of one slot: the splits' maxima and normalisers first (one thread a split), then 256 threads =
+// E / 4 column groups x the rest over the splits, added up in a fixed order.
 template <int D, int SLOTS>
-__global__ __launch_bounds__(2 * D) void da_join_kernel(DaArgs a) {
-  constexpr int E = 2 * D;
-  const int e = threadIdx.x;
+__global__ __launch_bounds__(256) void da_join_kernel(DaArgs a) {
+  constexpr int E = 2 * D, CG = E / 4, RG = 256 / CG;
+  __shared__ float wt[2][256], red[2][4][2];
+  __shared__ f32x4 sum[RG][CG];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int slot = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   const int blk = slot / SLOTS, in_blk = slot - blk * SLOTS;
   const int row = slot / a.share, head = hk * a.share + (slot - row * a.share);
-  float r[2];
   const long long rh = ((long long)b * a.Lq + row) * a.H + head;
+  const long long at0 = ((long long)(b * a.Hkv + hk) * a.n_blk + blk) * a.n_split * 2 * SLOTS + in_blk;
+  float l[2];
 #pragma unroll
-  for (int map = 0; map < 2; ++map) {
-    const long long at0 = (((long long)(b * a.Hkv + hk) * a.n_blk + blk) * a.n_split * 2 + map) * SLOTS + in_blk;
-    float m = -INFINITY;
-    for (int i = 0; i < a.n_split; ++i) m = fmaxf(m, a.part_ml[2 * (at0 + (long long)i * 2 * SLOTS)]);
-    float l = 0.f, o = 0.f;
-    for (int i = 0; i < a.n_split; ++i) {
-      const long long at = at0 + (long long)i * 2 * SLOTS;
-      const float li = a.part_ml[2 * at + 1];
-      if (li == 0.f) continue;                             // a split without a visible key
-      const float w = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - m);
-      l += w * li;
-      o += w * a.part[at * E + e];
-    }
-    const bool any = l > 0.f || l != l;
-    r[map] = any ? o / l : 0.f;
-    if (a.lse && e == 0) a.lse[2 * rh + map] = any ? m + __log2f(l) : INFINITY;
-    if (a.maps) a.maps[(2 * rh + map) * E + e] = r[map];
+  for (int m = 0; m < 2; ++m) {
+    f32x2 x = {-INFINITY, 0.f};
+    if (tid < a.n_split) x = *(const f32x2*)(a.part_ml + 2 * (at0 + (long long)(2 * tid + m) * SLOTS));
+    const float mx = bd_wave_max(x[0]);
+    if (lane == 0) red[m][wave][0] = mx;
+    __syncthreads();
+    const float top = fmaxf(fmaxf(red[m][0][0], red[m][1][0]), fmaxf(red[m][2][0], red[m][3][0]));
+    const float w = x[1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[0] - top);      // a split without a visible key weighs nothing
+    wt[m][tid] = w;
+    const float ls = bd_wave_sum(w * x[1]);
+    if (lane == 0) red[m][wave][1] = ls;
+    __syncthreads();
+    l[m] = (red[m][0][1] + red[m][1][1]) + (red[m][2][1] + red[m][3][1]);
+    if (a.lse && tid == 0) a.lse[2 * rh + m] = l[m] > 0.f || l[m] != l[m] ? top + __log2f(l[m]) : INFINITY;
   }
-  const float lam = da_lam(a, b * a.ls[0] + row * a.ls[1] + head * a.ls[2]);
-  a.out[b * a.os[0] + row * a.os[1] + head * a.os[2] + e] = bd_f32_to_bf16(r[0] - lam * r[1]);
+  const int cg = tid % CG, rg = tid / CG;
+  f32x4 r[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int i = rg; i < a.n_split; i += RG) {
+      const float w = wt[m][i];
+      if (w == 0.f) continue;
+      const f32x4 x = *(const f32x4*)(a.part + (at0 + (long long)(2 * i + m) * SLOTS) * E + 4 * cg);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += w * x[e];
+    }
+    sum[rg][cg] = o;
+    __syncthreads();
+    f32x4 all = sum[0][cg];
+#pragma unroll
+    for (int i = 1; i < RG; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) all[e] += sum[i][cg][e];
+    const float inv = l[m] > 0.f || l[m] != l[m] ? 1.0f / l[m] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[m][e] = all[e] * inv;
+    __syncthreads();
+    if (a.maps && rg == 0) *(f32x4*)(a.maps + (2 * rh + m) * E + 4 * cg) = r[m];
+  }
+  if (rg == 0) {
+    const float lam = da_lam(a, b * a.ls[0] + row * a.ls[1] + head * a.ls[2]);
+    u32x2 w;
+    w[0] = bd_pack_bf16x2(r[0][0] - lam * r[1][0], r[0][1] - lam * r[1][1]);
+    w[1] = bd_pack_bf16x2(r[0][2] - lam * r[1][2], r[0][3] - lam * r[1][3]);
+    *(u32x2*)(a.out + b * a.os[0] + row * a.os[1] + head * a.os[2] + 4 * cg) = w;
+  }
 }
 
 // =====================================================================================
@@ -415,22 +541,22 @@ __global__ __launch_bounds__(2 * D) void da_join_kernel(DaArgs a) {
 // From a bf16-rounded O it would miss sum_j dS_ij = 0 by 2^-9 of |dO||O| for all keys alike, as large as dS itself
 // where attention is nearly uniform.
 // =====================================================================================
-template <int D, int QB>
-__global__ __launch_bounds__(256, 1) void da_bwd_dq_kernel(DaArgs a) {
-  constexpr int E = 2 * D, KS = D / 32, ES = E / 32, DT = D / 16, NW = 4, RK = 2 * D, RV = 2 * E;
-  constexpr int TILE = KT * (2 * RK + RV), SLOTS = 64 * QB;
+template <int D, int QB, int NW, int OCC>
+__global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
+  constexpr int E = 2 * D, KS = D / 32, ES = E / 32, DT = D / 16, RK = 2 * D, RV = 2 * E;
+  constexpr int TILE = KT * (2 * RK + RV), SLOTS = 16 * QB * NW;
   extern __shared__ __attribute__((aligned(1024))) unsigned char da_smem[];
   __shared__ int red[NW];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, c = lane & 15, q4 = c >> 2, p4 = c & 3;
+  const int g = lane >> 4, c = lane & 15;
   int blk, hk, b;
-  da_block(a.n_blk, a.Hkv, blk, hk, b);
+  if (!da_block(a.n_blk, a.Hkv, a.B + (a.cu ? 1 : 0), blk, hk, b)) return;
   if (a.cu && b == a.B) {
     if (blk == 0) {
       const int first = min(max(a.cu[a.B], 0), a.total);
-      da_zero_tail(a.dq, a.dqs, first, a.total, 2 * hk * a.share, 2 * a.share, D, tid, 256);
-      for (long long i = tid; i < (long long)(a.total - first) * a.share; i += 256)
+      da_zero_tail(a.dq, a.dqs, first, a.total, 2 * hk * a.share, 2 * a.share, D, tid, 64 * NW);
+      for (long long i = tid; i < (long long)(a.total - first) * a.share; i += 64 * NW)
         a.dlam[(first + i / a.share) * a.H + hk * a.share + i % a.share] = 0.f;
     }
     return;
@@ -439,7 +565,7 @@ __global__ __launch_bounds__(256, 1) void da_bwd_dq_kernel(DaArgs a) {
   const int n_slots = sp.Lq * a.share;
   if (blk * SLOTS >= n_slots) return;
   const long long bq = a.cu ? 0 : b;
-  const int kend = da_visible_end<256>(a, b, sp.Lk, tid, red);
+  const int kend = da_visible_end<64 * NW>(a, b, sp.Lk, tid, red);
 
   const int s0 = blk * SLOTS + wave * 16 * QB;
   int row[QB], head[QB];
@@ -487,47 +613,35 @@ __global__ __launch_bounds__(256, 1) void da_bwd_dq_kernel(DaArgs a) {
       for (int i = 0; i < DT; ++i) acc[qb][m][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const float scale2 = a.scale * LOG2E;
 
-  const unsigned char* const kb0 = (const unsigned char*)(a.k + bq * a.ks[0] + sp.k0 * a.ks[1] + (long long)(2 * hk) * a.ks[2]);
-  const unsigned char* const kb1 = kb0 + 2 * a.ks[2];
-  const unsigned char* const vb = (const unsigned char*)(a.v + bq * a.vs[0] + sp.k0 * a.vs[1] + (long long)hk * a.vs[2]);
+  DaKeyStage<D, NW> keys;
+  keys.init(a, bq, sp.k0, hk, wave, lane);
   const unsigned lds0 = (unsigned)(size_t)(da_lds*)da_smem;
-  auto stage = [&](int kt0, unsigned long long vis, int buf) {
-    const unsigned base = lds0 + buf * TILE;
-    auto at = [&](const unsigned char* p, long long st) {
-      return [=](int r) { return ((vis >> r) & 1ull) ? p + 2 * st * (kt0 + r) : (const unsigned char*)nullptr; };
-    };
-    da_stage<RK, NW>(base, wave, lane, at(kb0, a.ks[1]));
-    da_stage<RK, NW>(base + KT * RK, wave, lane, at(kb1, a.ks[1]));
-    da_stage<RV, NW>(base + 2 * KT * RK, wave, lane, at(vb, a.vs[1]));
-  };
-  for (int walk = a.maps ? 1 : 0; walk < 2; ++walk) {
+  const unsigned knat = da_nat_base<RK>(g, c), ktr = da_tr_base<RK>(g, c), vnat = da_nat_base<RV>(g, c) + 2 * KT * RK;
+  auto walk_keys = [&](auto last) {                        // last: dQ is summed; else delta
+    constexpr bool LAST = decltype(last)::value;
     unsigned mb = da_mask_byte(a, b, lane, kend);
     unsigned long long vis = __ballot(mb != 0u);
     __syncthreads();                                       // (second walk: nobody reads the first one's last tile)
-    if (kend > 0) stage(0, vis, 0);
+    unsigned cur = lds0, other = lds0 + TILE;
+    if (kend > 0) keys.run(a, cur, 0, vis, wave, lane);
     mb = da_mask_byte(a, b, KT + lane, kend);
-    int buf = 0;
-    for (int kt0 = 0; kt0 < kend; kt0 += KT, buf ^= 1) {
+    for (int kt0 = 0; kt0 < kend; kt0 += KT) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
       const unsigned long long vis_next = __ballot(mb != 0u);
       mb = da_mask_byte(a, b, kt0 + 2 * KT + lane, kend);
-      if (kt0 + KT < kend) stage(kt0 + KT, vis_next, buf ^ 1);
-      const unsigned char* const K0 = da_smem + buf * TILE;
-      const unsigned char* const K1 = K0 + KT * RK;
-      const unsigned char* const Vs = K0 + 2 * KT * RK;
-#pragma unroll
+      if (kt0 + KT < kend) keys.run(a, other, kt0 + KT, vis_next, wave, lane);
+#pragma unroll 1                                           // (unrolled, the scheduler reads ahead more than the registers hold)
       for (int h2 = 0; h2 < 2; ++h2) {                     // 32 keys
+        const unsigned kn = cur + knat + 32 * RK * h2, kt = cur + ktr + 32 * RK * h2, vn = cur + vnat + 32 * RV * h2;
         bf16x8 dsf[QB][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const int krow = 32 * h2 + 8 * q4 + 4 * half + p4;
           f32x4 s[QB][2], dp[QB];
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb) s[qb][0] = s[qb][1] = dp[qb] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
-            const bf16x8 k0f = *(const bf16x8*)(K0 + da_off<RK>(krow, 4 * ks + g));
-            const bf16x8 k1f = *(const bf16x8*)(K1 + da_off<RK>(krow, 4 * ks + g));
+            const bf16x8 k0f = da_nat<RK>(kn, 0, half, ks), k1f = da_nat<RK>(kn + KT * RK, 0, half, ks);
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
               s[qb][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0f, qf[qb][0][ks], s[qb][0], 0, 0, 0);
@@ -536,27 +650,33 @@ __global__ __launch_bounds__(256, 1) void da_bwd_dq_kernel(DaArgs a) {
           }
 #pragma unroll
           for (int ks = 0; ks < ES; ++ks) {
-            const bf16x8 vf = *(const bf16x8*)(Vs + da_off<RV>(krow, 4 * ks + g));
+            const bf16x8 vf = da_nat<RV>(vn, 0, half, ks);
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) dp[qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, dof[qb][ks], dp[qb], 0, 0, 0);
           }
-          const unsigned m4 = (unsigned)(vis >> (32 * h2 + 8 * g + 4 * half)) & 0xfu;
+          if (vis != ~0ull) {
+            const unsigned m4 = (unsigned)(vis >> (32 * h2 + 8 * g + 4 * half)) & 0xfu;
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (!((m4 >> r) & 1u)) s[qb][0][r] = s[qb][1][r] = -INFINITY;        // weight 2^-inf = 0 (dP of a zero row is 0)
+          }
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const float p = ((m4 >> r) & 1u) ? __builtin_amdgcn_exp2f(s[qb][m][r] * scale2 - lse[qb][m]) : 0.f;
-                if (walk == 0) dl[qb][m] += p * dp[qb][r];
+                const float p = __builtin_amdgcn_exp2f(s[qb][m][r] * scale2 - lse[qb][m]);
+                if (!LAST) dl[qb][m] += p * dp[qb][r];
                 else dsf[qb][m][4 * half + r] = (__bf16)(p * (dp[qb][r] - dl[qb][m]));
               }
         }
-        if (walk == 1) {                                   // dQ^T += K^T dS^T
+        if (LAST) {                                        // dQ^T += K^T dS^T
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
-            const bf16x8 k0t = da_frag_tr<RK>(K0, 32 * h2 + 8 * g + q4, dt, p4);
-            const bf16x8 k1t = da_frag_tr<RK>(K1, 32 * h2 + 8 * g + q4, dt, p4);
+            const bf16x8 k0t = da_tr<RK>(kt, 0, dt), k1t = da_tr<RK>(kt + KT * RK, 0, dt);
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
               acc[qb][0][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0t, dsf[qb][0], acc[qb][0][dt], 0, 0, 0);
@@ -566,17 +686,20 @@ __global__ __launch_bounds__(256, 1) void da_bwd_dq_kernel(DaArgs a) {
         }
       }
       vis = vis_next;
+      const unsigned sw = cur; cur = other; other = sw;
     }
-    if (walk == 0) {
+  };
+  if (!a.maps) {
+    walk_keys(std::false_type());
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb)
+    for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          dl[qb][m] += __shfl_xor(dl[qb][m], 16, 64);
-          dl[qb][m] += __shfl_xor(dl[qb][m], 32, 64);
-        }
-    }
+      for (int m = 0; m < 2; ++m) {
+        dl[qb][m] += __shfl_xor(dl[qb][m], 16, 64);
+        dl[qb][m] += __shfl_xor(dl[qb][m], 32, 64);
+      }
   }
+  walk_keys(std::true_type());
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     if (!ok[qb]) continue;
@@ -604,21 +727,21 @@ __global__ __launch_bounds__(256, 1) void da_bwd_dq_kernel(DaArgs a) {
 // =====================================================================================
 // Backward, key side: a workgroup owns 64 KB keys of one key head and walks the query slots of all heads that share it.
 // =====================================================================================
-template <int D, int KB>
-__global__ __launch_bounds__(256, 1) void da_bwd_dkv_kernel(DaArgs a) {
-  constexpr int E = 2 * D, KS = D / 32, ES = E / 32, DT = D / 16, ET = E / 16, NW = 4, RK = 2 * D, RV = 2 * E;
-  constexpr int TILE = KT * (2 * RK + RV + 32), KEYS = 64 * KB;
+template <int D, int KB, int NW, int OCC>
+__global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
+  constexpr int E = 2 * D, KS = D / 32, ES = E / 32, DT = D / 16, ET = E / 16, RK = 2 * D, RV = 2 * E;
+  constexpr int TILE = KT * (2 * RK + RV + 32), KEYS = 16 * KB * NW;
   extern __shared__ __attribute__((aligned(1024))) unsigned char da_smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, c = lane & 15, q4 = c >> 2, p4 = c & 3;
+  const int g = lane >> 4, c = lane & 15;
   int blk, hk, b;
-  da_block(a.n_blk, a.Hkv, blk, hk, b);
+  if (!da_block(a.n_blk, a.Hkv, a.B + (a.cu ? 1 : 0), blk, hk, b)) return;
   if (a.cu && b == a.B) {
     if (blk == 0) {
       const int first = min(max(a.cu[a.B], 0), a.total);
-      da_zero_tail(a.dk, a.dks, first, a.total, 2 * hk, 2, D, tid, 256);
-      da_zero_tail(a.dv, a.dvs, first, a.total, hk, 1, E, tid, 256);
+      da_zero_tail(a.dk, a.dks, first, a.total, 2 * hk, 2, D, tid, 64 * NW);
+      da_zero_tail(a.dv, a.dvs, first, a.total, hk, 1, E, tid, 64 * NW);
     }
     return;
   }
@@ -657,52 +780,79 @@ __global__ __launch_bounds__(256, 1) void da_bwd_dkv_kernel(DaArgs a) {
   }
   const float scale2 = a.scale * LOG2E;
   const unsigned lds0 = (unsigned)(size_t)(da_lds*)da_smem;
-  auto stage = [&](int t0, int buf) {
-    const unsigned base = lds0 + buf * TILE;
-    auto at = [&](const unsigned short* p, const long long* st, int mul, int add) {
+  // Slot tiles: row s / share, head hk * share + s % share. Where share divides the tile a lane's offsets are the same for
+  // every whole tile and the base moves by KT / share rows.
+  typedef DaPieces<RK, NW> PQ;
+  typedef DaPieces<RV, NW> PD;
+  const unsigned char* const qb0 = (const unsigned char*)(a.q + bq * a.qs[0] + sp.q0 * a.qs[1] + (long long)(2 * hk * a.share) * a.qs[2]);
+  const unsigned char* const db0 = (const unsigned char*)(a.dout + bq * a.dos[0] + sp.q0 * a.dos[1] + (long long)(hk * a.share) * a.dos[2]);
+  const unsigned char* const sb0 = (const unsigned char*)(a.stats + 8 * ((bq * a.Lq + sp.q0) * a.H + hk * a.share));
+  const bool even = a.small_strides && KT % a.share == 0;
+  unsigned qo[PQ::N], dob[PD::N], so;
+  auto split = [&](int s, int& row, int& head) { row = s / a.share; head = s - row * a.share; };
+  {
+    int row, head;
+#pragma unroll
+    for (int j = 0; j < PQ::N; ++j) {
+      split(PQ::row(wave, lane, j), row, head);
+      qo[j] = (unsigned)(2 * a.qs[1]) * row + (unsigned)(4 * a.qs[2]) * head + 16 * PQ::chunk(wave, lane, j);
+    }
+#pragma unroll
+    for (int j = 0; j < PD::N; ++j) {
+      split(PD::row(wave, lane, j), row, head);
+      dob[j] = (unsigned)(2 * a.dos[1]) * row + (unsigned)(2 * a.dos[2]) * head + 16 * PD::chunk(wave, lane, j);
+    }
+    split(lane, row, head);
+    so = (unsigned)(row * a.H + head) * 32 + 16 * (wave & 1);
+  }
+  auto stage = [&](int t0, unsigned base) {
+    if (even && t0 + KT <= n_slots) {
+      const int row0 = t0 / a.share;
+      const unsigned char* const q0 = qb0 + 2 * a.qs[1] * row0;
+      da_stage_fast<RK, NW>(base, wave, q0, qo);
+      da_stage_fast<RK, NW>(base + KT * RK, wave, q0 + 2 * a.qs[2], qo);
+      da_stage_fast<RV, NW>(base + 2 * KT * RK, wave, db0 + 2 * a.dos[1] * row0, dob);
+      if (wave < 2) da_dma16s(da_uniform(sb0 + 32ll * row0 * a.H), so, base + KT * (2 * RK + RV) + wave * 1024);
+      return;
+    }
+    auto at = [&](const unsigned char* p, long long rs, long long hs) {
       return [=](int r) {
-        const int s = t0 + r;
-        if (s >= n_slots) return (const unsigned char*)nullptr;
-        const int row = s / a.share, head = hk * a.share + (s - row * a.share);
-        return (const unsigned char*)(p + bq * st[0] + (sp.q0 + row) * st[1] + (mul * head + add) * st[2]);
+        const int s = t0 + r, row = s / a.share;
+        return s < n_slots ? p + row * rs + (s - row * a.share) * hs : (const unsigned char*)nullptr;
       };
     };
-    da_stage<RK, NW>(base, wave, lane, at(a.q, a.qs, 2, 0));
-    da_stage<RK, NW>(base + KT * RK, wave, lane, at(a.q, a.qs, 2, 1));
-    da_stage<RV, NW>(base + 2 * KT * RK, wave, lane, at(a.dout, a.dos, 1, 0));
+    da_stage<RK, NW>(base, wave, lane, at(qb0, 2 * a.qs[1], 4 * a.qs[2]));
+    da_stage<RK, NW>(base + KT * RK, wave, lane, at(qb0 + 2 * a.qs[2], 2 * a.qs[1], 4 * a.qs[2]));
+    da_stage<RV, NW>(base + 2 * KT * RK, wave, lane, at(db0, 2 * a.dos[1], 2 * a.dos[2]));
     if (wave < 2) {                                        // the slots' statistics: lane = slot, 16 bytes a wave
-      const int s = t0 + lane;
-      const unsigned char* src = (const unsigned char*)bd_da_zero;
-      if (s < n_slots) {
-        const int row = s / a.share, head = hk * a.share + (s - row * a.share);
-        src = (const unsigned char*)(a.stats + 8 * ((bq * a.Lq + sp.q0 + row) * a.H + head) + 4 * wave);
-      }
-      da_dma16(src, base + KT * (2 * RK + RV) + wave * 1024);
+      const unsigned char* src = at(sb0, 32ll * a.H, 32)(lane);
+      da_dma16(src ? src + 16 * wave : (const unsigned char*)bd_da_zero, base + KT * (2 * RK + RV) + wave * 1024);
     }
   };
+  const unsigned qnat = da_nat_base<RK>(g, c), qtr = da_tr_base<RK>(g, c);
+  const unsigned dnat = da_nat_base<RV>(g, c) + 2 * KT * RK, dtr = da_tr_base<RV>(g, c) + 2 * KT * RK;
   if (__syncthreads_or(live)) {                            // no visible key in this workgroup: every gradient is zero
-    stage(0, 0);
-    int buf = 0;
-    for (int t0 = 0; t0 < n_slots; t0 += KT, buf ^= 1) {
+    unsigned cur = lds0, other = lds0 + TILE;
+    stage(0, cur);
+    for (int t0 = 0; t0 < n_slots; t0 += KT) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (t0 + KT < n_slots) stage(t0 + KT, buf ^ 1);
-      const unsigned char* const Q0 = da_smem + buf * TILE;
-      const unsigned char* const Q1 = Q0 + KT * RK;
-      const unsigned char* const Ds = Q0 + 2 * KT * RK;
-      const f32x4* const St = (const f32x4*)(Ds + KT * RV);        // [64] lse1, lse2, delta1, delta2; then [64] lam, ...
-#pragma unroll
+      if (t0 + KT < n_slots) stage(t0 + KT, other);
+      typedef __attribute__((address_space(3))) const f32x4 lds_f32x4;
+      typedef __attribute__((address_space(3))) const float lds_f32;
+#pragma unroll(D == 128 ? 1 : 2)                           // (head size 128: the unrolled body spills)
       for (int h2 = 0; h2 < 2; ++h2) {                     // 32 slots
+        const unsigned qn = cur + qnat + 32 * RK * h2, qt = cur + qtr + 32 * RK * h2;
+        const unsigned dn = cur + dnat + 32 * RV * h2, dt0 = cur + dtr + 32 * RV * h2;
+        const unsigned st0 = cur + KT * (2 * RK + RV) + 16 * (8 * g + 32 * h2);   // [64] lse1, lse2, delta1, delta2; then [64] lam, ...
         bf16x8 pf[KB], dsf[KB][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const int srow = 32 * h2 + 8 * q4 + 4 * half + p4;
           f32x4 s[KB][2], dp[KB];
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) s[kb][0] = s[kb][1] = dp[kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
-            const bf16x8 q0f = *(const bf16x8*)(Q0 + da_off<RK>(srow, 4 * ks + g));
-            const bf16x8 q1f = *(const bf16x8*)(Q1 + da_off<RK>(srow, 4 * ks + g));
+            const bf16x8 q0f = da_nat<RK>(qn, 0, half, ks), q1f = da_nat<RK>(qn + KT * RK, 0, half, ks);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
               s[kb][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q0f, kf[kb][0][ks], s[kb][0], 0, 0, 0);
@@ -711,15 +861,15 @@ __global__ __launch_bounds__(256, 1) void da_bwd_dkv_kernel(DaArgs a) {
           }
 #pragma unroll
           for (int ks = 0; ks < ES; ++ks) {
-            const bf16x8 df = *(const bf16x8*)(Ds + da_off<RV>(srow, 4 * ks + g));
+            const bf16x8 df = da_nat<RV>(dn, 0, half, ks);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) dp[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(df, vf[kb][ks], dp[kb], 0, 0, 0);
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int sl = 32 * h2 + 8 * g + 4 * half + r;
-            const f32x4 st = St[sl];
-            const float lam = *(const float*)(St + KT + sl);
+            const unsigned at = st0 + 16 * (4 * half + r);
+            const f32x4 st = *(lds_f32x4*)(size_t)at;
+            const float lam = *(lds_f32*)(size_t)(at + 1024);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
               const float p1 = __builtin_amdgcn_exp2f(s[kb][0][r] * scale2 - st[0]);
@@ -732,14 +882,13 @@ __global__ __launch_bounds__(256, 1) void da_bwd_dkv_kernel(DaArgs a) {
         }
 #pragma unroll
         for (int dt = 0; dt < ET; ++dt) {
-          const bf16x8 dt_ = da_frag_tr<RV>(Ds, 32 * h2 + 8 * g + q4, dt, p4);
+          const bf16x8 dt_ = da_tr<RV>(dt0, 0, dt);
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) av[kb][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(dt_, pf[kb], av[kb][dt], 0, 0, 0);
         }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const bf16x8 q0t = da_frag_tr<RK>(Q0, 32 * h2 + 8 * g + q4, dt, p4);
-          const bf16x8 q1t = da_frag_tr<RK>(Q1, 32 * h2 + 8 * g + q4, dt, p4);
+          const bf16x8 q0t = da_tr<RK>(qt, 0, dt), q1t = da_tr<RK>(qt + KT * RK, 0, dt);
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) {
             ak[kb][0][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q0t, dsf[kb][0], ak[kb][0][dt], 0, 0, 0);
@@ -747,6 +896,7 @@ __global__ __launch_bounds__(256, 1) void da_bwd_dkv_kernel(DaArgs a) {
           }
         }
       }
+      const unsigned sw = cur; cur = other; other = sw;
     }
   }
 #pragma unroll
@@ -814,14 +964,22 @@ __global__ __launch_bounds__(256) void da_dlam_cast_kernel(const float* __restri
 }
 
 // ---------------------------------------------------------------------------------------------- host side
-constexpr int FWD_QB = 2, FWD_NQG = 4, FWD_SLOTS = 16 * FWD_QB * FWD_NQG;      // 128 slots, 8 waves
+// Forward: blocks of 16 slots a wave holds, query groups of a workgroup (two waves each), waves of a SIMD. Measured, forward
+// alone: head size 64, 16 x 1024 tokens x 3 heads: (1, 4, 4) 64 us, (2, 2, 2) 72, (2, 4, 2) 84, (1, 2, 4) 91: with twice
+// the waves the exponentials of one hide behind the products of the others, though every operand read feeds one product
+// instead of two. Head size 128, 2 x 4096 x 8: (2, 4, 2) 470 us, (1, 4, 2) 584, (1, 2, 2) 999 (few slots a workgroup: the
+// tiles' way into LDS paces it). Head size 32, 96 ragged x 8: (2, 2, 4) 97 us, (1, 2, 4) 104, (4, 2, 2) 124, (2, 4, 2) 160.
+template <int B_, int NQG_, int OCC_> struct DaFCfg { static constexpr int B = B_, NQG = NQG_, OCC = OCC_, SLOTS = 16 * B_ * NQG_; };
+template <int D> struct DaFwd : DaFCfg<1, 4, 4> {};
+template <> struct DaFwd<32> : DaFCfg<2, 2, 4> {};
+template <> struct DaFwd<128> : DaFCfg<2, 4, 2> {};
 constexpr int ROWS_NQG = 2, ROWS_SLOTS = 16 * ROWS_NQG;                         // few slots: 32, 4 waves of 16
 
 int da_splits(const bd_diff_attn_args& p) {
   // few slots against many keys: enough splits of whole key tiles for two workgroups per CU, four tiles each at least
   if (p.cu_seqlens) return 1;
   const long long slots = (long long)p.Lq * (p.H / p.Hkv);
-  if (slots > FWD_SLOTS) return 1;
+  if (slots > 128) return 1;
   const long long blocks = (long long)p.B * p.Hkv * ((slots + ROWS_SLOTS - 1) / ROWS_SLOTS);
   const int tiles = (p.Lk + KT - 1) / KT;
   long long n = 512 / (blocks > 0 ? blocks : 1);
@@ -856,6 +1014,9 @@ int da_check(const bd_diff_attn_args& p, const char* what, DaArgs& a) {
   }
   a.B = p.B; a.Lq = p.Lq; a.Lk = p.Lk; a.H = p.H; a.Hkv = p.Hkv; a.share = p.H / p.Hkv; a.total = p.total_rows;
   a.lam_f32 = p.lam_dtype == BD_DTYPE_F32; a.scale = p.scale; a.n_split = 1;
+  a.small_strides = (long long)p.H * 32 * KT < (1ll << 31);
+  for (int i = 1; i < 3; ++i)
+    a.small_strides = a.small_strides && (p.q_stride[i] | p.k_stride[i] | p.v_stride[i] | p.dout_stride[i]) < (1ll << 24);
   a.lse = p.lse; a.maps = p.maps;
   return BD_OK;
 }
@@ -867,9 +1028,10 @@ int da_forward(const bd_diff_attn_args& p, DaArgs& a, hipStream_t s) {
   const int seqs = a.B + (a.cu ? 1 : 0);
   a.n_split = da_splits(p);
   const bool few = da_few(p);
-  const int per = few ? ROWS_SLOTS : FWD_SLOTS;
+  typedef DaFwd<D> F;
+  const int per = few ? ROWS_SLOTS : F::SLOTS;
   a.n_blk = (int)((slots + per - 1) / per);
-  const long long grid = (long long)a.n_blk * a.n_split * a.Hkv * seqs;
+  const long long grid = da_grid((long long)a.n_blk * a.n_split, (long long)a.Hkv * seqs);
   BD_REQUIRE(grid < (1ll << 31), "bd_diff_attention_fwd: too many workgroups");
   if (a.n_split > 1) {
     const long long ml = (long long)a.n_blk * a.n_split * a.Hkv * a.B * 2 * ROWS_SLOTS;
@@ -877,32 +1039,43 @@ int da_forward(const bd_diff_attn_args& p, DaArgs& a, hipStream_t s) {
     a.part = a.part_ml + ml * 2;
   }
   if (few) {
-    BD_SET_MAX_LDS((da_fwd_kernel<D, 1, ROWS_NQG>), LDS);
-    hipLaunchKernelGGL((da_fwd_kernel<D, 1, ROWS_NQG>), dim3((unsigned)grid), dim3(128 * ROWS_NQG), LDS, s, a);
+    BD_SET_MAX_LDS((da_fwd_kernel<D, 1, ROWS_NQG, 2>), LDS);
+    hipLaunchKernelGGL((da_fwd_kernel<D, 1, ROWS_NQG, 2>), dim3((unsigned)grid), dim3(128 * ROWS_NQG), LDS, s, a);
     if (a.n_split > 1)
-      hipLaunchKernelGGL((da_join_kernel<D, ROWS_SLOTS>), dim3((unsigned)slots, a.Hkv, a.B), dim3(2 * D), 0, s, a);
+      hipLaunchKernelGGL((da_join_kernel<D, ROWS_SLOTS>), dim3((unsigned)slots, a.Hkv, a.B), dim3(256), 0, s, a);
   } else {
-    BD_SET_MAX_LDS((da_fwd_kernel<D, FWD_QB, FWD_NQG>), LDS);
-    hipLaunchKernelGGL((da_fwd_kernel<D, FWD_QB, FWD_NQG>), dim3((unsigned)grid), dim3(128 * FWD_NQG), LDS, s, a);
+    BD_SET_MAX_LDS((da_fwd_kernel<D, F::B, F::NQG, F::OCC>), LDS);
+    hipLaunchKernelGGL((da_fwd_kernel<D, F::B, F::NQG, F::OCC>), dim3((unsigned)grid), dim3(128 * F::NQG), LDS, s, a);
   }
   return bd_check_launch("bd_diff_attention_fwd");
 }
 
+// Backward: blocks of 16 slots (dq) or keys (dkv) a wave holds, waves of a workgroup, waves of a SIMD. Measured, dq / dkv:
+// head size 64, 16 x 1024 x 3 heads: dq (1, 8, 4) 73 us, (1, 4, 3) 79; dkv (1, 4, 2) 86, (1, 4, 3) 108, (1, 8, 2) 113.
+// Head size 128, 2 x 4096 x 8: (1, 8, 2) 478 / 800 us, (2, 4, 1) 834 / 844, (1, 4, 1) 1058 / 1234. Head size 32, 96 ragged
+// x 8: (1, 4, 4) 90 / 96 us, (1, 8, 4) 110 / 121, dq (2, 4, 3) 99.
+template <int B_, int NW_, int OCC_> struct DaCfg { static constexpr int B = B_, NW = NW_, OCC = OCC_; };
+template <int D> struct DaBwd { typedef DaCfg<1, 8, 4> Q; typedef DaCfg<1, 4, 2> K; };
+template <> struct DaBwd<32> { typedef DaCfg<1, 4, 4> Q; typedef DaCfg<1, 4, 4> K; };
+template <> struct DaBwd<128> { typedef DaCfg<1, 8, 2> Q; typedef DaCfg<1, 8, 2> K; };
+
 template <int D>
 int da_backward(DaArgs& a, hipStream_t s) {
   constexpr int LDS = 2 * KT * 8 * D, LDS_KV = 2 * KT * (8 * D + 32);
+  typedef typename DaBwd<D>::Q Q;
+  typedef typename DaBwd<D>::K K;
   const long long slots = (long long)a.Lq * a.share;
   const int seqs = a.B + (a.cu ? 1 : 0);
-  a.n_blk = (int)((slots + 63) / 64);
-  long long grid = (long long)a.n_blk * a.Hkv * seqs;
+  a.n_blk = (int)((slots + 16 * Q::B * Q::NW - 1) / (16 * Q::B * Q::NW));
+  long long grid = da_grid(a.n_blk, (long long)a.Hkv * seqs);
   BD_REQUIRE(grid < (1ll << 31), "bd_diff_attention_bwd: too many workgroups");
-  BD_SET_MAX_LDS((da_bwd_dq_kernel<D, 1>), LDS);
-  hipLaunchKernelGGL((da_bwd_dq_kernel<D, 1>), dim3((unsigned)grid), dim3(256), LDS, s, a);
-  a.n_blk = (a.Lk + 63) / 64;
-  grid = (long long)a.n_blk * a.Hkv * seqs;
+  BD_SET_MAX_LDS((da_bwd_dq_kernel<D, Q::B, Q::NW, Q::OCC>), LDS);
+  hipLaunchKernelGGL((da_bwd_dq_kernel<D, Q::B, Q::NW, Q::OCC>), dim3((unsigned)grid), dim3(64 * Q::NW), LDS, s, a);
+  a.n_blk = (a.Lk + 16 * K::B * K::NW - 1) / (16 * K::B * K::NW);
+  grid = da_grid(a.n_blk, (long long)a.Hkv * seqs);
   BD_REQUIRE(grid < (1ll << 31), "bd_diff_attention_bwd: too many workgroups");
-  BD_SET_MAX_LDS((da_bwd_dkv_kernel<D, 1>), LDS_KV);
-  hipLaunchKernelGGL((da_bwd_dkv_kernel<D, 1>), dim3((unsigned)grid), dim3(256), LDS_KV, s, a);
+  BD_SET_MAX_LDS((da_bwd_dkv_kernel<D, K::B, K::NW, K::OCC>), LDS_KV);
+  hipLaunchKernelGGL((da_bwd_dkv_kernel<D, K::B, K::NW, K::OCC>), dim3((unsigned)grid), dim3(64 * K::NW), LDS_KV, s, a);
   return bd_check_launch("bd_diff_attention_bwd");
 }
 
