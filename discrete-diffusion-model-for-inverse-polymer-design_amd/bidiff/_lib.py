@@ -122,7 +122,7 @@ class DiffAttnArgs(C.Structure):
         ("lam_dtype", C.c_int), ("key_mask", VP), ("key_mask_stride", C.c_longlong), ("cu_seqlens", VP), ("total_rows", C.c_int),
         ("B", C.c_int), ("Lq", C.c_int), ("Lk", C.c_int), ("H", C.c_int), ("Hkv", C.c_int), ("head_dim", C.c_int),
         ("scale", C.c_float), ("out", VP), ("lse", VP), ("maps", VP), ("workspace", VP), ("workspace_bytes", C.c_longlong),
-        ("dout", VP), ("dq", VP), ("dk", VP), ("dv", VP), ("dlam", VP),
+        ("dout", VP), ("dq", VP), ("dk", VP), ("dv", VP), ("dlam", VP), ("dlam_dtype", C.c_int),
         ("dout_stride", _S3), ("dq_stride", _S3), ("dk_stride", _S3), ("dv_stride", _S3),
     ]
 
@@ -235,10 +235,10 @@ SIGNATURES = {
     "bd_host_dropout_factors": (C.c_int, [VP, C.c_uint, C.c_longlong, C.c_longlong, VP]),
     "bd_host_uniform_select": (C.c_float, [C.c_ulonglong, C.c_uint32, C.c_uint32, C.c_uint32]),
     "bd_host_uniform_token": (C.c_float, [C.c_ulonglong, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32]),
-    "bd_rotary": (C.c_int, [C.POINTER(RotaryTensor), C.c_int, VP, C.c_int, VP, C.c_longlong] + [C.c_int] * 7 + [VP]),
-    "bd_diff_attention_workspace_bytes": (C.c_longlong, [C.POINTER(DiffAttnArgs), C.c_int]),
-    "bd_diff_attention_fwd": (C.c_int, [C.POINTER(DiffAttnArgs), VP]),
-    "bd_diff_attention_bwd": (C.c_int, [C.POINTER(DiffAttnArgs), VP]),
+    "bd_rotary": (C.c_int, [VP, C.c_int, VP, C.c_int, VP, C.c_longlong] + [C.c_int] * 7 + [VP]),
+    "bd_diff_attention_workspace_bytes": (C.c_longlong, [VP, C.c_int]),
+    "bd_diff_attention_fwd": (C.c_int, [VP, VP]),
+    "bd_diff_attention_bwd": (C.c_int, [VP, VP]),
     "bd_diff_attention_dlam": (C.c_int, [VP, VP] + [C.c_int] * 7 + [VP]),
     "bd_linear_ce_state_bytes": (C.c_longlong, [C.c_longlong, C.c_int]),
     "bd_linear_ce_workspace_bytes": (C.c_longlong, [C.c_longlong, C.c_int, C.c_int, C.c_int]),

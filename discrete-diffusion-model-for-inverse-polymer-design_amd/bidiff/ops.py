@@ -8,7 +8,9 @@ their scratch memory from torch's allocator, repeat bit for bit, and may be capt
 with ``max_seqlen`` given). Operands on a CPU raise ``RuntimeError``: there is no other execution path.
 """
 import ctypes as C
+import functools
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -17,46 +19,57 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
-_S3 = C.c_longlong * 3
 # beyond this many keys the forward of a training step leaves each map's output in fp32 for the backward (16 * head_dim
 # bytes a row and head); up to here the backward walks the keys once more instead
 _MAPS_KEYS = 128
 
+# The argument blocks are packed by ``struct`` (a ctypes structure costs a call per field; a small call is host-bound)
+_ROTARY_TENSOR = struct.Struct("PP6qi4x")
+_ATTENTION = struct.Struct("4P15qi4xPqP7if4Pq5Pi4x12q")
+assert _ROTARY_TENSOR.size == C.sizeof(_lib.RotaryTensor) and _ATTENTION.size == C.sizeof(_lib.DiffAttnArgs)
 
-class _On:
-    """The operands' device made current for the launches inside (nothing to do in the usual case)."""
+
+class _Elsewhere:
+    """Makes the operands' device current for the launches inside."""
 
     def __init__(self, device):
-        self.ctx = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+        self.ctx = torch.cuda.device(device)
 
     def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
+        self.ctx.__enter__()
         return _lib.stream_handle()
 
     def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+        return self.ctx.__exit__(*exc)
+
+
+class _Here:
+    def __enter__(self):
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+    def __exit__(self, *exc):
         return False
 
 
+_HERE = _Here()
+
+
+def _on(device):
+    """Context for launches on ``device``: its current stream's handle, the device made current if it is not."""
+    return _HERE if torch.cuda.current_device() == device.index else _Elsewhere(device)
+
+
 def _same_device(what, first, *others):
+    dev = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"bidiff {what}: operands on {first.device} and {t.device}; all must be on one device")
+        if t is not None and t.device != dev:
+            raise ValueError(f"bidiff {what}: operands on {dev} and {t.device}; all must be on one device")
 
 
-def _strides(t, n):
-    """The leading strides of ``t`` as three values (batch, row, head), 0 where the axis has one entry; a tensor
-    without a batch axis gets batch stride 0."""
-    st = [0 if size == 1 else stride for size, stride in zip(t.shape, t.stride())][:n]
-    return [0] * (3 - len(st)) + st
-
-
-def _rows_of_16_bytes(t, n):
+def _rows_of_16_bytes(t):
     """``t`` or a copy of it whose rows the kernels can read in 16-byte pieces."""
-    per = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % per == 0 for s in _strides(t, n)):
+    *st, last = t.stride()
+    if last == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in st):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -105,23 +118,26 @@ def rotary_table(dim: int, max_positions: int, base: float = 10000.0, scaling: O
 def _rotary_launch(pairs, table, positions, interleaved, inverse):
     """pairs: one or two (source, destination) of [B, L, heads, D] (or [rows, heads, D])."""
     src = pairs[0][0]
-    B, L = (1, src.shape[0]) if src.dim() == 3 else src.shape[:2]
-    arr = (_lib.RotaryTensor * len(pairs))()
-    for a, (s, d) in zip(arr, pairs):
-        a.src, a.dst, a.n_heads = s.data_ptr(), d.data_ptr(), s.shape[-2]
-        a.src_stride, a.dst_stride = _S3(*_strides(s, s.dim() - 1)), _S3(*_strides(d, d.dim() - 1))
-    pos_stride = 0 if positions is None or positions.dim() == 1 else positions.stride(0)
-    with _On(src.device) as stream:
-        _lib.check(_lib.lib().bd_rotary(arr, len(pairs), _lib.ptr(table), table.shape[0], _lib.ptr(positions), pos_stride, B, L,
-                                        src.shape[-1], 2 * table.shape[1], int(interleaved), int(inverse), _DTYPES[src.dtype],
-                                        stream), "bd_rotary")
+    shape = src.shape
+    packed = len(shape) == 3
+    B, L = (1, shape[0]) if packed else shape[:2]
+    args = b""
+    for s, d in pairs:
+        st, dt = s.stride()[:-1], d.stride()[:-1]
+        if packed:
+            st, dt = (0,) + st, (0,) + dt
+        args += _ROTARY_TENSOR.pack(s.data_ptr(), d.data_ptr(), *st, *dt, s.shape[-2])
+    pos, pos_stride = (None, 0) if positions is None else (positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0)
+    with _on(src.device) as stream:
+        _lib.check(_lib.lib().bd_rotary(args, len(pairs), table.data_ptr(), table.shape[0], pos, pos_stride, B, L, shape[-1],
+                                        2 * table.shape[1], interleaved, inverse, _DTYPES[src.dtype], stream), "bd_rotary")
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, positions, interleaved, *xs):
         ctx.save_for_backward(table, positions)
-        ctx.interleaved, ctx.n = interleaved, len(xs)
+        ctx.interleaved = interleaved
         out = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
         _rotary_launch(list(zip(xs, out)), table, positions, interleaved, False)
         return out
@@ -130,13 +146,13 @@ class _Rotary(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, *grads):
         table, positions = ctx.saved_tensors
-        wanted = [i for i in range(ctx.n) if ctx.needs_input_grad[3 + i]]
-        dx = [None] * ctx.n
-        pairs = []
-        for i in wanted:
-            g = grads[i] if grads[i].stride(-1) == 1 else grads[i].contiguous()
-            dx[i] = torch.empty(g.shape, dtype=g.dtype, device=g.device)
-            pairs.append((g, dx[i]))
+        dx, pairs = [None] * len(grads), []
+        for i, g in enumerate(grads):
+            if ctx.needs_input_grad[3 + i]:
+                if g.stride(-1) != 1:
+                    g = g.contiguous()
+                dx[i] = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+                pairs.append((g, dx[i]))
         if pairs:
             _rotary_launch(pairs, table, positions, ctx.interleaved, True)
         return (None, None, None, *dx)
@@ -145,24 +161,24 @@ class _Rotary(torch.autograd.Function):
 def _rotary_check(xs, table, positions):
     q = xs[0]
     _same_device("rotary", q, *xs[1:], table, positions)
-    if q.dim() not in (3, 4):
-        raise ValueError(f"rotary: expected [batch, tokens, heads, head_dim] or [rows, heads, head_dim], got {tuple(q.shape)}")
-    for x in xs:
-        if x.dtype not in _DTYPES:
-            raise TypeError(f"rotary: bf16 or fp32 heads expected, got {x.dtype}")
-        if x.dtype != q.dtype or x.shape[:-2] != q.shape[:-2] or x.shape[-1] != q.shape[-1]:
-            raise ValueError("rotary: q and k must agree in dtype, tokens and head size")
+    shape = q.shape
+    if len(shape) not in (3, 4):
+        raise ValueError(f"rotary: expected [batch, tokens, heads, head_dim] or [rows, heads, head_dim], got {tuple(shape)}")
+    if q.dtype not in _DTYPES:
+        raise TypeError(f"rotary: bf16 or fp32 heads expected, got {q.dtype}")
+    lead = shape[:-2]
+    if len(xs) == 2 and (xs[1].dtype != q.dtype or xs[1].shape[:-2] != lead or xs[1].shape[-1] != shape[-1]):
+        raise ValueError("rotary: q and k must agree in dtype, tokens and head size")
     if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2 or not table.is_contiguous() or not table.numel():
         raise ValueError("rotary: table must be a contiguous fp32 [positions, rotary_dim / 2, 2] tensor (rotary_table makes one)")
-    if 2 * table.shape[1] > q.shape[-1]:
-        raise ValueError(f"rotary: the table turns {2 * table.shape[1]} values, a head has {q.shape[-1]}")
+    if 2 * table.shape[1] > shape[-1]:
+        raise ValueError(f"rotary: the table turns {2 * table.shape[1]} values, a head has {shape[-1]}")
     if table.requires_grad:
         raise NotImplementedError("rotary: the table has no gradient")
-    lead = tuple(q.shape[:-2])
     if positions is not None:
         if positions.dtype != torch.long:
             raise TypeError(f"rotary: positions must be int64, got {positions.dtype}")
-        if tuple(positions.shape) != lead and tuple(positions.shape) != lead[-1:]:
+        if positions.shape != lead and positions.shape != lead[-1:]:
             raise ValueError(f"rotary: positions must be {list(lead)} or {list(lead[-1:])}, got {tuple(positions.shape)}")
         if positions.stride(-1) != 1 and positions.shape[-1] > 1:
             positions = positions.contiguous()
@@ -213,90 +229,121 @@ def rotary_(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, pos
 
 
 # ------------------------------------------------------------------------------------------------ differential attention
-def _attention_args(q, k, v, lam, key_mask, cu, longest, scale):
+def _three(t):
+    """The strides of the leading axes as (batch, row, head); packed rows have no batch axis."""
+    st = t.stride()[:-1]
+    return st if len(st) == 3 else (0,) + st
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace(B, Lq, Lk, H, Hkv, D, packed, rows, backward):
     a = _lib.DiffAttnArgs()
-    a.q, a.k, a.v, a.lam = q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr()
-    n = q.dim() - 1
-    a.q_stride, a.k_stride, a.v_stride = _S3(*_strides(q, n)), _S3(*_strides(k, n)), _S3(*_strides(v, n))
-    a.lam_stride = _S3(*_strides(lam, n))
-    a.lam_dtype = _DTYPES[lam.dtype]
-    if key_mask is not None:
-        a.key_mask, a.key_mask_stride = key_mask.data_ptr(), key_mask.stride(0)
-    if cu is not None:
-        a.cu_seqlens, a.total_rows, a.B, a.Lq, a.Lk = cu.data_ptr(), q.shape[0], cu.numel() - 1, longest, longest
-    else:
-        a.B, a.Lq, a.Lk = q.shape[0], q.shape[1], k.shape[1]
-    a.H, a.Hkv, a.head_dim = v.shape[-2] * (q.shape[-2] // k.shape[-2]), v.shape[-2], q.shape[-1]
-    a.scale = scale
-    return a
-
-
-def _workspace(a, backward, device):
+    a.B, a.Lq, a.Lk, a.H, a.Hkv, a.head_dim, a.total_rows, a.cu_seqlens = B, Lq, Lk, H, Hkv, D, rows, 16 if packed else None
     need = _lib.lib().bd_diff_attention_workspace_bytes(C.byref(a), int(backward))
     if need < 0:
         _lib.check(-1, "bd_diff_attention_workspace_bytes")
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    a.workspace, a.workspace_bytes = (ws.data_ptr() if need else None), need
-    return ws
+    return need
 
 
-def _attention_forward(q, k, v, lam, key_mask, cu, longest, scale, training):
-    H, E = q.shape[-2] // 2, v.shape[-1]
-    a = _attention_args(q, k, v, lam, key_mask, cu, longest, scale)
-    out = torch.empty(*q.shape[:-2], H, E, dtype=q.dtype, device=q.device)
-    a.out, a.out_stride = out.data_ptr(), _S3(*_strides(out, out.dim() - 1))
-    lse = maps = None
+def _attention_sizes(q, k, v, cu, longest):
+    """(B, Lq, Lk, H, Hkv, D, packed, rows)"""
+    qs = q.shape
+    if cu is not None:
+        return cu.shape[0] - 1, longest, longest, qs[-2] // 2, v.shape[-2], qs[-1], True, qs[0]
+    return qs[0], qs[1], k.shape[1], qs[-2] // 2, v.shape[-2], qs[-1], False, qs[0] * qs[1]
+
+
+def _attention_call(entry, sizes, q, k, v, lam, lam_strides, key_mask, cu, scale, out=None, lse=0, maps=0, ws=0, ws_bytes=0, grads=None,
+                    stream=None):
+    B, Lq, Lk, H, Hkv, D, packed, rows = sizes
+    none3 = (0, 0, 0)
+    ptr = [0] * 5
+    gst = none3 * 4
+    dlam_dtype = 0
+    if grads is not None:
+        dout, dq, dk, dv, dlam, dlam_dtype = grads
+        ptr = [dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam]
+        gst = (*_three(dout), *_three(dq), *_three(dk), *_three(dv))
+    args = _ATTENTION.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), *_three(q), *_three(k), *_three(v), *lam_strides,
+        *(none3 if out is None else _three(out)), _DTYPES[lam.dtype],
+        0 if key_mask is None else key_mask.data_ptr(), 0 if key_mask is None else key_mask.stride(0),
+        cu.data_ptr() if packed else 0, rows if packed else 0, B, Lq, Lk, H, Hkv, D, scale,
+        0 if out is None else out.data_ptr(), lse, maps, ws, ws_bytes, *ptr, dlam_dtype, *gst)
+    _lib.check(getattr(_lib.lib(), entry)(args, stream), entry)
+
+
+def _lam_strides(lam, lead, H):
+    """(batch, row, head) strides of lam broadcast to lead + (H,) (0 along a broadcast axis), or None if it does not fit."""
+    want = (*lead, H) if len(lead) == 2 else (1, *lead, H)
+    off = 3 - lam.dim()
+    if off < 0 or (off == 0 and len(lead) == 1):
+        return None
+    st = [0, 0, 0]
+    for i, (n, s) in enumerate(zip(lam.shape, lam.stride())):
+        if n != want[off + i] and n != 1:
+            return None
+        st[off + i] = s if n != 1 else 0
+    return st
+
+
+def _attention_forward(q, k, v, lam, lam_strides, key_mask, cu, longest, scale, training):
+    sizes = _attention_sizes(q, k, v, cu, longest)
+    _, _, Lk, H, _, D, _, rows = sizes
+    dev = q.device
+    out = torch.empty(*q.shape[:-2], H, 2 * D, dtype=torch.bfloat16, device=dev)
+    ws_bytes = _attention_workspace(*sizes, False)
+    # one allocation for what the backward reads (log-sum-exps, then the maps), one for scratch
+    saved = ws = None
+    lse = maps = 0
     if training:
-        rows = q.shape[:-2].numel()
-        lse = torch.empty(rows, H, 2, dtype=torch.float32, device=q.device)
-        a.lse = lse.data_ptr()
-        if a.Lk > _MAPS_KEYS:
-            maps = torch.empty(rows, H, 2, E, dtype=torch.float32, device=q.device)
-            a.maps = maps.data_ptr()
-    with _On(q.device) as stream:
-        ws = _workspace(a, False, q.device)
-        _lib.check(_lib.lib().bd_diff_attention_fwd(C.byref(a), stream), "bd_diff_attention_fwd")
-        del ws
-    return out, lse, maps
+        n_lse = (rows * H * 2 + 3) // 4 * 4
+        saved = torch.empty(n_lse + (rows * H * 4 * D if Lk > _MAPS_KEYS else 0), dtype=torch.float32, device=dev)
+        lse = saved.data_ptr()
+        maps = lse + 4 * n_lse if Lk > _MAPS_KEYS else 0
+    if ws_bytes:
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _on(dev) as stream:
+        _attention_call("bd_diff_attention_fwd", sizes, q, k, v, lam, lam_strides, key_mask, cu, scale, out, lse, maps,
+                        ws.data_ptr() if ws_bytes else 0, ws_bytes, stream=stream)
+    return out, saved
 
 
 class _DiffAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, lam, key_mask, cu, longest, scale):
-        full = lam.expand(*q.shape[:-2], q.shape[-2] // 2)
-        out, lse, maps = _attention_forward(q, k, v, full, key_mask, cu, longest, scale, True)
-        ctx.save_for_backward(q, k, v, lam, key_mask, cu, lse, maps)
-        ctx.longest, ctx.scale = longest, scale
+    def forward(ctx, q, k, v, lam, lam_strides, key_mask, cu, longest, scale):
+        out, saved = _attention_forward(q, k, v, lam, lam_strides, key_mask, cu, longest, scale, True)
+        ctx.save_for_backward(q, k, v, lam, key_mask, cu, saved)
+        ctx.longest, ctx.scale, ctx.lam_strides = longest, scale, lam_strides
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, lam, key_mask, cu, lse, maps = ctx.saved_tensors
-        H = q.shape[-2] // 2
-        dout = _rows_of_16_bytes(dout, dout.dim() - 1)
-        a = _attention_args(q, k, v, lam.expand(*q.shape[:-2], H), key_mask, cu, ctx.longest, ctx.scale)
-        n = q.dim() - 1
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        rows = q.shape[:-2].numel()
-        dlam = torch.empty(rows, H, dtype=torch.float32, device=q.device)
-        a.dout, a.dout_stride = dout.data_ptr(), _S3(*_strides(dout, n))
-        a.lse, a.maps = lse.data_ptr(), (None if maps is None else maps.data_ptr())
-        a.dq, a.dk, a.dv, a.dlam = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam.data_ptr()
-        a.dq_stride, a.dk_stride, a.dv_stride = _S3(*_strides(dq, n)), _S3(*_strides(dk, n)), _S3(*_strides(dv, n))
-        with _On(q.device) as stream:
-            ws = _workspace(a, True, q.device)
-            _lib.check(_lib.lib().bd_diff_attention_bwd(C.byref(a), stream), "bd_diff_attention_bwd")
-            del ws
-            dl = None
-            if ctx.needs_input_grad[3]:
-                lead = (1,) * (3 - q.dim() + 1) + tuple(q.shape[:-2])                  # (batch, rows)
+        q, k, v, lam, key_mask, cu, saved = ctx.saved_tensors
+        sizes = _attention_sizes(q, k, v, cu, ctx.longest)
+        _, _, Lk, H, _, _, packed, rows = sizes
+        dev = q.device
+        dout = _rows_of_16_bytes(dout)
+        dq, dk, dv = (torch.empty(t.shape, dtype=torch.bfloat16, device=dev) for t in (q, k, v))
+        dl = torch.empty(lam.shape, dtype=lam.dtype, device=dev)
+        # a weight for every (row, head): its gradient is written as it comes; one that was broadcast: summed from fp32
+        whole = lam.numel() == rows * H
+        need = (_attention_workspace(*sizes, True) + 15) // 16 * 16
+        ws = torch.empty(need + (0 if whole else 4 * rows * H), dtype=torch.uint8, device=dev)
+        wp = ws.data_ptr()
+        lse = saved.data_ptr()
+        maps = lse + 4 * ((rows * H * 2 + 3) // 4 * 4) if Lk > _MAPS_KEYS else 0
+        with _on(dev) as stream:
+            _attention_call("bd_diff_attention_bwd", sizes, q, k, v, lam, ctx.lam_strides, key_mask, cu, ctx.scale, None, lse, maps,
+                            wp, need, (dout, dq, dk, dv, dl.data_ptr() if whole else wp + need, _DTYPES[lam.dtype] if whole else 1), stream)
+            if not whole and ctx.needs_input_grad[3]:
+                lead = (1, rows) if packed else q.shape[:2]
                 shape = (1,) * (3 - lam.dim()) + tuple(lam.shape)
-                dl = torch.empty(lam.shape, dtype=lam.dtype, device=lam.device)
-                _lib.check(_lib.lib().bd_diff_attention_dlam(
-                    _lib.ptr(dlam), _lib.ptr(dl), _DTYPES[lam.dtype], lead[0], lead[1], H, int(shape[0] == lead[0]),
-                    int(shape[1] == lead[1]), int(shape[2] == H), stream), "bd_diff_attention_dlam")
-        return dq, dk, dv, dl, None, None, None, None
+                _lib.check(_lib.lib().bd_diff_attention_dlam(wp + need, dl.data_ptr(), _DTYPES[lam.dtype], lead[0], lead[1], H,
+                                                             shape[0] == lead[0], shape[1] == lead[1], shape[2] == H, stream),
+                           "bd_diff_attention_dlam")
+        return dq, dk, dv, dl, None, None, None, None, None
 
 
 def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,
@@ -314,34 +361,31 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     _same_device("differential_attention", q, k, v, lam, key_mask, cu_seqlens)
     packed = cu_seqlens is not None
     dims = 3 if packed else 4
-    if q.dim() != dims or k.dim() != dims or v.dim() != dims:
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != dims or len(ks) != dims or len(vs) != dims:
         raise ValueError(f"differential_attention: q, k and v need {dims} axes"
-                         f"{' (packed rows have no batch axis)' if packed else ''}, got {q.dim()}, {k.dim()} and {v.dim()}")
-    for t in (q, k, v):
-        if t.dtype != torch.bfloat16:
-            raise TypeError(f"differential_attention: q, k and v must be bf16, got {t.dtype}")
+                         f"{' (packed rows have no batch axis)' if packed else ''}, got {len(qs)}, {len(ks)} and {len(vs)}")
+    if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise TypeError(f"differential_attention: q, k and v must be bf16, got {q.dtype}, {k.dtype} and {v.dtype}")
     if lam.dtype not in _DTYPES:
         raise TypeError(f"differential_attention: lam must be bf16 or fp32, got {lam.dtype}")
-    D, Hkv = q.shape[-1], v.shape[-2]
+    D, Hkv = qs[-1], vs[-2]
     if D not in (32, 64, 128):
         raise NotImplementedError(f"differential_attention: head sizes 32, 64 and 128 are supported, got {D}")
-    if k.shape[-1] != D or v.shape[-1] != 2 * D or k.shape[-2] != 2 * Hkv or q.shape[-2] % 2 or Hkv == 0 or q.shape[-2] == 0:
-        raise ValueError(f"differential_attention: heads do not fit: q {tuple(q.shape[-2:])}, k {tuple(k.shape[-2:])}, "
-                         f"v {tuple(v.shape[-2:])} (two maps a head, values twice as wide)")
-    H = q.shape[-2] // 2
+    if ks[-1] != D or vs[-1] != 2 * D or ks[-2] != 2 * Hkv or qs[-2] % 2 or Hkv == 0 or qs[-2] == 0:
+        raise ValueError(f"differential_attention: heads do not fit: q {tuple(qs[-2:])}, k {tuple(ks[-2:])}, "
+                         f"v {tuple(vs[-2:])} (two maps a head, values twice as wide)")
+    H = qs[-2] // 2
     if H % Hkv:
         raise ValueError(f"differential_attention: {H} heads cannot share {Hkv} key heads evenly")
-    if k.shape[:-2] != v.shape[:-2] or (packed and q.shape[0] != k.shape[0]) or (not packed and q.shape[0] != k.shape[0]):
+    if ks[:-2] != vs[:-2] or qs[0] != ks[0]:
         raise ValueError("differential_attention: q, k and v disagree in batch or rows")
-    lead = tuple(q.shape[:-2])
-    try:
-        fits = torch.broadcast_shapes(tuple(lam.shape), lead + (H,)) == torch.Size(lead + (H,))
-    except RuntimeError:
-        fits = False
-    if not fits:
-        raise ValueError(f"differential_attention: lam {tuple(lam.shape)} does not broadcast to {lead + (H,)}")
+    lead = qs[:-2]
     if lam.dim() == 0:
         lam = lam.reshape(1)
+    lam_strides = _lam_strides(lam, lead, H)
+    if lam_strides is None:
+        raise ValueError(f"differential_attention: lam {tuple(lam.shape)} does not broadcast to {(*lead, H)}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"differential_attention: scale must be positive and finite, got {scale}")
@@ -372,21 +416,30 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     _lib.require_device(q, "differential_attention")
     if q.numel() == 0 or k.numel() == 0:         # nothing to attend with or to: zeros that stay attached to the graph
         return q.new_zeros(*lead, H, 2 * D) + sum(t.reshape(-1)[:0].sum() for t in (q, k, v, lam)).to(q.dtype)
-    n = dims - 1
-    q, k, v = (_rows_of_16_bytes(t, n) for t in (q, k, v))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam)):
-        return _DiffAttention.apply(q, k, v, lam, key_mask, cu_seqlens, longest, scale)
-    return _attention_forward(q, k, v, lam.expand(*lead, H), key_mask, cu_seqlens, longest, scale, False)[0]
+    q, k, v = _rows_of_16_bytes(q), _rows_of_16_bytes(k), _rows_of_16_bytes(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or lam.requires_grad):
+        return _DiffAttention.apply(q, k, v, lam, lam_strides, key_mask, cu_seqlens, longest, scale)
+    return _attention_forward(q, k, v, lam, lam_strides, key_mask, cu_seqlens, longest, scale, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------ vocabulary head
 def _to_bf16(x, stream):
-    if x.dtype == torch.bfloat16:
-        return x.contiguous()
     x = x.contiguous()
+    if x.dtype == torch.bfloat16:
+        return x
     y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
-    _lib.check(_lib.lib().bd_cast_f32_to_bf16(_lib.ptr(x), _lib.ptr(y), x.numel(), stream), "bd_cast_f32_to_bf16")
+    _lib.check(_lib.lib().bd_cast_f32_to_bf16(x.data_ptr(), y.data_ptr(), x.numel(), stream), "bd_cast_f32_to_bf16")
     return y
+
+
+@functools.lru_cache(maxsize=256)
+def _head_sizes(M, d, V):
+    """Bytes of the state and of the two workspaces."""
+    L_ = _lib.lib()
+    sizes = (L_.bd_linear_ce_state_bytes(M, d), L_.bd_linear_ce_workspace_bytes(M, d, V, 0), L_.bd_linear_ce_workspace_bytes(M, d, V, 1))
+    if min(sizes) < 0:
+        _lib.check(-1, "bd_linear_ce_workspace_bytes")
+    return sizes
 
 
 class _LinearCE(torch.autograd.Function):
@@ -395,41 +448,45 @@ class _LinearCE(torch.autograd.Function):
         dev = hidden.device
         V, d = weight.shape
         M = targets.numel()
-        L_ = _lib.lib()
-        with _On(dev) as stream:
+        state_bytes, ws_bytes, _ = _head_sizes(M, d, V)
+        with _on(dev) as stream:
             h, w = _to_bf16(hidden, stream), _to_bf16(weight, stream)
             loss = torch.empty((), dtype=torch.float32, device=dev)
-            state = torch.empty(L_.bd_linear_ce_state_bytes(M, d), dtype=torch.uint8, device=dev)
-            ws = torch.empty(L_.bd_linear_ce_workspace_bytes(M, d, V, 0), dtype=torch.uint8, device=dev)
-            _lib.check(L_.bd_linear_ce_fwd(_lib.ptr(h), _lib.ptr(w), _lib.ptr(targets), _lib.ptr(indicator),
-                                           _lib.ptr(attention_mask), _lib.ptr(loss), M, d, V, _lib.ptr(state), state.numel(),
-                                           _lib.ptr(ws), ws.numel(), stream), "bd_linear_ce_fwd")
-        if any(ctx.needs_input_grad[:2]):
-            # (the weighted rows are in the state; of the head the bf16 copy is kept where one was made)
-            ctx.save_for_backward(weight if w is weight else None, None if w is weight else w, state)
+            state = torch.empty(state_bytes, dtype=torch.uint8, device=dev)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            _lib.check(_lib.lib().bd_linear_ce_fwd(
+                h.data_ptr(), w.data_ptr(), targets.data_ptr(), None if indicator is None else indicator.data_ptr(),
+                None if attention_mask is None else attention_mask.data_ptr(), loss.data_ptr(), M, d, V, state.data_ptr(), state_bytes,
+                ws.data_ptr(), ws_bytes, stream), "bd_linear_ce_fwd")
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
+            # (the weighted rows are in the state; of an fp32 head its bf16 copy is kept)
+            ctx.save_for_backward(w, state)
             ctx.like = (hidden.shape, hidden.dtype, weight.dtype)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gout):
-        weight, copy, state = ctx.saved_tensors
-        w = weight if copy is None else copy
+        w, state = ctx.saved_tensors
         shape, hidden_dtype, weight_dtype = ctx.like
         V, d = w.shape
         M = shape[:-1].numel()
-        L_ = _lib.lib()
         dev = w.device
-        with _On(dev) as stream:
-            g = gout.reshape(1).float().contiguous()
-            dh = torch.empty(shape, dtype=torch.bfloat16, device=dev) if ctx.needs_input_grad[0] else None
-            dw = None
-            if ctx.needs_input_grad[1]:      # fp32 gradients are accumulated into, bf16 ones written
-                dw = (torch.zeros if weight_dtype == torch.float32 else torch.empty)(V, d, dtype=weight_dtype, device=dev)
-            ws = torch.empty(L_.bd_linear_ce_workspace_bytes(M, d, V, 1), dtype=torch.uint8, device=dev)
-            _lib.check(L_.bd_linear_ce_bwd(_lib.ptr(w), _lib.ptr(g), _lib.ptr(dh), _lib.ptr(dw), _DTYPES[weight_dtype], M, d, V,
-                                           _lib.ptr(state), state.numel(), _lib.ptr(ws), ws.numel(), stream), "bd_linear_ce_bwd")
-        return (dh.to(hidden_dtype) if dh is not None else None), dw, None, None, None
+        state_bytes, _, ws_bytes = _head_sizes(M, d, V)
+        dh = torch.empty(shape, dtype=torch.bfloat16, device=dev) if ctx.needs_input_grad[0] else None
+        dw = None
+        if ctx.needs_input_grad[1]:      # fp32 gradients are accumulated into, bf16 ones written
+            dw = (torch.zeros if weight_dtype == torch.float32 else torch.empty)(V, d, dtype=weight_dtype, device=dev)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        if gout.dtype != torch.float32:
+            gout = gout.float()
+        with _on(dev) as stream:
+            _lib.check(_lib.lib().bd_linear_ce_bwd(
+                w.data_ptr(), gout.data_ptr(), None if dh is None else dh.data_ptr(), None if dw is None else dw.data_ptr(),
+                _DTYPES[weight_dtype], M, d, V, state.data_ptr(), state_bytes, ws.data_ptr(), ws_bytes, stream), "bd_linear_ce_bwd")
+        if dh is not None and hidden_dtype != torch.bfloat16:
+            dh = dh.to(hidden_dtype)
+        return dh, dw, None, None, None
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,

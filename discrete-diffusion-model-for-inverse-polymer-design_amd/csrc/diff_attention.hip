@@ -33,11 +33,12 @@ struct DaArgs {
   const unsigned short *q, *k, *v, *dout;
   const void* lam;
   unsigned short *out, *dq, *dk, *dv;
-  float *lse, *maps, *dlam, *stats, *part, *part_ml;
+  float *lse, *maps, *stats, *part, *part_ml;
+  void* dlam;
   const unsigned char* mask;
   const int* cu;
   long long qs[3], ks[3], vs[3], ls[3], os[3], dos[3], dqs[3], dks[3], dvs[3], mask_stride;
-  int B, Lq, Lk, H, Hkv, share, total, lam_f32, n_blk, n_split;
+  int B, Lq, Lk, H, Hkv, share, total, lam_f32, dlam_bf16, n_blk, n_split;
   int small_strides;             // 64 rows of every operand lie within 4 GiB: staged by 32-bit offsets
   float scale;
 };
@@ -185,6 +186,11 @@ __device__ __forceinline__ DaSpan da_span(const DaArgs& a, int b) {
 
 __device__ __forceinline__ float da_lam(const DaArgs& a, long long off) {
   return a.lam_f32 ? ((const float*)a.lam)[off] : bd_bf16_to_f32(((const unsigned short*)a.lam)[off]);
+}
+
+__device__ __forceinline__ void da_put_dlam(const DaArgs& a, long long at, float v) {
+  if (a.dlam_bf16) ((unsigned short*)a.dlam)[at] = bd_f32_to_bf16(v);
+  else ((float*)a.dlam)[at] = v;
 }
 
 // one past the last visible key of the sequence (the tiles behind it are not visited); all threads return it
@@ -557,7 +563,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
       const int first = min(max(a.cu[a.B], 0), a.total);
       da_zero_tail(a.dq, a.dqs, first, a.total, 2 * hk * a.share, 2 * a.share, D, tid, 64 * NW);
       for (long long i = tid; i < (long long)(a.total - first) * a.share; i += 64 * NW)
-        a.dlam[(first + i / a.share) * a.H + hk * a.share + i % a.share] = 0.f;
+        da_put_dlam(a, (first + i / a.share) * a.H + hk * a.share + i % a.share, 0.f);
     }
     return;
   }
@@ -707,7 +713,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
     if (g == 0) {
       *(f32x4*)(a.stats + 8 * rh[qb]) = (f32x4){lse[qb][0], lse[qb][1], dl[qb][0], dl[qb][1]};
       a.stats[8 * rh[qb] + 4] = lam;
-      a.dlam[rh[qb]] = -dl[qb][1];
+      da_put_dlam(a, rh[qb], -dl[qb][1]);
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -931,7 +937,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
 }
 
 // dlam [B, L, H] summed over the axes that lam was broadcast along (kept axes: kb, kl, kh), in a fixed order; one
-// workgroup per kept value (a wave's worth of values per workgroup where nothing is summed: a cast)
+// workgroup per kept value
 template <typename T>
 __global__ __launch_bounds__(256) void da_dlam_kernel(const float* __restrict__ dlam, T* __restrict__ out, int B, int L, int H, int kb, int kl,
                                                       int kh) {
@@ -953,14 +959,6 @@ __global__ __launch_bounds__(256) void da_dlam_kernel(const float* __restrict__ 
     if (sizeof(T) == 2) out[blockIdx.x] = (T)bd_f32_to_bf16(s);
     else ((float*)out)[blockIdx.x] = s;
   }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void da_dlam_cast_kernel(const float* __restrict__ dlam, T* __restrict__ out, long long n) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  if (sizeof(T) == 2) out[i] = (T)bd_f32_to_bf16(dlam[i]);
-  else ((float*)out)[i] = dlam[i];
 }
 
 // ---------------------------------------------------------------------------------------------- host side
@@ -1116,6 +1114,7 @@ extern "C" int bd_diff_attention_bwd(const bd_diff_attn_args* p, void* stream) {
   DaArgs a;
   const int rc = da_check(*p, "bd_diff_attention_bwd", a);
   if (rc != BD_OK) return rc;
+  BD_REQUIRE(p->dlam_dtype == BD_DTYPE_BF16 || p->dlam_dtype == BD_DTYPE_F32, "bd_diff_attention_bwd: dlam is neither bf16 nor fp32");
   BD_REQUIRE(p->dout && p->dq && p->dk && p->dv && p->dlam && p->lse, "bd_diff_attention_bwd: null operand");
   const void* aligned[] = {p->dout, p->dq, p->dk, p->dv, p->maps};
   for (const void* x : aligned) BD_REQUIRE(((uintptr_t)x & 15) == 0, "bd_diff_attention_bwd: operands must be 16-byte aligned");
@@ -1127,7 +1126,7 @@ extern "C" int bd_diff_attention_bwd(const bd_diff_attn_args* p, void* stream) {
              "bd_diff_attention_bwd: the workspace must hold %lld bytes, 16-byte aligned", need);
   a.dout = (const unsigned short*)p->dout;
   a.dq = (unsigned short*)p->dq; a.dk = (unsigned short*)p->dk; a.dv = (unsigned short*)p->dv;
-  a.dlam = p->dlam;
+  a.dlam = p->dlam; a.dlam_bf16 = p->dlam_dtype == BD_DTYPE_BF16;
   a.stats = (float*)p->workspace;
   bd_prof_scope prof(stream, 28.0 * p->B * p->H * (double)p->Lq * p->Lk * p->head_dim, BD_PROF_ATTN_BWD);
   switch (p->head_dim) {
@@ -1142,17 +1141,11 @@ extern "C" int bd_diff_attention_dlam(const float* dlam, void* out, int out_dtyp
   BD_REQUIRE(dlam && out && B > 0 && L > 0 && H > 0, "bd_diff_attention_dlam: null operand or empty shape");
   BD_REQUIRE(out_dtype == BD_DTYPE_BF16 || out_dtype == BD_DTYPE_F32, "bd_diff_attention_dlam: out is neither bf16 nor fp32");
   const long long all = (long long)B * L * H, kept = (keep_b ? B : 1ll) * (keep_l ? L : 1) * (keep_h ? H : 1);
-  BD_REQUIRE(all < (1ll << 38) && (kept == all || kept < (1ll << 31)), "bd_diff_attention_dlam: too many values");
+  BD_REQUIRE(all < (1ll << 38) && kept < (1ll << 31), "bd_diff_attention_dlam: too many values");
   hipStream_t s = (hipStream_t)stream;
   const bool bf = out_dtype == BD_DTYPE_BF16;
-  if (kept == all) {
-    const dim3 grid((unsigned)((all + 255) / 256));
-    if (bf) hipLaunchKernelGGL(da_dlam_cast_kernel<unsigned short>, grid, dim3(256), 0, s, dlam, (unsigned short*)out, all);
-    else hipLaunchKernelGGL(da_dlam_cast_kernel<float>, grid, dim3(256), 0, s, dlam, (float*)out, all);
-  } else {
-    const dim3 grid((unsigned)kept);
-    if (bf) hipLaunchKernelGGL(da_dlam_kernel<unsigned short>, grid, dim3(256), 0, s, dlam, (unsigned short*)out, B, L, H, keep_b, keep_l, keep_h);
-    else hipLaunchKernelGGL(da_dlam_kernel<float>, grid, dim3(256), 0, s, dlam, (float*)out, B, L, H, keep_b, keep_l, keep_h);
-  }
+  const dim3 grid((unsigned)kept);
+  if (bf) hipLaunchKernelGGL(da_dlam_kernel<unsigned short>, grid, dim3(256), 0, s, dlam, (unsigned short*)out, B, L, H, keep_b, keep_l, keep_h);
+  else hipLaunchKernelGGL(da_dlam_kernel<float>, grid, dim3(256), 0, s, dlam, (float*)out, B, L, H, keep_b, keep_l, keep_h);
   return bd_check_launch("bd_diff_attention_dlam");
 }

@@ -88,32 +88,36 @@ __global__ __launch_bounds__(256) void vl_gather_kernel(const unsigned short* __
   if (lane == 0) { before[wave] = nb; all[wave] = na; wsum[wave] = ws; }
   __syncthreads();
   const int first = before[0] + before[1] + before[2] + before[3], total = all[0] + all[1] + all[2] + all[3];
+  const bool lead = blockIdx.y == 0;
   if (wave == 0) {
     const int row = grp * SCAN + lane;
     const float w = row < M ? vl_weight(ind, attn, row) : 0.f;
     const unsigned long long live = __ballot(w != 0.f);
     const int at = __popcll(live & ((1ull << lane) - 1ull));
-    if (row < M) st.pos[row] = w != 0.f ? first + at : -1;
+    if (lead && row < M) st.pos[row] = w != 0.f ? first + at : -1;
     if (w != 0.f) {
       src[at] = row;
+    }
+    if (lead && w != 0.f) {
       st.idx[first + at] = row;
       st.w[first + at] = w;
       const long long t = targets[row];
       st.tgt[first + at] = t >= 0 && t < V ? (int)t : -1;      // outside the vocabulary: the row's loss is NaN
     }
     if (lane == 0) before[0] = __popcll(live);
-    if (grp == 0 && lane == 0) {
+    if (lead && grp == 0 && lane == 0) {
       st.head[0] = total;
       ((float*)st.head)[1] = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
     }
   }
   __syncthreads();
-  const int n = before[0], per = d / 8;
-  for (int i = tid; i < n * per; i += 256) {
-    const int r = i / per, ch = i - r * per;
+  // (the row's 16-byte chunks are dealt to the workgroups of a group, grid.y)
+  const int n = before[0], per = d / 8, wide = (per + gridDim.y - 1) / gridDim.y, ch0 = wide * blockIdx.y, chn = min(wide, per - ch0);
+  for (int i = tid; i < n * chn; i += 256) {
+    const int r = i / chn, ch = ch0 + i - r * chn;
     *(u32x4*)(st.hc + (long long)(first + r) * d + 8 * ch) = *(const u32x4*)(hidden + (long long)src[r] * d + 8 * ch);
   }
-  if (grp == groups - 1) {           // zeros behind the last row, to the end of its 256-row tile
+  if (grp == groups - 1 && blockIdx.y == 0) {      // zeros behind the last row, to the end of its 256-row tile
     const int end = (int)vl_up(total, 256);
     for (long long i = tid; i < (long long)(end - total) * per; i += 256)
       *(u32x4*)(st.hc + (long long)total * d + 8 * i) = (u32x4){0u, 0u, 0u, 0u};
@@ -123,9 +127,21 @@ __global__ __launch_bounds__(256) void vl_gather_kernel(const unsigned short* __
 // =====================================================================================
 // C[m, n] = sum_k A(m, k) B(n, k) on BM x BN tiles. AKC / BKC: the operand is stored along k (rows of K values) or, if
 // not, along its own axis (row k holds the values of all m / n). MFMA operand order: n is the A side and m the B side,
-// with n permuted inside 64 columns, so that a lane ends up with 16 consecutive n of one row m.
+// with n permuted inside 64 columns, so that a lane ends up with 2 x 8 consecutive n of one row m (columns 8 g and 32 + 8 g: the
+// four lanes of a row store 64 consecutive bytes at a time).
 // K is staged 64 at a time by LDS-DMA, two stages in turn.
 // =====================================================================================
+// Splits of a product's summed axis: one workgroup per CU, four stages each at least. For dh the tiles follow the row count
+// on the device, so the kernel and the one that adds the slabs up ask this themselves.
+__host__ __device__ inline int vl_splits(long long tiles, long long k_tiles, int most) {
+  long long n = tiles >= 256 ? 1 : tiles > 0 ? 256 / tiles : 1;
+  if (n > k_tiles / 4) n = k_tiles / 4;
+  return n < 1 ? 1 : n > most ? most : (int)n;
+}
+__device__ __forceinline__ int vl_dh_splits(int live, int bt, int d, int k, int most) {
+  return vl_splits((long long)((live + bt - 1) / bt) * ((d + bt - 1) / bt), (k + 63) >> 6, most);
+}
+
 struct VlGemm {
   const unsigned short *A, *B;
   long long lda, ldb;
@@ -133,10 +149,13 @@ struct VlGemm {
   int M, N, K;                        // capacities; m_live / k_live: M / K is the device's row count instead
   int n_rows;                         // rows of B that exist (BKC): columns behind them re-read the last one
   int m_live, k_live, n_split;
+  int dh_split;                       // dh: n_split is the most, the kernel takes what the row count asks for
+  unsigned short* dh;                 // dh from one piece and one split: written in bf16 to its rows, no slab
+  const int* idx;
   int v0, V;                          // VL_STATS, VL_DLOG: n is vocabulary column v0 + n, valid below V. VL_DW: m is
   const float *w, *lse;               // VL_DLOG
   const int* tgt;
-  f32x2* pairs;                       // VL_STATS: [64-column block][M] (maximum, sum) in base 2
+  f32x2* pairs;                       // VL_STATS: [tile column][M] (maximum, sum) in base 2
   unsigned short* dlog;               // VL_DLOG: [M, ldo]
   float* slab;                        // VL_SLAB: [split][M][N]
   long long slab_stride, ldo;
@@ -149,9 +168,7 @@ struct VlGemm {
 typedef __attribute__((address_space(3))) void vl_lds;
 
 template <int R> __device__ __forceinline__ int vl_kc(int row, int ch) { return R * row + 16 * (ch ^ ((row >> 1) & 7)); }
-template <int R, bool NSIDE> __device__ __forceinline__ int vl_mc(int row, int ch) {
-  return R * row + 16 * (ch ^ (NSIDE ? (((row & 1) << 3) | ((row >> 1) & 1)) : ((row & 3) << 2)));
-}
+template <int R> __device__ __forceinline__ int vl_mc(int row, int ch) { return R * row + 16 * (ch ^ ((row & 3) << 2)); }
 __device__ __forceinline__ s16x4 vl_read_tr(const unsigned char* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
 }
@@ -159,6 +176,26 @@ __device__ __forceinline__ bf16x8 vl_join(s16x4 a, s16x4 b) {
   union { struct { s16x4 a, b; } s; bf16x8 v; } u;
   u.s.a = a; u.s.b = b;
   return u.v;
+}
+
+// (maximum, sum of 2^(x - maximum)) of two parts
+__device__ __forceinline__ f32x2 vl_pair(f32x2 a, f32x2 b) {
+  const float m = fmaxf(a[0], b[0]), ref = m == -INFINITY ? 0.f : m;
+  return (f32x2){m, a[1] * __builtin_amdgcn_exp2f(a[0] - ref) + b[1] * __builtin_amdgcn_exp2f(b[0] - ref)};
+}
+
+// the columns a lane holds of a row (8 at o, 8 at o + 32), times f, in bf16
+__device__ __forceinline__ void vl_store_bf16(unsigned short* o, const f32x4 (&a)[4], float f, bool first, bool second) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[2 * i] = bd_pack_bf16x2(f * a[2 * h + i][0], f * a[2 * h + i][1]);
+      w[2 * i + 1] = bd_pack_bf16x2(f * a[2 * h + i][2], f * a[2 * h + i][3]);
+    }
+    if (h ? second : first) *(u32x4*)(o + 32 * h) = w;
+  }
 }
 
 template <int BM, int BN, bool AKC, bool BKC, int EPI>
@@ -173,7 +210,8 @@ __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGem
   const int live = p.head[0];
   const int M = p.m_live ? min(live, p.M) : p.M, K = p.k_live ? min((live + 63) & ~63, p.K) : p.K;      // (whole stages of rows: zeros behind the last)
   // tile list: groups of 8 tile rows, column by column inside a group; each XCD takes one contiguous part
-  const int tiles_m = (M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN, n_all = tiles_m * tiles_n * p.n_split;
+  const int tiles_m = (M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
+  const int n_split = p.dh_split ? vl_dh_splits(M, BM, p.N, p.K, p.n_split) : p.n_split, n_all = tiles_m * tiles_n * n_split;
   int tile;
   {
     const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, q = n_all >> 3, rr = n_all & 7;
@@ -184,7 +222,7 @@ __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGem
   tile -= split * tiles_m * tiles_n;
   const int group = tile / (8 * tiles_n), rows_here = min(tiles_m - 8 * group, 8), in_group = tile - group * 8 * tiles_n;
   const int m0 = (8 * group + in_group % rows_here) * BM, n0 = (in_group / rows_here) * BN;
-  const int kt_all = (K + 63) >> 6, kt_per = (kt_all + p.n_split - 1) / p.n_split;
+  const int kt_all = (K + 63) >> 6, kt_per = (kt_all + n_split - 1) / n_split;
   const int kt_beg = min(split * kt_per, kt_all), kt_end = min(kt_beg + kt_per, kt_all);
 
   // ---- staging: wave w sends pieces w, w + NW, ...; a lane's offset inside a stage's source is fixed but in a last
@@ -197,18 +235,18 @@ __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGem
       return (unsigned)(((long long)(min(m0 + row, p.M - 1) - m0) * p.lda + 8 * ch) * 2);
     }
     constexpr int R = 2 * BM;
-    const int row = at / R, ch = (vl_mc<R, false>(row, (at % R) >> 4) - R * row) >> 4;
+    const int row = at / R, ch = (vl_mc<R>(row, (at % R) >> 4) - R * row) >> 4;
     return (unsigned)(((long long)min(row, K - 1 - k0) * p.lda + min(m0 + 8 * ch, p.M - 8) - m0) * 2);
   };
   auto off_b = [&](int j, int k0) -> unsigned {
     const int at = (wave + NW * j) * 1024 + lane * 16;
     if (BKC) {
       const int rx = at >> 7, ch = ((at >> 4) & 7) ^ ((rx >> 1) & 7);
-      const int i = rx & 15, n = 64 * (rx >> 6) + 16 * (i >> 2) + 4 * ((rx >> 4) & 3) + (i & 3);     // permuted: see above
+      const int i = rx & 15, tn = (rx >> 4) & 3, n = 64 * (rx >> 6) + 32 * (tn >> 1) + 8 * (i >> 2) + 4 * (tn & 1) + (i & 3);   // permuted
       return (unsigned)(((long long)(min(n0 + n, p.n_rows - 1) - n0) * p.ldb + 8 * ch) * 2);
     }
     constexpr int R = 2 * BN;
-    const int row = at / R, ch = (vl_mc<R, true>(row, (at % R) >> 4) - R * row) >> 4;
+    const int row = at / R, ch = (vl_mc<R>(row, (at % R) >> 4) - R * row) >> 4;
     return (unsigned)(((long long)min(row, K - 1 - k0) * p.ldb + min(n0 + 8 * ch, p.N - 8) - n0) * 2);
   };
   unsigned va[PA], vb[PB];
@@ -252,8 +290,8 @@ __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGem
           x[tn] = *(const bf16x8*)(Bs + vl_kc<128>(64 * wn + 16 * tn + c, 4 * kk + g));
         } else {
           constexpr int R = 2 * BN;
-          const int r0 = 32 * kk + 8 * g + q4, ch = 8 * wn + 2 * p4 + (tn >> 1);
-          x[tn] = vl_join(vl_read_tr(Bs + vl_mc<R, true>(r0, ch) + 8 * (tn & 1)), vl_read_tr(Bs + vl_mc<R, true>(r0 + 4, ch) + 8 * (tn & 1)));
+          const int r0 = 32 * kk + 8 * g + q4, ch = 8 * wn + 4 * (tn >> 1) + p4;
+          x[tn] = vl_join(vl_read_tr(Bs + vl_mc<R>(r0, ch) + 8 * (tn & 1)), vl_read_tr(Bs + vl_mc<R>(r0 + 4, ch) + 8 * (tn & 1)));
         }
       }
 #pragma unroll
@@ -264,7 +302,7 @@ __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGem
         } else {
           constexpr int R = 2 * BM;
           const int r0 = 32 * kk + 8 * g + q4, ch = 2 * (TM * wm + tm) + (p4 >> 1);
-          y = vl_join(vl_read_tr(As + vl_mc<R, false>(r0, ch) + 8 * (p4 & 1)), vl_read_tr(As + vl_mc<R, false>(r0 + 4, ch) + 8 * (p4 & 1)));
+          y = vl_join(vl_read_tr(As + vl_mc<R>(r0, ch) + 8 * (p4 & 1)), vl_read_tr(As + vl_mc<R>(r0 + 4, ch) + 8 * (p4 & 1)));
         }
 #pragma unroll
         for (int tn = 0; tn < TN; ++tn) acc[tm][tn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[tn], y, acc[tm][tn], 0, 0, 0);
@@ -272,93 +310,109 @@ __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGem
     }
   }
 
-  // ---- lane: row m0 + 16 (TM wm + tm) + c, columns nb + 4 tn + j
-  const int nb = n0 + 64 * wn + 16 * g;
+  // ---- lane: row m0 + 16 (TM wm + tm) + c, columns nb + 32 (tn >> 1) + 4 (tn & 1) + j
+  const int nb = n0 + 64 * wn + 8 * g;
   float coef = 0.f;
-  if (EPI == VL_DW) {
+  if (EPI == VL_DW || EPI == VL_SLAB) {
     const float sw = ((const float*)p.head)[1];
-    coef = sw > 0.f ? p.gout[0] / sw : 0.f;
+    coef = sw > 0.f && p.gout ? p.gout[0] / sw : 0.f;
+  }
+  if (EPI == VL_STATS) {
+    // each wave's 64 columns to a pair (maximum, sum) per row, joined over the tile's columns through LDS
+    const bool whole = p.v0 + n0 + BN <= p.V;
+    f32x2* const pl = (f32x2*)vl_smem;                     // [WN][BM]
+    __syncthreads();
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) {
+      if (!whole) {
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (p.v0 + nb + 32 * (tn >> 1) + 4 * (tn & 1) + j >= p.V) acc[tm][tn][j] = -INFINITY;
+      }
+      float mx = -INFINITY, se = 0.f;
+#pragma unroll
+      for (int tn = 0; tn < TN; ++tn) mx = fmaxf(fmaxf(mx, fmaxf(acc[tm][tn][0], acc[tm][tn][1])), fmaxf(acc[tm][tn][2], acc[tm][tn][3]));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float ref = mx == -INFINITY ? 0.f : mx * VL_LOG2E;
+#pragma unroll
+      for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) se += __builtin_amdgcn_exp2f(acc[tm][tn][j] * VL_LOG2E - ref);
+      se += __shfl_xor(se, 16, 64);
+      se += __shfl_xor(se, 32, 64);
+      if (g == 0) pl[wn * BM + 16 * (TM * wm + tm) + c] = (f32x2){mx * VL_LOG2E, se};
+    }
+    __syncthreads();
+    if (tid < BM && m0 + tid < M) {
+      f32x2 x = pl[tid];
+#pragma unroll
+      for (int w = 1; w < WN; ++w) x = vl_pair(x, pl[w * BM + tid]);
+      p.pairs[(long long)(n0 / BN) * p.M + m0 + tid] = x;
+    }
+    return;
   }
 #pragma unroll
   for (int tm = 0; tm < TM; ++tm) {
     const int m = m0 + 16 * (TM * wm + tm) + c;
-    if (EPI == VL_STATS) {
-      float mx = -INFINITY, se = 0.f;
-#pragma unroll
-      for (int tn = 0; tn < TN; ++tn)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          acc[tm][tn][j] = p.v0 + nb + 4 * tn + j < p.V ? acc[tm][tn][j] * VL_LOG2E : -INFINITY;
-          mx = fmaxf(mx, acc[tm][tn][j]);
-        }
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float ref = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-      for (int tn = 0; tn < TN; ++tn)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) se += __builtin_amdgcn_exp2f(acc[tm][tn][j] - ref);
-      se += __shfl_xor(se, 16, 64);
-      se += __shfl_xor(se, 32, 64);
-      if (g == 0 && m < M && n0 + 64 * wn < p.N) p.pairs[(long long)((n0 >> 6) + wn) * p.M + m] = (f32x2){mx, se};
-    } else if (EPI == VL_DLOG) {
+    if (EPI == VL_DLOG) {
       // (rows behind the last weighted one: zeros, they are summed over by dW's product)
       const bool in = m < M;
       const int tcol = in ? p.tgt[m] - p.v0 - nb : -1;
-      const float lse = in ? p.lse[m] : 0.f, w = in ? p.w[m] : 0.f;
-      float v[16];
+      const float lse = in ? p.lse[m] : INFINITY, w = in ? p.w[m] : 0.f;
 #pragma unroll
       for (int tn = 0; tn < TN; ++tn)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int col = 4 * tn + j;
+          const int col = 32 * (tn >> 1) + 4 * (tn & 1) + j;
           const float pr = __builtin_amdgcn_exp2f(acc[tm][tn][j] * VL_LOG2E - lse);
-          v[col] = in && p.v0 + nb + col < p.V ? w * (pr - (col == tcol ? 1.f : 0.f)) : 0.f;
+          acc[tm][tn][j] = w * (col == tcol ? pr - 1.f : pr);
         }
-      if (nb < p.N) {
-        u32x4 lo, hi;
+      if (p.v0 + n0 + BN > p.V || !in) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { lo[i] = bd_pack_bf16x2(v[2 * i], v[2 * i + 1]); hi[i] = bd_pack_bf16x2(v[8 + 2 * i], v[9 + 2 * i]); }
-        unsigned short* o = p.dlog + (long long)m * p.ldo + nb;
-        *(u32x4*)o = lo;
-        *(u32x4*)(o + 8) = hi;
+        for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (!in || p.v0 + nb + 32 * (tn >> 1) + 4 * (tn & 1) + j >= p.V) acc[tm][tn][j] = 0.f;
       }
+      vl_store_bf16(p.dlog + (long long)m * p.ldo + nb, acc[tm], 1.f, nb < p.N, nb + 32 < p.N);
     } else if (EPI == VL_SLAB) {
-      if (m < M && nb < p.N) {
-        float* o = p.slab + split * p.slab_stride + (long long)m * p.ldo + nb;
+      if (m >= M) continue;
+      if (p.dh && n_split == 1) {
+        vl_store_bf16(p.dh + (long long)p.idx[m] * p.ldo + nb, acc[tm], coef, nb < p.N, nb + 32 < p.N);
+        continue;
+      }
+      float* o = p.slab + split * p.slab_stride + (long long)m * p.ldo + nb;
 #pragma unroll
-        for (int tn = 0; tn < TN; ++tn) {
-          f32x4 x = acc[tm][tn];
-          if (p.add) {
-            const f32x4 y = *(const f32x4*)(o + 4 * tn);
+      for (int tn = 0; tn < TN; ++tn) {
+        const int col = 32 * (tn >> 1) + 4 * (tn & 1);
+        if (nb + col >= p.N) continue;
+        f32x4 x = acc[tm][tn];
+        if (p.add) {
+          const f32x4 y = *(const f32x4*)(o + col);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] += y[j];
-          }
-          *(f32x4*)(o + 4 * tn) = x;
+          for (int j = 0; j < 4; ++j) x[j] += y[j];
         }
+        *(f32x4*)(o + col) = x;
       }
     } else {
-      if (p.v0 + m < p.V && nb < p.N) {
-        const long long at = (long long)(p.v0 + m) * p.ldo + nb;
-        if (p.dw_f32) {
-          float* o = (float*)p.dw + at;
+      if (p.v0 + m >= p.V) continue;
+      const long long at = (long long)(p.v0 + m) * p.ldo + nb;
+      if (!p.dw_f32) {
+        vl_store_bf16((unsigned short*)p.dw + at, acc[tm], coef, nb < p.N, nb + 32 < p.N);
+        continue;
+      }
+      float* o = (float*)p.dw + at;
 #pragma unroll
-          for (int tn = 0; tn < TN; ++tn) {
-            f32x4 y = *(const f32x4*)(o + 4 * tn);
+      for (int tn = 0; tn < TN; ++tn) {
+        const int col = 32 * (tn >> 1) + 4 * (tn & 1);
+        if (nb + col >= p.N) continue;
+        f32x4 y = *(const f32x4*)(o + col);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] += coef * acc[tm][tn][j];
-            *(f32x4*)(o + 4 * tn) = y;
-          }
-        } else {
-          u32x4 lo, hi;
-          lo[0] = bd_pack_bf16x2(coef * acc[tm][0][0], coef * acc[tm][0][1]); lo[1] = bd_pack_bf16x2(coef * acc[tm][0][2], coef * acc[tm][0][3]);
-          lo[2] = bd_pack_bf16x2(coef * acc[tm][1][0], coef * acc[tm][1][1]); lo[3] = bd_pack_bf16x2(coef * acc[tm][1][2], coef * acc[tm][1][3]);
-          hi[0] = bd_pack_bf16x2(coef * acc[tm][2][0], coef * acc[tm][2][1]); hi[1] = bd_pack_bf16x2(coef * acc[tm][2][2], coef * acc[tm][2][3]);
-          hi[2] = bd_pack_bf16x2(coef * acc[tm][3][0], coef * acc[tm][3][1]); hi[3] = bd_pack_bf16x2(coef * acc[tm][3][2], coef * acc[tm][3][3]);
-          unsigned short* o = (unsigned short*)p.dw + at;
-          *(u32x4*)o = lo;
-          *(u32x4*)(o + 8) = hi;
-        }
+        for (int j = 0; j < 4; ++j) y[j] += coef * acc[tm][tn][j];
+        *(f32x4*)(o + col) = y;
       }
     }
   }
@@ -369,14 +423,10 @@ __global__ __launch_bounds__(256) void vl_join_kernel(VlState st, const unsigned
                                                       float* __restrict__ rowloss, int cap, int blocks, int d) {
   const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= st.head[0]) return;
-  float m = -INFINITY, s = 0.f;
-  for (int i = lane; i < blocks; i += 64) {
-    const f32x2 x = pairs[(long long)i * cap + row];
-    const float mn = fmaxf(m, x[0]);
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    s = s * __builtin_amdgcn_exp2f(m - ref) + x[1] * __builtin_amdgcn_exp2f(x[0] - ref);
-    m = mn;
-  }
+  f32x2 ms = {-INFINITY, 0.f};
+  for (int i = lane; i < blocks; i += 64) ms = vl_pair(ms, pairs[(long long)i * cap + row]);
+  const float m = ms[0];
+  float s = ms[1];
   const float mm = bd_wave_max(m);
   const float ref = mm == -INFINITY ? 0.f : mm;
   s = bd_wave_sum(s * __builtin_amdgcn_exp2f(m - ref));
@@ -416,8 +466,8 @@ __global__ __launch_bounds__(1024) void vl_finish_kernel(VlState st, const float
 }
 
 // dhidden rows from the slabs (added in order), zeros at rows without a weight
-__global__ __launch_bounds__(256) void vl_dh_kernel(VlState st, const float* __restrict__ slab, long long slab_stride, int n_slab,
-                                                    const float* __restrict__ gout, unsigned short* __restrict__ dh, int M, int d) {
+__global__ __launch_bounds__(256) void vl_dh_kernel(VlState st, const float* __restrict__ slab, long long slab_stride, int most, int bt, int k,
+                                                    int pieces, const float* __restrict__ gout, unsigned short* __restrict__ dh, int M, int d) {
   const int per = d / 8;
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= (long long)M * per) return;
@@ -425,6 +475,8 @@ __global__ __launch_bounds__(256) void vl_dh_kernel(VlState st, const float* __r
   const int at = st.pos[row];
   u32x4 o = {0u, 0u, 0u, 0u};
   if (at >= 0) {
+    const int n_slab = vl_dh_splits(st.head[0], bt, d, k, most);
+    if (n_slab == 1 && pieces == 1) return;                // the product wrote the row itself
     const float sw = ((const float*)st.head)[1];
     const float coef = sw > 0.f ? gout[0] / sw : 0.f;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -472,48 +524,51 @@ __global__ __launch_bounds__(256) void vl_dw_kernel(VlState st, const float* __r
 struct VlPlan {
   long long m_pad;
   int piece, n_pieces;                // vocabulary columns per backward piece
-  int big;                            // 256 x 256 tiles
-  int split_h, split_w;               // splits of dh's product over the piece, of dW's over the rows
+  int big_z, big_h, big_w;            // 256 x 256 tiles for the scores, dh, dW (else 128 x 128)
+  int split_h, split_w;               // splits of dh's product over the piece (at most), of dW's over the rows
   long long slab_h, slab_w;           // floats of one slab
   long long fwd_bytes, bwd_bytes;
 };
 
 constexpr long long VL_PIECE_BYTES = 256ll << 20;      // dz of one piece: what stays near the card's last-level cache
 
-int vl_splits(long long tiles, long long k_tiles) {
-  // one workgroup per CU and more where the axis is long enough for four stages each
-  long long n = tiles >= 256 ? 1 : (256 + tiles - 1) / tiles;
-  if (n > k_tiles / 4) n = k_tiles / 4;
-  return n < 1 ? 1 : n > 64 ? 64 : (int)n;
-}
-
 VlPlan vl_plan(long long M, int d, int V) {
   VlPlan p;
   p.m_pad = vl_up(M, 256);
-  p.big = (p.m_pad / 256) * ((V + 255) / 256) >= 256;
-  const int bt = p.big ? 256 : 128;
+  // Tile sizes, each measured both ways (256 x 256 / 128 x 128, us; half of the rows weighted): the larger tile reads less LDS
+  // per product but leaves one workgroup on a CU, whose start and end nothing hides, and wastes more at ragged edges.
+  //   scores: 8192 x 2048 -> 65536: 881 / 986; x 1024: 502 / 526; 2000 x 1024 -> 65536: 149 / 139; 4096 x 512 -> 32000: 83 / 81;
+  //   3001 x 768 -> 32003: 111 / 96; 32768 x 384 -> 803: 19 / 19
+  //   dh (with the sum of its splits): in that order 889 / 1005, 520 / 686, 150 / 179, 83 / 91, 99 / 120, 38 / 26
+  //   dW (with the sum of its splits): 839 / 1040, 440 / 530, 140 / 162, 65 / 79, 106 / 103, 40 / 31
+  p.big_z = d >= 1024 && (p.m_pad / 256) * ((V + 255) / 256) >= 4096;
+  p.big_h = V >= 4096 && (d % 256 == 0 || d >= 768);
+  p.big_w = (long long)((V + 255) / 256) * ((d + 255) / 256) >= 200;
+  const int bh = p.big_h ? 256 : 128, bw = p.big_w ? 256 : 128;
   long long piece = VL_PIECE_BYTES / 2 / p.m_pad / 256 * 256;
   if (piece < 256) piece = 256;
   const long long v_pad = vl_up(V, 256);
   if (piece > v_pad) piece = v_pad;
   p.n_pieces = (int)((v_pad + piece - 1) / piece);
   p.piece = (int)vl_up((v_pad + p.n_pieces - 1) / p.n_pieces, 256);
-  p.split_h = vl_splits(vl_up(M, bt) / bt * (vl_up(d, bt) / bt), p.piece / 64);
-  p.split_w = vl_splits(vl_up(p.piece, bt) / bt * (vl_up(d, bt) / bt), p.m_pad / 64);
+  // (a quarter of the rows may carry weight: then dh has so many fewer tiles. At most 512 MB of slabs.)
   p.slab_h = p.m_pad * d;
+  p.split_h = vl_splits((vl_up(M, bh) / bh + 3) / 4 * (vl_up(d, bh) / bh), p.piece / 64, 64);
+  while (p.split_h > 1 && p.split_h * p.slab_h * 4 > (512ll << 20)) --p.split_h;
+  p.split_w = vl_splits(vl_up(p.piece, bw) / bw * (vl_up(d, bw) / bw), p.m_pad / 64, 64);
   p.slab_w = (long long)p.piece * d;
   const long long groups = (M + SCAN - 1) / SCAN;
-  p.fwd_bytes = vl_up(groups * 4, 256) * 2 + vl_up(p.m_pad * 4, 256) + (v_pad / 64) * p.m_pad * 8;
+  p.fwd_bytes = vl_up(groups * 4, 256) * 2 + vl_up(p.m_pad * 4, 256) + (v_pad / 128) * p.m_pad * 8;
   p.bwd_bytes = p.m_pad * p.piece * 2 + (p.split_h * p.slab_h + (p.split_w > 1 ? p.split_w * p.slab_w : 0)) * 4;
   return p;
 }
 
 template <bool AKC, bool BKC, int EPI>
-void vl_launch(const VlPlan& pl, const VlGemm& p, hipStream_t s) {
-  const int bt = pl.big ? 256 : 128;
+void vl_launch(int big, const VlGemm& p, hipStream_t s) {
+  const int bt = big ? 256 : 128;
   const long long n = vl_up(p.M, bt) / bt * (vl_up(p.N, bt) / bt) * p.n_split;
   const dim3 grid((unsigned)vl_up(n, 8));
-  if (pl.big) {
+  if (big) {
     BD_SET_MAX_LDS((vl_gemm_kernel<256, 256, AKC, BKC, EPI>), 131072);
     hipLaunchKernelGGL((vl_gemm_kernel<256, 256, AKC, BKC, EPI>), grid, dim3(512), 131072, s, p);
   } else {
@@ -557,16 +612,17 @@ extern "C" int bd_linear_ce_fwd(const void* hidden, const void* weight, const lo
   float* sums = (float*)w; w += vl_up(groups * 4ll, 256);
   float* rowloss = (float*)w; w += vl_up(pl.m_pad * 4, 256);
   f32x2* pairs = (f32x2*)w;
+  const int bz = pl.big_z ? 256 : 128;
   bd_prof_scope prof(stream, 2.0 * M * (double)V * d, BD_PROF_GEMM);
   hipLaunchKernelGGL(vl_count_kernel, dim3((groups + 3) / 4), dim3(256), 0, s, indicator, attention_mask, counts, sums, (int)M);
-  hipLaunchKernelGGL(vl_gather_kernel, dim3(groups), dim3(256), 0, s, (const unsigned short*)hidden, targets, indicator, attention_mask, counts,
+  hipLaunchKernelGGL(vl_gather_kernel, dim3(groups, (d + 511) / 512), dim3(256), 0, s, (const unsigned short*)hidden, targets, indicator, attention_mask, counts,
                      sums, st, (int)M, d, V);
   VlGemm p = {};
   p.A = st.hc; p.lda = d; p.B = (const unsigned short*)weight; p.ldb = d; p.head = st.head;
   p.M = (int)pl.m_pad; p.N = V; p.n_rows = V; p.K = d; p.m_live = 1; p.n_split = 1; p.V = V; p.pairs = pairs;
-  vl_launch<true, true, VL_STATS>(pl, p, s);
+  vl_launch<true, true, VL_STATS>(pl.big_z, p, s);
   hipLaunchKernelGGL(vl_join_kernel, dim3((unsigned)((M + 3) / 4)), dim3(256), 0, s, st, (const unsigned short*)weight, pairs, rowloss,
-                     (int)pl.m_pad, (V + 63) / 64, d);
+                     (int)pl.m_pad, (V + bz - 1) / bz, d);
   hipLaunchKernelGGL(vl_finish_kernel, dim3(1), dim3(1024), 0, s, st, rowloss, loss);
   return bd_check_launch("bd_linear_ce_fwd");
 }
@@ -595,12 +651,13 @@ extern "C" int bd_linear_ce_bwd(const void* weight, const float* grad_out, void*
     VlGemm p = {};
     p.A = st.hc; p.lda = d; p.B = wp; p.ldb = d; p.head = st.head; p.M = (int)pl.m_pad; p.N = n; p.n_rows = min(n, V - v0); p.K = d; p.m_live = 1; p.n_split = 1;
     p.v0 = v0; p.V = V; p.w = st.w; p.lse = st.lse; p.tgt = st.tgt; p.dlog = dlog; p.ldo = pl.piece;
-    vl_launch<true, true, VL_DLOG>(pl, p, s);
+    vl_launch<true, true, VL_DLOG>(pl.big_z, p, s);
     if (dhidden) {
       p = VlGemm();
       p.A = dlog; p.lda = pl.piece; p.B = wp; p.ldb = d; p.head = st.head; p.M = (int)pl.m_pad; p.N = d; p.K = min(n, V - v0); p.m_live = 1;
-      p.n_split = pl.split_h; p.slab = slab_h; p.slab_stride = pl.slab_h; p.ldo = d; p.add = i > 0;
-      vl_launch<true, false, VL_SLAB>(pl, p, s);
+      p.n_split = pl.split_h; p.dh_split = 1; p.slab = slab_h; p.slab_stride = pl.slab_h; p.ldo = d; p.add = i > 0;
+      if (pl.n_pieces == 1) { p.dh = (unsigned short*)dhidden; p.idx = st.idx; p.gout = grad_out; }
+      vl_launch<true, false, VL_SLAB>(pl.big_h, p, s);
     }
     if (dweight) {
       p = VlGemm();
@@ -608,19 +665,19 @@ extern "C" int bd_linear_ce_bwd(const void* weight, const float* grad_out, void*
       p.n_split = pl.split_w; p.v0 = v0; p.V = V; p.ldo = d;
       if (pl.split_w > 1) {
         p.slab = slab_w; p.slab_stride = pl.slab_w;
-        vl_launch<false, false, VL_SLAB>(pl, p, s);
+        vl_launch<false, false, VL_SLAB>(pl.big_w, p, s);
         const int rows = min(n, V - v0);
         const long long items = (long long)rows * (d / 8);
         hipLaunchKernelGGL(vl_dw_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, st, slab_w, pl.slab_w, pl.split_w, grad_out,
                            dweight, dweight_dtype == BD_DTYPE_F32, v0, rows, d);
       } else {
         p.gout = grad_out; p.dw = dweight; p.dw_f32 = dweight_dtype == BD_DTYPE_F32;
-        vl_launch<false, false, VL_DW>(pl, p, s);
+        vl_launch<false, false, VL_DW>(pl.big_w, p, s);
       }
     }
   }
   if (dhidden)
-    hipLaunchKernelGGL(vl_dh_kernel, dim3((unsigned)((M * (d / 8) + 255) / 256)), dim3(256), 0, s, st, slab_h, pl.slab_h, pl.split_h, grad_out,
-                       (unsigned short*)dhidden, (int)M, d);
+    hipLaunchKernelGGL(vl_dh_kernel, dim3((unsigned)((M * (d / 8) + 255) / 256)), dim3(256), 0, s, st, slab_h, pl.slab_h, pl.split_h,
+                       pl.big_h ? 256 : 128, min(pl.piece, V), pl.n_pieces, grad_out, (unsigned short*)dhidden, (int)M, d);
   return bd_check_launch("bd_linear_ce_bwd");
 }

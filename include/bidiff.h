@@ -797,7 +797,7 @@ int bd_rotary(const bd_rotary_tensor* tensors, int n_tensors, const float* table
  * Training: lse [rows, H, 2] fp32 (base-2 log-sum-exp of the scaled scores; rows counted through the batch) and, beyond
  * short sequences, maps [rows, H, 2, 2 head_dim] fp32 (each map's own output) are written by the forward and read by
  * the backward (maps may be null in both: the backward then walks the keys once more). Backward: dq, dk, dv bf16 and
- * dlam [rows, H] fp32 are overwritten. Workspaces of bd_diff_attention_workspace_bytes(args, backward) bytes; equal
+ * dlam [rows, H] (bf16 or fp32) are overwritten. Workspaces of bd_diff_attention_workspace_bytes(args, backward) bytes; equal
  * calls give equal bits. Stands beside bd_attention_fwd / bd_attention_bwd. */
 typedef struct {
   const void *q, *k, *v, *lam;
@@ -814,14 +814,14 @@ typedef struct {
   void* workspace;
   long long workspace_bytes;
   const void* dout;
-  void *dq, *dk, *dv;
-  float* dlam;
+  void *dq, *dk, *dv, *dlam;
+  int dlam_dtype;
   long long dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
 } bd_diff_attn_args;
 long long bd_diff_attention_workspace_bytes(const bd_diff_attn_args* args, int backward);
 int bd_diff_attention_fwd(const bd_diff_attn_args* args, void* stream);
 int bd_diff_attention_bwd(const bd_diff_attn_args* args, void* stream);
-/* dlam [B, L, H] fp32 as the backward leaves it, summed over the axes along which lam was broadcast (keep_* = 0), in
+/* dlam [B, L, H] as the backward leaves it in fp32, summed over the axes along which lam was broadcast (keep_* = 0), in
  * out_dtype (BD_DTYPE_*), kept axes in order (packed rows: B = 1). */
 int bd_diff_attention_dlam(const float* dlam, void* out, int out_dtype, int B, int L, int H, int keep_b, int keep_l, int keep_h,
                            void* stream);
