@@ -8,7 +8,7 @@ trainable parameters these raise (training runs through ``DiffusionBackbone`` / 
 dropout is not applied (``eval()`` semantics)."""
 import torch
 
-from .. import _lib
+from .. import _lib, ops
 
 
 def _pad_rows(w: torch.Tensor, mult: int = 128) -> torch.Tensor:
@@ -107,9 +107,101 @@ def _attention_core(mha, a_bf16, keymask, B, L, out_f32, epilogue):
     qkv = torch.empty(M, 3 * d, dtype=torch.bfloat16, device=a_bf16.device)
     _gemm(a_bf16, wqkv, bqkv, qkv, M, 3 * d, d, 0)
     att = torch.empty(M, d, dtype=torch.bfloat16, device=a_bf16.device)
-    _lib.check(_lib.lib().bd_attention_fwd(_lib.ptr(qkv), _lib.ptr(keymask), _lib.ptr(att), None, B, L, H, dh,
-                                           _lib.stream_handle()), "bd_attention_fwd")
+    if mha.rotary_base is not None:
+        turn_positions(mha, qkv.view(B, L, 3 * d), None, dh, L)
+    if mha.differential:
+        differential_heads(qkv.view(B, L, 3 * d), mha, keymask, None, None, dh, att.view(B, L, d), False)
+    else:
+        _lib.check(_lib.lib().bd_attention_fwd(_lib.ptr(qkv), _lib.ptr(keymask), _lib.ptr(att), None, B, L, H, dh,
+                                               _lib.stream_handle()), "bd_attention_fwd")
     _gemm(att, wo, bo, out_f32, M, d, d, epilogue)
+
+
+def split_qkv(qkv, n_maps, dh, differential):
+    """Views of a projection's output [..., 3 * heads * dh]: q and k [..., heads, dh] and v [..., heads, dh], or, for
+    differential attention, v [..., heads / 2, 2 dh] (both heads of a pair)."""
+    q, k, v = qkv.split(n_maps * dh, -1)
+    n_v, w_v = (n_maps // 2, 2 * dh) if differential else (n_maps, dh)
+    return q.unflatten(-1, (n_maps, dh)), k.unflatten(-1, (n_maps, dh)), v.unflatten(-1, (n_v, w_v))
+
+
+def turn_positions(mha, qkv, positions, dh_padded, n_positions, inverse=False):
+    """Rotary positions on the q and k parts of ``qkv`` [B, L, 3 * width] (or packed rows), in place. The head's own
+    values turn (a padded head's zeros behind them stay). The table is kept on the module."""
+    table = mha.__dict__.get("_rotary_table")
+    if table is None or table.device != qkv.device or table.shape[0] < n_positions:
+        table = ops.rotary_table(mha.head_dim, n_positions, base=mha.rotary_base, device=qkv.device)
+        mha.__dict__["_rotary_table"] = table
+    q, k, _ = split_qkv(qkv, mha.num_heads, dh_padded, False)
+    ops._rotary_launch([(q, q), (k, k)], table, positions, False, inverse)
+
+
+def differential_heads(qkv, mha, keymask, cu, longest, dh_padded, out, training):
+    """Differential attention of ``qkv`` [B, L, 3 * width] (or packed rows) into ``out`` [..., width]; returns what the
+    backward reads. The query projection carries sqrt(padded / own head size), as for the softmax kernels."""
+    q, k, v = split_qkv(qkv, mha.num_heads, dh_padded, True)
+    lam = mha.lambda_weight.detach()
+    o = out.unflatten(-1, (mha.num_heads // 2, 2 * dh_padded))
+    return ops._attention_forward(q, k, v, lam, [0, 0, 1], keymask, cu, longest, dh_padded ** -0.5, training, o)[1]
+
+
+def differential_heads_backward(qkv, mha, keymask, cu, longest, dh_padded, saved, dout, dqkv):
+    """Writes ``dqkv``; returns the gradient of ``mha.lambda_weight``."""
+    q, k, v = split_qkv(qkv, mha.num_heads, dh_padded, True)
+    dq, dk, dv = split_qkv(dqkv, mha.num_heads, dh_padded, True)
+    lam = mha.lambda_weight.detach()
+    dl = torch.empty_like(lam)
+    ops._attention_backward(q, k, v, lam, [0, 0, 1], keymask, cu, longest, dh_padded ** -0.5, saved,
+                            dout.unflatten(-1, (mha.num_heads // 2, 2 * dh_padded)), dq, dk, dv, dl)
+    return dl
+
+
+def backbone_forward_blocks(model, ids, timesteps, keymask, want_hidden=True, want_logits=False, hidden_out=None, logits_out=None,
+                            upto=None):
+    """Inference forward of a backbone whose attention the fused launches do not have (differential maps, rotary
+    positions): the per-layer kernels in the training forward's order, nothing kept. Returns (hidden bf16 [B, L, d] or
+    None, logits fp32 or None), or the fp32 residual stream after ``upto`` blocks."""
+    from ..training import autograd as ag
+    ag._enter()
+    B, L = ids.shape
+    M, d, F, V, H = B * L, model.hidden_size, model.ffn_hidden_size, model.vocab_size, model.num_heads
+    if d % 128 or F % 128:
+        raise ValueError("bidiff per-layer forward needs hidden and ffn sizes that are multiples of 128")
+    dev, bf, eps = ids.device, torch.bfloat16, float(model.final_norm.eps)
+    tw = ag._train_weights(model)
+    aw, st = tw.aw, ag._s()
+    x = torch.empty(M, d, device=dev)
+    _lib.check(_lib.lib().bd_embed(_lib.ptr(ids), _lib.ptr(timesteps), _lib.ptr(model.token_embedding.weight),
+                                   _lib.ptr(model.position_embedding.weight), _lib.ptr(model.timestep_embedding.weight), _lib.ptr(x),
+                                   B, L, d, V, model.max_position_embeddings, model.num_diffusion_steps + 1, st), "bd_embed")
+    h = torch.empty(M, d, dtype=bf, device=dev)
+    qkv = torch.empty(M, 3 * aw, dtype=bf, device=dev)
+    att = torch.empty(M, aw, dtype=bf, device=dev)
+    u = torch.empty(M, F, dtype=bf, device=dev)
+    n = len(model.layers) if upto is None else upto
+    for blk, w in list(zip(model.layers, tw.layers))[:n]:
+        ag._ln(x, blk.norm1.weight, blk.norm1.bias, h, None, M, d, eps)
+        ag._gemm(h, w["wqkv"], w["bqkv"], qkv, M, 3 * aw, 3 * aw, d, 3 * aw, 0)
+        if model.rotary_base is not None:
+            turn_positions(blk.attn, qkv.view(B, L, 3 * aw), None, tw.dhp, model.max_position_embeddings)
+        if blk.attn.differential:
+            differential_heads(qkv.view(B, L, 3 * aw), blk.attn, keymask, None, None, tw.dhp, att.view(B, L, aw), False)
+        else:
+            _lib.check(_lib.lib().bd_attention_fwd(_lib.ptr(qkv), _lib.ptr(keymask), _lib.ptr(att), None, B, L, H, tw.dhp, st),
+                       "bd_attention_fwd")
+        ag._gemm(att, w["wo"], blk.attn.out_proj.bias, x, M, d, d, aw, d, 2)
+        ag._ln(x, blk.norm2.weight, blk.norm2.bias, h, None, M, d, eps)
+        ag._gemm(h, w["w1"], blk.ffn.fc1.bias, u, M, F, F, d, F, 1)
+        ag._gemm(u, w["w2"], blk.ffn.fc2.bias, x, M, d, d, F, d, 2)
+    if upto is not None:
+        return x.view(B, L, d)
+    hidden = hidden_out if hidden_out is not None else torch.empty(B, L, d, dtype=bf, device=dev)
+    ag._ln(x, model.final_norm.weight, model.final_norm.bias, hidden, None, M, d, eps)
+    logits = None
+    if want_logits:
+        logits = logits_out if logits_out is not None else torch.empty(B, L, V, device=dev)
+        ag._gemm(hidden, tw.wout, None, logits, M, tw.vpad, V, d, V, 3)
+    return (hidden if want_hidden else None), logits
 
 
 def _ffn_core(ffn, a_bf16, M, out_f32, epilogue):

@@ -20,12 +20,26 @@ from .. import _lib
 
 
 class MultiHeadAttention(nn.Module):
-    """q/k/v/out projections (reference backbone.py:9-78)."""
+    """q/k/v/out projections (reference backbone.py:9-78).
 
-    def __init__(self, hidden_size: int, num_heads: int, dropout: float = 0.1):
+    ``differential``: the heads work in pairs; a pair attends with the difference of its two softmax maps, the second
+    times ``lambda_weight`` (one learned weight a pair), over both heads' values side by side. ``rotary_base``: queries and
+    keys are turned by their positions (``bidiff.ops.rotary``, half layout) before they meet. Both off by default: the
+    reference's attention."""
+
+    def __init__(self, hidden_size: int, num_heads: int, dropout: float = 0.1, differential: bool = False,
+                 rotary_base: Optional[float] = None, depth: int = 0):
         super().__init__()
         if hidden_size % num_heads != 0:
             raise AssertionError("hidden_size must be divisible by num_heads")
+        if differential and num_heads % 2:
+            raise ValueError(f"differential attention pairs the heads: num_heads must be even, got {num_heads}")
+        if rotary_base is not None and (not rotary_base > 0.0 or hidden_size // num_heads % 2):
+            raise ValueError("rotary positions need a positive base and an even head size")
+        self.differential = bool(differential)
+        self.rotary_base = None if rotary_base is None else float(rotary_base)
+        if self.differential:      # deeper layers start with more of the second map taken away
+            self.lambda_weight = nn.Parameter(torch.full((num_heads // 2,), 0.8 - 0.6 * math.exp(-0.3 * depth)))
         self.hidden_size = hidden_size
         self.num_heads = num_heads
         self.head_dim = hidden_size // num_heads
@@ -60,10 +74,11 @@ class FeedForward(nn.Module):
 class TransformerBlock(nn.Module):
     """One pre-norm block (reference backbone.py:104-129)."""
 
-    def __init__(self, hidden_size: int, num_heads: int, ffn_hidden_size: int, dropout: float = 0.1):
+    def __init__(self, hidden_size: int, num_heads: int, ffn_hidden_size: int, dropout: float = 0.1, differential: bool = False,
+                 rotary_base: Optional[float] = None, depth: int = 0):
         super().__init__()
         self.norm1 = nn.LayerNorm(hidden_size)
-        self.attn = MultiHeadAttention(hidden_size, num_heads, dropout)
+        self.attn = MultiHeadAttention(hidden_size, num_heads, dropout, differential, rotary_base, depth)
         self.norm2 = nn.LayerNorm(hidden_size)
         self.ffn = FeedForward(hidden_size, ffn_hidden_size, dropout)
 
@@ -105,7 +120,12 @@ class _Packed:
 
 
 class DiffusionBackbone(nn.Module):
-    """Transformer denoiser for discrete masking diffusion (reference backbone.py:132-377)."""
+    """Transformer denoiser for discrete masking diffusion (reference backbone.py:132-377).
+
+    Beyond the reference: ``attention="differential"`` pairs the heads of every layer (see ``MultiHeadAttention``; the
+    attention maps are then not dropped in training, the other three dropout sites are), ``rotary_base`` turns queries and
+    keys by their positions beside the learned position table. Such models train and sample through the per-layer kernels
+    in bf16 (no single-launch, chosen-row, ragged or fp32 forward)."""
 
     def __init__(
         self,
@@ -118,8 +138,14 @@ class DiffusionBackbone(nn.Module):
         num_diffusion_steps: int = 100,
         dropout: float = 0.1,
         pad_token_id: int = 0,
+        attention: str = "softmax",
+        rotary_base: Optional[float] = None,
     ):
         super().__init__()
+        if attention not in ("softmax", "differential"):
+            raise ValueError(f"attention must be 'softmax' or 'differential', got {attention!r}")
+        self.attention = attention
+        self.rotary_base = rotary_base
         self.vocab_size = vocab_size
         self.hidden_size = hidden_size
         self.num_layers = num_layers
@@ -135,7 +161,8 @@ class DiffusionBackbone(nn.Module):
         self.timestep_embedding = nn.Embedding(num_diffusion_steps + 1, hidden_size)
         self.embedding_dropout = nn.Dropout(dropout)
         self.layers = nn.ModuleList(
-            [TransformerBlock(hidden_size, num_heads, ffn_hidden_size, dropout) for _ in range(num_layers)]
+            [TransformerBlock(hidden_size, num_heads, ffn_hidden_size, dropout, attention == "differential", rotary_base, i)
+             for i in range(num_layers)]
         )
         self.final_norm = nn.LayerNorm(hidden_size)
         self.output_proj = nn.Linear(hidden_size, vocab_size, bias=False)
@@ -169,6 +196,11 @@ class DiffusionBackbone(nn.Module):
             elif isinstance(m, nn.LayerNorm):
                 nn.init.ones_(m.weight)
                 nn.init.zeros_(m.bias)
+
+    @property
+    def plain_attention(self) -> bool:
+        """The reference's attention: every fused forward applies."""
+        return self.attention == "softmax" and self.rotary_base is None
 
     def _next_dropout(self):
         """bd_dropout of the next training forward pass, or None when dropout is off (eval mode or
@@ -440,7 +472,7 @@ class DiffusionBackbone(nn.Module):
         32-row waves of the single-launch forward's workgroups: a sequence takes ceil(length / 32) adjacent waves,
         first-fit by decreasing size. Returns the int32 [n_blocks, 4] table for ``run_forward(wave_table=...)``, or
         None when this model / L has no such launch or the table would not save a tenth of the workgroups."""
-        if self.compute_dtype != "bf16" or L > 128:
+        if self.compute_dtype != "bf16" or L > 128 or not self.plain_attention:
             return None
         pk = self.packed()
         if _lib.lib().bd_backbone_mega_ragged_supported(C.byref(pk.desc), int(L)) != 1:
@@ -472,7 +504,7 @@ class DiffusionBackbone(nn.Module):
         """``ragged_wave_table`` for a [B, L] attention / key mask on the device (its last non-zero column + 1 is a
         sequence's length; one device -> host copy), or None when nothing would be saved."""
         B, L = mask.shape
-        if not (32 < L <= 128) or self.compute_dtype != "bf16" or B == 0:
+        if not (32 < L <= 128) or self.compute_dtype != "bf16" or B == 0 or not self.plain_attention:
             return None
         lens = ((mask != 0) * torch.arange(1, L + 1, device=mask.device)).amax(1)
         if int(lens.min().item()) > (L - 1) // 32 * 32:          # nobody needs fewer waves than the padded length
@@ -489,6 +521,13 @@ class DiffusionBackbone(nn.Module):
         timesteps = self._check_inputs(input_ids, timesteps)
         ids = input_ids.to(torch.long).contiguous()
         B, L = ids.shape
+        if not self.plain_attention:
+            if self.compute_dtype != "bf16":
+                raise NotImplementedError("differential attention and rotary positions run in bf16")
+            if wave_table is not None:
+                raise ValueError("wave_table: differential attention and rotary positions have no ragged forward")
+            from ._blocks import backbone_forward_blocks
+            return backbone_forward_blocks(self, ids, timesteps, keymask, want_hidden, want_logits, hidden_out, logits_out)
         if self.compute_dtype == "fp32":
             # fp32 mode: hidden comes back in fp32 (not the bf16 rows of the fused path)
             hidden, logits = self._forward_fp32(ids, timesteps, keymask, want_hidden, want_logits)
@@ -526,7 +565,7 @@ class DiffusionBackbone(nn.Module):
 
     def rows_forward_supported(self, L) -> bool:
         """Does ``run_forward_rows`` exist for this model and sequence length (the single-launch forward does)?"""
-        if self.compute_dtype != "bf16":
+        if self.compute_dtype != "bf16" or not self.plain_attention:
             return False
         return _lib.lib().bd_backbone_forward_rows_supported(C.byref(self.packed().desc), int(L)) == 1
 
@@ -534,7 +573,7 @@ class DiffusionBackbone(nn.Module):
         """Which chosen-row forward this model has for a [B, L] batch: "single_launch" (``need_all`` handled on the
         device), "per_layer" (large models on the per-layer kernels: the caller runs the full forward for a step that
         flagged a sequence in ``need_all``), or None."""
-        if self.compute_dtype != "bf16":
+        if self.compute_dtype != "bf16" or not self.plain_attention:
             return None
         desc = C.byref(self.packed().desc)
         if _lib.lib().bd_backbone_forward_rows_supported(desc, int(L)) == 1:
@@ -548,6 +587,8 @@ class DiffusionBackbone(nn.Module):
         final-norm rows at positions ``row_pos`` [B * row_cap] (int32, -1 = none) and every row of the sequences
         flagged in ``need_all`` [B] (uint8); its other rows keep what they held (``bd_sample_choose_rows`` writes
         both lists). The rows written equal ``run_forward``'s bit for bit."""
+        if not self.plain_attention:
+            raise NotImplementedError("differential attention and rotary positions have no chosen-row forward")
         timesteps = self._check_inputs(input_ids, timesteps)
         ids = input_ids.to(torch.long).contiguous()
         B, L = ids.shape
@@ -615,6 +656,12 @@ class DiffusionBackbone(nn.Module):
                 raise IndexError(f"layer_idx {layer_idx} out of range for {self.num_layers} layers")
             timesteps = self._check_inputs(input_ids, timesteps)
             B, L = input_ids.shape
+            if not self.plain_attention:
+                if self.compute_dtype != "bf16":
+                    raise NotImplementedError("differential attention and rotary positions run in bf16")
+                from ._blocks import backbone_forward_blocks
+                return backbone_forward_blocks(self, input_ids.to(torch.long).contiguous(), timesteps, keymask, False, False,
+                                               upto=layer_idx + 1)
             if self.compute_dtype == "fp32":
                 return self._forward_fp32(input_ids.to(torch.long).contiguous(), timesteps, keymask, False, False,
                                           upto=layer_idx + 1)[0]
@@ -689,6 +736,8 @@ class DiffusionBackbone(nn.Module):
             "num_diffusion_steps": self.num_diffusion_steps,
             "dropout": self.dropout,
             "pad_token_id": self.pad_token_id,
+            **({} if self.attention == "softmax" else {"attention": self.attention}),
+            **({} if self.rotary_base is None else {"rotary_base": self.rotary_base}),
         }
 
     def save_pretrained(self, path: str):

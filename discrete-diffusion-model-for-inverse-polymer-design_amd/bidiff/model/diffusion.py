@@ -101,6 +101,10 @@ class DiscreteMaskingDiffusion(nn.Module):
         # training forward: leave out the rows behind each sequence's last attended position (no loss, no gradient
         # and no influence on other rows comes from them; the returned logits are zero there). False = every row.
         self.skip_padded_rows = True
+        # True: the loss is computed from the final hidden rows without storing logits (bidiff.ops.linear_cross_entropy),
+        # forward and backward, in training and without autograd; "logits" is then built when it is first read. The loss
+        # is that of the logits to fp32 rounding. Off by default.
+        self.fused_head_loss = False
         self.register_buffer("mask_schedule", self._compute_mask_schedule())
 
     def _compute_mask_schedule(self) -> torch.Tensor:
@@ -169,6 +173,20 @@ class DiscreteMaskingDiffusion(nn.Module):
             from ..training.autograd import packed_training_loss
             loss, logits = packed_training_loss(self, noisy_ids, bb._check_inputs(noisy_ids, timesteps), attention_mask,
                                                 input_ids, mask_indicator, lengths)
+            return _Outputs({"loss": loss, "noisy_ids": noisy_ids, "mask_indicator": mask_indicator,
+                             "timesteps": timesteps}, {"logits": logits})
+        if self.fused_head_loss and getattr(bb, "compute_dtype", "bf16") == "bf16":
+            from .. import ops
+            from ..training import autograd as ag
+            if torch.is_grad_enabled() and any(p.requires_grad for p in bb.parameters()):
+                hidden = ag.backbone_forward_train(bb, noisy_ids, timesteps, attention_mask, hidden_states="bf16")
+            else:
+                hidden, _ = bb.run_forward(noisy_ids, timesteps, bb._keymask_bytes(attention_mask, noisy_ids))
+            loss = ops.linear_cross_entropy(hidden, bb.output_proj.weight, input_ids.to(torch.long), mask_indicator, attention_mask)
+
+            def logits():
+                with torch.no_grad():
+                    return ag.head_logits(bb, hidden.detach())
             return _Outputs({"loss": loss, "noisy_ids": noisy_ids, "mask_indicator": mask_indicator,
                              "timesteps": timesteps}, {"logits": logits})
         logits = self.backbone(noisy_ids, timesteps, attention_mask)

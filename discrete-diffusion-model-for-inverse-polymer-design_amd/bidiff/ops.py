@@ -287,11 +287,12 @@ def _lam_strides(lam, lead, H):
     return st
 
 
-def _attention_forward(q, k, v, lam, lam_strides, key_mask, cu, longest, scale, training):
+def _attention_forward(q, k, v, lam, lam_strides, key_mask, cu, longest, scale, training, out=None):
     sizes = _attention_sizes(q, k, v, cu, longest)
     _, _, Lk, H, _, D, _, rows = sizes
     dev = q.device
-    out = torch.empty(*q.shape[:-2], H, 2 * D, dtype=torch.bfloat16, device=dev)
+    if out is None:
+        out = torch.empty(*q.shape[:-2], H, 2 * D, dtype=torch.bfloat16, device=dev)
     ws_bytes = _attention_workspace(*sizes, False)
     # one allocation for what the backward reads (log-sum-exps, then the maps), one for scratch
     saved = ws = None
@@ -309,6 +310,27 @@ def _attention_forward(q, k, v, lam, lam_strides, key_mask, cu, longest, scale, 
     return out, saved
 
 
+def _attention_backward(q, k, v, lam, lam_strides, key_mask, cu, longest, scale, saved, dout, dq, dk, dv, dlam):
+    """Writes dq, dk, dv (any strides the kernels take) and dlam (lam's shape and dtype, contiguous)."""
+    sizes = _attention_sizes(q, k, v, cu, longest)
+    _, _, Lk, H, _, _, packed, rows = sizes
+    # a weight for every (row, head): its gradient is written as it comes; one that was broadcast: summed from fp32
+    whole = lam.numel() == rows * H
+    need = (_attention_workspace(*sizes, True) + 15) // 16 * 16
+    ws = torch.empty(need + (0 if whole else 4 * rows * H), dtype=torch.uint8, device=q.device)
+    wp, lse = ws.data_ptr(), saved.data_ptr()
+    maps = lse + 4 * ((rows * H * 2 + 3) // 4 * 4) if Lk > _MAPS_KEYS else 0
+    with _on(q.device) as stream:
+        _attention_call("bd_diff_attention_bwd", sizes, q, k, v, lam, lam_strides, key_mask, cu, scale, None, lse, maps, wp, need,
+                        (dout, dq, dk, dv, dlam.data_ptr() if whole else wp + need, _DTYPES[lam.dtype] if whole else 1), stream)
+        if not whole:
+            lead = (1, rows) if packed else q.shape[:2]
+            shape = (1,) * (3 - lam.dim()) + tuple(lam.shape)
+            _lib.check(_lib.lib().bd_diff_attention_dlam(wp + need, dlam.data_ptr(), _DTYPES[lam.dtype], lead[0], lead[1], H,
+                                                         shape[0] == lead[0], shape[1] == lead[1], shape[2] == H, stream),
+                       "bd_diff_attention_dlam")
+
+
 class _DiffAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lam, lam_strides, key_mask, cu, longest, scale):
@@ -321,28 +343,11 @@ class _DiffAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, lam, key_mask, cu, saved = ctx.saved_tensors
-        sizes = _attention_sizes(q, k, v, cu, ctx.longest)
-        _, _, Lk, H, _, _, packed, rows = sizes
         dev = q.device
-        dout = _rows_of_16_bytes(dout)
         dq, dk, dv = (torch.empty(t.shape, dtype=torch.bfloat16, device=dev) for t in (q, k, v))
         dl = torch.empty(lam.shape, dtype=lam.dtype, device=dev)
-        # a weight for every (row, head): its gradient is written as it comes; one that was broadcast: summed from fp32
-        whole = lam.numel() == rows * H
-        need = (_attention_workspace(*sizes, True) + 15) // 16 * 16
-        ws = torch.empty(need + (0 if whole else 4 * rows * H), dtype=torch.uint8, device=dev)
-        wp = ws.data_ptr()
-        lse = saved.data_ptr()
-        maps = lse + 4 * ((rows * H * 2 + 3) // 4 * 4) if Lk > _MAPS_KEYS else 0
-        with _on(dev) as stream:
-            _attention_call("bd_diff_attention_bwd", sizes, q, k, v, lam, ctx.lam_strides, key_mask, cu, ctx.scale, None, lse, maps,
-                            wp, need, (dout, dq, dk, dv, dl.data_ptr() if whole else wp + need, _DTYPES[lam.dtype] if whole else 1), stream)
-            if not whole and ctx.needs_input_grad[3]:
-                lead = (1, rows) if packed else q.shape[:2]
-                shape = (1,) * (3 - lam.dim()) + tuple(lam.shape)
-                _lib.check(_lib.lib().bd_diff_attention_dlam(wp + need, dl.data_ptr(), _DTYPES[lam.dtype], lead[0], lead[1], H,
-                                                             shape[0] == lead[0], shape[1] == lead[1], shape[2] == H, stream),
-                           "bd_diff_attention_dlam")
+        _attention_backward(q, k, v, lam, ctx.lam_strides, key_mask, cu, ctx.longest, ctx.scale, saved, _rows_of_16_bytes(dout),
+                            dq, dk, dv, dl)
         return dq, dk, dv, dl, None, None, None, None, None
 
 

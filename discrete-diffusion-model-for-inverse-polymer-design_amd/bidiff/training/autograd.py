@@ -251,6 +251,12 @@ class RowPacking:
         last = L - am.flip(1).to(torch.int8).argmax(dim=1)
         return torch.where(am.any(dim=1), last, torch.zeros_like(last)).cpu().numpy()
 
+    def positions(self):
+        """int64 position of each packed row inside its sequence (fillers: 0)."""
+        if getattr(self, "_positions", None) is None:
+            self._positions = self.rowmap.to(torch.long).clamp(min=0) % self.L
+        return self._positions
+
     def gather_index(self):
         """int64 index of each packed row's logical token (fillers point at token 0) and the filler mask."""
         if self._gather is None:
@@ -411,7 +417,9 @@ class _BackboneFn(torch.autograd.Function):
     def forward(ctx, model, ids, timesteps, keymask, mode, pk, *params):
         """mode 0: logits [B, L, V] (the diffusion training step); mode 1: the final-norm hidden states
         [B, L, d] in fp32 (what get_hidden_states / get_pooled_output return to a property head that
-        fine-tunes the last blocks, reference property_head.py:102-112)."""
+        fine-tunes the last blocks, reference property_head.py:102-112); mode 2: the same rows in bf16, as the
+        vocabulary head reads them."""
+        from ..model import _blocks as blocks
         _enter()
         lib = _lib.lib()
         B, L = ids.shape
@@ -450,8 +458,18 @@ class _BackboneFn(torch.autograd.Function):
             s["qkv"] = torch.empty(M, 3 * aw, dtype=bf, device=dev)
             _gemm(s["h1"], w["wqkv"], w["bqkv"], s["qkv"], M, 3 * aw, 3 * aw, d, 3 * aw, 0)
             s["att"] = att_all[li]
-            s["lse"] = torch.empty(B, H, L, device=dev)
-            if pk is None:
+            if model.rotary_base is not None:
+                blocks.turn_positions(blk.attn, s["qkv"] if pk is not None else s["qkv"].view(B, L, 3 * aw),
+                                      None if pk is None else pk.positions(), aw // H, model.max_position_embeddings)
+            if blk.attn.differential:
+                rows = (M,) if pk is not None else (B, L)
+                s["lse"] = blocks.differential_heads(s["qkv"].view(*rows, 3 * aw), blk.attn, keymask, None if pk is None else pk.cu, L,
+                                                     aw // H, s["att"].view(*rows, aw), True)
+            else:
+                s["lse"] = torch.empty(B, H, L, device=dev)
+            if blk.attn.differential:
+                pass
+            elif pk is None:
                 _ck(lib.bd_attention_fwd_drop(_lib.ptr(s["qkv"]), _lib.ptr(keymask), _lib.ptr(s["att"]), _lib.ptr(s["lse"]),
                                               B, L, H, aw // H, _dp(drop), 4 * li + 1, _s()), "bd_attention_fwd")
             else:
@@ -477,6 +495,11 @@ class _BackboneFn(torch.autograd.Function):
         stf = torch.empty(M, 2, device=dev)
         ctx.model, ctx.saved, ctx.tw, ctx.drop, ctx.mode, ctx.pk = model, saved, tw, drop, int(mode), pk
         ctx.ids, ctx.timesteps, ctx.keymask = ids, timesteps, keymask
+        if mode == 2:
+            hf = torch.empty(M, d, dtype=bf, device=dev)
+            _ln(x, model.final_norm.weight, model.final_norm.bias, hf, stf, M, d, eps)
+            ctx.x_last, ctx.stf, ctx.hf = x, stf, None
+            return hf if pk is not None else hf.view(B, L, d)
         if mode == 1:
             hid = torch.empty(B, L, d, device=dev) if pk is None else torch.empty(M, d, device=dev)
             _ck(lib.bd_layernorm(_lib.ptr(x), _lib.ptr(model.final_norm.weight), _lib.ptr(model.final_norm.bias), None,
@@ -492,6 +515,7 @@ class _BackboneFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dlogits):
+        from ..model import _blocks as blocks
         _enter()
         lib = _lib.lib()
         model, tw, drop, pk = ctx.model, ctx.tw, ctx.drop, ctx.pk
@@ -522,7 +546,9 @@ class _BackboneFn(torch.autograd.Function):
 
         dh_buf = torch.empty(M, d, dtype=bf, device=dev)
         head_job = None
-        if ctx.mode == 1:
+        if ctx.mode == 2:
+            dh_buf = dlogits.reshape(M, d).contiguous()
+        elif ctx.mode == 1:
             # the incoming gradient is that of the final-norm output itself
             _to_bf16(dlogits.reshape(M, d).float().contiguous(), dh_buf)
         else:
@@ -661,7 +687,12 @@ class _BackboneFn(torch.autograd.Function):
             wgrad_side(li, dy2, s["att"], tw.pad_views[li]["o"] if padded else gbuf(a.out_proj.weight), d, aw,
                        gbuf(a.out_proj.bias))
             _gemm(dy2, w["woT"], None, datt, M, aw, aw, d, aw, 0)
-            if pk is None:
+            if a.differential:
+                rows = (M,) if pk is not None else (B, L)
+                dlam = blocks.differential_heads_backward(s["qkv"].view(*rows, 3 * aw), a, keymask, None if pk is None else pk.cu, L, dhp,
+                                                          s["lse"], datt.view(*rows, aw), dqkv.view(*rows, 3 * aw))
+                gbuf(a.lambda_weight).add_(dlam)
+            elif pk is None:
                 _ck(lib.bd_attention_bwd_drop(_lib.ptr(s["qkv"]), _lib.ptr(keymask), _lib.ptr(s["att"]), _lib.ptr(datt),
                                               _lib.ptr(s["lse"]), _lib.ptr(delta), _lib.ptr(dqkv), B, L, H, aw // H,
                                               _dp(drop), 4 * li + 1, _s()), "bd_attention_bwd")
@@ -669,6 +700,9 @@ class _BackboneFn(torch.autograd.Function):
                 _ck(lib.bd_attention_bwd_varlen(_lib.ptr(s["qkv"]), _lib.ptr(keymask), _lib.ptr(s["att"]), _lib.ptr(datt),
                                                 _lib.ptr(s["lse"]), _lib.ptr(delta), _lib.ptr(dqkv), _lib.ptr(pk.cu), B, L,
                                                 H, aw // H, _dp(drop), 4 * li + 1, _s()), "bd_attention_bwd_varlen")
+            if model.rotary_base is not None:          # the gradient turns back
+                blocks.turn_positions(a, dqkv if pk is not None else dqkv.view(B, L, 3 * aw), None if pk is None else pk.positions(), dhp,
+                                      model.max_position_embeddings, inverse=True)
             projs = (a.q_proj, a.k_proj, a.v_proj)
             if not padded:      # the three row segments of the stacked gradient, one launch
                 wgrad_side(li, dqkv, s["h1"], [gbuf(pr.weight) for pr in projs], 3 * aw, d, [gbuf(pr.bias) for pr in projs])
@@ -714,8 +748,8 @@ class _BackboneFn(torch.autograd.Function):
 
 
 def backbone_forward_train(model, input_ids, timesteps, attention_mask, hidden_states=False, packing=None):
-    """Training forward: logits, or (``hidden_states=True``) the fp32 final-norm hidden states. With a
-    ``RowPacking`` the result holds the packed rows ([n_rows, V] or [n_rows, d]) instead of [B, L, .]."""
+    """Training forward: logits, or (``hidden_states=True``) the fp32 final-norm hidden states (``"bf16"``: the rows the
+    vocabulary head reads). With a ``RowPacking`` the result holds the packed rows ([n_rows, V] or [n_rows, d]) instead of [B, L, .]."""
     _lib.require_device(input_ids, "DiffusionBackbone.forward")
     if model.hidden_size % 128 or model.ffn_hidden_size % 128:
         raise ValueError("bidiff training path needs hidden and ffn sizes that are multiples of 128")
@@ -727,7 +761,8 @@ def backbone_forward_train(model, input_ids, timesteps, attention_mask, hidden_s
             raise RuntimeError("bidiff training path expects contiguous fp32 parameters")
     if packing is not None and (packing.B, packing.L) != tuple(ids.shape):
         raise ValueError("RowPacking was built for another batch shape")
-    return _BackboneFn.apply(model, ids, timesteps, keymask, 1 if hidden_states else 0, packing, *model._params())
+    mode = 2 if hidden_states == "bf16" else 1 if hidden_states else 0
+    return _BackboneFn.apply(model, ids, timesteps, keymask, mode, packing, *model._params())
 
 
 class _MaskedCE(torch.autograd.Function):
@@ -772,6 +807,17 @@ def masked_cross_entropy(logits, targets, mask_indicator, attention_mask=None):
     return _MaskedCE.apply(logits, targets, mask_indicator, attention_mask)
 
 
+def head_logits(model, hidden):
+    """fp32 logits [..., V] of bf16 final-norm rows [..., d] (the vocabulary head's product on its own)."""
+    _enter()
+    tw = _train_weights(model)
+    d, V = hidden.shape[-1], model.vocab_size
+    rows = hidden.reshape(-1, d).contiguous()
+    logits = torch.empty(*hidden.shape[:-1], V, device=hidden.device)
+    _gemm(rows, tw.wout, None, logits, rows.shape[0], tw.vpad, V, d, V, 3)
+    return logits
+
+
 def packed_training_loss(diffusion, noisy_ids, timesteps, attention_mask, targets, mask_indicator, lengths=None):
     """Denoiser + masked CE on the packed rows of the batch. Returns (loss, logits): the loss and its gradients
     equal the padded computation's (padded rows contribute to neither); ``logits()`` builds the [B, L, V] logits, a
@@ -782,7 +828,8 @@ def packed_training_loss(diffusion, noisy_ids, timesteps, attention_mask, target
     if lengths is None:
         lengths = RowPacking.lengths_from_mask(attention_mask)
     pk = RowPacking(lengths, B, L, noisy_ids.device)
-    logits_p = backbone_forward_train(backbone, noisy_ids, timesteps, attention_mask, packing=pk)
+    fused = bool(getattr(diffusion, "fused_head_loss", False))
+    rows_p = backbone_forward_train(backbone, noisy_ids, timesteps, attention_mask, hidden_states="bf16" if fused else False, packing=pk)
     # targets and loss flags of the packed rows (attention mask folded into the flag, fillers flagged off): one launch
     tg = torch.empty(pk.n_rows, dtype=torch.long, device=noisy_ids.device)
     ind = torch.empty(pk.n_rows, dtype=torch.uint8, device=noisy_ids.device)
@@ -792,13 +839,18 @@ def packed_training_loss(diffusion, noisy_ids, timesteps, attention_mask, target
     am_src = attention_mask.to(torch.long).contiguous()
     _ck(_lib.lib().bd_pack_targets(_lib.ptr(tg_src), _lib.ptr(ind_src), _lib.ptr(am_src), _lib.ptr(pk.rowmap), pk.n_rows,
                                    _lib.ptr(tg), _lib.ptr(ind), _s()), "bd_pack_targets")
-    loss = masked_cross_entropy(logits_p, tg, ind, None)
+    if fused:
+        from .. import ops
+        loss = ops.linear_cross_entropy(rows_p, backbone.output_proj.weight, tg, ind)
+    else:
+        loss = masked_cross_entropy(rows_p, tg, ind, None)
 
     def full_logits():
         """[B, L, V] copy of the packed logits, zeros at the rows that were left out (built when somebody asks)."""
         with torch.no_grad():
             idx, _ = pk.gather_index()
+            logits_p = head_logits(backbone, rows_p.detach()) if fused else rows_p.detach()
             full = torch.zeros(B * L, logits_p.shape[-1], device=logits_p.device, dtype=logits_p.dtype)
-            full.index_copy_(0, idx[:pk.n_real], logits_p.detach()[:pk.n_real])
+            full.index_copy_(0, idx[:pk.n_real], logits_p[:pk.n_real])
         return full.view(B, L, -1)
     return loss, full_logits

@@ -139,3 +139,34 @@ def linear_cross_entropy(hidden, weight, targets, w, gout=1.0, tol=False):
         res["dh_tol"][live] = abs(c) * (edz @ e.abs() + (dz.abs() @ e.abs()) * V * F) + U * 1.01 * res["dh"][live].abs()
         res["dw_tol"] = abs(c) * (edz.t() @ x.abs() + (dz.abs().t() @ x.abs()) * n * F) + U * 1.01 * res["dw"].abs()
     return res
+
+
+# ---------------------------------------------------------------- a block's attention with both
+def block_attention(rotary_base):
+    """``backbone_ref.attention`` with rotary positions (half layout, base ``rotary_base`` or None) and, where the state
+    dict holds ``lambda_weight``, differential maps. Differentiable torch, any dtype."""
+    import torch.nn.functional as Fn
+
+    def attention(x, sd, prefix, num_heads, attention_mask, dropout=None, site=0):
+        B, L, d = x.shape
+        dh = d // num_heads
+        q, k, v = (Fn.linear(x, sd[f"{prefix}.{n}_proj.weight"], sd[f"{prefix}.{n}_proj.bias"]).view(B, L, num_heads, dh) for n in "qkv")
+        if rotary_base is not None:
+            ang = torch.arange(L, dtype=torch.float64)[:, None] * rotary_base ** (-2.0 * torch.arange(dh // 2, dtype=torch.float64) / dh)
+            cos, sin = ang.cos().to(x.dtype)[:, None, :], ang.sin().to(x.dtype)[:, None, :]
+
+            def turn(t):
+                a, b = t[..., :dh // 2], t[..., dh // 2:]
+                return torch.cat([a * cos - b * sin, a * sin + b * cos], -1)
+            q, k = turn(q), turn(k)
+        s = torch.einsum("blhd,bmhd->bhlm", q, k) / math.sqrt(dh)
+        if attention_mask is not None:
+            s = s.masked_fill(~attention_mask.to(torch.bool)[:, None, None, :], -math.inf)
+        p = torch.nan_to_num(torch.softmax(s, -1), nan=0.0)
+        lam = sd.get(f"{prefix}.lambda_weight")
+        if lam is not None:
+            p = p[:, 0::2] - lam[None, :, None, None] * p[:, 1::2]
+            v = v.reshape(B, L, num_heads // 2, 2 * dh)
+        out = torch.einsum("bhlm,bmhd->blhd", p, v).reshape(B, L, d)
+        return Fn.linear(out, sd[f"{prefix}.out_proj.weight"], sd[f"{prefix}.out_proj.bias"])
+    return attention
