@@ -68,9 +68,9 @@ typedef __attribute__((address_space(3))) s16x4 da_lds_b64;
 template <int R>
 __device__ __forceinline__ unsigned da_nat_base(int g, int c) { return (unsigned)da_off<R>(8 * (c >> 2) + (c & 3), g); }
 template <int R>
-__device__ __forceinline__ bf16x8 da_nat(unsigned base, int h2, int half, int ks) {
+__device__ __forceinline__ bf16x8 da_nat(unsigned base, int h2, int half, int ks, int region = 0) {
   const unsigned flip = (R >= 128 && half ? 16u : 0u) | (64u * (unsigned)(ks & (R >= 256 ? 3 : 1)));
-  const unsigned add = (32 * h2 + 4 * half) * R + (R == 512 ? 256 * (ks >> 2) : 0);
+  const unsigned add = region + (32 * h2 + 4 * half) * R + (R == 512 ? 256 * (ks >> 2) : 0);
   return *(da_lds_b128*)(size_t)((base ^ flip) + add);
 }
 // transposed: 8 rows (32 h2 + 8 g ..) x 16 columns (16 dt ..) as an operand whose summed axis runs along the rows
@@ -79,14 +79,39 @@ __device__ __forceinline__ unsigned da_tr_base(int g, int c) {
   return (unsigned)(da_off<R>(8 * g + (c >> 2), (c & 3) >> 1) + 8 * (c & 1));
 }
 template <int R>
-__device__ __forceinline__ bf16x8 da_tr(unsigned base, int h2, int dt) {
+__device__ __forceinline__ bf16x8 da_tr(unsigned base, int h2, int dt, int region = 0) {
   const unsigned flip = 32u * (unsigned)(dt & (R >= 256 ? 7 : R == 128 ? 3 : 1));
-  const unsigned add = 32 * h2 * R + (R == 512 ? 256 * (dt >> 3) : 0);
+  const unsigned add = region + 32 * h2 * R + (R == 512 ? 256 * (dt >> 3) : 0);
   union { struct { s16x4 a, b; } s; bf16x8 v; } u;
   u.s.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_lds_b64*)(size_t)((base ^ flip) + add));
   u.s.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((da_lds_b64*)(size_t)((base ^ (flip | (R >= 128 ? 16u : 0u))) + add + 4 * R));
   return u.v;
 }
+
+// N operand fragments and the products each feeds, with AHEAD fragments read in advance: reads and products keep this order
+// (arithmetic may move between them). Left to itself the compiler reads a fragment, waits out the LDS latency and
+// multiplies, fragment by fragment, where registers are short (head size 128, 2 x 4096 x 8 heads: forward 432 -> 385 us,
+// dkv 819 -> 715; four deep for dkv, 2 and 3 gave 774 and 719).
+template <int AHEAD, int N, typename Load, typename Mul>
+__device__ __forceinline__ void da_pipe(Load load, Mul mul) {
+  constexpr int A = AHEAD < N ? AHEAD : N;
+  bf16x8 f[A];
+#pragma unroll
+  for (int i = 0; i < A; ++i) f[i] = load(i);
+  __builtin_amdgcn_sched_barrier(0x6);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    mul(i, f[i % A]);
+    if (i + A < N) f[i % A] = load(i + A);
+    __builtin_amdgcn_sched_barrier(0x6);
+  }
+}
+
+// Operands loaded into registers ahead of the staging loop pass through here: the compiler then waits for them once, now.
+// Left to itself it puts the wait in front of their first use inside the loop, where every turn would wait for the tile
+// just asked for as well (the loads' counter is one, and the compiler does not see the staging).
+template <typename V>
+__device__ __forceinline__ void da_landed(V& v) { asm volatile("" : "+v"(v)); }
 
 __device__ __forceinline__ void da_dma16(const void* src, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
@@ -167,6 +192,8 @@ struct DaKeyStage {
   }
 };
 
+__device__ __forceinline__ float da_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 struct DaSpan {          // one sequence: first row of queries / keys, their counts, the batch index for strides
   long long q0, k0;
   int Lq, Lk;
@@ -182,6 +209,23 @@ __device__ __forceinline__ DaSpan da_span(const DaArgs& a, int b) {
     s.q0 = 0; s.k0 = 0; s.Lq = a.Lq; s.Lk = a.Lk;
   }
   return s;
+}
+
+struct DaSlot { int row, head; bool ok; };     // (slots behind the last: the last one, ok = false)
+
+__device__ __forceinline__ DaSlot da_slot(const DaArgs& a, int s, int n_slots, int hk) {
+  DaSlot r;
+  r.ok = s < n_slots;
+  s = r.ok ? s : n_slots - 1;
+  r.row = s / a.share;
+  r.head = hk * a.share + (s - r.row * a.share);
+  return r;
+}
+// A value the compiler cannot connect with earlier ones: what is derived from it behind a loop is computed there instead of
+// being held in registers through it.
+__device__ __forceinline__ int da_again(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 __device__ __forceinline__ float da_lam(const DaArgs& a, long long off) {
@@ -208,7 +252,7 @@ __device__ __forceinline__ int da_visible_end(const DaArgs& a, int b, int Lk, in
       const unsigned long long v = __ballot(x[i] != 0);
       last = v ? 64 * i + 64 - __builtin_clzll(v) : last;
     }
-    return last;
+    return __builtin_amdgcn_readfirstlane(last);
   }
   for (int j = tid; j < Lk; j += NT) last = m[j] ? j + 1 : last;
 #pragma unroll
@@ -218,14 +262,15 @@ __device__ __forceinline__ int da_visible_end(const DaArgs& a, int b, int Lk, in
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) last = max(last, red[w]);
   __syncthreads();
-  return last;
+  return __builtin_amdgcn_readfirstlane(last);      // (one value: the loops over key tiles count on the scalar unit)
 }
 
 // mask byte of the lane's key of a tile (0 past the end); a volatile load stays where it is written
 __device__ __forceinline__ unsigned da_mask_byte(const DaArgs& a, int b, int key, int end) {
   if (key >= end) return 0u;
   if (!a.mask) return 1u;
-  return *(const volatile unsigned char*)(a.mask + b * a.mask_stride + key);
+  typedef __attribute__((address_space(1))) const volatile unsigned char global_byte;      // (a generic load would count as an LDS read)
+  return *(global_byte*)(a.mask + b * a.mask_stride + key);
 }
 
 // Workgroups are handed to the 8 XCDs in turn (blockIdx & 7). The blocks of one (sequence, key head) group share an XCD, so
@@ -245,8 +290,10 @@ __device__ __forceinline__ bool da_block(int n_blk, int n_heads, int seqs, int& 
     blk = lin % n_blk;
     grp = lin / n_blk;
   }
-  hk = grp % n_heads;
-  b = grp / n_heads;
+  // (the divisions ran on the vector unit: tell the compiler that every lane holds the same)
+  blk = __builtin_amdgcn_readfirstlane(blk);
+  hk = __builtin_amdgcn_readfirstlane(grp % n_heads);
+  b = __builtin_amdgcn_readfirstlane(grp / n_heads);
   return true;
 }
 inline long long da_grid(long long n_blk, long long groups) { return n_blk * ((groups + 7) / 8) * 8; }
@@ -267,7 +314,7 @@ __device__ __forceinline__ void da_zero_tail(unsigned short* p, const long long*
 // =====================================================================================
 template <int D, int QB, int NQG, int OCC>
 __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
-  constexpr int E = 2 * D, KS = D / 32, DT = E / 16, NW = 2 * NQG, RK = 2 * D, RV = 2 * E;
+  constexpr int E = 2 * D, AF = D == 128 ? 3 : 6, KS = D / 32, DT = E / 16, NW = 2 * NQG, RK = 2 * D, RV = 2 * E;
   constexpr int TILE = KT * (2 * RK + RV), SLOTS = 16 * QB * NQG;
   extern __shared__ __attribute__((aligned(1024))) unsigned char da_smem[];
   __shared__ int red[NW];
@@ -305,18 +352,12 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
   }
 
   // the lane's slots (column c of each block) and their query fragments
-  const int s0 = blk * SLOTS + grp * 16 * QB;
-  int row[QB], head[QB];
-  bool ok[QB];
+  const int s0 = blk * SLOTS + grp * 16 * QB + c;
   bf16x8 qf[QB][KS];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    int s = s0 + 16 * qb + c;
-    ok[qb] = s < n_slots;
-    s = ok[qb] ? s : n_slots - 1;
-    row[qb] = s / a.share;
-    head[qb] = hk * a.share + (s - row[qb] * a.share);
-    const unsigned short* qp = a.q + bq * a.qs[0] + (sp.q0 + row[qb]) * a.qs[1] + (2 * head[qb] + map) * a.qs[2] + 8 * g;
+    const DaSlot sl = da_slot(a, s0 + 16 * qb, n_slots, hk);
+    const unsigned short* qp = a.q + bq * a.qs[0] + (sp.q0 + sl.row) * a.qs[1] + (2 * sl.head + map) * a.qs[2] + 8 * g;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[qb][ks] = *(const bf16x8*)(qp + 32 * ks);
   }
@@ -332,6 +373,10 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
 
   DaKeyStage<D, NW> keys;
   keys.init(a, bq, sp.k0, hk, wave, lane);
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) da_landed(qf[qb][ks]);
   const unsigned lds0 = (unsigned)(size_t)(da_lds*)da_smem;
   const unsigned kbase = da_nat_base<RK>(g, c) + map * KT * RK, vbase = da_tr_base<RV>(g, c) + 2 * KT * RK;
   unsigned mb = da_mask_byte(a, b, kbeg + lane, kend);
@@ -349,16 +394,15 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
     // S^T: s[qb][t][r] <-> key 32 (t >> 1) + 8 g + 4 (t & 1) + r of the tile, slot c of block qb
     f32x4 s[QB][4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) s[qb][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < 4; ++t) s[qb][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    da_pipe<AF, 4 * KS>([&](int i) { return da_nat<RK>(kb, i / KS >> 1, i / KS & 1, i % KS); },
+                    [&](int i, bf16x8 kf) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const bf16x8 kf = da_nat<RK>(kb, t >> 1, t & 1, ks);
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) s[qb][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[qb][ks], s[qb][t], 0, 0, 0);
-      }
-    }
+                      for (int qb = 0; qb < QB; ++qb)
+                        s[qb][i / KS] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[qb][i % KS], s[qb][i / KS], 0, 0, 0);
+                    });
     bf16x8 pf[QB][2];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
@@ -371,9 +415,10 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
             if (!((m4 >> r) & 1u)) s[qb][t][r] = -INFINITY;
         }
       }
-      float mloc = -INFINITY;
+      // (the IEEE maximum of three values is one instruction here; fmaxf would first quiet each product's result)
+      float mloc = da_max(s[qb][0][0], s[qb][0][1]);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) mloc = fmaxf(fmaxf(mloc, fmaxf(s[qb][t][0], s[qb][t][1])), fmaxf(s[qb][t][2], s[qb][t][3]));
+      for (int i = 2; i < 16; i += 2) mloc = da_max(mloc, da_max(s[qb][i >> 2][i & 3], s[qb][i >> 2][(i & 3) + 1]));
       // The reference of the exponentials follows the maximum only when a score passes it by 2^8: weights then reach 2^8 at
       // most (no less exact in bf16 and fp32), and almost every tile goes without the exchange between a slot's four lanes
       // and without rescaling.
@@ -401,14 +446,12 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
         }
     }
     // O^T += V^T P^T
+    da_pipe<AF, 2 * DT>([&](int i) { return da_tr<RV>(vb, i & 1, i >> 1); },
+                    [&](int i, bf16x8 vf) {
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        const bf16x8 vf = da_tr<RV>(vb, h2, dt);
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) o[qb][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qb][h2], o[qb][dt], 0, 0, 0);
-      }
+                      for (int qb = 0; qb < QB; ++qb)
+                        o[qb][i >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qb][i & 1], o[qb][i >> 1], 0, 0, 0);
+                    });
     vis = vis_next;
     const unsigned sw = cur; cur = other; other = sw;
   }
@@ -418,16 +461,16 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
     l_run[qb] += __shfl_xor(l_run[qb], 16, 64);
     l_run[qb] += __shfl_xor(l_run[qb], 32, 64);
   }
+  const int s1 = da_again(s0), g1 = (da_again(lane) >> 4);
   if (a.n_split > 1) {
     const long long pb = ((long long)(b * a.Hkv + hk) * a.n_blk + blk) * a.n_split + split;
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      const long long at = (pb * 2 + map) * SLOTS + grp * 16 * QB + 16 * qb + c;
-      if (ok[qb]) {
+      if (s1 + 16 * qb >= n_slots) continue;
+      const long long at = (pb * 2 + map) * SLOTS + (s1 + 16 * qb - blk * SLOTS);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) *(f32x4*)(a.part + at * E + 16 * dt + 4 * g) = o[qb][dt];
-        if (g == 0) *(f32x2*)(a.part_ml + 2 * at) = (f32x2){m_run[qb] * scale2, l_run[qb]};
-      }
+      for (int dt = 0; dt < DT; ++dt) *(f32x4*)(a.part + at * E + 16 * dt + 4 * g1) = o[qb][dt];
+      if (g1 == 0) *(f32x2*)(a.part_ml + 2 * at) = (f32x2){m_run[qb] * scale2, l_run[qb]};
     }
     return;
   }
@@ -440,12 +483,15 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[qb][dt][r] *= inv;
-    const long long rh = (bq * a.Lq + sp.q0 + row[qb]) * a.H + head[qb];       // row and head, counted through the batch
-    if (ok[qb] && a.lse && g == 0)         // base 2, for the scaled scores; +inf: no visible key, every weight 2^-inf = 0
-      a.lse[2 * rh + map] = any ? m_run[qb] * scale2 + __log2f(l) : INFINITY;
-    if (ok[qb] && a.maps) {
+    if (a.lse) {
+      const DaSlot sl = da_slot(a, s1 + 16 * qb, n_slots, hk);
+      const long long rh = (bq * a.Lq + sp.q0 + sl.row) * a.H + sl.head;       // row and head, counted through the batch
+      if (sl.ok && g1 == 0)                // base 2, for the scaled scores; +inf: no visible key, every weight 2^-inf = 0
+        a.lse[2 * rh + map] = any ? m_run[qb] * scale2 + __log2f(l) : INFINITY;
+      if (sl.ok && a.maps) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) *(f32x4*)(a.maps + (2 * rh + map) * E + 16 * dt + 4 * g) = o[qb][dt];
+        for (int dt = 0; dt < DT; ++dt) *(f32x4*)(a.maps + (2 * rh + map) * E + 16 * dt + 4 * g1) = o[qb][dt];
+      }
     }
   }
   // map 1's sums go to their partner wave through LDS (same lane layout), which joins and stores
@@ -461,9 +507,10 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
   if (map == 0) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      if (!ok[qb]) continue;
-      const float lam = da_lam(a, bq * a.ls[0] + (sp.q0 + row[qb]) * a.ls[1] + head[qb] * a.ls[2]);
-      unsigned short* op = a.out + bq * a.os[0] + (sp.q0 + row[qb]) * a.os[1] + head[qb] * a.os[2] + 4 * g;
+      const DaSlot sl = da_slot(a, s1 + 16 * qb, n_slots, hk);
+      if (!sl.ok) continue;
+      const float lam = da_lam(a, bq * a.ls[0] + (sp.q0 + sl.row) * a.ls[1] + sl.head * a.ls[2]);
+      unsigned short* op = a.out + bq * a.os[0] + (sp.q0 + sl.row) * a.os[1] + sl.head * a.os[2] + 4 * g1;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const f32x4 o2 = xch[(qb * DT + dt) * 64 + lane];
@@ -549,7 +596,7 @@ __global__ __launch_bounds__(256) void da_join_kernel(DaArgs a) {
 // =====================================================================================
 template <int D, int QB, int NW, int OCC>
 __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
-  constexpr int E = 2 * D, KS = D / 32, ES = E / 32, DT = D / 16, RK = 2 * D, RV = 2 * E;
+  constexpr int E = 2 * D, AQ = D == 128 ? 4 : D == 64 ? 2 : 6, KS = D / 32, ES = E / 32, DT = D / 16, RK = 2 * D, RV = 2 * E;
   constexpr int TILE = KT * (2 * RK + RV), SLOTS = 16 * QB * NW;
   extern __shared__ __attribute__((aligned(1024))) unsigned char da_smem[];
   __shared__ int red[NW];
@@ -573,32 +620,25 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
   const long long bq = a.cu ? 0 : b;
   const int kend = da_visible_end<64 * NW>(a, b, sp.Lk, tid, red);
 
-  const int s0 = blk * SLOTS + wave * 16 * QB;
-  int row[QB], head[QB];
-  bool ok[QB];
-  long long rh[QB];
+  const int s0 = blk * SLOTS + wave * 16 * QB + c;
   bf16x8 qf[QB][2][KS], dof[QB][ES];
   float lse[QB][2], dl[QB][2];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    int s = s0 + 16 * qb + c;
-    ok[qb] = s < n_slots;
-    s = ok[qb] ? s : n_slots - 1;
-    row[qb] = s / a.share;
-    head[qb] = hk * a.share + (s - row[qb] * a.share);
-    rh[qb] = (bq * a.Lq + sp.q0 + row[qb]) * a.H + head[qb];
-    const unsigned short* dp = a.dout + bq * a.dos[0] + (sp.q0 + row[qb]) * a.dos[1] + head[qb] * a.dos[2] + 8 * g;
+    const DaSlot sl = da_slot(a, s0 + 16 * qb, n_slots, hk);
+    const long long rh = (bq * a.Lq + sp.q0 + sl.row) * a.H + sl.head;
+    const unsigned short* dp = a.dout + bq * a.dos[0] + (sp.q0 + sl.row) * a.dos[1] + sl.head * a.dos[2] + 8 * g;
 #pragma unroll
     for (int ks = 0; ks < ES; ++ks) dof[qb][ks] = *(const bf16x8*)(dp + 32 * ks);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      const unsigned short* qp = a.q + bq * a.qs[0] + (sp.q0 + row[qb]) * a.qs[1] + (2 * head[qb] + m) * a.qs[2] + 8 * g;
+      const unsigned short* qp = a.q + bq * a.qs[0] + (sp.q0 + sl.row) * a.qs[1] + (2 * sl.head + m) * a.qs[2] + 8 * g;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) qf[qb][m][ks] = *(const bf16x8*)(qp + 32 * ks);
-      lse[qb][m] = a.lse[2 * rh[qb] + m];
+      lse[qb][m] = a.lse[2 * rh + m];
       dl[qb][m] = 0.f;
       if (a.maps) {
-        const float* op = a.maps + (2 * rh[qb] + m) * E + 8 * g;
+        const float* op = a.maps + (2 * rh + m) * E + 8 * g;
 #pragma unroll
         for (int ks = 0; ks < ES; ++ks) {
           const f32x4 x = *(const f32x4*)(op + 32 * ks), y = *(const f32x4*)(op + 32 * ks + 4);
@@ -622,6 +662,18 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
   DaKeyStage<D, NW> keys;
   keys.init(a, bq, sp.k0, hk, wave, lane);
   const unsigned lds0 = (unsigned)(size_t)(da_lds*)da_smem;
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+#pragma unroll
+    for (int ks = 0; ks < ES; ++ks) da_landed(dof[qb][ks]);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      da_landed(lse[qb][m]);
+      da_landed(dl[qb][m]);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) da_landed(qf[qb][m][ks]);
+    }
+  }
   const unsigned knat = da_nat_base<RK>(g, c), ktr = da_tr_base<RK>(g, c), vnat = da_nat_base<RV>(g, c) + 2 * KT * RK;
   auto walk_keys = [&](auto last) {                        // last: dQ is summed; else delta
     constexpr bool LAST = decltype(last)::value;
@@ -645,21 +697,15 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
           f32x4 s[QB][2], dp[QB];
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb) s[qb][0] = s[qb][1] = dp[qb] = (f32x4){0.f, 0.f, 0.f, 0.f};
+          // fragments: keys of map 0 and 1 in turn, then the values
+          da_pipe<AQ, 2 * KS + ES>([&](int i) { return i < 2 * KS ? da_nat<RK>(kn, 0, half, i >> 1, (i & 1) * KT * RK) : da_nat<RV>(vn, 0, half, i - 2 * KS); },
+                               [&](int i, bf16x8 x) {
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            const bf16x8 k0f = da_nat<RK>(kn, 0, half, ks), k1f = da_nat<RK>(kn + KT * RK, 0, half, ks);
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) {
-              s[qb][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0f, qf[qb][0][ks], s[qb][0], 0, 0, 0);
-              s[qb][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1f, qf[qb][1][ks], s[qb][1], 0, 0, 0);
-            }
-          }
-#pragma unroll
-          for (int ks = 0; ks < ES; ++ks) {
-            const bf16x8 vf = da_nat<RV>(vn, 0, half, ks);
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) dp[qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, dof[qb][ks], dp[qb], 0, 0, 0);
-          }
+                                 for (int qb = 0; qb < QB; ++qb) {
+                                   if (i < 2 * KS) s[qb][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qf[qb][i & 1][i >> 1], s[qb][i & 1], 0, 0, 0);
+                                   else dp[qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, dof[qb][i - 2 * KS], dp[qb], 0, 0, 0);
+                                 }
+                               });
           if (vis != ~0ull) {
             const unsigned m4 = (unsigned)(vis >> (32 * h2 + 8 * g + 4 * half)) & 0xfu;
 #pragma unroll
@@ -679,17 +725,13 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
                 else dsf[qb][m][4 * half + r] = (__bf16)(p * (dp[qb][r] - dl[qb][m]));
               }
         }
-        if (LAST) {                                        // dQ^T += K^T dS^T
+        if (LAST)                                          // dQ^T += K^T dS^T
+          da_pipe<AQ, 2 * DT>([&](int i) { return da_tr<RK>(kt, 0, i >> 1, (i & 1) * KT * RK); },
+                          [&](int i, bf16x8 x) {
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const bf16x8 k0t = da_tr<RK>(kt, 0, dt), k1t = da_tr<RK>(kt + KT * RK, 0, dt);
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) {
-              acc[qb][0][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0t, dsf[qb][0], acc[qb][0][dt], 0, 0, 0);
-              acc[qb][1][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1t, dsf[qb][1], acc[qb][1][dt], 0, 0, 0);
-            }
-          }
-        }
+                            for (int qb = 0; qb < QB; ++qb)
+                              acc[qb][i & 1][i >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, dsf[qb][i & 1], acc[qb][i & 1][i >> 1], 0, 0, 0);
+                          });
       }
       vis = vis_next;
       const unsigned sw = cur; cur = other; other = sw;
@@ -706,19 +748,22 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
       }
   }
   walk_keys(std::true_type());
+  const int s1 = da_again(s0), g1 = da_again(lane) >> 4;
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    if (!ok[qb]) continue;
-    const float lam = da_lam(a, bq * a.ls[0] + (sp.q0 + row[qb]) * a.ls[1] + head[qb] * a.ls[2]);
-    if (g == 0) {
-      *(f32x4*)(a.stats + 8 * rh[qb]) = (f32x4){lse[qb][0], lse[qb][1], dl[qb][0], dl[qb][1]};
-      a.stats[8 * rh[qb] + 4] = lam;
-      da_put_dlam(a, rh[qb], -dl[qb][1]);
+    const DaSlot sl = da_slot(a, s1 + 16 * qb, n_slots, hk);
+    if (!sl.ok) continue;
+    const long long rh = (bq * a.Lq + sp.q0 + sl.row) * a.H + sl.head;
+    const float lam = da_lam(a, bq * a.ls[0] + (sp.q0 + sl.row) * a.ls[1] + sl.head * a.ls[2]);
+    if (g1 == 0) {
+      *(f32x4*)(a.stats + 8 * rh) = (f32x4){lse[qb][0], lse[qb][1], dl[qb][0], dl[qb][1]};
+      a.stats[8 * rh + 4] = lam;
+      da_put_dlam(a, rh, -dl[qb][1]);
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const float f = m ? -lam * a.scale : a.scale;
-      unsigned short* op = a.dq + bq * a.dqs[0] + (sp.q0 + row[qb]) * a.dqs[1] + (2 * head[qb] + m) * a.dqs[2] + 4 * g;
+      unsigned short* op = a.dq + bq * a.dqs[0] + (sp.q0 + sl.row) * a.dqs[1] + (2 * sl.head + m) * a.dqs[2] + 4 * g1;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         u32x2 w;
@@ -735,7 +780,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
 // =====================================================================================
 template <int D, int KB, int NW, int OCC>
 __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
-  constexpr int E = 2 * D, KS = D / 32, ES = E / 32, DT = D / 16, ET = E / 16, RK = 2 * D, RV = 2 * E;
+  constexpr int E = 2 * D, AK = D == 128 ? 4 : 6, KS = D / 32, ES = E / 32, DT = D / 16, ET = E / 16, RK = 2 * D, RV = 2 * E;
   constexpr int TILE = KT * (2 * RK + RV + 32), KEYS = 16 * KB * NW;
   extern __shared__ __attribute__((aligned(1024))) unsigned char da_smem[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -755,17 +800,13 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
   if (blk * KEYS >= sp.Lk) return;
   const long long bq = a.cu ? 0 : b;
   const int n_slots = sp.Lq * a.share;
-  const int k0 = blk * KEYS + wave * 16 * KB;
-  bool inside[KB], vis[KB];
+  const int k0 = blk * KEYS + wave * 16 * KB + c;
   bool live = false;
   bf16x8 kf[KB][2][KS], vf[KB][ES];
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
-    int key = k0 + 16 * kb + c;
-    inside[kb] = key < sp.Lk;
-    key = inside[kb] ? key : sp.Lk - 1;
-    vis[kb] = inside[kb] && (!a.mask || a.mask[b * a.mask_stride + key] != 0);
-    live = live || vis[kb];
+    const int key = min(k0 + 16 * kb, sp.Lk - 1);
+    live = live || (k0 + 16 * kb < sp.Lk && (!a.mask || a.mask[b * a.mask_stride + key] != 0));
     const unsigned short* vp = a.v + bq * a.vs[0] + (sp.k0 + key) * a.vs[1] + hk * a.vs[2] + 8 * g;
 #pragma unroll
     for (int ks = 0; ks < ES; ++ks) vf[kb][ks] = *(const bf16x8*)(vp + 32 * ks);
@@ -835,6 +876,15 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
       da_dma16(src ? src + 16 * wave : (const unsigned char*)bd_da_zero, base + KT * (2 * RK + RV) + wave * 1024);
     }
   };
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+    for (int ks = 0; ks < ES; ++ks) da_landed(vf[kb][ks]);
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) da_landed(kf[kb][m][ks]);
+  }
   const unsigned qnat = da_nat_base<RK>(g, c), qtr = da_tr_base<RK>(g, c);
   const unsigned dnat = da_nat_base<RV>(g, c) + 2 * KT * RK, dtr = da_tr_base<RV>(g, c) + 2 * KT * RK;
   if (__syncthreads_or(live)) {                            // no visible key in this workgroup: every gradient is zero
@@ -847,8 +897,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
       typedef __attribute__((address_space(3))) const float lds_f32;
 #pragma unroll(D == 128 ? 1 : 2)                           // (head size 128: the unrolled body spills)
       for (int h2 = 0; h2 < 2; ++h2) {                     // 32 slots
-        const unsigned qn = cur + qnat + 32 * RK * h2, qt = cur + qtr + 32 * RK * h2;
-        const unsigned dn = cur + dnat + 32 * RV * h2, dt0 = cur + dtr + 32 * RV * h2;
+        // (unrolled, h2 is a constant offset and both halves share their address registers)
+        constexpr bool U = D < 128;
+        const unsigned qn = cur + qnat + (U ? 0 : 32 * RK * h2), qt = cur + qtr + (U ? 0 : 32 * RK * h2);
+        const unsigned dn = cur + dnat + (U ? 0 : 32 * RV * h2), dt0 = cur + dtr + (U ? 0 : 32 * RV * h2);
+        const int hc = U ? h2 : 0;
         const unsigned st0 = cur + KT * (2 * RK + RV) + 16 * (8 * g + 32 * h2);   // [64] lse1, lse2, delta1, delta2; then [64] lam, ...
         bf16x8 pf[KB], dsf[KB][2];
 #pragma unroll
@@ -856,21 +909,14 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
           f32x4 s[KB][2], dp[KB];
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) s[kb][0] = s[kb][1] = dp[kb] = (f32x4){0.f, 0.f, 0.f, 0.f};
+          da_pipe<AK, 2 * KS + ES>([&](int i) { return i < 2 * KS ? da_nat<RK>(qn, hc, half, i >> 1, (i & 1) * KT * RK) : da_nat<RV>(dn, hc, half, i - 2 * KS); },
+                               [&](int i, bf16x8 x) {
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            const bf16x8 q0f = da_nat<RK>(qn, 0, half, ks), q1f = da_nat<RK>(qn + KT * RK, 0, half, ks);
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-              s[kb][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q0f, kf[kb][0][ks], s[kb][0], 0, 0, 0);
-              s[kb][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q1f, kf[kb][1][ks], s[kb][1], 0, 0, 0);
-            }
-          }
-#pragma unroll
-          for (int ks = 0; ks < ES; ++ks) {
-            const bf16x8 df = da_nat<RV>(dn, 0, half, ks);
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) dp[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(df, vf[kb][ks], dp[kb], 0, 0, 0);
-          }
+                                 for (int kb = 0; kb < KB; ++kb) {
+                                   if (i < 2 * KS) s[kb][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, kf[kb][i & 1][i >> 1], s[kb][i & 1], 0, 0, 0);
+                                   else dp[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, vf[kb][i - 2 * KS], dp[kb], 0, 0, 0);
+                                 }
+                               });
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const unsigned at = st0 + 16 * (4 * half + r);
@@ -886,48 +932,47 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
             }
           }
         }
+        // dV^T += dO^T P, dKm^T += Qm^T dSm
+        da_pipe<AK, ET + 2 * DT>([&](int i) { return i < ET ? da_tr<RV>(dt0, hc, i) : da_tr<RK>(qt, hc, (i - ET) >> 1, ((i - ET) & 1) * KT * RK); },
+                             [&](int i, bf16x8 x) {
 #pragma unroll
-        for (int dt = 0; dt < ET; ++dt) {
-          const bf16x8 dt_ = da_tr<RV>(dt0, 0, dt);
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) av[kb][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(dt_, pf[kb], av[kb][dt], 0, 0, 0);
-        }
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const bf16x8 q0t = da_tr<RK>(qt, 0, dt), q1t = da_tr<RK>(qt + KT * RK, 0, dt);
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
-            ak[kb][0][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q0t, dsf[kb][0], ak[kb][0][dt], 0, 0, 0);
-            ak[kb][1][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q1t, dsf[kb][1], ak[kb][1][dt], 0, 0, 0);
-          }
-        }
+                               for (int kb = 0; kb < KB; ++kb) {
+                                 if (i < ET) av[kb][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pf[kb], av[kb][i], 0, 0, 0);
+                                 else {
+                                   f32x4& z = ak[kb][(i - ET) & 1][(i - ET) >> 1];
+                                   z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, dsf[kb][(i - ET) & 1], z, 0, 0, 0);
+                                 }
+                               }
+                             });
       }
       const unsigned sw = cur; cur = other; other = sw;
     }
   }
+  const int k1 = da_again(k0), g1 = da_again(lane) >> 4;
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
-    if (!inside[kb]) continue;
-    const int key = k0 + 16 * kb + c;
+    const int key = k1 + 16 * kb;
+    if (key >= sp.Lk) continue;
+    const bool vis = !a.mask || a.mask[b * a.mask_stride + key] != 0;
     // a masked key's gradients are exact zeros whatever its column held
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      unsigned short* op = a.dk + bq * a.dks[0] + (sp.k0 + key) * a.dks[1] + (2 * hk + m) * a.dks[2] + 4 * g;
+      unsigned short* op = a.dk + bq * a.dks[0] + (sp.k0 + key) * a.dks[1] + (2 * hk + m) * a.dks[2] + 4 * g1;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         u32x2 w = {0u, 0u};
-        if (vis[kb]) {
+        if (vis) {
           w[0] = bd_pack_bf16x2(ak[kb][m][dt][0] * a.scale, ak[kb][m][dt][1] * a.scale);
           w[1] = bd_pack_bf16x2(ak[kb][m][dt][2] * a.scale, ak[kb][m][dt][3] * a.scale);
         }
         *(u32x2*)(op + 16 * dt) = w;
       }
     }
-    unsigned short* op = a.dv + bq * a.dvs[0] + (sp.k0 + key) * a.dvs[1] + hk * a.dvs[2] + 4 * g;
+    unsigned short* op = a.dv + bq * a.dvs[0] + (sp.k0 + key) * a.dvs[1] + hk * a.dvs[2] + 4 * g1;
 #pragma unroll
     for (int dt = 0; dt < ET; ++dt) {
       u32x2 w = {0u, 0u};
-      if (vis[kb]) {
+      if (vis) {
         w[0] = bd_pack_bf16x2(av[kb][dt][0], av[kb][dt][1]);
         w[1] = bd_pack_bf16x2(av[kb][dt][2], av[kb][dt][3]);
       }
@@ -1049,9 +1094,9 @@ int da_forward(const bd_diff_attn_args& p, DaArgs& a, hipStream_t s) {
 }
 
 // Backward: blocks of 16 slots (dq) or keys (dkv) a wave holds, waves of a workgroup, waves of a SIMD. Measured, dq / dkv:
-// head size 64, 16 x 1024 x 3 heads: dq (1, 8, 4) 73 us, (1, 4, 3) 79; dkv (1, 4, 2) 86, (1, 4, 3) 108, (1, 8, 2) 113.
-// Head size 128, 2 x 4096 x 8: (1, 8, 2) 478 / 800 us, (2, 4, 1) 834 / 844, (1, 4, 1) 1058 / 1234. Head size 32, 96 ragged
-// x 8: (1, 4, 4) 90 / 96 us, (1, 8, 4) 110 / 121, dq (2, 4, 3) 99.
+// head size 64, 16 x 1024 x 3 heads: dq (1, 8, 4) 67 us, (1, 4, 3) 79; dkv (1, 4, 2) 75, (1, 4, 3) 108, (1, 8, 2) 113.
+// Head size 128, 2 x 4096 x 8: (1, 8, 2) 428 / 715 us, (2, 4, 1) 834 / 844, (1, 4, 1) 1058 / 1234. Head size 32, 96 ragged
+// x 8: (1, 4, 4) 86 / 93 us, (1, 8, 4) 110 / 121, dq (2, 4, 3) 99.
 template <int B_, int NW_, int OCC_> struct DaCfg { static constexpr int B = B_, NW = NW_, OCC = OCC_; };
 template <int D> struct DaBwd { typedef DaCfg<1, 8, 4> Q; typedef DaCfg<1, 4, 2> K; };
 template <> struct DaBwd<32> { typedef DaCfg<1, 4, 4> Q; typedef DaCfg<1, 4, 4> K; };
