@@ -523,68 +523,78 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
   }
 }
 
-// Joins the key splits of one slot: the splits' maxima and normalisers first (one thread a split), then 256 threads =
-// E / 4 column groups x the rest over the splits, added up in a fixed order.
+// Joins the key splits of one slot, 16 columns a workgroup: waves 2 m and 2 m + 1 add up map m, 16 splits at a time each
+// with 4 lanes across the columns, in a fixed order. Bound by latency (one row, 65 521 keys, 4 x 4 heads of 64, 128
+// splits: 16.8 MB of partial sums in all): what a thread adds up is asked for before the splits' maxima and normalisers
+// are worked into weights, and many small workgroups wait at once.
+constexpr int JOIN_COLS = 16, JOIN_SPLITS = 256;
 template <int D, int SLOTS>
 __global__ __launch_bounds__(256) void da_join_kernel(DaArgs a) {
-  constexpr int E = 2 * D, CG = E / 4, RG = 256 / CG;
-  __shared__ float wt[2][256], red[2][4][2];
-  __shared__ f32x4 sum[RG][CG];
+  constexpr int E = 2 * D, CB = E / JOIN_COLS, N = JOIN_SPLITS / 32;
+  __shared__ float wt[2][JOIN_SPLITS], red[2][2][4];
+  __shared__ f32x4 sum[4][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int slot = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  const int slot = blockIdx.x / CB, col = (blockIdx.x % CB) * JOIN_COLS + 4 * (lane & 3), hk = blockIdx.y, b = blockIdx.z;
   const int blk = slot / SLOTS, in_blk = slot - blk * SLOTS;
   const int row = slot / a.share, head = hk * a.share + (slot - row * a.share);
   const long long rh = ((long long)b * a.Lq + row) * a.H + head;
   const long long at0 = ((long long)(b * a.Hkv + hk) * a.n_blk + blk) * a.n_split * 2 * SLOTS + in_blk;
-  float l[2];
+  const int map = wave >> 1, s0 = (wave & 1) * 16 + (lane >> 2);
+  f32x4 x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (s0 + 32 * i < a.n_split) x[i] = *(const f32x4*)(a.part + (at0 + (long long)(2 * (s0 + 32 * i) + map) * SLOTS) * E + col);
+  f32x2 ml[2] = {{-INFINITY, 0.f}, {-INFINITY, 0.f}};
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    f32x2 x = {-INFINITY, 0.f};
-    if (tid < a.n_split) x = *(const f32x2*)(a.part_ml + 2 * (at0 + (long long)(2 * tid + m) * SLOTS));
-    const float mx = bd_wave_max(x[0]);
-    if (lane == 0) red[m][wave][0] = mx;
-    __syncthreads();
-    const float top = fmaxf(fmaxf(red[m][0][0], red[m][1][0]), fmaxf(red[m][2][0], red[m][3][0]));
-    const float w = x[1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(x[0] - top);      // a split without a visible key weighs nothing
-    wt[m][tid] = w;
-    const float ls = bd_wave_sum(w * x[1]);
-    if (lane == 0) red[m][wave][1] = ls;
-    __syncthreads();
-    l[m] = (red[m][0][1] + red[m][1][1]) + (red[m][2][1] + red[m][3][1]);
-    if (a.lse && tid == 0) a.lse[2 * rh + m] = l[m] > 0.f || l[m] != l[m] ? top + __log2f(l[m]) : INFINITY;
+    if (tid < a.n_split) ml[m] = *(const f32x2*)(a.part_ml + 2 * (at0 + (long long)(2 * tid + m) * SLOTS));
+    const float mx = bd_wave_max(ml[m][0]);
+    if (lane == 0) red[0][m][wave] = mx;
   }
-  const int cg = tid % CG, rg = tid / CG;
+  __syncthreads();
+  float top[2], l[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    top[m] = fmaxf(fmaxf(red[0][m][0], red[0][m][1]), fmaxf(red[0][m][2], red[0][m][3]));
+    // a split without a visible key weighs nothing
+    const float w = ml[m][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[m][0] - top[m]);
+    wt[m][tid] = w;
+    const float ls = bd_wave_sum(w * ml[m][1]);
+    if (lane == 0) red[1][m][wave] = ls;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int m = 0; m < 2; ++m) l[m] = (red[1][m][0] + red[1][m][1]) + (red[1][m][2] + red[1][m][3]);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (s0 + 32 * i < a.n_split) {
+      const float w = wt[map][s0 + 32 * i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += w == 0.f ? 0.f : w * x[i][e];
+    }
+#pragma unroll
+  for (int s = 4; s < 64; s *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], s, 64);
+  if (lane < 4) sum[wave][lane] = o;
+  __syncthreads();
+  if (tid >= 4) return;
   f32x4 r[2];
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = rg; i < a.n_split; i += RG) {
-      const float w = wt[m][i];
-      if (w == 0.f) continue;
-      const f32x4 x = *(const f32x4*)(a.part + (at0 + (long long)(2 * i + m) * SLOTS) * E + 4 * cg);
+    const bool any = l[m] > 0.f || l[m] != l[m];
+    const float inv = any ? 1.0f / l[m] : 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += w * x[e];
-    }
-    sum[rg][cg] = o;
-    __syncthreads();
-    f32x4 all = sum[0][cg];
-#pragma unroll
-    for (int i = 1; i < RG; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) all[e] += sum[i][cg][e];
-    const float inv = l[m] > 0.f || l[m] != l[m] ? 1.0f / l[m] : 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[m][e] = all[e] * inv;
-    __syncthreads();
-    if (a.maps && rg == 0) *(f32x4*)(a.maps + (2 * rh + m) * E + 4 * cg) = r[m];
+    for (int e = 0; e < 4; ++e) r[m][e] = (sum[2 * m][tid][e] + sum[2 * m + 1][tid][e]) * inv;
+    if (a.maps) *(f32x4*)(a.maps + (2 * rh + m) * E + col) = r[m];
+    if (a.lse && tid == 0 && col == 0) a.lse[2 * rh + m] = any ? top[m] + __log2f(l[m]) : INFINITY;
   }
-  if (rg == 0) {
-    const float lam = da_lam(a, b * a.ls[0] + row * a.ls[1] + head * a.ls[2]);
-    u32x2 w;
-    w[0] = bd_pack_bf16x2(r[0][0] - lam * r[1][0], r[0][1] - lam * r[1][1]);
-    w[1] = bd_pack_bf16x2(r[0][2] - lam * r[1][2], r[0][3] - lam * r[1][3]);
-    *(u32x2*)(a.out + b * a.os[0] + row * a.os[1] + head * a.os[2] + 4 * cg) = w;
-  }
+  const float lam = da_lam(a, b * a.ls[0] + row * a.ls[1] + head * a.ls[2]);
+  u32x2 w;
+  w[0] = bd_pack_bf16x2(r[0][0] - lam * r[1][0], r[0][1] - lam * r[1][1]);
+  w[1] = bd_pack_bf16x2(r[0][2] - lam * r[1][2], r[0][3] - lam * r[1][3]);
+  *(u32x2*)(a.out + b * a.os[0] + row * a.os[1] + head * a.os[2] + col) = w;
 }
 
 // =====================================================================================
@@ -1027,7 +1037,7 @@ int da_splits(const bd_diff_attn_args& p) {
   const int tiles = (p.Lk + KT - 1) / KT;
   long long n = 512 / (blocks > 0 ? blocks : 1);
   if (n > tiles / 4) n = tiles / 4;
-  return n < 1 ? 1 : n > 256 ? 256 : (int)n;
+  return n < 1 ? 1 : n > JOIN_SPLITS ? JOIN_SPLITS : (int)n;
 }
 
 bool da_few(const bd_diff_attn_args& p) { return (long long)p.Lq * (p.H / p.Hkv) <= ROWS_SLOTS || da_splits(p) > 1; }
@@ -1085,7 +1095,7 @@ int da_forward(const bd_diff_attn_args& p, DaArgs& a, hipStream_t s) {
     BD_SET_MAX_LDS((da_fwd_kernel<D, 1, ROWS_NQG, 2>), LDS);
     hipLaunchKernelGGL((da_fwd_kernel<D, 1, ROWS_NQG, 2>), dim3((unsigned)grid), dim3(128 * ROWS_NQG), LDS, s, a);
     if (a.n_split > 1)
-      hipLaunchKernelGGL((da_join_kernel<D, ROWS_SLOTS>), dim3((unsigned)slots, a.Hkv, a.B), dim3(256), 0, s, a);
+      hipLaunchKernelGGL((da_join_kernel<D, ROWS_SLOTS>), dim3((unsigned)(slots * (2 * D / JOIN_COLS)), a.Hkv, a.B), dim3(256), 0, s, a);
   } else {
     BD_SET_MAX_LDS((da_fwd_kernel<D, F::B, F::NQG, F::OCC>), LDS);
     hipLaunchKernelGGL((da_fwd_kernel<D, F::B, F::NQG, F::OCC>), dim3((unsigned)grid), dim3(128 * F::NQG), LDS, s, a);
