@@ -66,6 +66,11 @@ def _same_device(what, first, *others):
             raise ValueError(f"bidiff {what}: operands on {dev} and {t.device}; all must be on one device")
 
 
+def _like(t):
+    """A contiguous tensor of ``t``'s shape, dtype and device, not filled."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _rows_of_16_bytes(t):
     """``t`` or a copy of it whose rows the kernels can read in 16-byte pieces."""
     *st, last = t.stride()
@@ -138,9 +143,9 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, table, positions, interleaved, *xs):
         ctx.save_for_backward(table, positions)
         ctx.interleaved = interleaved
-        out = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
+        out = [_like(x) for x in xs]
         _rotary_launch(list(zip(xs, out)), table, positions, interleaved, False)
-        return out
+        return tuple(out)
 
     @staticmethod
     @once_differentiable
@@ -151,7 +156,7 @@ class _Rotary(torch.autograd.Function):
             if ctx.needs_input_grad[3 + i]:
                 if g.stride(-1) != 1:
                     g = g.contiguous()
-                dx[i] = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+                dx[i] = _like(g)
                 pairs.append((g, dx[i]))
         if pairs:
             _rotary_launch(pairs, table, positions, ctx.interleaved, True)
@@ -203,7 +208,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, posi
     if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
         out = _Rotary.apply(table, positions, bool(interleaved), *xs)
     else:
-        out = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
+        out = [_like(x) for x in xs]
         _rotary_launch(list(zip(xs, out)), table, positions, interleaved, False)
     return out[0], out[1] if k is not None else None
 
@@ -343,9 +348,7 @@ class _DiffAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, lam, key_mask, cu, saved = ctx.saved_tensors
-        dev = q.device
-        dq, dk, dv = (torch.empty(t.shape, dtype=torch.bfloat16, device=dev) for t in (q, k, v))
-        dl = torch.empty(lam.shape, dtype=lam.dtype, device=dev)
+        dq, dk, dv, dl = _like(q), _like(k), _like(v), _like(lam)
         _attention_backward(q, k, v, lam, ctx.lam_strides, key_mask, cu, ctx.longest, ctx.scale, saved, _rows_of_16_bytes(dout),
                             dq, dk, dv, dl)
         return dq, dk, dv, dl, None, None, None, None, None
@@ -439,34 +442,40 @@ def _to_bf16(x, stream):
 
 @functools.lru_cache(maxsize=256)
 def _head_sizes(M, d, V):
-    """Bytes of the state and of the two workspaces."""
+    """Bytes of the state and of the workspaces: forward, backward, forward without state."""
     L_ = _lib.lib()
-    sizes = (L_.bd_linear_ce_state_bytes(M, d), L_.bd_linear_ce_workspace_bytes(M, d, V, 0), L_.bd_linear_ce_workspace_bytes(M, d, V, 1))
+    sizes = (L_.bd_linear_ce_state_bytes(M, d), *(L_.bd_linear_ce_workspace_bytes(M, d, V, kind) for kind in range(3)))
     if min(sizes) < 0:
         _lib.check(-1, "bd_linear_ce_workspace_bytes")
     return sizes
 
 
+def _head_loss(hidden, weight, targets, indicator, attention_mask, training):
+    """(loss, the head in bf16, what the backward needs or None)"""
+    dev = hidden.device
+    V, d = weight.shape
+    M = targets.numel()
+    state_bytes, with_state, _, alone = _head_sizes(M, d, V)
+    ws_bytes = with_state if training else alone
+    with _on(dev) as stream:
+        h, w = _to_bf16(hidden, stream), _to_bf16(weight, stream)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        state = torch.empty(state_bytes, dtype=torch.uint8, device=dev) if training else None
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        _lib.check(_lib.lib().bd_linear_ce_fwd(
+            h.data_ptr(), w.data_ptr(), targets.data_ptr(), None if indicator is None else indicator.data_ptr(),
+            None if attention_mask is None else attention_mask.data_ptr(), loss.data_ptr(), M, d, V,
+            state.data_ptr() if training else None, state_bytes, ws.data_ptr(), ws_bytes, stream), "bd_linear_ce_fwd")
+    return loss, w, state
+
+
 class _LinearCE(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, indicator, attention_mask):
-        dev = hidden.device
-        V, d = weight.shape
-        M = targets.numel()
-        state_bytes, ws_bytes, _ = _head_sizes(M, d, V)
-        with _on(dev) as stream:
-            h, w = _to_bf16(hidden, stream), _to_bf16(weight, stream)
-            loss = torch.empty((), dtype=torch.float32, device=dev)
-            state = torch.empty(state_bytes, dtype=torch.uint8, device=dev)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-            _lib.check(_lib.lib().bd_linear_ce_fwd(
-                h.data_ptr(), w.data_ptr(), targets.data_ptr(), None if indicator is None else indicator.data_ptr(),
-                None if attention_mask is None else attention_mask.data_ptr(), loss.data_ptr(), M, d, V, state.data_ptr(), state_bytes,
-                ws.data_ptr(), ws_bytes, stream), "bd_linear_ce_fwd")
-        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
-            # (the weighted rows are in the state; of an fp32 head its bf16 copy is kept)
-            ctx.save_for_backward(w, state)
-            ctx.like = (hidden.shape, hidden.dtype, weight.dtype)
+        loss, w, state = _head_loss(hidden, weight, targets, indicator, attention_mask, True)
+        # (the weighted rows are in the state; of an fp32 head its bf16 copy is kept)
+        ctx.save_for_backward(w, state)
+        ctx.like = (hidden.shape, hidden.dtype, weight.dtype)
         return loss
 
     @staticmethod
@@ -477,7 +486,7 @@ class _LinearCE(torch.autograd.Function):
         V, d = w.shape
         M = shape[:-1].numel()
         dev = w.device
-        state_bytes, _, ws_bytes = _head_sizes(M, d, V)
+        state_bytes, _, ws_bytes, _ = _head_sizes(M, d, V)
         dh = torch.empty(shape, dtype=torch.bfloat16, device=dev) if ctx.needs_input_grad[0] else None
         dw = None
         if ctx.needs_input_grad[1]:      # fp32 gradients are accumulated into, bf16 ones written
@@ -534,4 +543,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
         hidden = hidden.clone(memory_format=torch.contiguous_format)
     if weight.data_ptr() % 16:
         weight = weight.clone(memory_format=torch.contiguous_format)
-    return _LinearCE.apply(hidden, weight, targets.contiguous(), mask_indicator, attention_mask)
+    targets = targets.contiguous()
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _LinearCE.apply(hidden, weight, targets, mask_indicator, attention_mask)
+    return _head_loss(hidden, weight, targets, mask_indicator, attention_mask, False)[0]

@@ -831,12 +831,13 @@ int bd_diff_attention_dlam(const float* dlam, void* out, int out_dtype, int B, i
  * may be null = ones). loss[0] = sum(w * ce) / sum(w), exactly 0 when no row carries weight. Rows without weight are
  * never read; a weighted row whose target lies outside [0, V) makes the loss NaN. The forward leaves what the backward
  * needs (the weighted rows, their targets, weights and log-sum-exps) in state (bd_linear_ce_state_bytes(M, d) bytes);
- * workspaces of bd_linear_ce_workspace_bytes(M, d, V, backward) bytes are scratch. Backward, times grad_out[0]:
+ * a null state means that no backward follows. Workspaces are scratch of bd_linear_ce_workspace_bytes(M, d, V, kind)
+ * bytes, kind 0: forward, 1: backward, 2: forward without state. Backward, times grad_out[0]:
  * dhidden [M, d] bf16 (overwritten; zeros at rows without weight) and dweight [V, d], bf16 overwritten or fp32 ADDED to
  * (as the weight-gradient products of this library do); either may be null. Equal calls give equal bits.
  * Stands beside bd_masked_ce_fwd / bd_masked_ce_bwd, which read the logits from memory. */
 long long bd_linear_ce_state_bytes(long long M, int d);
-long long bd_linear_ce_workspace_bytes(long long M, int d, int V, int backward);
+long long bd_linear_ce_workspace_bytes(long long M, int d, int V, int kind);
 int bd_linear_ce_fwd(const void* hidden, const void* weight, const long long* targets, const unsigned char* indicator,
                      const long long* attention_mask, float* loss, long long M, int d, int V, void* state, long long state_bytes,
                      void* workspace, long long workspace_bytes, void* stream);
