@@ -329,7 +329,11 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
   if (a.cu && b == a.B) {                                  // (packed: one more sequence, the rows behind the last one)
     if (blk == 0) {
       da_zero_tail(a.out, a.os, min(max(a.cu[a.B], 0), a.total), a.total, hk * a.share, a.share, E, tid, 64 * NW);
-      for (int i = 0; i < a.B; ++i) {                      // a sequence longer than Lq: its rows past Lq are NaN, not silence
+      // a sequence longer than Lq: its rows past Lq are NaN, not silence
+      int longer = 0;
+      for (int i = tid; i < a.B; i += 64 * NW) longer |= min(a.cu[i + 1], a.total) - max(a.cu[i], 0) > a.Lq;
+      const int n = __syncthreads_or(longer) ? a.B : 0;
+      for (int i = 0; i < n; ++i) {
         const int lo = min(max(a.cu[i], 0), a.total), hi = min(max(a.cu[i + 1], lo), a.total);
         for (long long r = lo + (long long)a.Lq; r < hi; ++r)
           for (int e = tid; e < a.share * E; e += 64 * NW)
