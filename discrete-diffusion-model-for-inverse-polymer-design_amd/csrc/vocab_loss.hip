@@ -167,6 +167,7 @@ struct VlGemm {
 
 typedef __attribute__((address_space(3))) void vl_lds;
 
+// 16-byte chunk ch of a row: what 16 lanes read at a time covers every bank once
 template <int R> __device__ __forceinline__ int vl_kc(int row, int ch) { return R * row + 16 * (ch ^ ((row >> 1) & 7)); }
 template <int R> __device__ __forceinline__ int vl_mc(int row, int ch) { return R * row + 16 * (ch ^ ((row & 3) << 2)); }
 __device__ __forceinline__ s16x4 vl_read_tr(const unsigned char* p) {
@@ -177,6 +178,9 @@ __device__ __forceinline__ bf16x8 vl_join(s16x4 a, s16x4 b) {
   u.s.a = a; u.s.b = b;
   return u.v;
 }
+
+// (the IEEE maximum: fmaxf would first quiet each product's result)
+__device__ __forceinline__ float vl_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // (maximum, sum of 2^(x - maximum)) of two parts
 __device__ __forceinline__ f32x2 vl_pair(f32x2 a, f32x2 b) {
@@ -199,9 +203,10 @@ __device__ __forceinline__ void vl_store_bf16(unsigned short* o, const f32x4 (&a
 }
 
 template <int BM, int BN, bool AKC, bool BKC, int EPI>
-__global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGemm p) {
+__global__ __launch_bounds__(2 * BN, 2) void vl_gemm_kernel(VlGemm p) {
   constexpr int WM = 2, WN = BN / 64, NW = WM * WN, TM = BM / WM / 16, TN = 4;
-  constexpr int SA = BM * 128, SB = BN * 128, STAGE = SA + SB;      // bytes of a 64-deep stage, either layout
+  constexpr int BK = 64, AHEAD = 2;
+  constexpr int SA = BM * BK * 2, SB = BN * BK * 2, STAGE = SA + SB;      // bytes of a stage, either layout
   extern __shared__ __attribute__((aligned(1024))) unsigned char vl_smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -231,7 +236,8 @@ __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGem
   auto off_a = [&](int j, int k0) -> unsigned {
     const int at = (wave + NW * j) * 1024 + lane * 16;
     if (AKC) {
-      const int row = at >> 7, ch = ((at >> 4) & 7) ^ ((row >> 1) & 7);
+      constexpr int R = 2 * BK;
+      const int row = at / R, ch = (vl_kc<R>(row, (at % R) >> 4) - R * row) >> 4;
       return (unsigned)(((long long)(min(m0 + row, p.M - 1) - m0) * p.lda + 8 * ch) * 2);
     }
     constexpr int R = 2 * BM;
@@ -241,7 +247,8 @@ __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGem
   auto off_b = [&](int j, int k0) -> unsigned {
     const int at = (wave + NW * j) * 1024 + lane * 16;
     if (BKC) {
-      const int rx = at >> 7, ch = ((at >> 4) & 7) ^ ((rx >> 1) & 7);
+      constexpr int R = 2 * BK;
+      const int rx = at / R, ch = (vl_kc<R>(rx, (at % R) >> 4) - R * rx) >> 4;
       const int i = rx & 15, tn = (rx >> 4) & 3, n = 64 * (rx >> 6) + 32 * (tn >> 1) + 8 * (i >> 2) + 4 * (tn & 1) + (i & 3);   // permuted
       return (unsigned)(((long long)(min(n0 + n, p.n_rows - 1) - n0) * p.ldb + 8 * ch) * 2);
     }
@@ -260,13 +267,13 @@ __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGem
   };
   auto issue = [&](int kt, int buf) {
     const unsigned base = lds0 + buf * STAGE;
-    const unsigned char* sa = (const unsigned char*)(AKC ? p.A + (long long)m0 * p.lda + 64ll * kt : p.A + 64ll * kt * p.lda + m0);
-    const unsigned char* sb = (const unsigned char*)(BKC ? p.B + (long long)n0 * p.ldb + 64ll * kt : p.B + 64ll * kt * p.ldb + n0);
-    const bool ragged = 64 * kt + 64 > K;
+    const unsigned char* sa = (const unsigned char*)(AKC ? p.A + (long long)m0 * p.lda + (long long)BK * kt : p.A + (long long)BK * kt * p.lda + m0);
+    const unsigned char* sb = (const unsigned char*)(BKC ? p.B + (long long)n0 * p.ldb + (long long)BK * kt : p.B + (long long)BK * kt * p.ldb + n0);
+    const bool ragged = BK * kt + BK > K;
 #pragma unroll
-    for (int j = 0; j < PA; ++j) glds(sa, !AKC && ragged ? off_a(j, 64 * kt) : va[j], base + (wave + NW * j) * 1024);
+    for (int j = 0; j < PA; ++j) glds(sa, !AKC && ragged ? off_a(j, BK * kt) : va[j], base + (wave + NW * j) * 1024);
 #pragma unroll
-    for (int j = 0; j < PB; ++j) glds(sb, !BKC && ragged ? off_b(j, 64 * kt) : vb[j], base + SA + (wave + NW * j) * 1024);
+    for (int j = 0; j < PB; ++j) glds(sb, !BKC && ragged ? off_b(j, BK * kt) : vb[j], base + SA + (wave + NW * j) * 1024);
   };
 
   f32x4 acc[TM][TN];
@@ -281,32 +288,35 @@ __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGem
     if (kt + 1 < kt_end) issue(kt + 1, buf ^ 1);
     const unsigned char* const As = vl_smem + buf * STAGE;
     const unsigned char* const Bs = As + SA;
+    auto load_x = [&](int kk, int tn) -> bf16x8 {
+      if (BKC) return *(const bf16x8*)(Bs + vl_kc<2 * BK>(64 * wn + 16 * tn + c, 4 * kk + g));
+      constexpr int R = 2 * BN;
+      const int r0 = 32 * kk + 8 * g + q4, ch = 8 * wn + 4 * (tn >> 1) + p4;
+      return vl_join(vl_read_tr(Bs + vl_mc<R>(r0, ch) + 8 * (tn & 1)), vl_read_tr(Bs + vl_mc<R>(r0 + 4, ch) + 8 * (tn & 1)));
+    };
+    auto load_y = [&](int kk, int tm) -> bf16x8 {
+      if (AKC) return *(const bf16x8*)(As + vl_kc<2 * BK>(16 * TM * wm + 16 * tm + c, 4 * kk + g));
+      constexpr int R = 2 * BM;
+      const int r0 = 32 * kk + 8 * g + q4, ch = 2 * (TM * wm + tm) + (p4 >> 1);
+      return vl_join(vl_read_tr(As + vl_mc<R>(r0, ch) + 8 * (p4 & 1)), vl_read_tr(As + vl_mc<R>(r0 + 4, ch) + 8 * (p4 & 1)));
+    };
+    // operand fragments are read AHEAD of their products, in this order (the compiler left alone reads one, waits for it and
+    // multiplies: scores of 4096 x 2048 -> 65536 in 867 us instead of 746)
+    constexpr int STEPS = BK / 32 * TM;
+    bf16x8 x[2][TN], y[AHEAD];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      bf16x8 x[TN];
+    for (int tn = 0; tn < TN; ++tn) x[0][tn] = load_x(0, tn);
 #pragma unroll
-      for (int tn = 0; tn < TN; ++tn) {
-        if (BKC) {
-          x[tn] = *(const bf16x8*)(Bs + vl_kc<128>(64 * wn + 16 * tn + c, 4 * kk + g));
-        } else {
-          constexpr int R = 2 * BN;
-          const int r0 = 32 * kk + 8 * g + q4, ch = 8 * wn + 4 * (tn >> 1) + p4;
-          x[tn] = vl_join(vl_read_tr(Bs + vl_mc<R>(r0, ch) + 8 * (tn & 1)), vl_read_tr(Bs + vl_mc<R>(r0 + 4, ch) + 8 * (tn & 1)));
-        }
-      }
+    for (int i = 0; i < AHEAD; ++i) y[i] = load_y(i / TM, i % TM);
+    __builtin_amdgcn_sched_barrier(0x6);
 #pragma unroll
-      for (int tm = 0; tm < TM; ++tm) {
-        bf16x8 y;
-        if (AKC) {
-          y = *(const bf16x8*)(As + vl_kc<128>(16 * TM * wm + 16 * tm + c, 4 * kk + g));
-        } else {
-          constexpr int R = 2 * BM;
-          const int r0 = 32 * kk + 8 * g + q4, ch = 2 * (TM * wm + tm) + (p4 >> 1);
-          y = vl_join(vl_read_tr(As + vl_mc<R>(r0, ch) + 8 * (p4 & 1)), vl_read_tr(As + vl_mc<R>(r0 + 4, ch) + 8 * (p4 & 1)));
-        }
+    for (int i = 0; i < STEPS; ++i) {
+      const int kk = i / TM, tm = i % TM;
 #pragma unroll
-        for (int tn = 0; tn < TN; ++tn) acc[tm][tn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[tn], y, acc[tm][tn], 0, 0, 0);
-      }
+      for (int tn = 0; tn < TN; ++tn) acc[tm][tn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[kk & 1][tn], y[i % AHEAD], acc[tm][tn], 0, 0, 0);
+      if (i + AHEAD < STEPS) y[i % AHEAD] = load_y((i + AHEAD) / TM, (i + AHEAD) % TM);
+      if (kk + 1 < BK / 32 && tm < TN) x[(kk + 1) & 1][tm] = load_x(kk + 1, tm);
+      __builtin_amdgcn_sched_barrier(0x6);
     }
   }
 
@@ -333,7 +343,7 @@ __global__ __launch_bounds__(BM == 256 ? 512 : 256, 2) void vl_gemm_kernel(VlGem
       }
       float mx = -INFINITY, se = 0.f;
 #pragma unroll
-      for (int tn = 0; tn < TN; ++tn) mx = fmaxf(fmaxf(mx, fmaxf(acc[tm][tn][0], acc[tm][tn][1])), fmaxf(acc[tm][tn][2], acc[tm][tn][3]));
+      for (int tn = 0; tn < TN; ++tn) mx = vl_max(vl_max(mx, vl_max(acc[tm][tn][0], acc[tm][tn][1])), vl_max(acc[tm][tn][2], acc[tm][tn][3]));
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
       const float ref = mx == -INFINITY ? 0.f : mx * VL_LOG2E;
@@ -620,7 +630,7 @@ __global__ __launch_bounds__(1024) void vl_narrow_finish_kernel(const f32x2* __r
 struct VlPlan {
   long long m_pad;
   int piece, n_pieces;                // vocabulary columns per backward piece
-  int big_z, big_h, big_w;            // 256 x 256 tiles for the scores, dh, dW (else 128 x 128)
+  int big_s, big_z, big_h, big_w;     // 256 x 256 tiles for the scores, dz, dh, dW (else 128 x 128)
   int split_h, split_w;               // splits of dh's product over the piece (at most), of dW's over the rows
   long long slab_h, slab_w;           // floats of one slab
   long long fwd_bytes, bwd_bytes;
@@ -632,14 +642,23 @@ VlPlan vl_plan(long long M, int d, int V) {
   VlPlan p;
   p.m_pad = vl_up(M, 256);
   // Tile sizes, each measured both ways (256 x 256 / 128 x 128, us; half of the rows weighted): the larger tile reads less LDS
-  // per product but leaves one workgroup on a CU, whose start and end nothing hides, and wastes more at ragged edges.
-  //   scores: 8192 x 2048 -> 65536: 881 / 986; x 1024: 502 / 526; 2000 x 1024 -> 65536: 149 / 139; 4096 x 512 -> 32000: 83 / 81;
-  //   3001 x 768 -> 32003: 111 / 96; 32768 x 384 -> 803: 19 / 19
-  //   dh (with the sum of its splits): in that order 889 / 1005, 520 / 686, 150 / 179, 83 / 91, 99 / 120, 38 / 26
-  //   dW (with the sum of its splits): 839 / 1040, 440 / 530, 140 / 162, 65 / 79, 106 / 103, 40 / 31
-  p.big_z = d >= 1024 && (p.m_pad / 256) * ((V + 255) / 256) >= 4096;
-  p.big_h = V >= 4096 && (d % 256 == 0 || d >= 768);
-  p.big_w = (long long)((V + 255) / 256) * ((d + 255) / 256) >= 200;
+  // per product but leaves one workgroup on a CU, whose start and end nothing hides, and wastes more at ragged edges and
+  // in a last round of few tiles.
+  //                     scores      scores again, to dz   dh (with the sum of its splits)   dW (with the sum of its splits)
+  //   8192 x 2048 -> 65536  804 / 1011   979 / 1076   917 / 987   899 / 951
+  //   8192 x 1024 -> 65536  420 / 504    567 / 610    494 / 684   433 / 458
+  //   2000 x 1024 -> 65536  130 / 136    155 / 137    141 / 178   137 / 147
+  //   4096 x 512 -> 32000    73 / 76      97 / 92      79 / 91     64 / 67
+  //   3001 x 768 -> 32003    92 / 88     114 / 104     93 / 120   102 / 87
+  //   8192 x 768 -> 8192     48 / 53      60 / 62      67 / 86     74 / 57
+  //   32768 x 384 -> 4096    58 / 64      82 / 80      76 / 66     74 / 90
+  //   32768 x 384 -> 803     17 / 18      25 / 25      37 / 25     39 / 28
+  //   8192 x 4096 -> 2048    88 / 63      96 / 64      73 / 83     82 / 66
+  const long long tiles_z = (p.m_pad / 256) * ((V + 255) / 256), tiles_w = (long long)((V + 255) / 256) * ((d + 255) / 256);
+  p.big_s = tiles_z >= 512;
+  p.big_z = d >= 1024 && tiles_z >= 4096;
+  p.big_h = V >= 2048 && (d % 256 == 0 || d >= 768);
+  p.big_w = 10 * tiles_w >= 9 * vl_up(tiles_w, 256);      // whole rounds of the CUs
   const int bh = p.big_h ? 256 : 128, bw = p.big_w ? 256 : 128;
   long long piece = VL_PIECE_BYTES / 2 / p.m_pad / 256 * 256;
   if (piece < 256) piece = 256;
@@ -659,17 +678,17 @@ VlPlan vl_plan(long long M, int d, int V) {
   return p;
 }
 
+template <int BT, bool AKC, bool BKC, int EPI>
+void vl_launch_tile(const VlGemm& p, hipStream_t s) {
+  constexpr int LDS = 2 * (BT + BT) * 128;
+  const long long n = vl_up(p.M, BT) / BT * (vl_up(p.N, BT) / BT) * p.n_split;
+  BD_SET_MAX_LDS((vl_gemm_kernel<BT, BT, AKC, BKC, EPI>), LDS);
+  hipLaunchKernelGGL((vl_gemm_kernel<BT, BT, AKC, BKC, EPI>), dim3((unsigned)vl_up(n, 8)), dim3(2 * BT), LDS, s, p);
+}
 template <bool AKC, bool BKC, int EPI>
 void vl_launch(int big, const VlGemm& p, hipStream_t s) {
-  const int bt = big ? 256 : 128;
-  const long long n = vl_up(p.M, bt) / bt * (vl_up(p.N, bt) / bt) * p.n_split;
-  const dim3 grid((unsigned)vl_up(n, 8));
-  if (big) {
-    BD_SET_MAX_LDS((vl_gemm_kernel<256, 256, AKC, BKC, EPI>), 131072);
-    hipLaunchKernelGGL((vl_gemm_kernel<256, 256, AKC, BKC, EPI>), grid, dim3(512), 131072, s, p);
-  } else {
-    hipLaunchKernelGGL((vl_gemm_kernel<128, 128, AKC, BKC, EPI>), grid, dim3(256), 65536, s, p);
-  }
+  if (big) vl_launch_tile<256, AKC, BKC, EPI>(p, s);
+  else vl_launch_tile<128, AKC, BKC, EPI>(p, s);
 }
 
 int vl_check(long long M, int d, int V, const char* what) {
@@ -726,11 +745,11 @@ extern "C" int bd_linear_ce_fwd(const void* hidden, const void* weight, const lo
     hipLaunchKernelGGL(vl_narrow_finish_kernel, dim3(1), dim3(1024), 0, s, parts, blocks, loss);
     return bd_check_launch("bd_linear_ce_fwd");
   }
-  const int bz = pl.big_z ? 256 : 128;
+  const int bz = pl.big_s ? 256 : 128;
   VlGemm p = {};
   p.A = st.hc; p.lda = d; p.B = (const unsigned short*)weight; p.ldb = d; p.head = st.head;
   p.M = (int)pl.m_pad; p.N = V; p.n_rows = V; p.K = d; p.m_live = 1; p.n_split = 1; p.V = V; p.pairs = pairs;
-  vl_launch<true, true, VL_STATS>(pl.big_z, p, s);
+  vl_launch<true, true, VL_STATS>(pl.big_s, p, s);
   hipLaunchKernelGGL(vl_join_kernel, dim3((unsigned)((M + 3) / 4)), dim3(256), 0, s, st, (const unsigned short*)weight, pairs, rowloss,
                      (int)pl.m_pad, (V + bz - 1) / bz, d);
   hipLaunchKernelGGL(vl_finish_kernel, dim3(1), dim3(1024), 0, s, st, rowloss, loss);
