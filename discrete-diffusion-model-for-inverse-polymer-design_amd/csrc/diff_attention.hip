@@ -312,7 +312,7 @@ __device__ __forceinline__ void da_zero_tail(unsigned short* p, const long long*
 // Forward. Waves work in pairs: wave 2 w + m holds map m of the 16 QB slots of query group w (NQG groups in a
 // workgroup). Split over keys (n_split > 1): each split leaves its unnormalised sums, maximum and normaliser.
 // =====================================================================================
-template <int D, int QB, int NQG, int OCC>
+template <int D, int QB, int NQG, int OCC, bool TWO>
 __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
   constexpr int E = 2 * D, AF = D == 128 ? 3 : 6, KS = D / 32, DT = E / 16, NW = 2 * NQG, RK = 2 * D, RV = 2 * E;
   constexpr int TILE = KT * (2 * RK + RV), SLOTS = 16 * QB * NQG;
@@ -407,7 +407,7 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
                       for (int qb = 0; qb < QB; ++qb)
                         s[qb][i / KS] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[qb][i % KS], s[qb][i / KS], 0, 0, 0);
                     });
-    bf16x8 pf[QB][2];
+    bf16x8 pf[QB][2], pl[QB][2];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       if (vis != ~0ull) {
@@ -445,16 +445,23 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
         for (int r = 0; r < 4; ++r) {
           const float p = __builtin_amdgcn_exp2f(s[qb][t][r] * scale2 - msc);
           l_run[qb] += p;                                  // the lane's own keys; the four lanes of a slot are added up at the end
-          // weights to bf16 for the second product (half a step: 2^-8 of each weight; the normaliser keeps them in fp32)
-          pf[qb][t >> 1][4 * (t & 1) + r] = (__bf16)p;
+          // Weights to bf16 for the second product (half a step: 2^-8 of each weight; the normaliser keeps them in fp32). Split
+          // over the keys, the products wait for memory: there a second bf16 holds what the first left out (2^-16), for
+          // 23.2 -> 23.8 us at one row against 65 521 keys; with all keys in one workgroup it would be 16.9 -> 18.8 us (2 rows
+          // against 512 keys), and the large products would grow by half.
+          const __bf16 hi = (__bf16)p;
+          pf[qb][t >> 1][4 * (t & 1) + r] = hi;
+          if (TWO) pl[qb][t >> 1][4 * (t & 1) + r] = (__bf16)(p - (float)hi);
         }
     }
     // O^T += V^T P^T
     da_pipe<AF, 2 * DT>([&](int i) { return da_tr<RV>(vb, i & 1, i >> 1); },
                     [&](int i, bf16x8 vf) {
 #pragma unroll
-                      for (int qb = 0; qb < QB; ++qb)
+                      for (int qb = 0; qb < QB; ++qb) {
                         o[qb][i >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qb][i & 1], o[qb][i >> 1], 0, 0, 0);
+                        if (TWO) o[qb][i >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[qb][i & 1], o[qb][i >> 1], 0, 0, 0);
+                      }
                     });
     vis = vis_next;
     const unsigned sw = cur; cur = other; other = sw;
@@ -1095,14 +1102,16 @@ int da_forward(const bd_diff_attn_args& p, DaArgs& a, hipStream_t s) {
     a.part_ml = (float*)p.workspace;
     a.part = a.part_ml + ml * 2;
   }
-  if (few) {
-    BD_SET_MAX_LDS((da_fwd_kernel<D, 1, ROWS_NQG, 2>), LDS);
-    hipLaunchKernelGGL((da_fwd_kernel<D, 1, ROWS_NQG, 2>), dim3((unsigned)grid), dim3(128 * ROWS_NQG), LDS, s, a);
-    if (a.n_split > 1)
-      hipLaunchKernelGGL((da_join_kernel<D, ROWS_SLOTS>), dim3((unsigned)(slots * (2 * D / JOIN_COLS)), a.Hkv, a.B), dim3(256), 0, s, a);
+  if (a.n_split > 1) {
+    BD_SET_MAX_LDS((da_fwd_kernel<D, 1, ROWS_NQG, 2, true>), LDS);
+    hipLaunchKernelGGL((da_fwd_kernel<D, 1, ROWS_NQG, 2, true>), dim3((unsigned)grid), dim3(128 * ROWS_NQG), LDS, s, a);
+    hipLaunchKernelGGL((da_join_kernel<D, ROWS_SLOTS>), dim3((unsigned)(slots * (2 * D / JOIN_COLS)), a.Hkv, a.B), dim3(256), 0, s, a);
+  } else if (few) {
+    BD_SET_MAX_LDS((da_fwd_kernel<D, 1, ROWS_NQG, 2, false>), LDS);
+    hipLaunchKernelGGL((da_fwd_kernel<D, 1, ROWS_NQG, 2, false>), dim3((unsigned)grid), dim3(128 * ROWS_NQG), LDS, s, a);
   } else {
-    BD_SET_MAX_LDS((da_fwd_kernel<D, F::B, F::NQG, F::OCC>), LDS);
-    hipLaunchKernelGGL((da_fwd_kernel<D, F::B, F::NQG, F::OCC>), dim3((unsigned)grid), dim3(128 * F::NQG), LDS, s, a);
+    BD_SET_MAX_LDS((da_fwd_kernel<D, F::B, F::NQG, F::OCC, false>), LDS);
+    hipLaunchKernelGGL((da_fwd_kernel<D, F::B, F::NQG, F::OCC, false>), dim3((unsigned)grid), dim3(128 * F::NQG), LDS, s, a);
   }
   return bd_check_launch("bd_diff_attention_fwd");
 }
