@@ -39,9 +39,16 @@ struct DaArgs {
   const int* cu;
   long long qs[3], ks[3], vs[3], ls[3], os[3], dos[3], dqs[3], dks[3], dvs[3], mask_stride;
   int B, Lq, Lk, H, Hkv, share, total, lam_f32, dlam_bf16, n_blk, n_split;
+  unsigned share_mul, share_log; // s / share = (4 s share_mul >> 32) >> share_log for s < 2^30
   int small_strides;             // 64 rows of every operand lie within 4 GiB: staged by 32-bit offsets
   float scale;
 };
+
+// row and head (of those that share a key head) of slot s
+__device__ __forceinline__ void da_split(const DaArgs& a, int s, int& row, int& head) {
+  row = (int)(__umulhi(4u * (unsigned)s, a.share_mul) >> a.share_log);
+  head = s - row * a.share;
+}
 
 __device__ __attribute__((aligned(64))) const unsigned int bd_da_zero[16] = {};
 
@@ -217,8 +224,8 @@ __device__ __forceinline__ DaSlot da_slot(const DaArgs& a, int s, int n_slots, i
   DaSlot r;
   r.ok = s < n_slots;
   s = r.ok ? s : n_slots - 1;
-  r.row = s / a.share;
-  r.head = hk * a.share + (s - r.row * a.share);
+  da_split(a, s, r.row, r.head);
+  r.head += hk * a.share;
   return r;
 }
 // A value the compiler cannot connect with earlier ones: what is derived from it behind a loop is computed there instead of
@@ -237,6 +244,8 @@ __device__ __forceinline__ void da_put_dlam(const DaArgs& a, long long at, float
   else ((float*)a.dlam)[at] = v;
 }
 
+typedef __attribute__((address_space(1))) const unsigned char da_global_byte;      // (a generic load would count as an LDS read)
+
 // one past the last visible key of the sequence (the tiles behind it are not visited); all threads return it
 template <int NT>
 __device__ __forceinline__ int da_visible_end(const DaArgs& a, int b, int Lk, int tid, int* red) {
@@ -244,12 +253,12 @@ __device__ __forceinline__ int da_visible_end(const DaArgs& a, int b, int Lk, in
   const unsigned char* m = a.mask + b * a.mask_stride;
   int last = 0;
   if (Lk <= 512) {                                         // every wave by itself: eight loads in flight, no barrier
-    unsigned char x[8];
+    unsigned x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 64 * i + (tid & 63) < Lk ? m[64 * i + (tid & 63)] : 0;
+    for (int i = 0; i < 8; ++i) x[i] = *(da_global_byte*)(m + min(64 * i + (tid & 63), Lk - 1));
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const unsigned long long v = __ballot(x[i] != 0);
+      const unsigned long long v = __ballot(x[i] != 0u && 64 * i + (tid & 63) < Lk);
       last = v ? 64 * i + 64 - __builtin_clzll(v) : last;
     }
     return __builtin_amdgcn_readfirstlane(last);
@@ -265,12 +274,11 @@ __device__ __forceinline__ int da_visible_end(const DaArgs& a, int b, int Lk, in
   return __builtin_amdgcn_readfirstlane(last);      // (one value: the loops over key tiles count on the scalar unit)
 }
 
-// mask byte of the lane's key of a tile (0 past the end); a volatile load stays where it is written
+// mask byte of the lane's key of a tile (0 past the end)
 __device__ __forceinline__ unsigned da_mask_byte(const DaArgs& a, int b, int key, int end) {
   if (key >= end) return 0u;
   if (!a.mask) return 1u;
-  typedef __attribute__((address_space(1))) const volatile unsigned char global_byte;      // (a generic load would count as an LDS read)
-  return *(global_byte*)(a.mask + b * a.mask_stride + key);
+  return *(da_global_byte*)(a.mask + b * a.mask_stride + key);
 }
 
 // Workgroups are handed to the 8 XCDs in turn (blockIdx & 7). The blocks of one (sequence, key head) group share an XCD, so
@@ -857,20 +865,19 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
   const unsigned char* const sb0 = (const unsigned char*)(a.stats + 8 * ((bq * a.Lq + sp.q0) * a.H + hk * a.share));
   const bool even = a.small_strides && KT % a.share == 0;
   unsigned qo[PQ::N], dob[PD::N], so;
-  auto split = [&](int s, int& row, int& head) { row = s / a.share; head = s - row * a.share; };
   {
     int row, head;
 #pragma unroll
     for (int j = 0; j < PQ::N; ++j) {
-      split(PQ::row(wave, lane, j), row, head);
+      da_split(a, PQ::row(wave, lane, j), row, head);
       qo[j] = (unsigned)(2 * a.qs[1]) * row + (unsigned)(4 * a.qs[2]) * head + 16 * PQ::chunk(wave, lane, j);
     }
 #pragma unroll
     for (int j = 0; j < PD::N; ++j) {
-      split(PD::row(wave, lane, j), row, head);
+      da_split(a, PD::row(wave, lane, j), row, head);
       dob[j] = (unsigned)(2 * a.dos[1]) * row + (unsigned)(2 * a.dos[2]) * head + 16 * PD::chunk(wave, lane, j);
     }
-    split(lane, row, head);
+    da_split(a, lane, row, head);
     so = (unsigned)(row * a.H + head) * 32 + 16 * (wave & 1);
   }
   auto stage = [&](int t0, unsigned base) {
@@ -885,8 +892,10 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
     }
     auto at = [&](const unsigned char* p, long long rs, long long hs) {
       return [=](int r) {
-        const int s = t0 + r, row = s / a.share;
-        return s < n_slots ? p + row * rs + (s - row * a.share) * hs : (const unsigned char*)nullptr;
+        int row, head;
+        const int s = da_again(t0 + r);                    // (a last tile's: nothing of it is held through the loop)
+        da_split(a, s, row, head);
+        return s < n_slots ? p + row * rs + head * hs : (const unsigned char*)nullptr;
       };
     };
     da_stage<RK, NW>(base, wave, lane, at(qb0, 2 * a.qs[1], 4 * a.qs[2]));
@@ -1077,6 +1086,8 @@ int da_check(const bd_diff_attn_args& p, const char* what, DaArgs& a) {
     a.dos[i] = p.dout_stride[i]; a.dqs[i] = p.dq_stride[i]; a.dks[i] = p.dk_stride[i]; a.dvs[i] = p.dv_stride[i];
   }
   a.B = p.B; a.Lq = p.Lq; a.Lk = p.Lk; a.H = p.H; a.Hkv = p.Hkv; a.share = p.H / p.Hkv; a.total = p.total_rows;
+  for (a.share_log = 0; (1 << a.share_log) < a.share;) ++a.share_log;
+  a.share_mul = (unsigned)((1ull << (30 + a.share_log)) / a.share) + 1u;
   a.lam_f32 = p.lam_dtype == BD_DTYPE_F32; a.scale = p.scale; a.n_split = 1;
   a.small_strides = (long long)p.H * 32 * KT < (1ll << 31);
   for (int i = 1; i < 3; ++i)
