@@ -39,6 +39,7 @@ struct DaArgs {
   const int* cu;
   long long qs[3], ks[3], vs[3], ls[3], os[3], dos[3], dqs[3], dks[3], dvs[3], mask_stride;
   int B, Lq, Lk, H, Hkv, share, total, lam_f32, dlam_bf16, n_blk, n_split;
+  int per;                       // split over keys: slots of a workgroup of the forward
   unsigned share_mul, share_log; // s / share = (4 s share_mul >> 32) >> share_log for s < 2^30
   int small_strides;             // 64 rows of every operand lie within 4 GiB: staged by 32-bit offsets
   float scale;
@@ -453,10 +454,10 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
         for (int r = 0; r < 4; ++r) {
           const float p = __builtin_amdgcn_exp2f(s[qb][t][r] * scale2 - msc);
           l_run[qb] += p;                                  // the lane's own keys; the four lanes of a slot are added up at the end
-          // Weights to bf16 for the second product (half a step: 2^-8 of each weight; the normaliser keeps them in fp32). Split
-          // over the keys, the products wait for memory: there a second bf16 holds what the first left out (2^-16), for
-          // 23.2 -> 23.8 us at one row against 65 521 keys; with all keys in one workgroup it would be 16.9 -> 18.8 us (2 rows
-          // against 512 keys), and the large products would grow by half.
+          // Weights to bf16 for the second product (half a step: 2^-8 of each weight; the normaliser keeps them in fp32). A few
+          // rows split over the keys wait for memory, not for products: there a second bf16 holds what the first left out
+          // (2^-16), for 23.2 -> 23.8 us at one row against 65 521 keys; with all keys in one workgroup it would be 16.9 ->
+          // 18.8 us (2 rows against 512 keys), and the large products would grow by half.
           const __bf16 hi = (__bf16)p;
           pf[qb][t >> 1][4 * (t & 1) + r] = hi;
           if (TWO) pl[qb][t >> 1][4 * (t & 1) + r] = (__bf16)(p - (float)hi);
@@ -542,31 +543,56 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
   }
 }
 
-// Joins the key splits of one slot, 16 columns a workgroup: waves 2 m and 2 m + 1 add up map m, 16 splits at a time each
+// first of a slot's partial sums: [sequence and key head][block of slots][split][map][slot of the block]
+__device__ __forceinline__ long long da_part(const DaArgs& a, int b, int hk, int slot) {
+  const int blk = slot / a.per;
+  return ((long long)(b * a.Hkv + hk) * a.n_blk + blk) * a.n_split * 2 * a.per + (slot - blk * a.per);
+}
+
+// four columns of a slot whose maps' sums, maxima and normalisers are joined
+template <int D>
+__device__ __forceinline__ void da_joined(const DaArgs& a, int b, const DaSlot& sl, long long rh, int col, f32x4 (&r)[2], const float (&top)[2],
+                                          const float (&l)[2]) {
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const bool any = l[m] > 0.f || l[m] != l[m];
+    const float inv = any ? 1.0f / l[m] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[m][e] *= inv;
+    if (a.maps) *(f32x4*)(a.maps + (2 * rh + m) * 2 * D + col) = r[m];
+    if (a.lse && col == 0) a.lse[2 * rh + m] = any ? top[m] + __log2f(l[m]) : INFINITY;
+  }
+  const float lam = da_lam(a, b * a.ls[0] + sl.row * a.ls[1] + sl.head * a.ls[2]);
+  u32x2 w;
+  w[0] = bd_pack_bf16x2(r[0][0] - lam * r[1][0], r[0][1] - lam * r[1][1]);
+  w[1] = bd_pack_bf16x2(r[0][2] - lam * r[1][2], r[0][3] - lam * r[1][3]);
+  *(u32x2*)(a.out + b * a.os[0] + sl.row * a.os[1] + sl.head * a.os[2] + col) = w;
+}
+
+// Joins more than 16 key splits of one slot, 16 columns a workgroup: waves 2 m and 2 m + 1 add up map m, 16 splits at a time each
 // with 4 lanes across the columns, in a fixed order. Bound by latency (one row, 65 521 keys, 4 x 4 heads of 64, 128
 // splits: 16.8 MB of partial sums in all): what a thread adds up is asked for before the splits' maxima and normalisers
 // are worked into weights, and many small workgroups wait at once.
-constexpr int JOIN_COLS = 16, JOIN_SPLITS = 256;
-template <int D, int SLOTS>
+constexpr int JOIN_COLS = 16, JOIN_SPLITS = 256, JOIN_LANES = 16;
+template <int D>
 __global__ __launch_bounds__(256) void da_join_kernel(DaArgs a) {
   constexpr int E = 2 * D, CB = E / JOIN_COLS, N = JOIN_SPLITS / 32;
   __shared__ float wt[2][JOIN_SPLITS], red[2][2][4];
   __shared__ f32x4 sum[4][4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int slot = blockIdx.x / CB, col = (blockIdx.x % CB) * JOIN_COLS + 4 * (lane & 3), hk = blockIdx.y, b = blockIdx.z;
-  const int blk = slot / SLOTS, in_blk = slot - blk * SLOTS;
-  const int row = slot / a.share, head = hk * a.share + (slot - row * a.share);
-  const long long rh = ((long long)b * a.Lq + row) * a.H + head;
-  const long long at0 = ((long long)(b * a.Hkv + hk) * a.n_blk + blk) * a.n_split * 2 * SLOTS + in_blk;
+  const DaSlot sl = da_slot(a, slot, a.Lq * a.share, hk);
+  const long long rh = ((long long)b * a.Lq + sl.row) * a.H + sl.head;
+  const long long at0 = da_part(a, b, hk, slot);
   const int map = wave >> 1, s0 = (wave & 1) * 16 + (lane >> 2);
   f32x4 x[N];
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (s0 + 32 * i < a.n_split) x[i] = *(const f32x4*)(a.part + (at0 + (long long)(2 * (s0 + 32 * i) + map) * SLOTS) * E + col);
+    if (s0 + 32 * i < a.n_split) x[i] = *(const f32x4*)(a.part + (at0 + (long long)(2 * (s0 + 32 * i) + map) * a.per) * E + col);
   f32x2 ml[2] = {{-INFINITY, 0.f}, {-INFINITY, 0.f}};
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    if (tid < a.n_split) ml[m] = *(const f32x2*)(a.part_ml + 2 * (at0 + (long long)(2 * tid + m) * SLOTS));
+    if (tid < a.n_split) ml[m] = *(const f32x2*)(a.part_ml + 2 * (at0 + (long long)(2 * tid + m) * a.per));
     const float mx = bd_wave_max(ml[m][0]);
     if (lane == 0) red[0][m][wave] = mx;
   }
@@ -601,19 +627,50 @@ __global__ __launch_bounds__(256) void da_join_kernel(DaArgs a) {
   if (tid >= 4) return;
   f32x4 r[2];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    const bool any = l[m] > 0.f || l[m] != l[m];
-    const float inv = any ? 1.0f / l[m] : 0.f;
+  for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r[m][e] = (sum[2 * m][tid][e] + sum[2 * m + 1][tid][e]) * inv;
-    if (a.maps) *(f32x4*)(a.maps + (2 * rh + m) * E + col) = r[m];
-    if (a.lse && tid == 0 && col == 0) a.lse[2 * rh + m] = any ? top[m] + __log2f(l[m]) : INFINITY;
+    for (int e = 0; e < 4; ++e) r[m][e] = sum[2 * m][tid][e] + sum[2 * m + 1][tid][e];
+  da_joined<D>(a, b, sl, rh, col, r, top, l);
+}
+
+// The same for at most 16 splits (many slots: the launch is bound by the partial sums' way through memory): a wave takes
+// 16 (slot, split) pairs, four lanes across 16 columns each, and adds up by exchanges alone (2048 slots, 2 splits of 64-wide heads: 8.3 us).
+template <int D>
+__global__ __launch_bounds__(256) void da_join_few_kernel(DaArgs a) {
+  constexpr int E = 2 * D, CB = E / JOIN_COLS;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hk = blockIdx.y, b = blockIdx.z;
+  int lanes = 2;                                           // lanes (of four) that share a slot
+  while (lanes < a.n_split) lanes *= 2;
+  const int n_slots = a.Lq * a.share, pair = lane >> 2, split = pair & (lanes - 1), here = JOIN_LANES / lanes;
+  const int slot = ((int)(blockIdx.x / CB) * 4 + wave) * here + pair / lanes, col = (int)(blockIdx.x % CB) * JOIN_COLS + 4 * (lane & 3);
+  const DaSlot sl = da_slot(a, slot, n_slots, hk);
+  const long long rh = ((long long)b * a.Lq + sl.row) * a.H + sl.head;
+  const long long at0 = da_part(a, b, hk, min(slot, n_slots - 1));
+  f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  f32x2 ml[2] = {{-INFINITY, 0.f}, {-INFINITY, 0.f}};
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+    if (split < a.n_split) {
+      const long long at = at0 + (long long)(2 * split + m) * a.per;
+      ml[m] = *(const f32x2*)(a.part_ml + 2 * at);
+      x[m] = *(const f32x4*)(a.part + at * E + col);
+    }
+  float top[2], l[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    top[m] = ml[m][0];
+    for (int s = 4; s < 4 * lanes; s *= 2) top[m] = fmaxf(top[m], __shfl_xor(top[m], s, 64));
+    const float w = ml[m][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[m][0] - top[m]);
+    l[m] = w * ml[m][1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[m][e] = w == 0.f ? 0.f : w * x[m][e];
+    for (int s = 4; s < 4 * lanes; s *= 2) {
+      l[m] += __shfl_xor(l[m], s, 64);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[m][e] += __shfl_xor(x[m][e], s, 64);
+    }
   }
-  const float lam = da_lam(a, b * a.ls[0] + row * a.ls[1] + head * a.ls[2]);
-  u32x2 w;
-  w[0] = bd_pack_bf16x2(r[0][0] - lam * r[1][0], r[0][1] - lam * r[1][1]);
-  w[1] = bd_pack_bf16x2(r[0][2] - lam * r[1][2], r[0][3] - lam * r[1][3]);
-  *(u32x2*)(a.out + b * a.os[0] + row * a.os[1] + head * a.os[2] + col) = w;
+  if (split == 0 && sl.ok) da_joined<D>(a, b, sl, rh, col, x, top, l);
 }
 
 // =====================================================================================
@@ -1048,19 +1105,28 @@ template <> struct DaFwd<32> : DaFCfg<2, 2, 4> {};
 template <> struct DaFwd<128> : DaFCfg<2, 4, 2> {};
 constexpr int ROWS_NQG = 2, ROWS_SLOTS = 16 * ROWS_NQG;                         // few slots: 32, 4 waves of 16
 
-int da_splits(const bd_diff_attn_args& p) {
-  // few slots against many keys: enough splits of whole key tiles for two workgroups per CU, four tiles each at least
-  if (p.cu_seqlens) return 1;
-  const long long slots = (long long)p.Lq * (p.H / p.Hkv);
-  if (slots > 128) return 1;
-  const long long blocks = (long long)p.B * p.Hkv * ((slots + ROWS_SLOTS - 1) / ROWS_SLOTS);
-  const int tiles = (p.Lk + KT - 1) / KT;
-  long long n = 512 / (blocks > 0 ? blocks : 1);
-  if (n > tiles / 4) n = tiles / 4;
-  return n < 1 ? 1 : n > JOIN_SPLITS ? JOIN_SPLITS : (int)n;
-}
+// The forward of a call. Half of the large workgroup's slots or fewer: the workgroup of 32 (measured, this / the large one: 2
+// rows against 512 keys x 6 heads of 64 in 64 sequences 15.6 / 20.1 us, 32 rows 16.1 / 21.1, 64 rows 23.4 / 22.5; heads of
+// 128, 32 rows 31.5 / 57.5, 64 rows 46.4 / 58.8). Split over the keys where the workgroups leave CUs without work, one a CU,
+// if that gives a split enough key tiles: 2 for the workgroup of 32 (one row against 4096 keys, 4 heads of 64 over
+// 4 key heads: 10.3 us, with 4 tiles 11.9, with 8 15.5), else 16 (1024 rows against 1024 keys, 8 heads of 64: 20.0 us unsplit,
+// 28.5 with 8 tiles, 33.0 with 4; 128 rows against 4096 keys, 16 heads over 4: unsplit 62, split in four 30). 65 521 keys, 16 heads over
+// 4, split / unsplit: 16 rows 37 / 927 us, 128 rows 150 / 937, 512 rows 561 / 944.
+struct DaPlan { bool few; int per, n_blk, n_split; };
 
-bool da_few(const bd_diff_attn_args& p) { return (long long)p.Lq * (p.H / p.Hkv) <= ROWS_SLOTS || da_splits(p) > 1; }
+DaPlan da_plan(const bd_diff_attn_args& p) {
+  const long long slots = (long long)p.Lq * (p.H / p.Hkv);
+  const int large = p.head_dim == 128 ? DaFwd<128>::SLOTS : p.head_dim == 64 ? DaFwd<64>::SLOTS : DaFwd<32>::SLOTS;
+  DaPlan r;
+  r.few = 2 * slots <= large;
+  r.per = r.few ? ROWS_SLOTS : large;
+  r.n_blk = (int)((slots + r.per - 1) / r.per);
+  const int most = (p.Lk + KT - 1) / KT / (r.few ? 2 : 16);
+  long long n = 256 / ((long long)p.B * p.Hkv * r.n_blk);
+  if (n > most) n = most;
+  r.n_split = p.cu_seqlens || n < 1 ? 1 : n > JOIN_SPLITS ? JOIN_SPLITS : (int)n;
+  return r;
+}
 
 int da_check(const bd_diff_attn_args& p, const char* what, DaArgs& a) {
   BD_REQUIRE(p.q && p.k && p.v && p.lam, "%s: null operand", what);
@@ -1101,28 +1167,34 @@ int da_forward(const bd_diff_attn_args& p, DaArgs& a, hipStream_t s) {
   constexpr int LDS = 2 * KT * 8 * D;
   const long long slots = (long long)a.Lq * a.share;
   const int seqs = a.B + (a.cu ? 1 : 0);
-  a.n_split = da_splits(p);
-  const bool few = da_few(p);
-  typedef DaFwd<D> F;
-  const int per = few ? ROWS_SLOTS : F::SLOTS;
-  a.n_blk = (int)((slots + per - 1) / per);
+  const DaPlan pl = da_plan(p);
+  a.n_split = pl.n_split; a.n_blk = pl.n_blk; a.per = pl.per;
   const long long grid = da_grid((long long)a.n_blk * a.n_split, (long long)a.Hkv * seqs);
   BD_REQUIRE(grid < (1ll << 31), "bd_diff_attention_fwd: too many workgroups");
   if (a.n_split > 1) {
-    const long long ml = (long long)a.n_blk * a.n_split * a.Hkv * a.B * 2 * ROWS_SLOTS;
     a.part_ml = (float*)p.workspace;
-    a.part = a.part_ml + ml * 2;
+    a.part = a.part_ml + (long long)a.n_blk * a.n_split * a.Hkv * a.B * 2 * a.per * 2;
   }
-  if (a.n_split > 1) {
-    BD_SET_MAX_LDS((da_fwd_kernel<D, 1, ROWS_NQG, 2, true>), LDS);
-    hipLaunchKernelGGL((da_fwd_kernel<D, 1, ROWS_NQG, 2, true>), dim3((unsigned)grid), dim3(128 * ROWS_NQG), LDS, s, a);
-    hipLaunchKernelGGL((da_join_kernel<D, ROWS_SLOTS>), dim3((unsigned)(slots * (2 * D / JOIN_COLS)), a.Hkv, a.B), dim3(256), 0, s, a);
-  } else if (few) {
+  typedef DaFwd<D> F;
+  if (!pl.few) {
+    BD_SET_MAX_LDS((da_fwd_kernel<D, F::B, F::NQG, F::OCC, false>), LDS);
+    hipLaunchKernelGGL((da_fwd_kernel<D, F::B, F::NQG, F::OCC, false>), dim3((unsigned)grid), dim3(128 * F::NQG), LDS, s, a);
+  } else if (a.n_split == 1) {
     BD_SET_MAX_LDS((da_fwd_kernel<D, 1, ROWS_NQG, 2, false>), LDS);
     hipLaunchKernelGGL((da_fwd_kernel<D, 1, ROWS_NQG, 2, false>), dim3((unsigned)grid), dim3(128 * ROWS_NQG), LDS, s, a);
   } else {
-    BD_SET_MAX_LDS((da_fwd_kernel<D, F::B, F::NQG, F::OCC, false>), LDS);
-    hipLaunchKernelGGL((da_fwd_kernel<D, F::B, F::NQG, F::OCC, false>), dim3((unsigned)grid), dim3(128 * F::NQG), LDS, s, a);
+    BD_SET_MAX_LDS((da_fwd_kernel<D, 1, ROWS_NQG, 2, true>), LDS);
+    hipLaunchKernelGGL((da_fwd_kernel<D, 1, ROWS_NQG, 2, true>), dim3((unsigned)grid), dim3(128 * ROWS_NQG), LDS, s, a);
+  }
+  if (a.n_split > 1) {
+    constexpr int CB = 2 * D / JOIN_COLS;
+    int lanes = 2;
+    while (lanes < a.n_split) lanes *= 2;
+    if (a.n_split <= JOIN_LANES)      // (16 splits of 512 slots x 4 key heads: 14.8 us, the other way 39.6)
+      hipLaunchKernelGGL((da_join_few_kernel<D>), dim3((unsigned)((slots * lanes + 4 * JOIN_LANES - 1) / (4 * JOIN_LANES) * CB), a.Hkv, a.B), dim3(256),
+                         0, s, a);
+    else
+      hipLaunchKernelGGL((da_join_kernel<D>), dim3((unsigned)(slots * CB), a.Hkv, a.B), dim3(256), 0, s, a);
   }
   return bd_check_launch("bd_diff_attention_fwd");
 }
@@ -1162,10 +1234,8 @@ extern "C" long long bd_diff_attention_workspace_bytes(const bd_diff_attn_args* 
   if (!p || p->B <= 0 || p->Lq <= 0 || p->Lk <= 0 || p->H <= 0 || p->Hkv <= 0 || p->H % p->Hkv) return -1;
   const long long rows = p->cu_seqlens ? p->total_rows : (long long)p->B * p->Lq;
   if (backward) return rows * p->H * 32;
-  const int n = da_splits(*p);
-  if (n == 1) return 0;
-  const long long slots = (long long)p->Lq * (p->H / p->Hkv), blocks = (slots + ROWS_SLOTS - 1) / ROWS_SLOTS;
-  return blocks * n * p->Hkv * p->B * 2 * ROWS_SLOTS * (2 + 2 * (long long)p->head_dim) * 4;
+  const DaPlan r = da_plan(*p);
+  return r.n_split == 1 ? 0 : (long long)r.n_blk * r.n_split * p->Hkv * p->B * 2 * r.per * (2 + 2 * (long long)p->head_dim) * 4;
 }
 
 extern "C" int bd_diff_attention_fwd(const bd_diff_attn_args* p, void* stream) {

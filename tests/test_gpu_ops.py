@@ -265,6 +265,23 @@ def test_differential_attention_extreme_scores(gpu_device):
                 within(x, r[name].view(x.shape), r[name + "_tol"].view(x.shape), name)
 
 
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D,mask,lam", [
+    (1, 40, 2100, 2, 2, 64, "holes", "token"), (2, 33, 2049, 4, 2, 64, "empty", "head"), (1, 70, 4200, 4, 1, 128, None, "token"), (1, 100, 3300, 2, 1, 32, "tail", "row"),
+    (1, 16, 9000, 4, 1, 64, None, "token"), (1, 9, 1200, 6, 1, 128, "holes", "token"), (3, 5, 260, 3, 3, 32, "tail", "negative"), (1, 31, 2048, 1, 1, 64, "holes", "one"),
+])
+def test_differential_attention_split_over_keys(gpu_device, B, Lq, Lk, H, Hkv, D, mask, lam):
+    """Workgroups of either size with their keys split, joined from few and from many splits; splits without a visible key."""
+    q, k, v, lm, m, dout = attention_case(gpu_device, B, Lq, Lk, H, Hkv, D, mask, lam, seed=Lk)
+    r = reference(q, k, v, lm, m, dout, H)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lm)]
+    out = ops.differential_attention(*leaves, m)
+    within(out.detach(), r["out"].view(out.shape), r["out_tol"].view(out.shape), "out")
+    for name, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, dout)):
+        within(x, r[name].view(x.shape), r[name + "_tol"].view(x.shape), name)
+    with torch.no_grad():
+        assert torch.equal(ops.differential_attention(*leaves, m), out)
+
+
 def test_differential_attention_long_cache_offsets(gpu_device):
     """Keys whose byte offset passes 32 bits: rows of a buffer of more than 4 GiB, strided."""
     dev = gpu_device
