@@ -19,9 +19,6 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
-# beyond this many keys the forward of a training step leaves each map's output in fp32 for the backward (16 * head_dim
-# bytes a row and head); up to here the backward walks the keys once more instead
-_MAPS_KEYS = 128
 
 # The argument blocks are packed by ``struct`` (a ctypes structure costs a call per field; a small call is host-bound)
 _ROTARY_TENSOR = struct.Struct("PP6qi4x")
@@ -69,6 +66,15 @@ def _same_device(what, first, *others):
 def _like(t):
     """A contiguous tensor of ``t``'s shape, dtype and device, not filled."""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _keeps_maps(Lk, D):
+    """Beyond 8 keys for each value of a head the forward of a training step leaves each map's output in fp32 for the backward
+    (16 * head_dim bytes a row and head); up to there the backward walks the keys once more instead. Measured, all kernels of
+    a step, maps kept / keys walked twice: 3 heads of 64, 256 x 128 tokens 140 / 122 us, 64 x 512 211 / 203, 42 x 768 262 / 272,
+    16 x 2048 440 / 479; heads of 128, 32 x 512 263 / 243, 16 x 1024 447 / 458, 8 x 2048 736 / 813; heads of 32, 256 x 128
+    73 / 69, 128 x 256 92 / 90, 96 packed sequences of up to 509 267 / 282."""
+    return Lk > 8 * D
 
 
 def _rows_of_16_bytes(t):
@@ -304,9 +310,9 @@ def _attention_forward(q, k, v, lam, lam_strides, key_mask, cu, longest, scale, 
     lse = maps = 0
     if training:
         n_lse = (rows * H * 2 + 3) // 4 * 4
-        saved = torch.empty(n_lse + (rows * H * 4 * D if Lk > _MAPS_KEYS else 0), dtype=torch.float32, device=dev)
+        saved = torch.empty(n_lse + (rows * H * 4 * D if _keeps_maps(Lk, D) else 0), dtype=torch.float32, device=dev)
         lse = saved.data_ptr()
-        maps = lse + 4 * n_lse if Lk > _MAPS_KEYS else 0
+        maps = lse + 4 * n_lse if _keeps_maps(Lk, D) else 0
     if ws_bytes:
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with _on(dev) as stream:
@@ -318,13 +324,13 @@ def _attention_forward(q, k, v, lam, lam_strides, key_mask, cu, longest, scale, 
 def _attention_backward(q, k, v, lam, lam_strides, key_mask, cu, longest, scale, saved, dout, dq, dk, dv, dlam):
     """Writes dq, dk, dv (any strides the kernels take) and dlam (lam's shape and dtype, contiguous)."""
     sizes = _attention_sizes(q, k, v, cu, longest)
-    _, _, Lk, H, _, _, packed, rows = sizes
+    _, _, Lk, H, _, D, packed, rows = sizes
     # a weight for every (row, head): its gradient is written as it comes; one that was broadcast: summed from fp32
     whole = lam.numel() == rows * H
     need = (_attention_workspace(*sizes, True) + 15) // 16 * 16
     ws = torch.empty(need + (0 if whole else 4 * rows * H), dtype=torch.uint8, device=q.device)
     wp, lse = ws.data_ptr(), saved.data_ptr()
-    maps = lse + 4 * ((rows * H * 2 + 3) // 4 * 4) if Lk > _MAPS_KEYS else 0
+    maps = lse + 4 * ((rows * H * 2 + 3) // 4 * 4) if _keeps_maps(Lk, D) else 0
     with _on(q.device) as stream:
         _attention_call("bd_diff_attention_bwd", sizes, q, k, v, lam, lam_strides, key_mask, cu, scale, None, lse, maps, wp, need,
                         (dout, dq, dk, dv, dlam.data_ptr() if whole else wp + need, _DTYPES[lam.dtype] if whole else 1), stream)

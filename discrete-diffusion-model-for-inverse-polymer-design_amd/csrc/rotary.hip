@@ -10,6 +10,9 @@
 // Bound by memory: every value is read and written once. A thread turns one unit of 2 x 16 bytes (8 bf16 or 4 fp32
 // pairs) of up to four heads: the unit's table entries stay in its registers, neighbouring lanes take neighbouring
 // units and heads of one token (whole lines, the same table row), and the loads of all its heads are in flight together.
+// Measured: 30 011 tokens x 20 heads of 128 in fp32, half of each turned, 115 us (614 MB read and written: 5.3 TB/s; a large
+// copy runs at 4.9); 256 x 128 tokens x 6 heads of 128 in bf16 18.2 us (101 MB: 5.5 TB/s, part of it from the last-level
+// cache); 64 x 2 tokens x 24 heads of 64 3.5 us, a launch's latency.
 #include "bd_common.h"
 #include "bd_prof.h"
 #include "bidiff.h"
@@ -182,7 +185,8 @@ int rotary_launch(RotArgs& a, bool vec, bool in_place, hipStream_t s) {
   if (vec) {
     a.units = a.rd / (2 * N);
     a.tail = in_place ? 0 : (a.D - a.rd) / N;
-    // four heads a thread where that still leaves more threads than the card holds at once (256 CUs x 2048)
+    // four heads a thread where that still leaves more threads than the card holds at once (256 CUs x 2048). Measured, one head
+    // a thread / four: the fp32 case above 117.5 / 116.2 us (the 2 it takes: 115.5), 64 x 2 tokens x 24 heads 3.5 / 5.1
     const int per = a.units + a.tail;
     int g = 1;
     while (g < 4 && tokens * ((a.heads + 2 * g - 1) / (2 * g)) * per >= 256 * 2048) g *= 2;
