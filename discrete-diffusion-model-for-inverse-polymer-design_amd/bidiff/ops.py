@@ -221,11 +221,14 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, posi
 
 def rotary_(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, positions: Optional[torch.Tensor] = None,
             interleaved: bool = False, inverse: bool = False):
-    """``rotary`` in place, for inference and for kernels' own buffers (no gradient is recorded). ``inverse`` turns back."""
+    """``rotary`` in place, for inference and for kernels' own buffers (no gradient is recorded; q and k must not share values).
+    ``inverse`` turns back."""
     xs = [q] if k is None else [q, k]
     positions = _rotary_check(xs, table, positions)
     if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
         raise RuntimeError("rotary_: in place on a tensor that requires grad; use rotary")
+    if k is not None and q.numel() and q.data_ptr() == k.data_ptr():
+        raise ValueError("rotary_: q and k are the same memory; it would turn twice")
     for x in xs:
         if x.numel() and x.stride(-1) != 1:
             raise ValueError("rotary_: the last axis must be contiguous")
@@ -369,9 +372,9 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     D = 32, 64 or 128, H a multiple of Hkv; returns [B, Lq, H, 2 D]. ``lam`` (bf16 or fp32) broadcasts to [B, Lq, H]: a
     weight per head, or one for each row. ``key_mask`` [B, Lk]: non-zero = visible; a query without a visible key gives
     zeros, and what masked keys and values hold reaches nothing (their gradients are zeros). Packed rows: the same tensors
-    without the batch axis, ``cu_seqlens`` int [sequences + 1] (rows cu[b] .. cu[b + 1] - 1 belong to sequence b, rows
-    behind the last come out zero), ``max_seqlen`` the longest (None: read back from the device; rows of a longer sequence
-    come out NaN), ``key_mask`` [sequences, max_seqlen]. ``scale`` defaults to 1 / sqrt(D)."""
+    without the batch axis, ``cu_seqlens`` int [sequences + 1] (rows cu[b] .. cu[b + 1] - 1 belong to sequence b; offsets
+    that do not fall; rows before the first and behind the last sequence come out zero), ``max_seqlen`` the longest (None: read
+    back from the device; a longer sequence's rows from there on come out NaN, in the gradients too), ``key_mask`` [sequences, max_seqlen]. ``scale`` defaults to 1 / sqrt(D)."""
     _same_device("differential_attention", q, k, v, lam, key_mask, cu_seqlens)
     packed = cu_seqlens is not None
     dims = 3 if packed else 4

@@ -307,13 +307,27 @@ __device__ __forceinline__ bool da_block(int n_blk, int n_heads, int seqs, int& 
 }
 inline long long da_grid(long long n_blk, long long groups) { return n_blk * ((groups + 7) / 8) * 8; }
 
-// packed rows that belong to no sequence (behind cu[B]): zeros, heads hk * share .. of width W
-__device__ __forceinline__ void da_zero_tail(unsigned short* p, const long long* st, int first, int end, int head0, int heads,
-                                             int W, int tid, int nt) {
+// rows first .. end - 1 of heads head0 .. of width W, every 32 bits of them set to `word`
+__device__ __forceinline__ void da_fill(unsigned short* p, const long long* st, int first, int end, unsigned word, int head0, int heads, int W,
+                                        int tid, int nt) {
   const int per = heads * (W / 8);
   for (long long i = tid; i < (long long)(end - first) * per; i += nt) {
     const int row = first + (int)(i / per), r = (int)(i % per);
-    *(u32x4*)(p + row * st[1] + (long long)(head0 + r / (W / 8)) * st[2] + 8 * (r % (W / 8))) = (u32x4){0u, 0u, 0u, 0u};
+    *(u32x4*)(p + row * st[1] + (long long)(head0 + r / (W / 8)) * st[2] + 8 * (r % (W / 8))) = (u32x4){word, word, word, word};
+  }
+}
+// Packed rows that no sequence's workgroups write (one workgroup a head, all NT threads): zeros before the first and behind
+// the last sequence, NaN (no silence) in a sequence longer than announced, from its row Lq on.
+template <int NT, typename Fill>
+__device__ __forceinline__ void da_unclaimed(const DaArgs& a, int tid, Fill fill) {
+  fill(0, min(max(a.cu[0], 0), a.total), 0u);
+  fill(min(max(a.cu[a.B], 0), a.total), a.total, 0u);
+  int longer = 0;
+  for (int i = tid; i < a.B; i += NT) longer |= min(a.cu[i + 1], a.total) - max(a.cu[i], 0) > a.Lq;
+  const int n = __syncthreads_or(longer) ? a.B : 0;
+  for (int i = 0; i < n; ++i) {
+    const int lo = min(max(a.cu[i], 0), a.total), hi = min(max(a.cu[i + 1], lo), a.total);
+    if (hi - lo > a.Lq) fill(lo + a.Lq, hi, 0x7fc07fc0u);
   }
 }
 
@@ -335,20 +349,11 @@ __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
   if (!da_block(a.n_blk * a.n_split, a.Hkv, a.B + (a.cu ? 1 : 0), blk, hk, b)) return;
   const int split = blk % a.n_split;
   blk /= a.n_split;
-  if (a.cu && b == a.B) {                                  // (packed: one more sequence, the rows behind the last one)
-    if (blk == 0) {
-      da_zero_tail(a.out, a.os, min(max(a.cu[a.B], 0), a.total), a.total, hk * a.share, a.share, E, tid, 64 * NW);
-      // a sequence longer than Lq: its rows past Lq are NaN, not silence
-      int longer = 0;
-      for (int i = tid; i < a.B; i += 64 * NW) longer |= min(a.cu[i + 1], a.total) - max(a.cu[i], 0) > a.Lq;
-      const int n = __syncthreads_or(longer) ? a.B : 0;
-      for (int i = 0; i < n; ++i) {
-        const int lo = min(max(a.cu[i], 0), a.total), hi = min(max(a.cu[i + 1], lo), a.total);
-        for (long long r = lo + (long long)a.Lq; r < hi; ++r)
-          for (int e = tid; e < a.share * E; e += 64 * NW)
-            a.out[r * a.os[1] + (long long)(hk * a.share + e / E) * a.os[2] + e % E] = 0x7fc0;
-      }
-    }
+  if (a.cu && b == a.B) {                                  // (packed: one more sequence, the rows of none)
+    if (blk == 0)
+      da_unclaimed<64 * NW>(a, tid, [&](int first, int end, unsigned word) {
+        da_fill(a.out, a.os, first, end, word, hk * a.share, a.share, E, tid, 64 * NW);
+      });
     return;
   }
   const DaSpan sp = da_span(a, b);
@@ -692,12 +697,12 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
   int blk, hk, b;
   if (!da_block(a.n_blk, a.Hkv, a.B + (a.cu ? 1 : 0), blk, hk, b)) return;
   if (a.cu && b == a.B) {
-    if (blk == 0) {
-      const int first = min(max(a.cu[a.B], 0), a.total);
-      da_zero_tail(a.dq, a.dqs, first, a.total, 2 * hk * a.share, 2 * a.share, D, tid, 64 * NW);
-      for (long long i = tid; i < (long long)(a.total - first) * a.share; i += 64 * NW)
-        da_put_dlam(a, (first + i / a.share) * a.H + hk * a.share + i % a.share, 0.f);
-    }
+    if (blk == 0)
+      da_unclaimed<64 * NW>(a, tid, [&](int first, int end, unsigned word) {
+        da_fill(a.dq, a.dqs, first, end, word, 2 * hk * a.share, 2 * a.share, D, tid, 64 * NW);
+        for (long long i = tid; i < (long long)(end - first) * a.share; i += 64 * NW)
+          da_put_dlam(a, (first + i / a.share) * a.H + hk * a.share + i % a.share, word ? __uint_as_float(0x7fc00000u) : 0.f);
+      });
     return;
   }
   const DaSpan sp = da_span(a, b);
@@ -875,11 +880,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
   int blk, hk, b;
   if (!da_block(a.n_blk, a.Hkv, a.B + (a.cu ? 1 : 0), blk, hk, b)) return;
   if (a.cu && b == a.B) {
-    if (blk == 0) {
-      const int first = min(max(a.cu[a.B], 0), a.total);
-      da_zero_tail(a.dk, a.dks, first, a.total, 2 * hk, 2, D, tid, 64 * NW);
-      da_zero_tail(a.dv, a.dvs, first, a.total, hk, 1, E, tid, 64 * NW);
-    }
+    if (blk == 0)
+      da_unclaimed<64 * NW>(a, tid, [&](int first, int end, unsigned word) {
+        da_fill(a.dk, a.dks, first, end, word, 2 * hk, 2, D, tid, 64 * NW);
+        da_fill(a.dv, a.dvs, first, end, word, hk, 1, E, tid, 64 * NW);
+      });
     return;
   }
   const DaSpan sp = da_span(a, b);
@@ -1157,7 +1162,7 @@ int da_check(const bd_diff_attn_args& p, const char* what, DaArgs& a) {
   a.lam_f32 = p.lam_dtype == BD_DTYPE_F32; a.scale = p.scale; a.n_split = 1;
   a.small_strides = (long long)p.H * 32 * KT < (1ll << 31);
   for (int i = 1; i < 3; ++i)
-    a.small_strides = a.small_strides && (p.q_stride[i] | p.k_stride[i] | p.v_stride[i] | p.dout_stride[i]) < (1ll << 24);
+    a.small_strides = a.small_strides && (unsigned long long)(p.q_stride[i] | p.k_stride[i] | p.v_stride[i] | p.dout_stride[i]) < (1ull << 24);
   a.lse = p.lse; a.maps = p.maps;
   return BD_OK;
 }

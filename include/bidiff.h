@@ -791,8 +791,8 @@ int bd_rotary(const bd_rotary_tensor* tensors, int n_tensors, const float* table
  * (width 2 head_dim), hk = h / (H / Hkv). lam: one weight per (row, head), bf16 or fp32 (BD_DTYPE_*).
  * Padded batches: B sequences of Lq queries and Lk keys; key_mask (non-zero = visible) or null. Packed rows: cu_seqlens
  * [B + 1] (int32, device), sequence b = rows cu[b] .. cu[b + 1] - 1 of all operands, Lq = Lk = the longest sequence,
- * total_rows rows in all (batch strides are not used; rows behind cu[B] become zero in every output, rows of a sequence
- * behind Lq become NaN in out). What masked keys hold never reaches a result. Strides are in elements (batch, row,
+ * total_rows rows in all (batch strides are not used; offsets must not fall; rows before cu[0] and behind cu[B] become
+ * zero in every output, rows of a sequence from its row Lq on NaN). What masked keys hold never reaches a result. Strides are in elements (batch, row,
  * head), multiples of 8 but for lam's (0 = shared), the last axis is contiguous; operands are 16-byte aligned.
  * Training: lse [rows, H, 2] fp32 (base-2 log-sum-exp of the scaled scores; rows counted through the batch) and, beyond
  * short sequences, maps [rows, H, 2, 2 head_dim] fp32 (each map's own output) are written by the forward and read by

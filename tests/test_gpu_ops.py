@@ -238,6 +238,26 @@ def test_differential_attention_packed_rows_longer_than_announced_are_nan(gpu_de
     assert bool(torch.isnan(out[12:16]).all()) and bool(torch.isfinite(out[:12]).all()) and bool(torch.isfinite(out[16:]).all())
 
 
+def test_differential_attention_packed_rows_of_no_sequence(gpu_device):
+    """Zeros before the first and behind the last sequence; in a sequence longer than announced NaN from there on, in every
+    gradient as well; the rows of the other sequences as if they were alone."""
+    dev, g = gpu_device, gen(gpu_device, 21)
+    x = [torch.randn(70, h, w, generator=g, device=dev).to(BF).requires_grad_(True) for h, w in ((4, 32), (4, 32), (2, 64))]
+    lam = torch.rand(70, 2, generator=g, device=dev).requires_grad_(True)
+    dout = torch.randn(70, 2, 64, generator=g, device=dev).to(BF)
+    cu = torch.tensor([3, 9, 9, 40, 60], dtype=torch.int32, device=dev)
+    out = ops.differential_attention(*x, lam, cu_seqlens=cu, max_seqlen=25)
+    grads = torch.autograd.grad(out, (*x, lam), dout)
+    for y in (out.detach(), *grads):
+        assert not bool(y[:3].any()) and not bool(y[60:].any())
+        assert bool(torch.isnan(y[34:40].float()).all()) and bool(torch.isfinite(y[:34].float()).all()) and bool(torch.isfinite(y[40:].float()).all())
+    for a, b in ((3, 9), (40, 60)):
+        one = [t.detach()[a:b].requires_grad_(True) for t in (*x, lam)]
+        alone = ops.differential_attention(*one, cu_seqlens=torch.tensor([0, b - a], dtype=torch.int32, device=dev), max_seqlen=25)
+        assert torch.equal(alone, out[a:b])
+        assert all(torch.equal(s, t[a:b]) for s, t in zip(torch.autograd.grad(alone, one, dout[a:b]), grads))
+
+
 def test_differential_attention_without_rows_or_keys(gpu_device):
     dev = gpu_device
     for B, Lq, Lk in ((0, 3, 4), (2, 0, 4), (2, 3, 0)):

@@ -176,3 +176,11 @@ def test_rotary_refuses_at_the_c_abi(change):
         x.src_stride[:], x.dst_stride[:] = (8, 8, 8), a["dst_stride"]
     assert _lib.lib().bd_rotary(t, a["n"], a["table"], a["rows"], None, 0, a["B"], a["L"], a["D"], a["rd"], 0, 0, a["dtype"], None) == -1
     assert b"bd_rotary" in _lib.lib().bd_last_error()
+
+
+def test_rotary_in_place_refuses_the_same_memory_twice():
+    x = z(1, 3, 4, 8)
+    with pytest.raises(ValueError, match="same memory"):
+        ops.rotary_(x, x, TABLE)
+    with pytest.raises(ValueError, match="same memory"):
+        ops.rotary_(x, x[:, :, :2], TABLE)
