@@ -56,13 +56,13 @@ __device__ __attribute__((aligned(64))) const unsigned int bd_da_zero[16] = {};
 typedef __attribute__((address_space(3))) void da_lds;
 
 // A staged tile has rows of R bytes; 16-byte chunk ch of row `row` sits at chunk ch ^ f(row). The XOR spreads what is read
-// at a time over the banks: eight rows 0-3 / 8-11 (or 4-7 / 12-15) at one chunk by ds_read_b128, four neighbouring rows of
-// 32 bytes by the transposing read.
+// at a time over the banks: by ds_read_b128 four times four neighbouring rows, two groups at one chunk and two at its neighbour;
+// by the transposing read two groups of four neighbouring rows, 32 bytes each.
 template <int R>
 __device__ __forceinline__ int da_off(int row, int ch) {
   const int f = R >= 256 ? (((row & 3) << 2) | ((row >> 2) & 3))
               : R == 128 ? ((((row >> 1) & 1) << 2) | (((row >> 3) & 1) << 1) | ((row >> 2) & 1))
-                         : ((row >> 3) & 3);
+                         : ((row >> 3) & 1) << 1;
   return R * row + 16 * (ch ^ f);
 }
 
