@@ -134,6 +134,13 @@ __device__ __forceinline__ void da_dma16s(const void* base, unsigned off, unsign
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 
+// A value the compiler cannot connect with earlier ones: what is derived from it behind a loop is computed there instead of
+// being held in registers through it.
+__device__ __forceinline__ int da_again(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // Staging of KT rows of R bytes in 1-KiB pieces dealt to NW waves: where in the tile a lane's 16 bytes of piece j land
 template <int R, int NW>
 struct DaPieces {
@@ -154,7 +161,21 @@ __device__ __forceinline__ void da_stage_fast(unsigned lds, int wave, const unsi
   for (int j = 0; j < DaPieces<R, NW>::N; ++j)
     if (DaPieces<R, NW>::any(wave, j)) da_dma16s(from, off[j], lds + (wave + NW * j) * 1024);
 }
-// row_ptr(row) = the row's first byte, or null for a row that is to be zeros
+// The same for a tile of which some rows are to be zeros: there(row) tells which are fetched. The zeros are written by the
+// lanes whose rows are not (the buffer is nobody's until the next barrier, which waits for both).
+template <int R, int NW, typename There>
+__device__ __forceinline__ void da_stage_some(unsigned lds, int wave, int lane, const unsigned char* base, const unsigned (&off)[DaPieces<R, NW>::N],
+                                              There there) {
+  const unsigned char* const from = da_uniform(base);
+  lane = da_again(lane);                                   // (few tiles come here: nothing of it is held through the loop)
+#pragma unroll
+  for (int j = 0; j < DaPieces<R, NW>::N; ++j) {
+    if (!DaPieces<R, NW>::any(wave, j)) break;
+    if (there(DaPieces<R, NW>::row(wave, lane, j))) da_dma16s(from, off[j], lds + (wave + NW * j) * 1024);
+    else *(__attribute__((address_space(3))) u32x4*)(size_t)(lds + (wave + NW * j) * 1024 + 16 * lane) = (u32x4){0u, 0u, 0u, 0u};
+  }
+}
+// Strides too far apart for 32-bit offsets: row_ptr(row) = the row's first byte, or null for a row that is to be zeros
 template <int R, int NW, typename F>
 __device__ __forceinline__ void da_stage(unsigned lds, int wave, int lane, F row_ptr) {
 #pragma unroll
@@ -189,6 +210,13 @@ struct DaKeyStage {
       da_stage_fast<RK, NW>(base, wave, k0 + ks * kt0, ko);
       da_stage_fast<RK, NW>(base + KT * RK, wave, k1 + ks * kt0, ko);
       da_stage_fast<RV, NW>(base + 2 * KT * RK, wave, v + vs * kt0, vo);
+      return;
+    }
+    if (a.small_strides) {
+      auto there = [&](int r) { return ((vis >> r) & 1ull) != 0ull; };
+      da_stage_some<RK, NW>(base, wave, lane, k0 + ks * kt0, ko, there);
+      da_stage_some<RK, NW>(base + KT * RK, wave, lane, k1 + ks * kt0, ko, there);
+      da_stage_some<RV, NW>(base + 2 * KT * RK, wave, lane, v + vs * kt0, vo, there);
       return;
     }
     auto at = [&](const unsigned char* p, long long st) {
@@ -229,13 +257,6 @@ __device__ __forceinline__ DaSlot da_slot(const DaArgs& a, int s, int n_slots, i
   r.head += hk * a.share;
   return r;
 }
-// A value the compiler cannot connect with earlier ones: what is derived from it behind a loop is computed there instead of
-// being held in registers through it.
-__device__ __forceinline__ int da_again(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
 __device__ __forceinline__ float da_lam(const DaArgs& a, long long off) {
   return a.lam_f32 ? ((const float*)a.lam)[off] : bd_bf16_to_f32(((const unsigned short*)a.lam)[off]);
 }
@@ -253,15 +274,20 @@ __device__ __forceinline__ int da_visible_end(const DaArgs& a, int b, int Lk, in
   if (!a.mask) return Lk;
   const unsigned char* m = a.mask + b * a.mask_stride;
   int last = 0;
-  if (Lk <= 512) {                                         // every wave by itself: eight loads in flight, no barrier
-    unsigned x[8];
+  if (Lk <= 512) {                                         // every wave by itself: all loads in flight, no barrier
+    auto scan = [&](auto loads) {
+      constexpr int N = decltype(loads)::value;
+      unsigned x[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = *(da_global_byte*)(m + min(64 * i + (tid & 63), Lk - 1));
+      for (int i = 0; i < N; ++i) x[i] = *(da_global_byte*)(m + min(64 * i + (tid & 63), Lk - 1));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned long long v = __ballot(x[i] != 0u && 64 * i + (tid & 63) < Lk);
-      last = v ? 64 * i + 64 - __builtin_clzll(v) : last;
-    }
+      for (int i = 0; i < N; ++i) {
+        const unsigned long long v = __ballot(x[i] != 0u && 64 * i + (tid & 63) < Lk);
+        last = v ? 64 * i + 64 - __builtin_clzll(v) : last;
+      }
+    };
+    if (Lk <= 128) scan(std::integral_constant<int, 2>());
+    else scan(std::integral_constant<int, 8>());
     return __builtin_amdgcn_readfirstlane(last);
   }
   for (int j = tid; j < Lk; j += NT) last = m[j] ? j + 1 : last;
