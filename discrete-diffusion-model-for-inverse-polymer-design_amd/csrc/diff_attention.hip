@@ -360,6 +360,9 @@ __device__ __forceinline__ void da_unclaimed(const DaArgs& a, int tid, Fill fill
 // =====================================================================================
 // Forward. Waves work in pairs: wave 2 w + m holds map m of the 16 QB slots of query group w (NQG groups in a
 // workgroup). Split over keys (n_split > 1): each split leaves its unnormalised sums, maximum and normaliser.
+// Head size 128 (2 x 4096 tokens, 8 heads over 4: 391 us, 1.05 PFLOP/s): matrix cores busy 52 % of the cycles, vector units
+// 44 %: the exponentials of one wave of a SIMD run under the products of the other. Head sizes 32 and 64: bound by the vector units (67 % and
+// 60 % busy): about 4 instructions a score in the loop, the rest around it (many short sequences).
 // =====================================================================================
 template <int D, int QB, int NQG, int OCC, bool TWO>
 __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
@@ -710,10 +713,11 @@ __global__ __launch_bounds__(256) void da_join_few_kernel(DaArgs a) {
 // (dO . O_m) or, where none were kept, from a first walk over the keys: sums of the very P and dP that form dS.
 // From a bf16-rounded O it would miss sum_j dS_ij = 0 by 2^-9 of |dO||O| for all keys alike, as large as dS itself
 // where attention is nearly uniform.
+// Head size 128 as above: 435 us, 0.95 PFLOP/s, matrix cores busy 45 %, vector units 42 %.
 // =====================================================================================
 template <int D, int QB, int NW, int OCC>
 __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
-  constexpr int E = 2 * D, AQ = D == 128 ? 4 : D == 64 ? 2 : 6, KS = D / 32, ES = E / 32, DT = D / 16, RK = 2 * D, RV = 2 * E;
+  constexpr int E = 2 * D, AQ = D == 32 ? 6 : 4, KS = D / 32, ES = E / 32, DT = D / 16, RK = 2 * D, RV = 2 * E;
   constexpr int TILE = KT * (2 * RK + RV), SLOTS = 16 * QB * NW;
   extern __shared__ __attribute__((aligned(1024))) unsigned char da_smem[];
   __shared__ int red[NW];
@@ -893,7 +897,10 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
 }
 
 // =====================================================================================
-// Backward, key side: a workgroup owns 64 KB keys of one key head and walks the query slots of all heads that share it.
+// Backward, key side: a workgroup owns 16 KB NW keys of one key head and walks the query slots of all heads that share it.
+// Head size 128 as above: 713 us, 0.77 PFLOP/s. Every operand fragment read from LDS feeds one product (a wave cannot hold the
+// sums, keys and values of 32 keys beside a second wave on its SIMD): 64 KB a wave for 32 slots, at 128 bytes a cycle 4100
+// cycles a CU for 2048 of products. Waves of 32 keys alone on their SIMD lose more to what they cannot overlap (above).
 // =====================================================================================
 template <int D, int KB, int NW, int OCC>
 __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
@@ -1126,10 +1133,10 @@ __global__ __launch_bounds__(256) void da_dlam_kernel(const float* __restrict__ 
 
 // ---------------------------------------------------------------------------------------------- host side
 // Forward: blocks of 16 slots a wave holds, query groups of a workgroup (two waves each), waves of a SIMD. Measured, forward
-// alone: head size 64, 16 x 1024 tokens x 3 heads: (1, 4, 4) 64 us, (2, 2, 2) 72, (2, 4, 2) 84, (1, 2, 4) 91: with twice
-// the waves the exponentials of one hide behind the products of the others, though every operand read feeds one product
-// instead of two. Head size 128, 2 x 4096 x 8: (2, 4, 2) 470 us, (1, 4, 2) 584, (1, 2, 2) 999 (few slots a workgroup: the
-// tiles' way into LDS paces it). Head size 32, 96 ragged x 8: (2, 2, 4) 97 us, (1, 2, 4) 104, (4, 2, 2) 124, (2, 4, 2) 160.
+// alone: head size 64, 16 x 1024 tokens x 3 heads: (1, 4, 4) 59 us, (2, 2, 2) 60, (2, 4, 2) 70, (1, 2, 4) 70; 256 x 128 padded tokens
+// 32.6, 34.1, 36.7, 43.7. Head size 128, 2 x 4096 x 8 over 4: (2, 4, 2) 391 us, (1, 4, 2) 492, (2, 2, 2) 558, (1, 2, 2) 722 (few slots
+// a workgroup: the tiles' way into LDS paces it). Head size 32, 96 ragged sequences x 8: (2, 2, 4) 85 us, (1, 4, 6) 98, (1, 4, 5)
+// 109, (1, 2, 6) 118, (2, 1, 4) 129, (1, 8, 4) 151.
 template <int B_, int NQG_, int OCC_> struct DaFCfg { static constexpr int B = B_, NQG = NQG_, OCC = OCC_, SLOTS = 16 * B_ * NQG_; };
 template <int D> struct DaFwd : DaFCfg<1, 4, 4> {};
 template <> struct DaFwd<32> : DaFCfg<2, 2, 4> {};
@@ -1230,12 +1237,13 @@ int da_forward(const bd_diff_attn_args& p, DaArgs& a, hipStream_t s) {
   return bd_check_launch("bd_diff_attention_fwd");
 }
 
-// Backward: blocks of 16 slots (dq) or keys (dkv) a wave holds, waves of a workgroup, waves of a SIMD. Measured, dq / dkv:
-// head size 64, 16 x 1024 x 3 heads: dq (1, 8, 4) 67 us, (1, 4, 3) 79; dkv (1, 4, 2) 75, (1, 4, 3) 108, (1, 8, 2) 113.
-// Head size 128, 2 x 4096 x 8: (1, 8, 2) 428 / 715 us, (2, 4, 1) 834 / 844, (1, 4, 1) 1058 / 1234. Head size 32, 96 ragged
-// x 8: (1, 4, 4) 86 / 93 us, (1, 8, 4) 110 / 121, dq (2, 4, 3) 99.
+// Backward: blocks of 16 slots (dq) or keys (dkv) a wave holds, waves of a workgroup, waves of a SIMD. Measured: head size 64,
+// 16 x 1024 x 3 heads: dq (2, 4, 2) 72 us, (1, 8, 4) 74, (1, 4, 4) 77, (2, 2, 2) 143; dkv (1, 4, 2) 79, (1, 8, 2) 94, (2, 4, 1) 116,
+// (1, 4, 3) 308 (spills). Head size 128, 2 x 4096 x 8 over 4: dq (1, 8, 2) 435 us, (2, 4, 1) 497, (1, 4, 2) 1034; dkv (1, 8, 2) 713, (1, 4, 1)
+// 819, (2, 4, 1) 872. Head size 32, 96 ragged x 8: dq (1, 4, 4) 86 us, (1, 4, 5) 95, (2, 4, 2) 97 (but 152 against 176 at 96 x 512), (1, 8, 5)
+// 118; dkv (1, 4, 4) 94, (2, 2, 2) 95, (1, 4, 3) 98, (2, 4, 2) 112, (1, 8, 4) 115.
 template <int B_, int NW_, int OCC_> struct DaCfg { static constexpr int B = B_, NW = NW_, OCC = OCC_; };
-template <int D> struct DaBwd { typedef DaCfg<1, 8, 4> Q; typedef DaCfg<1, 4, 2> K; };
+template <int D> struct DaBwd { typedef DaCfg<2, 4, 2> Q; typedef DaCfg<1, 4, 2> K; };
 template <> struct DaBwd<32> { typedef DaCfg<1, 4, 4> Q; typedef DaCfg<1, 4, 4> K; };
 template <> struct DaBwd<128> { typedef DaCfg<1, 8, 2> Q; typedef DaCfg<1, 8, 2> K; };
 
