@@ -532,6 +532,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     lead = hidden.shape[:-1]
     if weight.shape[1] == 0 or weight.shape[1] % 64:
         raise NotImplementedError(f"linear_cross_entropy: the hidden size must be a multiple of 64, got {weight.shape[1]}")
+    if lead.numel() >= 1 << 24 or weight.shape[0] >= 1 << 28 or weight.shape[1] > 65536:
+        raise NotImplementedError(f"linear_cross_entropy: at most 2^24 - 1 rows, 2^28 - 1 classes and a hidden size of 65536, got "
+                                  f"{lead.numel()}, {weight.shape[0]} and {weight.shape[1]}")
     if targets.dtype != torch.long:
         raise TypeError(f"linear_cross_entropy: targets must be int64, got {targets.dtype}")
     for t, name in ((targets, "targets"), (mask_indicator, "mask_indicator"), (attention_mask, "attention_mask")):

@@ -184,3 +184,12 @@ def test_rotary_in_place_refuses_the_same_memory_twice():
         ops.rotary_(x, x, TABLE)
     with pytest.raises(ValueError, match="same memory"):
         ops.rotary_(x, x[:, :, :2], TABLE)
+
+
+def test_linear_cross_entropy_refuses_more_rows_than_it_counts():
+    h, w = z(1, 64, dtype=torch.bfloat16).expand(1 << 24, 64), z(5, 64, dtype=torch.bfloat16)
+    t = torch.zeros(1, dtype=torch.long).expand(1 << 24)
+    with pytest.raises(NotImplementedError, match="rows"):
+        ops.linear_cross_entropy(h, w, t)
+    with pytest.raises(RuntimeError):                    # one row fewer is only refused for where it lies
+        ops.linear_cross_entropy(h[1:], w, t[1:])
