@@ -1243,24 +1243,36 @@ int da_forward(const bd_diff_attn_args& p, DaArgs& a, hipStream_t s) {
 // 819, (2, 4, 1) 872. Head size 32, 96 ragged x 8: dq (1, 4, 4) 86 us, (1, 4, 5) 95, (2, 4, 2) 97 (but 152 against 176 at 96 x 512), (1, 8, 5)
 // 118; dkv (1, 4, 4) 94, (2, 2, 2) 95, (1, 4, 3) 98, (2, 4, 2) 112, (1, 8, 4) 115.
 template <int B_, int NW_, int OCC_> struct DaCfg { static constexpr int B = B_, NW = NW_, OCC = OCC_; };
-template <int D> struct DaBwd { typedef DaCfg<2, 4, 2> Q; typedef DaCfg<1, 4, 2> K; };
-template <> struct DaBwd<32> { typedef DaCfg<1, 4, 4> Q; typedef DaCfg<1, 4, 4> K; };
-template <> struct DaBwd<128> { typedef DaCfg<1, 8, 2> Q; typedef DaCfg<1, 8, 2> K; };
+template <int D> struct DaBwd { typedef DaCfg<2, 4, 2> Q; typedef DaCfg<1, 4, 2> K; typedef DaCfg<1, 4, 3> QS; };
+template <> struct DaBwd<32> { typedef DaCfg<1, 4, 4> Q; typedef DaCfg<1, 4, 4> K; typedef Q QS; };
+template <> struct DaBwd<128> { typedef DaCfg<1, 8, 2> Q; typedef DaCfg<1, 8, 2> K; typedef DaCfg<1, 4, 2> QS; };
+
+template <int D, typename C>
+void da_launch_dq(DaArgs& a, hipStream_t s, long long grid) {
+  constexpr int LDS = 2 * KT * 8 * D;
+  BD_SET_MAX_LDS((da_bwd_dq_kernel<D, C::B, C::NW, C::OCC>), LDS);
+  hipLaunchKernelGGL((da_bwd_dq_kernel<D, C::B, C::NW, C::OCC>), dim3((unsigned)grid), dim3(64 * C::NW), LDS, s, a);
+}
 
 template <int D>
 int da_backward(DaArgs& a, hipStream_t s) {
-  constexpr int LDS = 2 * KT * 8 * D, LDS_KV = 2 * KT * (8 * D + 32);
+  constexpr int LDS_KV = 2 * KT * (8 * D + 32);
   typedef typename DaBwd<D>::Q Q;
+  typedef typename DaBwd<D>::QS QS;
   typedef typename DaBwd<D>::K K;
-  const long long slots = (long long)a.Lq * a.share;
-  const int seqs = a.B + (a.cu ? 1 : 0);
-  a.n_blk = (int)((slots + 16 * Q::B * Q::NW - 1) / (16 * Q::B * Q::NW));
-  long long grid = da_grid(a.n_blk, (long long)a.Hkv * seqs);
+  const long long slots = (long long)a.Lq * a.share, groups = (long long)a.Hkv * (a.B + (a.cu ? 1 : 0));
+  auto blocks = [](long long rows, int per) { return (rows + per - 1) / per; };
+  // Workgroups for at most half of the CUs: smaller ones (dq, this / the large ones: 4096 tokens x 4 heads of 64 96 / 130 us, 1024 tokens 27 / 40;
+  // 4096 tokens x 4 heads of 128 146 / 180; 8192 x 3 heads of 128, three quarters of the CUs, 541 / 374. dk / dv with half the keys a
+  // workgroup: 4096 x 4 heads of 128 338 / 306, 2048 x 7 of 64 78 / 64: not worth it)
+  const bool small = 2 * (long long)a.Hkv * a.B * blocks(slots, 16 * Q::B * Q::NW) <= 256;
+  a.n_blk = (int)blocks(slots, small ? 16 * QS::B * QS::NW : 16 * Q::B * Q::NW);
+  long long grid = da_grid(a.n_blk, groups);
   BD_REQUIRE(grid < (1ll << 31), "bd_diff_attention_bwd: too many workgroups");
-  BD_SET_MAX_LDS((da_bwd_dq_kernel<D, Q::B, Q::NW, Q::OCC>), LDS);
-  hipLaunchKernelGGL((da_bwd_dq_kernel<D, Q::B, Q::NW, Q::OCC>), dim3((unsigned)grid), dim3(64 * Q::NW), LDS, s, a);
-  a.n_blk = (a.Lk + 16 * K::B * K::NW - 1) / (16 * K::B * K::NW);
-  grid = da_grid(a.n_blk, (long long)a.Hkv * seqs);
+  if (small) da_launch_dq<D, QS>(a, s, grid);
+  else da_launch_dq<D, Q>(a, s, grid);
+  a.n_blk = (int)blocks(a.Lk, 16 * K::B * K::NW);
+  grid = da_grid(a.n_blk, groups);
   BD_REQUIRE(grid < (1ll << 31), "bd_diff_attention_bwd: too many workgroups");
   BD_SET_MAX_LDS((da_bwd_dkv_kernel<D, K::B, K::NW, K::OCC>), LDS_KV);
   hipLaunchKernelGGL((da_bwd_dkv_kernel<D, K::B, K::NW, K::OCC>), dim3((unsigned)grid), dim3(64 * K::NW), LDS_KV, s, a);

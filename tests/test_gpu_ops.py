@@ -302,6 +302,25 @@ def test_differential_attention_split_over_keys(gpu_device, B, Lq, Lk, H, Hkv, D
         assert torch.equal(ops.differential_attention(*leaves, m), out)
 
 
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D,mask", [
+    (70, 65, 64, 2, 2, 64, "holes"), (44, 130, 520, 3, 3, 64, "tail"), (66, 129, 130, 2, 1, 128, "empty"), (33, 100, 1030, 4, 4, 128, None), (150, 40, 70, 4, 2, 32, "tail"),
+])
+def test_differential_attention_many_workgroups(gpu_device, B, Lq, Lk, H, Hkv, D, mask):
+    """Enough queries for every CU: the larger workgroups of the query side's gradient, keys walked once and twice."""
+    q, k, v, lm, m, dout = attention_case(gpu_device, B, Lq, Lk, H, Hkv, D, mask, "token", seed=B + D)
+    r = reference(q, k, v, lm, m, dout, H)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lm)]
+    out = ops.differential_attention(*leaves, m)
+    within(out.detach(), r["out"].view(out.shape), r["out_tol"].view(out.shape), "out")
+    grads = torch.autograd.grad(out, leaves, dout)
+    for name, x in zip(("dq", "dk", "dv"), grads):
+        within(x, r[name].view(x.shape), r[name + "_tol"].view(x.shape), name)
+    want, tol = lam_gradient(r, lm, (B, Lq), H)
+    within(grads[3], want, tol, "dlam")
+    again = torch.autograd.grad(ops.differential_attention(*leaves, m), leaves, dout)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
 def test_differential_attention_long_cache_offsets(gpu_device):
     """Keys whose byte offset passes 32 bits: rows of a buffer of more than 4 GiB, strided."""
     dev = gpu_device
@@ -349,6 +368,27 @@ def test_linear_cross_entropy(gpu_device, M, d, V, live, wdt):
     with torch.no_grad():
         assert torch.equal(ops.linear_cross_entropy(*leaves, t, ind, am), loss)
     again = torch.autograd.grad(ops.linear_cross_entropy(*leaves, t, ind, am) / 4, leaves)
+    assert torch.equal(again[0], dh) and torch.equal(again[1], de)
+
+
+@pytest.mark.parametrize("M,d,V,live,wdt", [(5000, 1024, 65000, 0.3, BF), (9000, 256, 65000, 0.2, torch.float32)])
+def test_linear_cross_entropy_in_pieces_of_the_vocabulary(gpu_device, M, d, V, live, wdt):
+    """The largest tiles of every product, and a backward in several pieces of the vocabulary."""
+    dev, g = gpu_device, gen(gpu_device, M + V)
+    h = torch.randn(M, d, generator=g, device=dev).to(BF)
+    e = (torch.randn(V, d, generator=g, device=dev) * 2.0 / d ** 0.5).to(wdt)
+    t = torch.randint(0, V, (M,), generator=g, device=dev)
+    ind = torch.rand(M, generator=g, device=dev) < live
+    rows = ind.nonzero()[:, 0]
+    r = R.linear_cross_entropy(h[rows], e.to(BF), t[rows], torch.ones(len(rows), device=dev), gout=1.0, tol=True)
+    leaves = [h.requires_grad_(True), e.requires_grad_(True)]
+    loss = ops.linear_cross_entropy(*leaves, t, ind)
+    within(loss.detach(), r["loss"], r["loss_tol"], "loss")
+    dh, de = torch.autograd.grad(loss, leaves)
+    within(dh[rows], r["dh"], r["dh_tol"], "dhidden")
+    within(de, r["dw"], r["dw_tol"], "dweight")
+    assert not bool(dh[~ind].any())
+    again = torch.autograd.grad(ops.linear_cross_entropy(*leaves, t, ind), leaves)
     assert torch.equal(again[0], dh) and torch.equal(again[1], de)
 
 
