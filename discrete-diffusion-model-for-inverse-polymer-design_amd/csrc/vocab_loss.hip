@@ -152,6 +152,8 @@ struct VlGemm {
   int dh_split;                       // dh: n_split is the most, the kernel takes what the row count asks for
   unsigned short* dh;                 // dh from one piece and one split: written in bf16 to its rows, no slab
   const int* idx;
+  const int* pos;                     // dh without a kernel behind it: the rows_all rows without weight are cleared here
+  int rows_all;
   int v0, V;                          // VL_STATS, VL_DLOG: n is vocabulary column v0 + n, valid below V. VL_DW: m is
   const float *w, *lse;               // VL_DLOG
   const int* tgt;
@@ -214,6 +216,13 @@ __global__ __launch_bounds__(2 * BN, 2) void vl_gemm_kernel(VlGemm p) {
   const int g = lane >> 4, c = lane & 15, q4 = c >> 2, p4 = c & 3;
   const int live = p.head[0];
   const int M = p.m_live ? min(live, p.M) : p.M, K = p.k_live ? min((live + 63) & ~63, p.K) : p.K;      // (whole stages of rows: zeros behind the last)
+  if (EPI == VL_SLAB && p.pos) {                           // (every workgroup its share, with or without a tile)
+    const int share = (p.rows_all + gridDim.x - 1) / gridDim.x, first = blockIdx.x * share, per = p.N / 8;
+    for (int i = tid; i < min(share, p.rows_all - first) * per; i += 64 * NW) {
+      const int row = first + i / per;
+      if (p.pos[row] < 0) *(u32x4*)(p.dh + (long long)row * p.ldo + 8 * (i % per)) = (u32x4){0u, 0u, 0u, 0u};
+    }
+  }
   // tile list: groups of 8 tile rows, column by column inside a group; each XCD takes one contiguous part
   const int tiles_m = (M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
   const int n_split = p.dh_split ? vl_dh_splits(M, BM, p.N, p.K, p.n_split) : p.n_split, n_all = tiles_m * tiles_n * n_split;
@@ -463,7 +472,11 @@ __global__ __launch_bounds__(1024) void vl_finish_kernel(VlState st, const float
   __shared__ float part[16];
   const int n = st.head[0];
   float s = 0.f;
-  for (int i = threadIdx.x; i < n; i += 1024) s += rowloss[i];
+#pragma unroll 4
+  for (int i = 4 * threadIdx.x; i < n; i += 4096) {        // (rows behind the last: whatever is there, not added)
+    const f32x4 x = *(const f32x4*)(rowloss + i);
+    s += (x[0] + (i + 1 < n ? x[1] : 0.f)) + ((i + 2 < n ? x[2] : 0.f) + (i + 3 < n ? x[3] : 0.f));
+  }
   s = bd_wave_sum(s);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
@@ -772,6 +785,7 @@ extern "C" int bd_linear_ce_bwd(const void* weight, const float* grad_out, void*
   unsigned short* dlog = (unsigned short*)workspace;
   float* slab_h = (float*)((char*)workspace + pl.m_pad * pl.piece * 2);
   float* slab_w = slab_h + pl.split_h * pl.slab_h;
+  const bool dh_alone = pl.n_pieces == 1 && pl.split_h == 1;       // the product writes every row of dh, no slab to add up
   bd_prof_scope prof(stream, 6.0 * M * (double)V * d, BD_PROF_GEMM);
   for (int i = 0; i < pl.n_pieces; ++i) {
     const int v0 = i * pl.piece, n = min(pl.piece, (int)vl_up(V - v0, 64));       // columns of the piece, whole 64s
@@ -786,6 +800,7 @@ extern "C" int bd_linear_ce_bwd(const void* weight, const float* grad_out, void*
       p.A = dlog; p.lda = pl.piece; p.B = wp; p.ldb = d; p.head = st.head; p.M = (int)pl.m_pad; p.N = d; p.K = min(n, V - v0); p.m_live = 1;
       p.n_split = pl.split_h; p.dh_split = 1; p.slab = slab_h; p.slab_stride = pl.slab_h; p.ldo = d; p.add = i > 0;
       if (pl.n_pieces == 1) { p.dh = (unsigned short*)dhidden; p.idx = st.idx; p.gout = grad_out; }
+      if (dh_alone) { p.pos = st.pos; p.rows_all = (int)M; }
       vl_launch<true, false, VL_SLAB>(pl.big_h, p, s);
     }
     if (dweight) {
@@ -805,7 +820,7 @@ extern "C" int bd_linear_ce_bwd(const void* weight, const float* grad_out, void*
       }
     }
   }
-  if (dhidden)
+  if (dhidden && !dh_alone)
     hipLaunchKernelGGL(vl_dh_kernel, dim3((unsigned)((M * (d / 8) + 255) / 256)), dim3(256), 0, s, st, slab_h, pl.slab_h, pl.split_h,
                        pl.big_h ? 256 : 128, min(pl.piece, V), pl.n_pieces, grad_out, (unsigned short*)dhidden, (int)M, d);
   return bd_check_launch("bd_linear_ce_bwd");
