@@ -710,12 +710,13 @@ __global__ __launch_bounds__(256) void da_join_few_kernel(DaArgs a) {
 // =====================================================================================
 // Backward, query side: dQ and what the key side needs of each slot (stats: lse1, lse2, delta1, delta2, lam), dlam.
 // A wave owns 16 QB slots and both of their maps (dP = dO V^T is shared). delta_m comes from the forward's fp32 maps
-// (dO . O_m) or, where none were kept, from a first walk over the keys: sums of the very P and dP that form dS.
+// (dO . O_m) or, where none were kept, from a first walk over the keys (SHORT: from what the only walk leaves in registers): sums of
+// the very P and dP that form dS.
 // From a bf16-rounded O it would miss sum_j dS_ij = 0 by 2^-9 of |dO||O| for all keys alike, as large as dS itself
 // where attention is nearly uniform.
 // Head size 128 as above: 435 us, 0.95 PFLOP/s, matrix cores busy 45 %, vector units 42 %.
 // =====================================================================================
-template <int D, int QB, int NW, int OCC>
+template <int D, int QB, int NW, int OCC, bool SHORT>
 __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
   constexpr int E = 2 * D, AQ = D == 32 ? 6 : 4, KS = D / 32, ES = E / 32, DT = D / 16, RK = 2 * D, RV = 2 * E;
   constexpr int TILE = KT * (2 * RK + RV), SLOTS = 16 * QB * NW;
@@ -796,6 +797,36 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
     }
   }
   const unsigned knat = da_nat_base<RK>(g, c), ktr = da_tr_base<RK>(g, c), vnat = da_nat_base<RV>(g, c) + 2 * KT * RK;
+  // scores of 16 keys (half a 32-key group) against the wave's slots, and dP; masked keys' scores are -inf
+  auto scores = [&](unsigned kn, unsigned vn, int half, unsigned long long vis32, f32x4 (&s)[QB][2], f32x4 (&dp)[QB]) {
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) s[qb][0] = s[qb][1] = dp[qb] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    // fragments: keys of map 0 and 1 in turn, then the values
+    da_pipe<AQ, 2 * KS + ES>([&](int i) { return i < 2 * KS ? da_nat<RK>(kn, 0, half, i >> 1, (i & 1) * KT * RK) : da_nat<RV>(vn, 0, half, i - 2 * KS); },
+                         [&](int i, bf16x8 x) {
+#pragma unroll
+                           for (int qb = 0; qb < QB; ++qb) {
+                             if (i < 2 * KS) s[qb][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qf[qb][i & 1][i >> 1], s[qb][i & 1], 0, 0, 0);
+                             else dp[qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, dof[qb][i - 2 * KS], dp[qb], 0, 0, 0);
+                           }
+                         });
+    if ((unsigned)vis32 != ~0u) {
+      const unsigned m4 = (unsigned)(vis32 >> (8 * g + 4 * half)) & 0xfu;
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!((m4 >> r) & 1u)) s[qb][0][r] = s[qb][1][r] = -INFINITY;        // weight 2^-inf = 0 (dP of a zero row is 0)
+    }
+  };
+  auto add_dq = [&](unsigned kt, const bf16x8 (&dsf)[QB][2]) {                 // dQ^T += K^T dS^T
+    da_pipe<AQ, 2 * DT>([&](int i) { return da_tr<RK>(kt, 0, i >> 1, (i & 1) * KT * RK); },
+                    [&](int i, bf16x8 x) {
+#pragma unroll
+                      for (int qb = 0; qb < QB; ++qb)
+                        acc[qb][i & 1][i >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, dsf[qb][i & 1], acc[qb][i & 1][i >> 1], 0, 0, 0);
+                    });
+  };
   auto walk_keys = [&](auto last) {                        // last: dQ is summed; else delta
     constexpr bool LAST = decltype(last)::value;
     unsigned mb = da_mask_byte(a, b, lane, kend);
@@ -816,25 +847,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           f32x4 s[QB][2], dp[QB];
-#pragma unroll
-          for (int qb = 0; qb < QB; ++qb) s[qb][0] = s[qb][1] = dp[qb] = (f32x4){0.f, 0.f, 0.f, 0.f};
-          // fragments: keys of map 0 and 1 in turn, then the values
-          da_pipe<AQ, 2 * KS + ES>([&](int i) { return i < 2 * KS ? da_nat<RK>(kn, 0, half, i >> 1, (i & 1) * KT * RK) : da_nat<RV>(vn, 0, half, i - 2 * KS); },
-                               [&](int i, bf16x8 x) {
-#pragma unroll
-                                 for (int qb = 0; qb < QB; ++qb) {
-                                   if (i < 2 * KS) s[qb][i & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, qf[qb][i & 1][i >> 1], s[qb][i & 1], 0, 0, 0);
-                                   else dp[qb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, dof[qb][i - 2 * KS], dp[qb], 0, 0, 0);
-                                 }
-                               });
-          if (vis != ~0ull) {
-            const unsigned m4 = (unsigned)(vis >> (32 * h2 + 8 * g + 4 * half)) & 0xfu;
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb)
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (!((m4 >> r) & 1u)) s[qb][0][r] = s[qb][1][r] = -INFINITY;        // weight 2^-inf = 0 (dP of a zero row is 0)
-          }
+          scores(kn, vn, half, vis >> (32 * h2), s, dp);
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
@@ -846,20 +859,13 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
                 else dsf[qb][m][4 * half + r] = (__bf16)(p * (dp[qb][r] - dl[qb][m]));
               }
         }
-        if (LAST)                                          // dQ^T += K^T dS^T
-          da_pipe<AQ, 2 * DT>([&](int i) { return da_tr<RK>(kt, 0, i >> 1, (i & 1) * KT * RK); },
-                          [&](int i, bf16x8 x) {
-#pragma unroll
-                            for (int qb = 0; qb < QB; ++qb)
-                              acc[qb][i & 1][i >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, dsf[qb][i & 1], acc[qb][i & 1][i >> 1], 0, 0, 0);
-                          });
+        if (LAST) add_dq(kt, dsf);
       }
       vis = vis_next;
       const unsigned sw = cur; cur = other; other = sw;
     }
   };
-  if (!a.maps) {
-    walk_keys(std::false_type());
+  auto join_delta = [&] {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
@@ -867,8 +873,60 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
         dl[qb][m] += __shfl_xor(dl[qb][m], 16, 64);
         dl[qb][m] += __shfl_xor(dl[qb][m], 32, 64);
       }
+  };
+  if constexpr (SHORT) {                                   // both tiles stay in LDS, their weights and dP in registers
+    f32x4 p[2][2][2][QB][2], dp[2][2][2][QB];              // [tile][32 keys][16 of them]
+    unsigned long long vis[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      vis[t] = __ballot(da_mask_byte(a, b, KT * t + lane, kend) != 0u);
+      if (KT * t < kend) keys.run(a, lds0 + t * TILE, KT * t, vis[t], wave, lane);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (KT * t >= kend) continue;
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          f32x4 (&s)[QB][2] = p[t][h2][half];
+          f32x4 (&d)[QB] = dp[t][h2][half];
+          scores(lds0 + t * TILE + knat + 32 * RK * h2, lds0 + t * TILE + vnat + 32 * RV * h2, half, vis[t] >> (32 * h2), s, d);
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                s[qb][m][r] = __builtin_amdgcn_exp2f(s[qb][m][r] * scale2 - lse[qb][m]);
+                dl[qb][m] += s[qb][m][r] * d[qb][r];
+              }
+        }
+    }
+    join_delta();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (KT * t >= kend) continue;
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) {
+        bf16x8 dsf[QB][2];
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dsf[qb][m][i] = (__bf16)(p[t][h2][i >> 2][qb][m][i & 3] * (dp[t][h2][i >> 2][qb][i & 3] - dl[qb][m]));
+        add_dq(lds0 + t * TILE + ktr + 32 * RK * h2, dsf);
+      }
+    }
+  } else {
+    if (!a.maps) {
+      walk_keys(std::false_type());
+      join_delta();
+    }
+    walk_keys(std::true_type());
   }
-  walk_keys(std::true_type());
   const int s1 = da_again(s0), g1 = da_again(lane) >> 4;
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
@@ -1243,15 +1301,15 @@ int da_forward(const bd_diff_attn_args& p, DaArgs& a, hipStream_t s) {
 // 819, (2, 4, 1) 872. Head size 32, 96 ragged x 8: dq (1, 4, 4) 86 us, (1, 4, 5) 95, (2, 4, 2) 97 (but 152 against 176 at 96 x 512), (1, 8, 5)
 // 118; dkv (1, 4, 4) 94, (2, 2, 2) 95, (1, 4, 3) 98, (2, 4, 2) 112, (1, 8, 4) 115.
 template <int B_, int NW_, int OCC_> struct DaCfg { static constexpr int B = B_, NW = NW_, OCC = OCC_; };
-template <int D> struct DaBwd { typedef DaCfg<2, 4, 2> Q; typedef DaCfg<1, 4, 2> K; typedef DaCfg<1, 4, 3> QS; };
-template <> struct DaBwd<32> { typedef DaCfg<1, 4, 4> Q; typedef DaCfg<1, 4, 4> K; typedef Q QS; };
-template <> struct DaBwd<128> { typedef DaCfg<1, 8, 2> Q; typedef DaCfg<1, 8, 2> K; typedef DaCfg<1, 4, 2> QS; };
+template <int D> struct DaBwd { typedef DaCfg<2, 4, 2> Q; typedef DaCfg<1, 4, 2> K; typedef DaCfg<1, 4, 3> QS; typedef DaCfg<1, 4, 3> QR; };
+template <> struct DaBwd<32> { typedef DaCfg<1, 4, 4> Q; typedef DaCfg<1, 4, 4> K; typedef Q QS; typedef DaCfg<1, 4, 3> QR; };
+template <> struct DaBwd<128> { typedef DaCfg<1, 8, 2> Q; typedef DaCfg<1, 8, 2> K; typedef DaCfg<1, 4, 2> QS; typedef Q QR; };
 
-template <int D, typename C>
+template <int D, typename C, bool SHORT>
 void da_launch_dq(DaArgs& a, hipStream_t s, long long grid) {
   constexpr int LDS = 2 * KT * 8 * D;
-  BD_SET_MAX_LDS((da_bwd_dq_kernel<D, C::B, C::NW, C::OCC>), LDS);
-  hipLaunchKernelGGL((da_bwd_dq_kernel<D, C::B, C::NW, C::OCC>), dim3((unsigned)grid), dim3(64 * C::NW), LDS, s, a);
+  BD_SET_MAX_LDS((da_bwd_dq_kernel<D, C::B, C::NW, C::OCC, SHORT>), LDS);
+  hipLaunchKernelGGL((da_bwd_dq_kernel<D, C::B, C::NW, C::OCC, SHORT>), dim3((unsigned)grid), dim3(64 * C::NW), LDS, s, a);
 }
 
 template <int D>
@@ -1259,6 +1317,7 @@ int da_backward(DaArgs& a, hipStream_t s) {
   constexpr int LDS_KV = 2 * KT * (8 * D + 32);
   typedef typename DaBwd<D>::Q Q;
   typedef typename DaBwd<D>::QS QS;
+  typedef typename DaBwd<D>::QR QR;
   typedef typename DaBwd<D>::K K;
   const long long slots = (long long)a.Lq * a.share, groups = (long long)a.Hkv * (a.B + (a.cu ? 1 : 0));
   auto blocks = [](long long rows, int per) { return (rows + per - 1) / per; };
@@ -1266,11 +1325,15 @@ int da_backward(DaArgs& a, hipStream_t s) {
   // 4096 tokens x 4 heads of 128 146 / 180; 8192 x 3 heads of 128, three quarters of the CUs, 541 / 374. dk / dv with half the keys a
   // workgroup: 4096 x 4 heads of 128 338 / 306, 2048 x 7 of 64 78 / 64: not worth it)
   const bool small = 2 * (long long)a.Hkv * a.B * blocks(slots, 16 * Q::B * Q::NW) <= 256;
-  a.n_blk = (int)blocks(slots, small ? 16 * QS::B * QS::NW : 16 * Q::B * Q::NW);
+  // At most two key tiles: both stay in LDS, weights and dP in registers, the keys are walked once (this / the general form: 256 x 128
+  // padded tokens x 3 heads of 64 35.4 / 40.8 us, 8 x 128 8.9 / 12.0, 256 x 64 18.5 / 25.7; heads of 32, 256 x 128 21.3 / 26.6)
+  const bool keeps = D <= 64 && !a.maps && a.Lk <= 2 * KT;
+  a.n_blk = (int)blocks(slots, keeps ? 16 * QR::B * QR::NW : small ? 16 * QS::B * QS::NW : 16 * Q::B * Q::NW);
   long long grid = da_grid(a.n_blk, groups);
   BD_REQUIRE(grid < (1ll << 31), "bd_diff_attention_bwd: too many workgroups");
-  if (small) da_launch_dq<D, QS>(a, s, grid);
-  else da_launch_dq<D, Q>(a, s, grid);
+  if (keeps) da_launch_dq<D, QR, D <= 64>(a, s, grid);
+  else if (small) da_launch_dq<D, QS, false>(a, s, grid);
+  else da_launch_dq<D, Q, false>(a, s, grid);
   a.n_blk = (int)blocks(a.Lk, 16 * K::B * K::NW);
   grid = da_grid(a.n_blk, groups);
   BD_REQUIRE(grid < (1ll << 31), "bd_diff_attention_bwd: too many workgroups");

@@ -304,6 +304,7 @@ def test_differential_attention_split_over_keys(gpu_device, B, Lq, Lk, H, Hkv, D
 
 @pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D,mask", [
     (70, 65, 64, 2, 2, 64, "holes"), (44, 130, 520, 3, 3, 64, "tail"), (66, 129, 130, 2, 1, 128, "empty"), (33, 100, 1030, 4, 4, 128, None), (150, 40, 70, 4, 2, 32, "tail"),
+    (70, 65, 140, 2, 2, 64, "holes"), (3, 70, 200, 2, 1, 64, "empty"), (80, 70, 129, 2, 2, 32, "empty"), (20, 128, 128, 6, 2, 64, "holes"),
 ])
 def test_differential_attention_many_workgroups(gpu_device, B, Lq, Lk, H, Hkv, D, mask):
     """Enough queries for every CU: the larger workgroups of the query side's gradient, keys walked once and twice."""
