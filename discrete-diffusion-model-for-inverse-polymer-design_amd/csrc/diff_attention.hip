@@ -604,8 +604,8 @@ __device__ __forceinline__ void da_joined(const DaArgs& a, int b, const DaSlot& 
 }
 
 // Joins more than 16 key splits of one slot, 16 columns a workgroup: waves 2 m and 2 m + 1 add up map m, 16 splits at a time each
-// with 4 lanes across the columns, in a fixed order. Bound by latency (one row, 65 521 keys, 4 x 4 heads of 64, 128
-// splits: 16.8 MB of partial sums in all): what a thread adds up is asked for before the splits' maxima and normalisers
+// with 4 lanes across the columns, in a fixed order. Bound by latency (one row, 65 521 keys, 4 x 4 heads of 64, 64
+// splits: 1 MB of partial sums, 4.7 us): what a thread adds up is asked for before the splits' maxima and normalisers
 // are worked into weights, and many small workgroups wait at once.
 constexpr int JOIN_COLS = 16, JOIN_SPLITS = 256, JOIN_LANES = 16;
 template <int D>
@@ -1165,25 +1165,35 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
 }
 
 // dlam [B, L, H] summed over the axes that lam was broadcast along (kept axes: kb, kl, kh), in a fixed order; one
-// workgroup per kept value
+// workgroup per kept value, eight loads of a thread in flight (a weight per head, 32 768 rows: 6 us; one load at a time 59)
 template <typename T>
-__global__ __launch_bounds__(256) void da_dlam_kernel(const float* __restrict__ dlam, T* __restrict__ out, int B, int L, int H, int kb, int kl,
-                                                      int kh) {
-  __shared__ float part[4];
+__global__ __launch_bounds__(1024) void da_dlam_kernel(const float* __restrict__ dlam, T* __restrict__ out, int B, int L, int H, int kb, int kl,
+                                                       int kh) {
+  __shared__ float part[16];
   const int nh = kh ? H : 1, nl = kl ? L : 1;
   const int h = blockIdx.x % nh, l = (blockIdx.x / nh) % nl, b = blockIdx.x / nh / nl;
-  const int sb = kb ? 1 : B, sl = kl ? 1 : L, sh = kh ? 1 : H;
-  const long long n = (long long)sb * sl * sh;
+  // the values summed: `rows` of them `step` apart, and, where the heads are summed too, H neighbours of each
+  const float* p = dlam + ((long long)b * L + l) * H + h;
+  long long rows = (kb ? 1ll : B) * (kl ? 1 : L), step = kl ? (long long)L * H : H, near = kh ? 1 : H;
+  if (near > 1 && (step == H || rows == 1)) { rows *= near; step = near = 1; }
+  const long long n = rows * near;
   float s = 0.f;
-  for (long long i = threadIdx.x; i < n; i += 256) {
-    const int ih = (int)(i % sh), il = (int)(i / sh % sl), ib = (int)(i / sh / sl);
-    s += dlam[((long long)(b + ib) * L + l + il) * H + h + ih];
+  for (long long i = threadIdx.x; i < n; i += 8 * 1024) {
+    float x[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const long long k = i + 1024 * u;
+      x[u] = k < n ? p[near == 1 ? k * step : k / near * step + k % near] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += x[u];
   }
   s = bd_wave_sum(s);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
-    s = (part[0] + part[1]) + (part[2] + part[3]);
+    s = 0.f;
+    for (int w = 0; w < 16; ++w) s += part[w];
     if (sizeof(T) == 2) out[blockIdx.x] = (T)bd_f32_to_bf16(s);
     else ((float*)out)[blockIdx.x] = s;
   }
@@ -1408,7 +1418,7 @@ extern "C" int bd_diff_attention_dlam(const float* dlam, void* out, int out_dtyp
   hipStream_t s = (hipStream_t)stream;
   const bool bf = out_dtype == BD_DTYPE_BF16;
   const dim3 grid((unsigned)kept);
-  if (bf) hipLaunchKernelGGL(da_dlam_kernel<unsigned short>, grid, dim3(256), 0, s, dlam, (unsigned short*)out, B, L, H, keep_b, keep_l, keep_h);
-  else hipLaunchKernelGGL(da_dlam_kernel<float>, grid, dim3(256), 0, s, dlam, (float*)out, B, L, H, keep_b, keep_l, keep_h);
+  if (bf) hipLaunchKernelGGL(da_dlam_kernel<unsigned short>, grid, dim3(1024), 0, s, dlam, (unsigned short*)out, B, L, H, keep_b, keep_l, keep_h);
+  else hipLaunchKernelGGL(da_dlam_kernel<float>, grid, dim3(1024), 0, s, dlam, (float*)out, B, L, H, keep_b, keep_l, keep_h);
   return bd_check_launch("bd_diff_attention_dlam");
 }

