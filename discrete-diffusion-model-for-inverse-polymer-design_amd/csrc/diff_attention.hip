@@ -361,8 +361,8 @@ __device__ __forceinline__ void da_unclaimed(const DaArgs& a, int tid, Fill fill
 // Forward. Waves work in pairs: wave 2 w + m holds map m of the 16 QB slots of query group w (NQG groups in a
 // workgroup). Split over keys (n_split > 1): each split leaves its unnormalised sums, maximum and normaliser.
 // Head size 128 (2 x 4096 tokens, 8 heads over 4: 391 us, 1.05 PFLOP/s): matrix cores busy 52 % of the cycles, vector units
-// 44 %: the exponentials of one wave of a SIMD run under the products of the other. Head sizes 32 and 64: bound by the vector units (67 % and
-// 60 % busy): about 4 instructions a score in the loop, the rest around it (many short sequences).
+// 44 %: the exponentials of one wave of a SIMD run under the products of the other. Head sizes 32 and 64: bound by the
+// vector units (66 % and 56 % busy): about 4 instructions a score in the loop, the rest around it (many short sequences).
 // =====================================================================================
 template <int D, int QB, int NQG, int OCC, bool TWO>
 __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
@@ -819,6 +819,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
           if (!((m4 >> r) & 1u)) s[qb][0][r] = s[qb][1][r] = -INFINITY;        // weight 2^-inf = 0 (dP of a zero row is 0)
     }
   };
+  // (dS goes to bf16 as the product's operand: half a step is 2^-8 of each, and its sum over the keys misses zero by no more)
   auto add_dq = [&](unsigned kt, const bf16x8 (&dsf)[QB][2]) {                 // dQ^T += K^T dS^T
     da_pipe<AQ, 2 * DT>([&](int i) { return da_tr<RK>(kt, 0, i >> 1, (i & 1) * KT * RK); },
                     [&](int i, bf16x8 x) {
@@ -1109,6 +1110,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
             for (int kb = 0; kb < KB; ++kb) {
               const float p1 = __builtin_amdgcn_exp2f(s[kb][0][r] * scale2 - st[0]);
               const float p2 = __builtin_amdgcn_exp2f(s[kb][1][r] * scale2 - st[1]) * lam;
+              // to bf16 as the products' operands, the maps' difference taken before: 2^-8 of each difference, of each dS
               pf[kb][4 * half + r] = (__bf16)(p1 - p2);
               dsf[kb][0][4 * half + r] = (__bf16)(p1 * (dp[kb][r] - st[2]));
               dsf[kb][1][4 * half + r] = (__bf16)(p2 * (st[3] - dp[kb][r]));
