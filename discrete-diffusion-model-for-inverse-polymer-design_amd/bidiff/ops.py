@@ -374,7 +374,8 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     zeros, and what masked keys and values hold reaches nothing (their gradients are zeros). Packed rows: the same tensors
     without the batch axis, ``cu_seqlens`` int [sequences + 1] (rows cu[b] .. cu[b + 1] - 1 belong to sequence b; offsets
     that do not fall; rows before the first and behind the last sequence come out zero), ``max_seqlen`` the longest (None: read
-    back from the device; a longer sequence's rows from there on come out NaN, in the gradients too), ``key_mask`` [sequences, max_seqlen]. ``scale`` defaults to 1 / sqrt(D)."""
+    back from the device; a longer sequence's rows from there on come out NaN, in the gradients too), ``key_mask``
+    [sequences, max_seqlen]. ``scale`` defaults to 1 / sqrt(D)."""
     _same_device("differential_attention", q, k, v, lam, key_mask, cu_seqlens)
     packed = cu_seqlens is not None
     dims = 3 if packed else 4

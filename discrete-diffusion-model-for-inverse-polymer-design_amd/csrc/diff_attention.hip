@@ -56,8 +56,8 @@ __device__ __attribute__((aligned(64))) const unsigned int bd_da_zero[16] = {};
 typedef __attribute__((address_space(3))) void da_lds;
 
 // A staged tile has rows of R bytes; 16-byte chunk ch of row `row` sits at chunk ch ^ f(row). The XOR spreads what is read
-// at a time over the banks: by ds_read_b128 four times four neighbouring rows, two groups at one chunk and two at its neighbour;
-// by the transposing read two groups of four neighbouring rows, 32 bytes each.
+// at a time over the banks: by ds_read_b128 four times four neighbouring rows, two groups at one chunk and two at its
+// neighbour; by the transposing read two groups of four neighbouring rows, 32 bytes each.
 template <int R>
 __device__ __forceinline__ int da_off(int row, int ch) {
   const int f = R >= 256 ? (((row & 3) << 2) | ((row >> 2) & 3))
@@ -603,10 +603,10 @@ __device__ __forceinline__ void da_joined(const DaArgs& a, int b, const DaSlot& 
   *(u32x2*)(a.out + b * a.os[0] + sl.row * a.os[1] + sl.head * a.os[2] + col) = w;
 }
 
-// Joins more than 16 key splits of one slot, 16 columns a workgroup: waves 2 m and 2 m + 1 add up map m, 16 splits at a time each
-// with 4 lanes across the columns, in a fixed order. Bound by latency (one row, 65 521 keys, 4 x 4 heads of 64, 64
-// splits: 1 MB of partial sums, 4.7 us): what a thread adds up is asked for before the splits' maxima and normalisers
-// are worked into weights, and many small workgroups wait at once.
+// Joins more than 16 key splits of one slot, 16 columns a workgroup: waves 2 m and 2 m + 1 add up map m, 16 splits at a time
+// each with 4 lanes across the columns, in a fixed order. Bound by latency (one row, 65 521 keys, 4 x 4 heads of 64, 64
+// splits: 1 MB of partial sums, 4.7 us): what a thread adds up is asked for before the splits' maxima and normalisers are
+// worked into weights, and many small workgroups wait at once.
 constexpr int JOIN_COLS = 16, JOIN_SPLITS = 256, JOIN_LANES = 16;
 template <int D>
 __global__ __launch_bounds__(256) void da_join_kernel(DaArgs a) {
@@ -667,8 +667,9 @@ __global__ __launch_bounds__(256) void da_join_kernel(DaArgs a) {
   da_joined<D>(a, b, sl, rh, col, r, top, l);
 }
 
-// The same for at most 16 splits (many slots: the launch is bound by the partial sums' way through memory): a wave takes
-// 16 (slot, split) pairs, four lanes across 16 columns each, and adds up by exchanges alone (2048 slots, 2 splits of 64-wide heads: 8.3 us).
+// The same for at most 16 splits (many slots: the launch is bound by the partial sums' way through memory): a wave takes 16
+// (slot, split) pairs, four lanes across 16 columns each, and adds up by exchanges alone (2048 slots, 2 splits of 64-wide
+// heads: 8.3 us).
 template <int D>
 __global__ __launch_bounds__(256) void da_join_few_kernel(DaArgs a) {
   constexpr int E = 2 * D, CB = E / JOIN_COLS;
@@ -708,13 +709,12 @@ __global__ __launch_bounds__(256) void da_join_few_kernel(DaArgs a) {
 }
 
 // =====================================================================================
-// Backward, query side: dQ and what the key side needs of each slot (stats: lse1, lse2, delta1, delta2, lam), dlam.
-// A wave owns 16 QB slots and both of their maps (dP = dO V^T is shared). delta_m comes from the forward's fp32 maps
-// (dO . O_m) or, where none were kept, from a first walk over the keys (SHORT: from what the only walk leaves in registers): sums of
-// the very P and dP that form dS.
-// From a bf16-rounded O it would miss sum_j dS_ij = 0 by 2^-9 of |dO||O| for all keys alike, as large as dS itself
-// where attention is nearly uniform.
-// Head size 128 as above: 435 us, 0.95 PFLOP/s, matrix cores busy 45 %, vector units 42 %.
+// Backward, query side: dQ and what the key side needs of each slot (stats: lse1, lse2, delta1, delta2, lam), dlam. A wave
+// owns 16 QB slots and both of their maps (dP = dO V^T is shared). delta_m comes from the forward's fp32 maps (dO . O_m) or,
+// where none were kept, from a first walk over the keys (SHORT: from what the only walk leaves in registers): sums of the
+// very P and dP that form dS. From a bf16-rounded O it would miss sum_j dS_ij = 0 by 2^-9 of |dO||O| for all keys alike, as
+// large as dS itself where attention is nearly uniform. Head size 128 as above: 435 us, 0.95 PFLOP/s, matrix cores busy 45
+// %, vector units 42 %.
 // =====================================================================================
 template <int D, int QB, int NW, int OCC, bool SHORT>
 __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
@@ -1203,23 +1203,23 @@ __global__ __launch_bounds__(1024) void da_dlam_kernel(const float* __restrict__
 
 // ---------------------------------------------------------------------------------------------- host side
 // Forward: blocks of 16 slots a wave holds, query groups of a workgroup (two waves each), waves of a SIMD. Measured, forward
-// alone: head size 64, 16 x 1024 tokens x 3 heads: (1, 4, 4) 59 us, (2, 2, 2) 60, (2, 4, 2) 70, (1, 2, 4) 70; 256 x 128 padded tokens
-// 32.6, 34.1, 36.7, 43.7. Head size 128, 2 x 4096 x 8 over 4: (2, 4, 2) 391 us, (1, 4, 2) 492, (2, 2, 2) 558, (1, 2, 2) 722 (few slots
-// a workgroup: the tiles' way into LDS paces it). Head size 32, 96 ragged sequences x 8: (2, 2, 4) 85 us, (1, 4, 6) 98, (1, 4, 5)
-// 109, (1, 2, 6) 118, (2, 1, 4) 129, (1, 8, 4) 151.
+// alone: head size 64, 16 x 1024 tokens x 3 heads: (1, 4, 4) 59 us, (2, 2, 2) 60, (2, 4, 2) 70, (1, 2, 4) 70; 256 x 128
+// padded tokens 32.6, 34.1, 36.7, 43.7. Head size 128, 2 x 4096 x 8 over 4: (2, 4, 2) 391 us, (1, 4, 2) 492, (2, 2, 2) 558,
+// (1, 2, 2) 722 (few slots a workgroup: the tiles' way into LDS paces it). Head size 32, 96 ragged sequences x 8: (2, 2, 4)
+// 85 us, (1, 4, 6) 98, (1, 4, 5) 109, (1, 2, 6) 118, (2, 1, 4) 129, (1, 8, 4) 151.
 template <int B_, int NQG_, int OCC_> struct DaFCfg { static constexpr int B = B_, NQG = NQG_, OCC = OCC_, SLOTS = 16 * B_ * NQG_; };
 template <int D> struct DaFwd : DaFCfg<1, 4, 4> {};
 template <> struct DaFwd<32> : DaFCfg<2, 2, 4> {};
 template <> struct DaFwd<128> : DaFCfg<2, 4, 2> {};
 constexpr int ROWS_NQG = 2, ROWS_SLOTS = 16 * ROWS_NQG;                         // few slots: 32, 4 waves of 16
 
-// The forward of a call. Half of the large workgroup's slots or fewer: the workgroup of 32 (measured, this / the large one: 2
-// rows against 512 keys x 6 heads of 64 in 64 sequences 15.6 / 20.1 us, 32 rows 16.1 / 21.1, 64 rows 23.4 / 22.5; heads of
+// The forward of a call. Half of the large workgroup's slots or fewer: the workgroup of 32 (measured, this / the large one:
+// 2 rows against 512 keys x 6 heads of 64 in 64 sequences 15.6 / 20.1 us, 32 rows 16.1 / 21.1, 64 rows 23.4 / 22.5; heads of
 // 128, 32 rows 31.5 / 57.5, 64 rows 46.4 / 58.8). Split over the keys where the workgroups leave CUs without work, one a CU,
-// if that gives a split enough key tiles: 2 for the workgroup of 32 (one row against 4096 keys, 4 heads of 64 over
-// 4 key heads: 10.3 us, with 4 tiles 11.9, with 8 15.5), else 16 (1024 rows against 1024 keys, 8 heads of 64: 20.0 us unsplit,
-// 28.5 with 8 tiles, 33.0 with 4; 128 rows against 4096 keys, 16 heads over 4: unsplit 62, split in four 30). 65 521 keys, 16 heads over
-// 4, split / unsplit: 16 rows 37 / 927 us, 128 rows 150 / 937, 512 rows 561 / 944.
+// if that gives a split enough key tiles: 2 for the workgroup of 32 (one row against 4096 keys, 4 heads of 64 over 4 key
+// heads: 10.3 us, with 4 tiles 11.9, with 8 15.5), else 16 (1024 rows against 1024 keys, 8 heads of 64: 20.0 us unsplit,
+// 28.5 with 8 tiles, 33.0 with 4; 128 rows against 4096 keys, 16 heads over 4: unsplit 62, split in four 30). 65 521 keys,
+// 16 heads over 4, split / unsplit: 16 rows 37 / 927 us, 128 rows 150 / 937, 512 rows 561 / 944.
 struct DaPlan { bool few; int per, n_blk, n_split; };
 
 DaPlan da_plan(const bd_diff_attn_args& p) {
@@ -1307,11 +1307,12 @@ int da_forward(const bd_diff_attn_args& p, DaArgs& a, hipStream_t s) {
   return bd_check_launch("bd_diff_attention_fwd");
 }
 
-// Backward: blocks of 16 slots (dq) or keys (dkv) a wave holds, waves of a workgroup, waves of a SIMD. Measured: head size 64,
-// 16 x 1024 x 3 heads: dq (2, 4, 2) 72 us, (1, 8, 4) 74, (1, 4, 4) 77, (2, 2, 2) 143; dkv (1, 4, 2) 79, (1, 8, 2) 94, (2, 4, 1) 116,
-// (1, 4, 3) 308 (spills). Head size 128, 2 x 4096 x 8 over 4: dq (1, 8, 2) 435 us, (2, 4, 1) 497, (1, 4, 2) 1034; dkv (1, 8, 2) 713, (1, 4, 1)
-// 819, (2, 4, 1) 872. Head size 32, 96 ragged x 8: dq (1, 4, 4) 86 us, (1, 4, 5) 95, (2, 4, 2) 97 (but 152 against 176 at 96 x 512), (1, 8, 5)
-// 118; dkv (1, 4, 4) 94, (2, 2, 2) 95, (1, 4, 3) 98, (2, 4, 2) 112, (1, 8, 4) 115.
+// Backward: blocks of 16 slots (dq) or keys (dkv) a wave holds, waves of a workgroup, waves of a SIMD. Measured: head size
+// 64, 16 x 1024 x 3 heads: dq (2, 4, 2) 72 us, (1, 8, 4) 74, (1, 4, 4) 77, (2, 2, 2) 143; dkv (1, 4, 2) 79, (1, 8, 2) 94,
+// (2, 4, 1) 116, (1, 4, 3) 308 (spills). Head size 128, 2 x 4096 x 8 over 4: dq (1, 8, 2) 435 us, (2, 4, 1) 497, (1, 4, 2)
+// 1034; dkv (1, 8, 2) 713, (1, 4, 1) 819, (2, 4, 1) 872. Head size 32, 96 ragged x 8: dq (1, 4, 4) 86 us, (1, 4, 5) 95, (2,
+// 4, 2) 97 (but 152 against 176 at 96 x 512), (1, 8, 5) 118; dkv (1, 4, 4) 94, (2, 2, 2) 95, (1, 4, 3) 98, (2, 4, 2) 112,
+// (1, 8, 4) 115.
 template <int B_, int NW_, int OCC_> struct DaCfg { static constexpr int B = B_, NW = NW_, OCC = OCC_; };
 template <int D> struct DaBwd { typedef DaCfg<2, 4, 2> Q; typedef DaCfg<1, 4, 2> K; typedef DaCfg<1, 4, 3> QS; typedef DaCfg<1, 4, 3> QR; };
 template <> struct DaBwd<32> { typedef DaCfg<1, 4, 4> Q; typedef DaCfg<1, 4, 4> K; typedef Q QS; typedef DaCfg<1, 4, 3> QR; };
@@ -1333,12 +1334,13 @@ int da_backward(DaArgs& a, hipStream_t s) {
   typedef typename DaBwd<D>::K K;
   const long long slots = (long long)a.Lq * a.share, groups = (long long)a.Hkv * (a.B + (a.cu ? 1 : 0));
   auto blocks = [](long long rows, int per) { return (rows + per - 1) / per; };
-  // Workgroups for at most half of the CUs: smaller ones (dq, this / the large ones: 4096 tokens x 4 heads of 64 96 / 130 us, 1024 tokens 27 / 40;
-  // 4096 tokens x 4 heads of 128 146 / 180; 8192 x 3 heads of 128, three quarters of the CUs, 541 / 374. dk / dv with half the keys a
-  // workgroup: 4096 x 4 heads of 128 338 / 306, 2048 x 7 of 64 78 / 64: not worth it)
+  // Workgroups for at most half of the CUs: smaller ones (dq, this / the large ones: 4096 tokens x 4 heads of 64 96 / 130
+  // us, 1024 tokens 27 / 40; 4096 tokens x 4 heads of 128 146 / 180; 8192 x 3 heads of 128, three quarters of the CUs, 541 /
+  // 374. dk / dv with half the keys a workgroup: 4096 x 4 heads of 128 338 / 306, 2048 x 7 of 64 78 / 64: not worth it)
   const bool small = 2 * (long long)a.Hkv * a.B * blocks(slots, 16 * Q::B * Q::NW) <= 256;
-  // At most two key tiles: both stay in LDS, weights and dP in registers, the keys are walked once (this / the general form: 256 x 128
-  // padded tokens x 3 heads of 64 35.4 / 40.8 us, 8 x 128 8.9 / 12.0, 256 x 64 18.5 / 25.7; heads of 32, 256 x 128 21.3 / 26.6)
+  // At most two key tiles: both stay in LDS, weights and dP in registers, the keys are walked once (this / the general form:
+  // 256 x 128 padded tokens x 3 heads of 64 35.4 / 40.8 us, 8 x 128 8.9 / 12.0, 256 x 64 18.5 / 25.7; heads of 32, 256 x 128
+  // 21.3 / 26.6)
   const bool keeps = D <= 64 && !a.maps && a.Lk <= 2 * KT;
   a.n_blk = (int)blocks(slots, keeps ? 16 * QR::B * QR::NW : small ? 16 * QS::B * QS::NW : 16 * Q::B * Q::NW);
   long long grid = da_grid(a.n_blk, groups);

@@ -68,8 +68,8 @@ __global__ __launch_bounds__(256) void vl_count_kernel(const unsigned char* __re
 }
 
 // the group's weighted rows to their places: the counts of the groups before it are added up first (in order). Bound by
-// memory behind that sum's latency (16 384 of 32 768 rows of 768 bytes: 25 MB in 8-9 us); a row's chunks are dealt to more workgroups from
-// 512 values on.
+// memory behind that sum's latency (16 384 of 32 768 rows of 768 bytes: 25 MB in 8-9 us); a row's chunks are dealt to more
+// workgroups from 512 values on.
 __global__ __launch_bounds__(256) void vl_gather_kernel(const unsigned short* __restrict__ hidden, const long long* __restrict__ targets,
                                                         const unsigned char* __restrict__ ind, const long long* __restrict__ attn,
                                                         const int* __restrict__ counts, const float* __restrict__ sums, VlState st,
@@ -127,13 +127,13 @@ __global__ __launch_bounds__(256) void vl_gather_kernel(const unsigned short* __
 }
 
 // =====================================================================================
-// C[m, n] = sum_k A(m, k) B(n, k) on BM x BN tiles. AKC / BKC: the operand is stored along k (rows of K values) or, if
-// not, along its own axis (row k holds the values of all m / n). MFMA operand order: n is the A side and m the B side,
-// with n permuted inside 64 columns, so that a lane ends up with 2 x 8 consecutive n of one row m (columns 8 g and 32 + 8 g: the
-// four lanes of a row store 64 consecutive bytes at a time).
-// K is staged 64 at a time by LDS-DMA, two stages in turn (three or four stages of 32: 4-15 % slower).
-// Bound by the matrix cores where the summed axis is long: 4096 x 2048 -> 65536 scores 746 us = 1.47 PFLOP/s (65 % of the cycles; the
-// clock gives way under the load), dz 1.15, dh 1.3, dW 1.3; by the tiles' start and end at short ones: 16384 x 384 -> 803 0.4-0.6.
+// C[m, n] = sum_k A(m, k) B(n, k) on BM x BN tiles. AKC / BKC: the operand is stored along k (rows of K values) or, if not,
+// along its own axis (row k holds the values of all m / n). MFMA operand order: n is the A side and m the B side, with n
+// permuted inside 64 columns, so that a lane ends up with 2 x 8 consecutive n of one row m (columns 8 g and 32 + 8 g: the
+// four lanes of a row store 64 consecutive bytes at a time). K is staged 64 at a time by LDS-DMA, two stages in turn (three
+// or four stages of 32: 4-15 % slower). Bound by the matrix cores where the summed axis is long: 4096 x 2048 -> 65536 scores
+// 746 us = 1.47 PFLOP/s (65 % of the cycles; the clock gives way under the load), dz 1.15, dh 1.3, dW 1.3; by the tiles'
+// start and end at short ones: 16384 x 384 -> 803 0.4-0.6.
 // =====================================================================================
 // Splits of a product's summed axis: one workgroup per CU, four stages each at least. For dh the tiles follow the row count
 // on the device, so the kernel and the one that adds the slabs up ask this themselves.
@@ -472,7 +472,8 @@ __global__ __launch_bounds__(256) void vl_join_kernel(VlState st, const unsigned
   }
 }
 
-// loss = sum rowloss / sum w, in a fixed order; an exact zero without a weighted row (16 384 rows: 4 us, one workgroup's latency)
+// loss = sum rowloss / sum w, in a fixed order; an exact zero without a weighted row (16 384 rows: 4 us, one workgroup's
+// latency)
 __global__ __launch_bounds__(1024) void vl_finish_kernel(VlState st, const float* __restrict__ rowloss, float* __restrict__ loss) {
   __shared__ float part[16];
   const int n = st.head[0];
@@ -550,12 +551,13 @@ __global__ __launch_bounds__(256) void vl_dw_kernel(VlState st, const float* __r
 
 // =====================================================================================
 // Forward for a vocabulary of at most 64 classes: 16 rows a workgroup, straight from where they lie (they are gathered
-// beside it only where a backward follows; it then leaves their log-sum-exps at their compact places). The waves share the rows and deal the hidden size among them (32 values in turn; the small call is bound by latency: every load
-// of a wave is asked for before its first product); their scores meet in LDS, where 16 threads finish a row. Transposed
-// products (z^T = W h^T): a lane's scores are one row's. Then the workgroups' sums are added in order.
-// Measured, hidden size 384, half of the rows weighted, this / gathered rows and tiles, without a backward, us: 512 rows, 39
-// classes 8.6 / 23; 32768 rows, 39 classes 18 / 36 (beside the gathering for a backward 18 / 21). At 128 classes it is
-// 34 / 36 and 37 / 21: every workgroup reads the head's rows again.
+// beside it only where a backward follows; it then leaves their log-sum-exps at their compact places). The waves share the
+// rows and deal the hidden size among them (32 values in turn; the small call is bound by latency: every load of a wave is
+// asked for before its first product); their scores meet in LDS, where 16 threads finish a row. Transposed products (z^T = W
+// h^T): a lane's scores are one row's. Then the workgroups' sums are added in order. Measured, hidden size 384, half of the
+// rows weighted, this / gathered rows and tiles, without a backward, us: 512 rows, 39 classes 8.6 / 23; 32768 rows, 39
+// classes 18 / 36 (beside the gathering for a backward 18 / 21). At 128 classes it is 34 / 36 and 37 / 21: every workgroup
+// reads the head's rows again.
 // =====================================================================================
 constexpr int VL_NARROW = 64, VL_NROWS = 16;
 __global__ __launch_bounds__(256, 2) void vl_narrow_kernel(const unsigned short* __restrict__ hidden, const unsigned short* __restrict__ weight,
