@@ -29,7 +29,7 @@ struct VlState {                      // what the forward leaves for the backwar
   int* head;                          // [0] weighted rows, [1] sum of weights (float bits)
   int *idx, *pos, *tgt;               // compact row -> row; row -> compact row or -1; target of a compact row
   float *w, *lse;                     // weight and log2-sum-exp2 of z * log2(e) of a compact row
-  unsigned short* hc;                 // [m_pad, d] compact rows, zeros behind the last
+  unsigned short* hc;                 // [m_pad, d] compact rows, zeros to the end of the last 64
   long long bytes;
 };
 
@@ -80,6 +80,7 @@ __global__ __launch_bounds__(256) void vl_gather_kernel(const unsigned short* __
   const int groups = (M + SCAN - 1) / SCAN, grp = blockIdx.x;
   int nb = 0, na = 0;
   float ws = 0.f;
+#pragma unroll 4
   for (int i = tid; i < groups; i += 256) {
     const int n = counts[i];
     na += n;
@@ -119,10 +120,12 @@ __global__ __launch_bounds__(256) void vl_gather_kernel(const unsigned short* __
     const int r = i / chn, ch = ch0 + i - r * chn;
     *(u32x4*)(st.hc + (long long)(first + r) * d + 8 * ch) = *(const u32x4*)(hidden + (long long)src[r] * d + 8 * ch);
   }
-  if (grp == groups - 1 && blockIdx.y == 0) {      // zeros behind the last row, to the end of its 256-row tile
-    const int end = (int)vl_up(total, 256);
-    for (long long i = tid; i < (long long)(end - total) * per; i += 256)
-      *(u32x4*)(st.hc + (long long)total * d + 8 * i) = (u32x4){0u, 0u, 0u, 0u};
+  if (grp == groups - 1) {      // zeros behind the last row to the end of its 64: dW sums whole stages of rows (what a tile's
+    const int tail = (int)vl_up(total, 64) - total;      // further rows hold reaches no row but their own)
+    for (int i = tid; i < tail * chn; i += 256) {
+      const int r = i / chn;
+      *(u32x4*)(st.hc + (long long)(total + r) * d + 8 * (ch0 + i - r * chn)) = (u32x4){0u, 0u, 0u, 0u};
+    }
   }
 }
 
@@ -509,6 +512,7 @@ __global__ __launch_bounds__(256) void vl_dh_kernel(VlState st, const float* __r
     const float sw = ((const float*)st.head)[1];
     const float coef = sw > 0.f ? gout[0] / sw : 0.f;
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int s = 0; s < n_slab; ++s) {
       const float* p = slab + s * slab_stride + (long long)at * d + 8 * ch;
       const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
@@ -521,21 +525,36 @@ __global__ __launch_bounds__(256) void vl_dh_kernel(VlState st, const float* __r
   *(u32x4*)(dh + (long long)row * d + 8 * ch) = o;
 }
 
-// dW rows v0 .. v0 + rows from the slabs of their splits. Bound by memory (803 x 384, 12 slabs: 5 us)
+// dW rows v0 .. v0 + rows from the slabs of their splits: 32 units of 8 values a workgroup, each added up by eight threads that
+// take every eighth slab, then in order. Bound by memory (803 x 384, 12 slabs) or latency (39 x 64, 256 slabs: 3.4 us, one
+// thread a unit 21)
 __global__ __launch_bounds__(256) void vl_dw_kernel(VlState st, const float* __restrict__ slab, long long slab_stride, int n_slab,
                                                     const float* __restrict__ gout, void* __restrict__ dw, int dw_f32, int v0, int rows, int d) {
-  const int per = d / 8;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long long)rows * per) return;
+  __shared__ float part[7][32][9];
+  const int tid = threadIdx.x, unit = tid & 31, from = tid >> 5;
+  const long long i = (long long)blockIdx.x * 32 + unit, all = (long long)rows * (d / 8);
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (i < all) {
+#pragma unroll 4
+    for (int s = from; s < n_slab; s += 8) {
+      const float* p = slab + s * slab_stride + 8 * i;
+      const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { v[e] += a[e]; v[4 + e] += b[e]; }
+    }
+  }
+  if (from > 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[from - 1][unit][e] = v[e];
+  }
+  __syncthreads();
+  if (from > 0 || i >= all) return;
+#pragma unroll
+  for (int f = 0; f < 7; ++f)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += part[f][unit][e];
   const float sw = ((const float*)st.head)[1];
   const float coef = sw > 0.f ? gout[0] / sw : 0.f;
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < n_slab; ++s) {
-    const float* p = slab + s * slab_stride + 8 * i;
-    const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { v[e] += a[e]; v[4 + e] += b[e]; }
-  }
   const long long at = (long long)v0 * d + 8 * i;
   if (dw_f32) {
     float* o = (float*)dw + at;
@@ -819,7 +838,7 @@ extern "C" int bd_linear_ce_bwd(const void* weight, const float* grad_out, void*
         vl_launch<false, false, VL_SLAB>(pl.big_w, p, s);
         const int rows = min(n, V - v0);
         const long long items = (long long)rows * (d / 8);
-        hipLaunchKernelGGL(vl_dw_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256), 0, s, st, slab_w, pl.slab_w, pl.split_w, grad_out,
+        hipLaunchKernelGGL(vl_dw_kernel, dim3((unsigned)((items + 31) / 32)), dim3(256), 0, s, st, slab_w, pl.slab_w, pl.split_w, grad_out,
                            dweight, dweight_dtype == BD_DTYPE_F32, v0, rows, d);
       } else {
         p.gout = grad_out; p.dw = dweight; p.dw_f32 = dweight_dtype == BD_DTYPE_F32;
