@@ -709,7 +709,7 @@ __global__ __launch_bounds__(256) void da_join_few_kernel(DaArgs a) {
 }
 
 // =====================================================================================
-// Backward, query side: dQ and what the key side needs of each slot (stats: lse1, lse2, delta1, delta2, lam), dlam. A wave
+// Backward, query side: dQ and what the key side needs of each slot (stats: lse1, lse2, delta1, delta2, lam, scale of dK), dlam. A wave
 // owns 16 QB slots and both of their maps (dP = dO V^T is shared). delta_m comes from the forward's fp32 maps (dO . O_m) or,
 // where none were kept, from a first walk over the keys (SHORT: from what the only walk leaves in registers): sums of the
 // very P and dP that form dS. From a bf16-rounded O it would miss sum_j dS_ij = 0 by 2^-9 of |dO||O| for all keys alike, as
@@ -828,6 +828,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
                         acc[qb][i & 1][i >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, dsf[qb][i & 1], acc[qb][i & 1][i >> 1], 0, 0, 0);
                     });
   };
+  int seen = 0;                                            // keys that the mask leaves
   auto walk_keys = [&](auto last) {                        // last: dQ is summed; else delta
     constexpr bool LAST = decltype(last)::value;
     unsigned mb = da_mask_byte(a, b, lane, kend);
@@ -841,6 +842,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
       const unsigned long long vis_next = __ballot(mb != 0u);
       mb = da_mask_byte(a, b, kt0 + 2 * KT + lane, kend);
       if (kt0 + KT < kend) keys.run(a, other, kt0 + KT, vis_next, wave, lane);
+      if (LAST) seen += __popcll(vis);
 #pragma unroll 1                                           // (unrolled, the scheduler reads ahead more than the registers hold)
       for (int h2 = 0; h2 < 2; ++h2) {                     // 32 keys
         const unsigned kn = cur + knat + 32 * RK * h2, kt = cur + ktr + 32 * RK * h2, vn = cur + vnat + 32 * RV * h2;
@@ -881,6 +883,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       vis[t] = __ballot(da_mask_byte(a, b, KT * t + lane, kend) != 0u);
+      seen += __popcll(vis[t]);
       if (KT * t < kend) keys.run(a, lds0 + t * TILE, KT * t, vis[t], wave, lane);
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -928,6 +931,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
     }
     walk_keys(std::true_type());
   }
+  // One key alone has weight 1 whatever its score: dQ and dK are exact zeros, where 2^(s - lse) rounds beside 1
+  const float scale = seen == 1 ? 0.f : a.scale;
   const int s1 = da_again(s0), g1 = da_again(lane) >> 4;
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
@@ -937,12 +942,12 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
     const float lam = da_lam(a, bq * a.ls[0] + (sp.q0 + sl.row) * a.ls[1] + sl.head * a.ls[2]);
     if (g1 == 0) {
       *(f32x4*)(a.stats + 8 * rh) = (f32x4){lse[qb][0], lse[qb][1], dl[qb][0], dl[qb][1]};
-      a.stats[8 * rh + 4] = lam;
+      *(f32x2*)(a.stats + 8 * rh + 4) = (f32x2){lam, scale};
       da_put_dlam(a, rh, -dl[qb][1]);
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      const float f = m ? -lam * a.scale : a.scale;
+      const float f = m ? -lam * scale : scale;
       unsigned short* op = a.dq + bq * a.dqs[0] + (sp.q0 + sl.row) * a.dqs[1] + (2 * sl.head + m) * a.dqs[2] + 4 * g1;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
@@ -1134,6 +1139,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
     }
   }
   const int k1 = da_again(k0), g1 = da_again(lane) >> 4;
+  const float scale = n_slots > 0 ? *(const float*)(sb0 + 20) : 0.f;   // (the same of every slot: they see the same keys)
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
     const int key = k1 + 16 * kb;
@@ -1147,8 +1153,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dkv_kernel(DaArgs a) {
       for (int dt = 0; dt < DT; ++dt) {
         u32x2 w = {0u, 0u};
         if (vis) {
-          w[0] = bd_pack_bf16x2(ak[kb][m][dt][0] * a.scale, ak[kb][m][dt][1] * a.scale);
-          w[1] = bd_pack_bf16x2(ak[kb][m][dt][2] * a.scale, ak[kb][m][dt][3] * a.scale);
+          w[0] = bd_pack_bf16x2(ak[kb][m][dt][0] * scale, ak[kb][m][dt][1] * scale);
+          w[1] = bd_pack_bf16x2(ak[kb][m][dt][2] * scale, ak[kb][m][dt][3] * scale);
         }
         *(u32x2*)(op + 16 * dt) = w;
       }

@@ -230,6 +230,52 @@ def test_differential_attention_packed_rows(gpu_device, lens, total, H, Hkv, D, 
         within(dh, r2["dlam"].sum(0), r2["dlam_tol"].sum(0) + r2["dlam"].abs().sum(0) * (total + 8) * R.F + R.F * r2["dlam"].sum(0).abs(), "dlam by head")
 
 
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [
+    (1, 1, 1, 1, 1, 64), (3, 5, 1, 4, 2, 32), (4, 70, 1, 2, 1, 128), (2, 9, 40, 2, 2, 64), (3, 129, 128, 3, 3, 64), (2, 20, 200, 4, 1, 64),
+    (2, 33, 300, 2, 2, 32), (2, 300, 150, 2, 1, 128), (2, 17, 1100, 2, 2, 128),
+])
+def test_differential_attention_one_key_seen(gpu_device, B, Lq, Lk, H, Hkv, D):
+    """One key has weight 1 whatever its score: out = (1 - lam) v, and q and k have a gradient of exactly zero."""
+    dev = gpu_device
+    q, k, v, lam, _, dout = attention_case(dev, B, Lq, Lk, H, Hkv, D, None, "token")
+    m = torch.zeros(B, Lk, dtype=torch.bool, device=dev)
+    m[torch.arange(B), torch.arange(B) * 37 % Lk] = True
+    r = reference(q, k, v, lam, m, dout, H)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lam)]
+    for mask in (m, None) if Lk == 1 else (m,):
+        out = ops.differential_attention(*leaves, key_mask=mask)
+        within(out.detach(), r["out"].view(out.shape), r["out_tol"].view(out.shape), "out")
+        dq, dk, dv, dlam = torch.autograd.grad(out, leaves, dout)
+        assert not bool(dq.any()) and not bool(dk.any())
+        within(dv, r["dv"].view(dv.shape), r["dv_tol"].view(dv.shape), "dv")
+        want, tol = lam_gradient(r, lam, (B, Lq), H)
+        within(dlam, want, tol, "dlam")
+    if Lk > 1:                                             # a second key for the last entry: its gradients are back, the others' stay zero
+        m[-1, (B * 37 - 36) % Lk] = True
+        r = reference(q, k, v, lam, m, dout, H)
+        dq, dk = torch.autograd.grad(ops.differential_attention(*leaves, key_mask=m), leaves[:2], dout)
+        assert not bool(dq[:-1].any()) and not bool(dk[:-1].any()) and bool(dq[-1].any()) and bool(dk[-1].any())
+        within(dq, r["dq"].view(dq.shape), r["dq_tol"].view(dq.shape), "dq")
+        within(dk, r["dk"].view(dk.shape), r["dk_tol"].view(dk.shape), "dk")
+
+
+@pytest.mark.parametrize("lens,D", [([1], 32), ([1] * 9, 64), ([1, 0, 1, 1], 128), ([1, 2, 1, 70, 1], 64)])
+def test_differential_attention_packed_rows_of_one_token(gpu_device, lens, D):
+    dev, total, H, Hkv = gpu_device, sum(lens) + 2, 4, 2
+    g = gen(dev, total + D)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=dev).to(BF)  # noqa: E731
+    leaves = [t.requires_grad_(True) for t in (rnd(total, 2 * H, D), rnd(total, 2 * Hkv, D), rnd(total, Hkv, 2 * D), rnd(total, H))]
+    cu = torch.tensor([0, *np.cumsum(lens)], dtype=torch.int32, device=dev)
+    out = ops.differential_attention(*leaves, cu_seqlens=cu)
+    dq, dk, dv, _ = torch.autograd.grad(out, leaves, rnd(total, H, 2 * D))
+    alone = torch.zeros(total, dtype=torch.bool, device=dev)
+    for n, at in zip(lens, cu.tolist()):
+        alone[at:at + n] = n == 1
+    assert not bool(dq[alone].any()) and not bool(dk[alone].any()) and bool(dv[alone].any())
+    seen = ~alone & (torch.arange(total, device=dev) < cu[-1])
+    assert bool((dq[seen].flatten(1) != 0).any(1).all()) and bool((dk[seen].flatten(1) != 0).any(1).all())
+
+
 def test_differential_attention_packed_rows_longer_than_announced_are_nan(gpu_device):
     dev = gpu_device
     x = [torch.randn(20, h, w, device=dev).to(BF) for h, w in ((4, 32), (4, 32), (2, 64))]
