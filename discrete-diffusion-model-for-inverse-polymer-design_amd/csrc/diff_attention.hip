@@ -713,7 +713,9 @@ __global__ __launch_bounds__(256) void da_join_few_kernel(DaArgs a) {
 // owns 16 QB slots and both of their maps (dP = dO V^T is shared). delta_m comes from the forward's fp32 maps (dO . O_m) or,
 // where none were kept, from a first walk over the keys (SHORT: from what the only walk leaves in registers): sums of the
 // very P and dP that form dS. From a bf16-rounded O it would miss sum_j dS_ij = 0 by 2^-9 of |dO||O| for all keys alike, as
-// large as dS itself where attention is nearly uniform. Head size 128 as above: 435 us, 0.95 PFLOP/s, matrix cores busy 45
+// large as dS itself where attention is nearly uniform. dlam is always -sum_j P2 dP of the walk: the fp32 maps hold the
+// forward's bf16 weights (1.7e-3 of a row), which a weight per head, summed over rows that cancel, does not bear (5.9e-3 of
+// 36 x 739 rows' sum, now the 2^-8 of its own rounding; one fma a pair, 1 % of dq at head size 32, 3 % at 128). Head size 128 as above: 435 us, 0.95 PFLOP/s, matrix cores busy 45
 // %, vector units 42 %.
 // =====================================================================================
 template <int D, int QB, int NW, int OCC, bool SHORT>
@@ -829,8 +831,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
                     });
   };
   int seen = 0;                                            // keys that the mask leaves
-  auto walk_keys = [&](auto last) {                        // last: dQ is summed; else delta
-    constexpr bool LAST = decltype(last)::value;
+  float dm[QB];                                            // dP . P2 of the rows, for dlam
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) dm[qb] = 0.f;
+  auto walk_keys = [&](auto last, auto only) {             // last: dQ is summed; else delta. only: dlam's sums too
+    constexpr bool LAST = decltype(last)::value, ONLY = decltype(only)::value;
     unsigned mb = da_mask_byte(a, b, lane, kend);
     unsigned long long vis = __ballot(mb != 0u);
     __syncthreads();                                       // (second walk: nobody reads the first one's last tile)
@@ -858,6 +863,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 const float p = __builtin_amdgcn_exp2f(s[qb][m][r] * scale2 - lse[qb][m]);
+                if (ONLY && m == 1) dm[qb] += p * dp[qb][r];
                 if (!LAST) dl[qb][m] += p * dp[qb][r];
                 else dsf[qb][m][4 * half + r] = (__bf16)(p * (dp[qb][r] - dl[qb][m]));
               }
@@ -868,14 +874,17 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
       const unsigned sw = cur; cur = other; other = sw;
     }
   };
+  auto join = [&](float& x) {                              // the lanes that share a slot
+    x += __shfl_xor(x, 16, 64);
+    x += __shfl_xor(x, 32, 64);
+  };
   auto join_delta = [&] {
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb)
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        dl[qb][m] += __shfl_xor(dl[qb][m], 16, 64);
-        dl[qb][m] += __shfl_xor(dl[qb][m], 32, 64);
-      }
+    for (int qb = 0; qb < QB; ++qb) {
+      join(dl[qb][0]);
+      join(dl[qb][1]);
+      dm[qb] = dl[qb][1];
+    }
   };
   if constexpr (SHORT) {                                   // both tiles stay in LDS, their weights and dP in registers
     f32x4 p[2][2][2][QB][2], dp[2][2][2][QB];              // [tile][32 keys][16 of them]
@@ -925,11 +934,15 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
       }
     }
   } else {
-    if (!a.maps) {
-      walk_keys(std::false_type());
+    if (a.maps) {
+      walk_keys(std::true_type(), std::true_type());
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) join(dm[qb]);
+    } else {
+      walk_keys(std::false_type(), std::false_type());
       join_delta();
+      walk_keys(std::true_type(), std::false_type());
     }
-    walk_keys(std::true_type());
   }
   // One key alone has weight 1 whatever its score: dQ and dK are exact zeros, where 2^(s - lse) rounds beside 1
   const float scale = seen == 1 ? 0.f : a.scale;
@@ -943,7 +956,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
     if (g1 == 0) {
       *(f32x4*)(a.stats + 8 * rh) = (f32x4){lse[qb][0], lse[qb][1], dl[qb][0], dl[qb][1]};
       *(f32x2*)(a.stats + 8 * rh + 4) = (f32x2){lam, scale};
-      da_put_dlam(a, rh, -dl[qb][1]);
+      da_put_dlam(a, rh, -dm[qb]);
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {

@@ -259,6 +259,24 @@ def test_differential_attention_one_key_seen(gpu_device, B, Lq, Lk, H, Hkv, D):
         within(dk, r["dk"].view(dk.shape), r["dk_tol"].view(dk.shape), "dk")
 
 
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [(2, 60, 300, 2, 1, 32), (1, 130, 513, 2, 2, 64), (1, 40, 1100, 1, 1, 128), (2, 60, 120, 2, 1, 32), (1, 40, 400, 2, 2, 64)])
+def test_differential_attention_weight_gradient_keeps_fp32(gpu_device, B, Lq, Lk, H, Hkv, D):
+    """Every value row holds x in one column: a row's dlam is -x dout of that column, with no error of weights in bf16
+    (about 1e-4 here). Relative: both sums over the keys Lk steps of 2^-24, the scores' dot products D steps of their
+    absolute sum in each pass, the exponents a step of their size."""
+    dev = gpu_device
+    q, k, _, _, _, dout = attention_case(dev, B, Lq, Lk, H, Hkv, D, None, "token")
+    v = torch.zeros(B, Lk, Hkv, 2 * D, dtype=BF, device=dev)
+    v[..., 5] = 1.5
+    lam = torch.full((B, Lq, H), 0.5, device=dev, requires_grad=True)
+    out = ops.differential_attention(q.requires_grad_(True), k, v, lam)
+    (dlam,) = torch.autograd.grad(out, (lam,), dout)
+    want = -1.5 * dout[..., 5].double()
+    absolute = float((q.detach().float().norm(dim=-1).max() * k.float().norm(dim=-1).max()).item()) / D ** 0.5
+    rel = R.F * (2 * Lk + 2 * D * absolute + 8 * absolute + 16)
+    within(dlam, want, rel * want.abs(), "dlam")
+
+
 @pytest.mark.parametrize("lens,D", [([1], 32), ([1] * 9, 64), ([1, 0, 1, 1], 128), ([1, 2, 1, 70, 1], 64)])
 def test_differential_attention_packed_rows_of_one_token(gpu_device, lens, D):
     dev, total, H, Hkv = gpu_device, sum(lens) + 2, 4, 2
