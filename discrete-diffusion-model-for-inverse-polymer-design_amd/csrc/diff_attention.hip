@@ -709,14 +709,14 @@ __global__ __launch_bounds__(256) void da_join_few_kernel(DaArgs a) {
 }
 
 // =====================================================================================
-// Backward, query side: dQ and what the key side needs of each slot (stats: lse1, lse2, delta1, delta2, lam, scale of dK), dlam. A wave
-// owns 16 QB slots and both of their maps (dP = dO V^T is shared). delta_m comes from the forward's fp32 maps (dO . O_m) or,
-// where none were kept, from a first walk over the keys (SHORT: from what the only walk leaves in registers): sums of the
-// very P and dP that form dS. From a bf16-rounded O it would miss sum_j dS_ij = 0 by 2^-9 of |dO||O| for all keys alike, as
-// large as dS itself where attention is nearly uniform. dlam is always -sum_j P2 dP of the walk: the fp32 maps hold the
-// forward's bf16 weights (1.7e-3 of a row), which a weight per head, summed over rows that cancel, does not bear (5.9e-3 of
-// 36 x 739 rows' sum, now the 2^-8 of its own rounding; one fma a pair, 1 % of dq at head size 32, 3 % at 128). Head size 128 as above: 435 us, 0.95 PFLOP/s, matrix cores busy 45
-// %, vector units 42 %.
+// Backward, query side: dQ and what the key side needs of each slot (stats: lse1, lse2, delta1, delta2, lam, scale of
+// dK), dlam. A wave owns 16 QB slots and both of their maps (dP = dO V^T is shared). delta_m comes from the forward's
+// fp32 maps (dO . O_m) or, where none were kept, from a first walk over the keys (SHORT: from what the only walk leaves
+// in registers): sums of the very P and dP that form dS. From a bf16-rounded O it would miss sum_j dS_ij = 0 by 2^-9 of
+// |dO||O| for all keys alike, as large as dS itself where attention is nearly uniform. dlam is always -sum_j P2 dP of the
+// walk: the fp32 maps hold the forward's bf16 weights (1.7e-3 of a row), which a weight per head, summed over rows that
+// cancel, does not bear (5.9e-3 of 36 x 739 rows' sum, now the 2^-8 of its own rounding; one fma a pair, 1 % of dq at
+// head size 32, 3 % at 128). Head size 128 as above: 440 us, 0.94 PFLOP/s, matrix cores busy 45 %, vector units 42 %.
 // =====================================================================================
 template <int D, int QB, int NW, int OCC, bool SHORT>
 __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
