@@ -546,8 +546,9 @@ class _BackboneFn(torch.autograd.Function):
 
         dh_buf = torch.empty(M, d, dtype=bf, device=dev)
         head_job = None
-        if ctx.mode == 2:
-            dh_buf = dlogits.reshape(M, d).contiguous()
+        dh_top = dh_buf              # gradient of the final norm's rows
+        if ctx.mode == 2:            # (autograd's own tensor: read by the final norm alone, the layers write dh_buf)
+            dh_top = dlogits.reshape(M, d).contiguous()
         elif ctx.mode == 1:
             # the incoming gradient is that of the final-norm output itself
             _to_bf16(dlogits.reshape(M, d).float().contiguous(), dh_buf)
@@ -658,7 +659,7 @@ class _BackboneFn(torch.autograd.Function):
         top = (n_layers - 1) % len(dyb) if n_layers else 0
         lnp = tw.ln_parts(d, dev)
         lnp.begin()
-        _ln_bwd(dh_buf, ctx.x_last, ctx.stf, model.final_norm.weight, None, dx, gbuf(model.final_norm.weight),
+        _ln_bwd(dh_top, ctx.x_last, ctx.stf, model.final_norm.weight, None, dx, gbuf(model.final_norm.weight),
                 gbuf(model.final_norm.bias), M, d, dx_bf16=dyb[top] if n_layers else None, drop=drop,
                 site=max(0, 4 * (n_layers - 1) + 3), parts=lnp)
 
