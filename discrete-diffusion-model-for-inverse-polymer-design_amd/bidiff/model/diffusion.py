@@ -179,10 +179,11 @@ class DiscreteMaskingDiffusion(nn.Module):
             from .. import ops
             from ..training import autograd as ag
             if torch.is_grad_enabled() and any(p.requires_grad for p in bb.parameters()):
-                hidden = ag.backbone_forward_train(bb, noisy_ids, timesteps, attention_mask, hidden_states="bf16")
+                hidden, head = ag.backbone_forward_train(bb, noisy_ids, timesteps, attention_mask, hidden_states="head")
             else:
                 hidden, _ = bb.run_forward(noisy_ids, timesteps, bb._keymask_bytes(attention_mask, noisy_ids))
-            loss = ops.linear_cross_entropy(hidden, bb.output_proj.weight, input_ids.to(torch.long), mask_indicator, attention_mask)
+                head = bb.output_proj.weight
+            loss = ops.linear_cross_entropy(hidden, head, input_ids.to(torch.long), mask_indicator, attention_mask)
 
             def logits():
                 with torch.no_grad():

@@ -418,7 +418,8 @@ class _BackboneFn(torch.autograd.Function):
         """mode 0: logits [B, L, V] (the diffusion training step); mode 1: the final-norm hidden states
         [B, L, d] in fp32 (what get_hidden_states / get_pooled_output return to a property head that
         fine-tunes the last blocks, reference property_head.py:102-112); mode 2: the same rows in bf16, as the
-        vocabulary head reads them."""
+        vocabulary head reads them, and the head's weight itself (None if it is frozen): a loss that reads the weight
+        through this output sends its gradient through the backward pass below."""
         from ..model import _blocks as blocks
         _enter()
         lib = _lib.lib()
@@ -499,7 +500,9 @@ class _BackboneFn(torch.autograd.Function):
             hf = torch.empty(M, d, dtype=bf, device=dev)
             _ln(x, model.final_norm.weight, model.final_norm.bias, hf, stf, M, d, eps)
             ctx.x_last, ctx.stf, ctx.hf = x, stf, None
-            return hf if pk is not None else hf.view(B, L, d)
+            ctx.set_materialize_grads(False)          # (nobody may read the weight through here)
+            head = model.output_proj.weight
+            return (hf if pk is not None else hf.view(B, L, d)), (head if head.requires_grad else None)
         if mode == 1:
             hid = torch.empty(B, L, d, device=dev) if pk is None else torch.empty(M, d, device=dev)
             _ck(lib.bd_layernorm(_lib.ptr(x), _lib.ptr(model.final_norm.weight), _lib.ptr(model.final_norm.bias), None,
@@ -514,7 +517,7 @@ class _BackboneFn(torch.autograd.Function):
         return logits
 
     @staticmethod
-    def backward(ctx, dlogits):
+    def backward(ctx, dlogits, dhead=None):
         from ..model import _blocks as blocks
         _enter()
         lib = _lib.lib()
@@ -548,7 +551,7 @@ class _BackboneFn(torch.autograd.Function):
         head_job = None
         dh_top = dh_buf              # gradient of the final norm's rows
         if ctx.mode == 2:            # (autograd's own tensor: read by the final norm alone, the layers write dh_buf)
-            dh_top = dlogits.reshape(M, d).contiguous()
+            dh_top = dh_buf.zero_() if dlogits is None else dlogits.reshape(M, d).contiguous()
         elif ctx.mode == 1:
             # the incoming gradient is that of the final-norm output itself
             _to_bf16(dlogits.reshape(M, d).float().contiguous(), dh_buf)
@@ -615,6 +618,16 @@ class _BackboneFn(torch.autograd.Function):
             handed[li] = done
 
         hook_fn, hook_layer = _tail_hook_of(model)
+        if ctx.mode == 2:
+            # The hook promises the head's gradient too: it is added here, ahead of the hook, where it came through this
+            # pass, and a head whose gradient goes another way leaves the hook out (whoever waits for it asks at the end).
+            head = model.output_proj.weight
+            if dhead is not None and direct and hook_fn is not None:
+                head.grad.add_(dhead)
+            elif dhead is not None:
+                grads[head] = dhead
+            elif head.requires_grad:
+                hook_fn = None
 
         def tail_hook(li):
             """Every gradient of the layers >= li is enqueued (main stream: this layer's kernels; second stream: the
@@ -750,7 +763,9 @@ class _BackboneFn(torch.autograd.Function):
 
 def backbone_forward_train(model, input_ids, timesteps, attention_mask, hidden_states=False, packing=None):
     """Training forward: logits, or (``hidden_states=True``) the fp32 final-norm hidden states (``"bf16"``: the rows the
-    vocabulary head reads). With a ``RowPacking`` the result holds the packed rows ([n_rows, V] or [n_rows, d]) instead of [B, L, .]."""
+    vocabulary head reads; ``"head"``: (those rows, the head's weight), for a loss whose gradient of the weight is to be
+    complete when the hook of ``set_tail_ready_hook`` is called). With a ``RowPacking`` the result holds the packed rows
+    ([n_rows, V] or [n_rows, d]) instead of [B, L, .]."""
     _lib.require_device(input_ids, "DiffusionBackbone.forward")
     if model.hidden_size % 128 or model.ffn_hidden_size % 128:
         raise ValueError("bidiff training path needs hidden and ffn sizes that are multiples of 128")
@@ -762,8 +777,12 @@ def backbone_forward_train(model, input_ids, timesteps, attention_mask, hidden_s
             raise RuntimeError("bidiff training path expects contiguous fp32 parameters")
     if packing is not None and (packing.B, packing.L) != tuple(ids.shape):
         raise ValueError("RowPacking was built for another batch shape")
-    mode = 2 if hidden_states == "bf16" else 1 if hidden_states else 0
-    return _BackboneFn.apply(model, ids, timesteps, keymask, mode, packing, *model._params())
+    mode = 2 if hidden_states in ("bf16", "head") else 1 if hidden_states else 0
+    out = _BackboneFn.apply(model, ids, timesteps, keymask, mode, packing, *model._params())
+    if mode != 2:
+        return out
+    rows, head = out
+    return (rows, model.output_proj.weight if head is None else head) if hidden_states == "head" else rows
 
 
 class _MaskedCE(torch.autograd.Function):
@@ -830,7 +849,9 @@ def packed_training_loss(diffusion, noisy_ids, timesteps, attention_mask, target
         lengths = RowPacking.lengths_from_mask(attention_mask)
     pk = RowPacking(lengths, B, L, noisy_ids.device)
     fused = bool(getattr(diffusion, "fused_head_loss", False))
-    rows_p = backbone_forward_train(backbone, noisy_ids, timesteps, attention_mask, hidden_states="bf16" if fused else False, packing=pk)
+    rows_p = backbone_forward_train(backbone, noisy_ids, timesteps, attention_mask, hidden_states="head" if fused else False, packing=pk)
+    if fused:
+        rows_p, head = rows_p
     # targets and loss flags of the packed rows (attention mask folded into the flag, fillers flagged off): one launch
     tg = torch.empty(pk.n_rows, dtype=torch.long, device=noisy_ids.device)
     ind = torch.empty(pk.n_rows, dtype=torch.uint8, device=noisy_ids.device)
@@ -842,7 +863,7 @@ def packed_training_loss(diffusion, noisy_ids, timesteps, attention_mask, target
                                    _lib.ptr(tg), _lib.ptr(ind), _s()), "bd_pack_targets")
     if fused:
         from .. import ops
-        loss = ops.linear_cross_entropy(rows_p, backbone.output_proj.weight, tg, ind)
+        loss = ops.linear_cross_entropy(rows_p, head, tg, ind)
     else:
         loss = masked_cross_entropy(rows_p, tg, ind, None)
 

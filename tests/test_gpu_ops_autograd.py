@@ -37,3 +37,61 @@ def test_gradient_of_the_heads_rows_is_left_alone(gpu_device):
     loss = ops.linear_cross_entropy(hidden, bb.output_proj.weight.detach(), ids, None, attn)
     got = torch.autograd.grad(loss, (hidden, bb.final_norm.weight))[0]
     assert torch.equal(got, want) and torch.equal(kept[0], want)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("heads,attention", [(3, "softmax"), (8, "softmax"), (6, "differential")])
+def test_tail_hook_of_the_fused_head_loss(gpu_device, heads, attention, packed):
+    """The hook inside the backward pass (data-parallel training starts the all-reduce of ``flat_grad[split:]`` there) sees
+    the final gradients of the upper layers, the final norm and the vocabulary head, whose gradient the fused loss makes."""
+    from bidiff.parallel import tail_split_offset
+    bb, model, ids, attn, _ = small_model(gpu_device, heads, attention, dropout=0.1)
+    model.fused_head_loss, model.skip_padded_rows = True, packed
+    opt = FlatAdamW(model.parameters(), lr=1e-3)
+    off = tail_split_offset(opt, bb, 2)
+    seen = []
+    AG.set_tail_ready_hook(lambda: seen.append((opt.flat_grad[off:].clone(), opt.flat_grad[:off].clone())), 2, model=bb)
+    try:
+        for _ in range(3):
+            opt.zero_grad()
+            seen.clear()
+            model(ids, attn)["loss"].backward()
+            torch.cuda.synchronize()
+            assert len(seen) == 1
+            assert float(bb.output_proj.weight.grad.abs().max()) > 0
+            assert torch.equal(seen[0][0], opt.flat_grad[off:]), "tail complete when the hook fires"
+            assert not torch.equal(seen[0][1], opt.flat_grad[:off]), "head still in progress"
+        bb.dropout = 0.0               # no dropout decisions: the passes differ in nothing but the hook
+        grads = []
+        for hook in (lambda: None, None):
+            AG.set_tail_ready_hook(hook, 2, model=bb)
+            opt.zero_grad()
+            torch.manual_seed(5)       # same timesteps and corruption
+            (model(ids, attn)["loss"] / 2).backward()
+            (model(ids, attn)["loss"] / 2).backward()      # a second micro-batch adds to the first's gradients
+            grads.append(opt.flat_grad.clone())
+        assert float((grads[0] - grads[1]).norm() / grads[1].norm()) < 1e-4      # (atomic sums: another order each time)
+    finally:
+        AG.set_tail_ready_hook(None, model=bb)
+
+
+def test_tail_hook_waits_for_a_head_outside_the_backbone(gpu_device):
+    """Rows of ``backbone_forward_train(hidden_states="bf16")`` under a loss of the caller's own: the head's gradient does not
+    pass through the backbone's backward pass, which therefore cannot report the tail as complete."""
+    from bidiff.parallel import tail_split_offset
+    bb, model, ids, attn, t = small_model(gpu_device)
+    opt = FlatAdamW(model.parameters(), lr=1e-3)
+    off = tail_split_offset(opt, bb, 2)
+    seen = []
+    AG.set_tail_ready_hook(lambda: seen.append(opt.flat_grad[off:].clone()), 2, model=bb)
+    try:
+        for frozen in (False, True):
+            opt.zero_grad()
+            seen.clear()
+            hidden = AG.backbone_forward_train(bb, ids, t, attn, hidden_states="bf16")
+            w = bb.output_proj.weight
+            ops.linear_cross_entropy(hidden, w.detach() if frozen else w, ids, None, attn).backward()
+            torch.cuda.synchronize()
+            assert all(torch.equal(s, opt.flat_grad[off:]) for s in seen)
+    finally:
+        AG.set_tail_ready_hook(None, model=bb)
