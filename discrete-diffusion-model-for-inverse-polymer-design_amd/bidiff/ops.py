@@ -237,6 +237,9 @@ def rotary_(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, pos
     _lib.require_device(q, "rotary_")
     if all(x.numel() for x in xs):
         _rotary_launch([(x, x) for x in xs], table, positions, interleaved, inverse)
+        for x in xs:                     # a graph that saved the old values has to notice, as with torch's in-place operations
+            if not x.is_inference():
+                torch.autograd.graph.increment_version(x)
     elif q.shape[:-2].numel():
         raise ValueError("rotary_: q and k need at least one head")
     return q, k

@@ -95,3 +95,28 @@ def test_tail_hook_waits_for_a_head_outside_the_backbone(gpu_device):
             assert all(torch.equal(s, opt.flat_grad[off:]) for s in seen)
     finally:
         AG.set_tail_ready_hook(None, model=bb)
+
+
+def test_rotary_in_place_is_seen_by_autograd(gpu_device):
+    """A tensor that a living graph saved and ``rotary_`` then turned: the backward pass raises, as after any in-place operation."""
+    dev = gpu_device
+    table = ops.rotary_table(32, 8, device=dev)
+    x, y = (torch.randn(2, 8, 3, 32, device=dev) for _ in range(2))
+    w = torch.randn(32, device=dev, requires_grad=True)
+    for a, b in ((x, None), (y, x)):
+        loss = ((a * w).sum() if b is None else (b * w).sum())
+        ops.rotary_(a, b, table)
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+    loss = (x * w).sum()
+    with torch.no_grad():
+        ops.rotary_(x.detach()[:, 2:5], None, table)           # through a detached view
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+    with torch.inference_mode():
+        z = torch.randn(2, 8, 3, 32, device=dev, dtype=BF)      # no version to count
+        before = z.clone()
+        ops.rotary_(z, None, table)
+        ops.rotary_(z, None, table, inverse=True)
+        # two roundings of values that turn twice: half a step of a pair's length each
+        assert float((z.float() - before.float()).abs().max()) <= 4 * 2.0 ** -8 * float(before.abs().max())
