@@ -14,6 +14,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -61,6 +62,12 @@ def _same_device(what, first, *others):
     for t in others:
         if t is not None and t.device != dev:
             raise ValueError(f"bidiff {what}: operands on {dev} and {t.device}; all must be on one device")
+
+
+def _no_tangents(what, *operands):
+    """The kernels have no forward-mode derivative: a dual operand is refused (its tangent would be lost)."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in operands):
+        raise NotImplementedError(f"bidiff {what}: no forward-mode derivative; an operand carries a tangent")
 
 
 def _like(t):
@@ -172,6 +179,7 @@ class _Rotary(torch.autograd.Function):
 def _rotary_check(xs, table, positions):
     q = xs[0]
     _same_device("rotary", q, *xs[1:], table, positions)
+    _no_tangents("rotary", *xs, table)
     shape = q.shape
     if len(shape) not in (3, 4):
         raise ValueError(f"rotary: expected [batch, tokens, heads, head_dim] or [rows, heads, head_dim], got {tuple(shape)}")
@@ -380,6 +388,7 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     back from the device; a longer sequence's rows from there on come out NaN, in the gradients too), ``key_mask``
     [sequences, max_seqlen]. ``scale`` defaults to 1 / sqrt(D)."""
     _same_device("differential_attention", q, k, v, lam, key_mask, cu_seqlens)
+    _no_tangents("differential_attention", q, k, v, lam)
     packed = cu_seqlens is not None
     dims = 3 if packed else 4
     qs, ks, vs = q.shape, k.shape, v.shape
@@ -528,6 +537,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     zero gradients; a counted row whose target lies outside the vocabulary makes the loss NaN. Gradients come in their
     operand's dtype, that of an fp32 weight accumulated in fp32."""
     _same_device("linear_cross_entropy", hidden, weight, targets, mask_indicator, attention_mask)
+    _no_tangents("linear_cross_entropy", hidden, weight)
     for t, name in ((hidden, "hidden"), (weight, "weight")):
         if t.dtype not in _DTYPES:
             raise TypeError(f"linear_cross_entropy: {name} must be bf16 or fp32, got {t.dtype}")
