@@ -183,7 +183,9 @@ class DiscreteMaskingDiffusion(nn.Module):
             else:
                 hidden, _ = bb.run_forward(noisy_ids, timesteps, bb._keymask_bytes(attention_mask, noisy_ids))
                 head = bb.output_proj.weight
-            loss = ops.linear_cross_entropy(hidden, head, input_ids.to(torch.long), mask_indicator, attention_mask)
+            # (a mask in floating point counts as in the logits form)
+            loss = ops.linear_cross_entropy(hidden, head, input_ids.to(torch.long), mask_indicator,
+                                            None if attention_mask is None else attention_mask.to(torch.long))
 
             def logits():
                 with torch.no_grad():

@@ -533,9 +533,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
 
     hidden [..., d] (the rows behind the final norm) and weight [V, d] in bf16 or fp32 (fp32 operands are rounded to bf16
     once, as the head's product does), d a multiple of 64, any V; targets int64 [...]; ``mask_indicator`` [...] (non-zero =
-    counts) and ``attention_mask`` [...] (the row's weight) may be None. Rows that do not count are never read and get
-    zero gradients; a counted row whose target lies outside the vocabulary makes the loss NaN. Gradients come in their
-    operand's dtype, that of an fp32 weight accumulated in fp32."""
+    counts) and ``attention_mask`` [...] (the row's weight, a whole number: bool or an integer type) may be None. Rows that
+    do not count are never read and get zero gradients; a counted row whose target lies outside the vocabulary makes the
+    loss NaN. Gradients come in their operand's dtype, that of an fp32 weight accumulated in fp32."""
     _same_device("linear_cross_entropy", hidden, weight, targets, mask_indicator, attention_mask)
     _no_tangents("linear_cross_entropy", hidden, weight)
     for t, name in ((hidden, "hidden"), (weight, "weight")):
@@ -554,6 +554,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     for t, name in ((targets, "targets"), (mask_indicator, "mask_indicator"), (attention_mask, "attention_mask")):
         if t is not None and t.shape != lead:
             raise ValueError(f"linear_cross_entropy: {name} must be {list(lead)}, got {tuple(t.shape)}")
+    if attention_mask is not None and (attention_mask.is_floating_point() or attention_mask.is_complex()):
+        raise TypeError(f"linear_cross_entropy: attention_mask holds whole numbers (bool or integers), got {attention_mask.dtype}")
     _lib.require_device(hidden, "linear_cross_entropy")
     if targets.numel() == 0:                     # no row at all: a zero that stays attached to the graph
         return (hidden.reshape(-1)[:0].sum() + weight.reshape(-1)[:0].sum()).float()

@@ -120,3 +120,18 @@ def test_rotary_in_place_is_seen_by_autograd(gpu_device):
         ops.rotary_(z, None, table, inverse=True)
         # two roundings of values that turn twice: half a step of a pair's length each
         assert float((z.float() - before.float()).abs().max()) <= 4 * 2.0 ** -8 * float(before.abs().max())
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_fused_head_loss_under_a_mask_in_floating_point(gpu_device, packed):
+    """The diffusion step takes its 0 / 1 mask in any type, with the fused loss as with logits."""
+    _, model, ids, attn, t = small_model(gpu_device)
+    model.fused_head_loss, model.skip_padded_rows = True, packed
+    losses = []
+    for mask in (attn, attn.float(), attn.bool()):
+        torch.manual_seed(4)
+        losses.append(model(ids, mask, t)["loss"])
+        with torch.no_grad():
+            torch.manual_seed(4)
+            losses.append(model(ids, mask, t)["loss"])
+    assert all(torch.equal(a, b) for a, b in zip(losses, losses[2:]))

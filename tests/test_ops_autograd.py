@@ -55,3 +55,10 @@ def test_forward_mode_of_the_rotary_table_is_refused():
     with forward_ad.dual_level():
         with pytest.raises(NotImplementedError, match="forward-mode"):
             ops.rotary(z(1, 3, 2, 8), None, forward_ad.make_dual(TABLE.clone(), TABLE + 1))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, BF, torch.float64, torch.complex64])
+def test_weights_of_rows_that_are_not_whole_numbers_are_refused(dtype):
+    """``attention_mask`` holds whole numbers: 0.5 would count as 0 and 1.9 as 1."""
+    with pytest.raises(TypeError, match="attention_mask"):
+        ops.linear_cross_entropy(z(3, 64), z(7, 64), torch.zeros(3, dtype=torch.long), None, torch.ones(3, dtype=dtype))
