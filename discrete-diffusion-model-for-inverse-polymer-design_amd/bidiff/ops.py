@@ -286,9 +286,9 @@ def _attention_call(entry, sizes, q, k, v, lam, lam_strides, key_mask, cu, scale
     gst = none3 * 4
     dlam_dtype = 0
     if grads is not None:
-        dout, dq, dk, dv, dlam, dlam_dtype = grads
-        ptr = [dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dlam]
-        gst = (*_three(dout), *_three(dq), *_three(dk), *_three(dv))
+        *tensors, dlam, dlam_dtype = grads
+        ptr = [0 if t is None else t.data_ptr() for t in tensors] + [dlam]
+        gst = sum((none3 if t is None else tuple(_three(t)) for t in tensors), ())
     args = _ATTENTION.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), *_three(q), *_three(k), *_three(v), *lam_strides,
         *(none3 if out is None else _three(out)), _DTYPES[lam.dtype],
@@ -336,11 +336,12 @@ def _attention_forward(q, k, v, lam, lam_strides, key_mask, cu, longest, scale, 
 
 
 def _attention_backward(q, k, v, lam, lam_strides, key_mask, cu, longest, scale, saved, dout, dq, dk, dv, dlam):
-    """Writes dq, dk, dv (any strides the kernels take) and dlam (lam's shape and dtype, contiguous)."""
+    """Writes dq, dk, dv (any strides the kernels take) and dlam (lam's shape and dtype, contiguous). None: not asked for (dk
+    and dv together)."""
     sizes = _attention_sizes(q, k, v, cu, longest)
     _, _, Lk, H, _, D, packed, rows = sizes
     # a weight for every (row, head): its gradient is written as it comes; one that was broadcast: summed from fp32
-    whole = lam.numel() == rows * H
+    whole = dlam is not None and lam.numel() == rows * H
     need = (_attention_workspace(*sizes, True) + 15) // 16 * 16
     ws = torch.empty(need + (0 if whole else 4 * rows * H), dtype=torch.uint8, device=q.device)
     wp, lse = ws.data_ptr(), saved.data_ptr()
@@ -348,7 +349,7 @@ def _attention_backward(q, k, v, lam, lam_strides, key_mask, cu, longest, scale,
     with _on(q.device) as stream:
         _attention_call("bd_diff_attention_bwd", sizes, q, k, v, lam, lam_strides, key_mask, cu, scale, None, lse, maps, wp, need,
                         (dout, dq, dk, dv, dlam.data_ptr() if whole else wp + need, _DTYPES[lam.dtype] if whole else 1), stream)
-        if not whole:
+        if dlam is not None and not whole:
             lead = (1, rows) if packed else q.shape[:2]
             shape = (1,) * (3 - lam.dim()) + tuple(lam.shape)
             _lib.check(_lib.lib().bd_diff_attention_dlam(wp + need, dlam.data_ptr(), _DTYPES[lam.dtype], lead[0], lead[1], H,
@@ -368,10 +369,12 @@ class _DiffAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, lam, key_mask, cu, saved = ctx.saved_tensors
-        dq, dk, dv, dl = _like(q), _like(k), _like(v), _like(lam)
+        for_q, for_k, for_v, for_lam = ctx.needs_input_grad[:4]
+        dq, dl = _like(q) if for_q else None, _like(lam) if for_lam else None
+        dk, dv = (_like(k), _like(v)) if for_k or for_v else (None, None)      # (one kernel makes both)
         _attention_backward(q, k, v, lam, ctx.lam_strides, key_mask, cu, ctx.longest, ctx.scale, saved, _rows_of_16_bytes(dout),
                             dq, dk, dv, dl)
-        return dq, dk, dv, dl, None, None, None, None, None
+        return dq, dk if for_k else None, dv if for_v else None, dl, None, None, None, None, None
 
 
 def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,

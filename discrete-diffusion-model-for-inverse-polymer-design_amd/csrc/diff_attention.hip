@@ -732,7 +732,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
   if (a.cu && b == a.B) {
     if (blk == 0)
       da_unclaimed<64 * NW>(a, tid, [&](int first, int end, unsigned word) {
-        da_fill(a.dq, a.dqs, first, end, word, 2 * hk * a.share, 2 * a.share, D, tid, 64 * NW);
+        if (a.dq) da_fill(a.dq, a.dqs, first, end, word, 2 * hk * a.share, 2 * a.share, D, tid, 64 * NW);
         for (long long i = tid; i < (long long)(end - first) * a.share; i += 64 * NW)
           da_put_dlam(a, (first + i / a.share) * a.H + hk * a.share + i % a.share, word ? __uint_as_float(0x7fc00000u) : 0.f);
       });
@@ -834,7 +834,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
   float dm[QB];                                            // dP . P2 of the rows, for dlam
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) dm[qb] = 0.f;
-  auto walk_keys = [&](auto last, auto only) {             // last: dQ is summed; else delta. only: dlam's sums too
+  // last: dQ is summed; only: dlam's sums, delta is there from the maps; neither: delta (and dlam with it)
+  auto walk_keys = [&](auto last, auto only) {
     constexpr bool LAST = decltype(last)::value, ONLY = decltype(only)::value;
     unsigned mb = da_mask_byte(a, b, lane, kend);
     unsigned long long vis = __ballot(mb != 0u);
@@ -847,7 +848,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
       const unsigned long long vis_next = __ballot(mb != 0u);
       mb = da_mask_byte(a, b, kt0 + 2 * KT + lane, kend);
       if (kt0 + KT < kend) keys.run(a, other, kt0 + KT, vis_next, wave, lane);
-      if (LAST) seen += __popcll(vis);
+      if (!LAST || ONLY) seen += __popcll(vis);            // (in the first walk)
 #pragma unroll 1                                           // (unrolled, the scheduler reads ahead more than the registers hold)
       for (int h2 = 0; h2 < 2; ++h2) {                     // 32 keys
         const unsigned kn = cur + knat + 32 * RK * h2, kt = cur + ktr + 32 * RK * h2, vn = cur + vnat + 32 * RV * h2;
@@ -864,8 +865,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
               for (int r = 0; r < 4; ++r) {
                 const float p = __builtin_amdgcn_exp2f(s[qb][m][r] * scale2 - lse[qb][m]);
                 if (ONLY && m == 1) dm[qb] += p * dp[qb][r];
-                if (!LAST) dl[qb][m] += p * dp[qb][r];
-                else dsf[qb][m][4 * half + r] = (__bf16)(p * (dp[qb][r] - dl[qb][m]));
+                if (LAST) dsf[qb][m][4 * half + r] = (__bf16)(p * (dp[qb][r] - dl[qb][m]));
+                else if (!ONLY) dl[qb][m] += p * dp[qb][r];
               }
         }
         if (LAST) add_dq(kt, dsf);
@@ -920,7 +921,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
     join_delta();
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      if (KT * t >= kend) continue;
+      if (KT * t >= kend || !a.dq) continue;
 #pragma unroll
       for (int h2 = 0; h2 < 2; ++h2) {
         bf16x8 dsf[QB][2];
@@ -935,13 +936,14 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
     }
   } else {
     if (a.maps) {
-      walk_keys(std::true_type(), std::true_type());
+      if (a.dq) walk_keys(std::true_type(), std::true_type());
+      else walk_keys(std::false_type(), std::true_type());
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) join(dm[qb]);
     } else {
       walk_keys(std::false_type(), std::false_type());
       join_delta();
-      walk_keys(std::true_type(), std::false_type());
+      if (a.dq) walk_keys(std::true_type(), std::false_type());
     }
   }
   // One key alone has weight 1 whatever its score: dQ and dK are exact zeros, where 2^(s - lse) rounds beside 1
@@ -958,6 +960,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
       *(f32x2*)(a.stats + 8 * rh + 4) = (f32x2){lam, scale};
       da_put_dlam(a, rh, -dm[qb]);
     }
+    if (!a.dq) continue;                                   // q needs no gradient
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const float f = m ? -lam * scale : scale;
@@ -1367,6 +1370,7 @@ int da_backward(DaArgs& a, hipStream_t s) {
   if (keeps) da_launch_dq<D, QR, D <= 64>(a, s, grid);
   else if (small) da_launch_dq<D, QS, false>(a, s, grid);
   else da_launch_dq<D, Q, false>(a, s, grid);
+  if (!a.dk) return bd_check_launch("bd_diff_attention_bwd");
   a.n_blk = (int)blocks(a.Lk, 16 * K::B * K::NW);
   grid = da_grid(a.n_blk, groups);
   BD_REQUIRE(grid < (1ll << 31), "bd_diff_attention_bwd: too many workgroups");
@@ -1411,7 +1415,7 @@ extern "C" int bd_diff_attention_bwd(const bd_diff_attn_args* p, void* stream) {
   const int rc = da_check(*p, "bd_diff_attention_bwd", a);
   if (rc != BD_OK) return rc;
   BD_REQUIRE(p->dlam_dtype == BD_DTYPE_BF16 || p->dlam_dtype == BD_DTYPE_F32, "bd_diff_attention_bwd: dlam is neither bf16 nor fp32");
-  BD_REQUIRE(p->dout && p->dq && p->dk && p->dv && p->dlam && p->lse, "bd_diff_attention_bwd: null operand");
+  BD_REQUIRE(p->dout && p->dlam && p->lse && !p->dk == !p->dv, "bd_diff_attention_bwd: null operand (dq may be, dk and dv together)");
   const void* aligned[] = {p->dout, p->dq, p->dk, p->dv, p->maps};
   for (const void* x : aligned) BD_REQUIRE(((uintptr_t)x & 15) == 0, "bd_diff_attention_bwd: operands must be 16-byte aligned");
   for (int i = 0; i < 3; ++i)

@@ -797,7 +797,8 @@ int bd_rotary(const bd_rotary_tensor* tensors, int n_tensors, const float* table
  * Training: lse [rows, H, 2] fp32 (base-2 log-sum-exp of the scaled scores; rows counted through the batch) and, beyond
  * short sequences, maps [rows, H, 2, 2 head_dim] fp32 (each map's own output) are written by the forward and read by
  * the backward (maps may be null in both: the backward then walks the keys once more). Backward: dq, dk, dv bf16 and
- * dlam [rows, H] (bf16 or fp32) are overwritten. Workspaces of bd_diff_attention_workspace_bytes(args, backward) bytes; equal
+ * dlam [rows, H] (bf16 or fp32) are overwritten; dq may be null, and dk and dv together: what only they need is not run.
+ * Workspaces of bd_diff_attention_workspace_bytes(args, backward) bytes; equal
  * calls give equal bits. Stands beside bd_attention_fwd / bd_attention_bwd. */
 typedef struct {
   const void *q, *k, *v, *lam;

@@ -135,3 +135,47 @@ def test_fused_head_loss_under_a_mask_in_floating_point(gpu_device, packed):
             torch.manual_seed(4)
             losses.append(model(ids, mask, t)["loss"])
     assert all(torch.equal(a, b) for a, b in zip(losses, losses[2:]))
+
+
+FORMS = {"kept maps": (2, 70, 300, 4, 2, 32, False), "keys walked twice": (2, 70, 150, 4, 2, 64, False), "two key tiles": (3, 40, 100, 2, 2, 64, False),
+         "wide heads": (1, 33, 90, 2, 1, 128, False), "packed": (3, 60, 60, 4, 2, 32, True)}
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_frozen_operands_of_differential_attention(gpu_device, monkeypatch, form):
+    """Any subset of q, k, v and lam may need a gradient. Theirs have the bits of the full backward; for the others nothing is
+    computed into memory: no dq where q is frozen, no launch for the keys' side where k and v are."""
+    dev = gpu_device
+    B, Lq, Lk, H, Hkv, D, packed = FORMS[form]
+    g = torch.Generator(device=dev).manual_seed(21)
+    lead_q, lead_k = ((B * Lq,), (B * Lk,)) if packed else ((B, Lq), (B, Lk))
+    base = {n: torch.randn(*s, generator=g, device=dev).to(BF) for n, s in
+            (("q", (*lead_q, 2 * H, D)), ("k", (*lead_k, 2 * Hkv, D)), ("v", (*lead_k, Hkv, 2 * D)))}
+    base["lam"] = torch.rand(H, generator=g, device=dev)
+    dout = torch.randn(*lead_q, H, 2 * D, generator=g, device=dev).to(BF)
+    # (packed: rows before the first and behind the last sequence, too)
+    kw = dict(cu_seqlens=torch.tensor([2, 60, 61, B * Lq - 3], dtype=torch.int32, device=dev), max_seqlen=115) if packed else {}
+    written = []
+    call = ops._attention_call
+
+    def spy(entry, *args, **kwargs):
+        if kwargs.get("grads") or entry == "bd_diff_attention_bwd":
+            grads = kwargs.get("grads") or next(a for a in args if isinstance(a, tuple) and len(a) == 6)
+            written.append(tuple(t is not None for t in grads[1:4]))
+        return call(entry, *args, **kwargs)
+    monkeypatch.setattr(ops, "_attention_call", spy)
+
+    def run(names):
+        x = {n: t.clone().requires_grad_(n in names) for n, t in base.items()}
+        out = ops.differential_attention(*x.values(), **kw)
+        return dict(zip(names, torch.autograd.grad(out, [x[n] for n in names], dout)))
+
+    def same(a, b):                # (one packed sequence is longer than announced: NaN there)
+        return torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+    full = run(("q", "k", "v", "lam"))
+    assert written.pop() == (True, True, True)
+    for names in (("q",), ("k",), ("v",), ("lam",), ("q", "lam"), ("k", "v"), ("q", "v"), ("k", "lam")):
+        got = run(names)
+        assert all(same(got[n], full[n]) for n in names), names
+        keys = "k" in names or "v" in names
+        assert written.pop() == ("q" in names, keys, keys), names
