@@ -467,9 +467,10 @@ def _to_bf16(x, stream):
 
 @functools.lru_cache(maxsize=256)
 def _head_sizes(M, d, V):
-    """Bytes of the state and of the workspaces: forward, backward, forward without state."""
+    """Bytes of the state and of the workspaces: forward, backward, forward without state, backward for the head's gradient
+    alone, for the rows' alone."""
     L_ = _lib.lib()
-    sizes = (L_.bd_linear_ce_state_bytes(M, d), *(L_.bd_linear_ce_workspace_bytes(M, d, V, kind) for kind in range(3)))
+    sizes = (L_.bd_linear_ce_state_bytes(M, d), *(L_.bd_linear_ce_workspace_bytes(M, d, V, kind) for kind in range(5)))
     if min(sizes) < 0:
         _lib.check(-1, "bd_linear_ce_workspace_bytes")
     return sizes
@@ -480,8 +481,8 @@ def _head_loss(hidden, weight, targets, indicator, attention_mask, training):
     dev = hidden.device
     V, d = weight.shape
     M = targets.numel()
-    state_bytes, with_state, _, alone = _head_sizes(M, d, V)
-    ws_bytes = with_state if training else alone
+    sizes = _head_sizes(M, d, V)
+    state_bytes, ws_bytes = sizes[0], sizes[1 if training else 3]
     with _on(dev) as stream:
         h, w = _to_bf16(hidden, stream), _to_bf16(weight, stream)
         loss = torch.empty((), dtype=torch.float32, device=dev)
@@ -511,10 +512,12 @@ class _LinearCE(torch.autograd.Function):
         V, d = w.shape
         M = shape[:-1].numel()
         dev = w.device
-        state_bytes, _, ws_bytes, _ = _head_sizes(M, d, V)
-        dh = torch.empty(shape, dtype=torch.bfloat16, device=dev) if ctx.needs_input_grad[0] else None
+        sizes = _head_sizes(M, d, V)
+        for_rows, for_head = ctx.needs_input_grad[:2]
+        state_bytes, ws_bytes = sizes[0], sizes[2 if for_rows and for_head else 5 if for_rows else 4]
+        dh = torch.empty(shape, dtype=torch.bfloat16, device=dev) if for_rows else None
         dw = None
-        if ctx.needs_input_grad[1]:      # fp32 gradients are accumulated into, bf16 ones written
+        if for_head:                     # fp32 gradients are accumulated into, bf16 ones written
             dw = (torch.zeros if weight_dtype == torch.float32 else torch.empty)(V, d, dtype=weight_dtype, device=dev)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         if gout.dtype != torch.float32:

@@ -672,10 +672,13 @@ struct VlPlan {
   int big_s, big_z, big_h, big_w;     // 256 x 256 tiles for the scores, dz, dh, dW (else 128 x 128)
   int split_h, split_w;               // splits of dh's product over the piece (at most), of dW's over the rows
   long long slab_h, slab_w;           // floats of one slab
-  long long fwd_bytes, bwd_bytes;
+  bool dh_alone;                      // one piece, one split: the product writes every row of dh, no slab to add up
+  long long fwd_bytes;
 };
 
-constexpr long long VL_PIECE_BYTES = 256ll << 20;      // dz of one piece: what stays near the card's last-level cache
+// dz of one piece: what stays near the card's last-level cache (a piece has 256 columns at least: from 2^19 rows on it is
+// 512 bytes a row)
+constexpr long long VL_PIECE_BYTES = 256ll << 20;
 
 VlPlan vl_plan(long long M, int d, int V) {
   VlPlan p;
@@ -705,16 +708,24 @@ VlPlan vl_plan(long long M, int d, int V) {
   if (piece > v_pad) piece = v_pad;
   p.n_pieces = (int)((v_pad + piece - 1) / piece);
   p.piece = (int)vl_up((v_pad + p.n_pieces - 1) / p.n_pieces, 256);
-  // (a quarter of the rows may carry weight: then dh has so many fewer tiles. At most 512 MB of slabs.)
+  // (a quarter of the rows may carry weight: then dh has so many fewer tiles. At most 512 MB of slabs, or a single one.)
   p.slab_h = p.m_pad * d;
   p.split_h = vl_splits((vl_up(M, bh) / bh + 3) / 4 * (vl_up(d, bh) / bh), p.piece / 64, 64);
   while (p.split_h > 1 && p.split_h * p.slab_h * 4 > (512ll << 20)) --p.split_h;
+  p.dh_alone = p.n_pieces == 1 && p.split_h == 1;
+  // (fewer than 256 tiles times splits of a tile: at most 64 MB of slabs)
   p.split_w = vl_splits(vl_up(p.piece, bw) / bw * (vl_up(d, bw) / bw), p.m_pad / 64, 64);
   p.slab_w = (long long)p.piece * d;
   const long long groups = (M + SCAN - 1) / SCAN;
   p.fwd_bytes = vl_up(groups * 4, 256) * 2 + vl_up(p.m_pad * 4, 256) + (v_pad / 128) * p.m_pad * 8;
-  p.bwd_bytes = p.m_pad * p.piece * 2 + (p.split_h * p.slab_h + (p.split_w > 1 ? p.split_w * p.slab_w : 0)) * 4;
   return p;
+}
+
+// floats of all slabs of dh, of dW
+long long vl_dh_slabs(const VlPlan& p) { return p.dh_alone ? 0 : p.split_h * p.slab_h; }
+long long vl_dw_slabs(const VlPlan& p) { return p.split_w > 1 ? p.split_w * p.slab_w : 0; }
+long long vl_bwd_bytes(const VlPlan& p, bool dh, bool dw) {
+  return p.m_pad * p.piece * 2 + ((dh ? vl_dh_slabs(p) : 0) + (dw ? vl_dw_slabs(p) : 0)) * 4;
 }
 
 template <int BT, bool AKC, bool BKC, int EPI>
@@ -745,7 +756,8 @@ extern "C" long long bd_linear_ce_workspace_bytes(long long M, int d, int V, int
   if (M <= 0 || d <= 0 || V <= 0) return -1;
   if (kind == 2 && V <= VL_NARROW) return vl_up(vl_up(M, VL_NROWS) / VL_NROWS * 8, 256);
   const VlPlan p = vl_plan(M, d, V);
-  return kind == 1 ? p.bwd_bytes : p.fwd_bytes + (kind == 2 ? bd_linear_ce_state_bytes(M, d) : 0);
+  if (kind == 1 || kind == 3 || kind == 4) return vl_bwd_bytes(p, kind != 3, kind != 4);
+  return p.fwd_bytes + (kind == 2 ? bd_linear_ce_state_bytes(M, d) : 0);
 }
 
 extern "C" int bd_linear_ce_fwd(const void* hidden, const void* weight, const long long* targets, const unsigned char* indicator,
@@ -805,13 +817,13 @@ extern "C" int bd_linear_ce_bwd(const void* weight, const float* grad_out, void*
   BD_REQUIRE(dweight_dtype == BD_DTYPE_BF16 || dweight_dtype == BD_DTYPE_F32, "bd_linear_ce_bwd: dweight is neither bf16 nor fp32");
   const VlPlan pl = vl_plan(M, d, V);
   BD_REQUIRE(state_bytes >= bd_linear_ce_state_bytes(M, d), "bd_linear_ce_bwd: the state must hold %lld bytes", bd_linear_ce_state_bytes(M, d));
-  BD_REQUIRE(workspace_bytes >= pl.bwd_bytes, "bd_linear_ce_bwd: the workspace must hold %lld bytes", pl.bwd_bytes);
+  const long long need = vl_bwd_bytes(pl, dhidden != nullptr, dweight != nullptr);
+  BD_REQUIRE(workspace_bytes >= need, "bd_linear_ce_bwd: the workspace must hold %lld bytes", need);
   hipStream_t s = (hipStream_t)stream;
   const VlState st = vl_state((void*)state, M, d);
   unsigned short* dlog = (unsigned short*)workspace;
   float* slab_h = (float*)((char*)workspace + pl.m_pad * pl.piece * 2);
-  float* slab_w = slab_h + pl.split_h * pl.slab_h;
-  const bool dh_alone = pl.n_pieces == 1 && pl.split_h == 1;       // the product writes every row of dh, no slab to add up
+  float* slab_w = slab_h + (dhidden ? vl_dh_slabs(pl) : 0);
   bd_prof_scope prof(stream, 6.0 * M * (double)V * d, BD_PROF_GEMM);
   for (int i = 0; i < pl.n_pieces; ++i) {
     const int v0 = i * pl.piece, n = min(pl.piece, (int)vl_up(V - v0, 64));       // columns of the piece, whole 64s
@@ -826,7 +838,7 @@ extern "C" int bd_linear_ce_bwd(const void* weight, const float* grad_out, void*
       p.A = dlog; p.lda = pl.piece; p.B = wp; p.ldb = d; p.head = st.head; p.M = (int)pl.m_pad; p.N = d; p.K = min(n, V - v0); p.m_live = 1;
       p.n_split = pl.split_h; p.dh_split = 1; p.slab = slab_h; p.slab_stride = pl.slab_h; p.ldo = d; p.add = i > 0;
       if (pl.n_pieces == 1) { p.dh = (unsigned short*)dhidden; p.idx = st.idx; p.gout = grad_out; }
-      if (dh_alone) { p.pos = st.pos; p.rows_all = (int)M; }
+      if (pl.dh_alone) { p.pos = st.pos; p.rows_all = (int)M; }
       vl_launch<true, false, VL_SLAB>(pl.big_h, p, s);
     }
     if (dweight) {
@@ -846,7 +858,7 @@ extern "C" int bd_linear_ce_bwd(const void* weight, const float* grad_out, void*
       }
     }
   }
-  if (dhidden && !dh_alone)
+  if (dhidden && !pl.dh_alone)
     hipLaunchKernelGGL(vl_dh_kernel, dim3((unsigned)((M * (d / 8) + 255) / 256)), dim3(256), 0, s, st, slab_h, pl.slab_h, pl.split_h,
                        pl.big_h ? 256 : 128, min(pl.piece, V), pl.n_pieces, grad_out, (unsigned short*)dhidden, (int)M, d);
   return bd_check_launch("bd_linear_ce_bwd");

@@ -833,7 +833,10 @@ int bd_diff_attention_dlam(const float* dlam, void* out, int out_dtype, int B, i
  * never read; a weighted row whose target lies outside [0, V) makes the loss NaN. The forward leaves what the backward
  * needs (the weighted rows, their targets, weights and log-sum-exps) in state (bd_linear_ce_state_bytes(M, d) bytes);
  * a null state means that no backward follows. Workspaces are scratch of bd_linear_ce_workspace_bytes(M, d, V, kind)
- * bytes, kind 0: forward, 1: backward, 2: forward without state. Backward, times grad_out[0]:
+ * bytes, kind 0: forward, 1: backward, 2: forward without state, 3: backward without dhidden, 4: backward without dweight.
+ * The backward's hold the bf16 gradients of a piece of the scores (256 MB, or 256 columns where those are more, from 2^19
+ * rows on), dhidden's fp32 sums where pieces or splits have to be added (512 MB, or one [M, d]) and 64 MB for dweight's.
+ * Backward, times grad_out[0]:
  * dhidden [M, d] bf16 (overwritten; zeros at rows without weight) and dweight [V, d], bf16 overwritten or fp32 ADDED to
  * (as the weight-gradient products of this library do); either may be null. Equal calls give equal bits.
  * Stands beside bd_masked_ce_fwd / bd_masked_ce_bwd, which read the logits from memory. */

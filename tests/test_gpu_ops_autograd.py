@@ -179,3 +179,20 @@ def test_frozen_operands_of_differential_attention(gpu_device, monkeypatch, form
         assert all(same(got[n], full[n]) for n in names), names
         keys = "k" in names or "v" in names
         assert written.pop() == ("q" in names, keys, keys), names
+
+
+@pytest.mark.parametrize("M,d,V", [(33000, 64, 39), (20000, 256, 803), (700, 128, 300), (3000, 64, 65000)])
+@pytest.mark.parametrize("wdt", [BF, torch.float32])
+def test_either_gradient_of_the_head_loss_alone(gpu_device, M, d, V, wdt):
+    """The rows' gradient alone and the head's alone, each in the scratch it asks for (with and without slabs, in one piece of
+    the vocabulary and in two), have the bits that they have together."""
+    dev = gpu_device
+    g = torch.Generator(device=dev).manual_seed(31)
+    h, w = torch.randn(M, d, generator=g, device=dev).to(BF), (torch.randn(V, d, generator=g, device=dev) / d ** 0.5).to(wdt)
+    t, ind = torch.randint(0, V, (M,), generator=g, device=dev), torch.rand(M, generator=g, device=dev) < 0.6
+
+    def run(*need):
+        leaves = [x.clone().requires_grad_(n) for x, n in zip((h, w), need)]
+        return torch.autograd.grad(ops.linear_cross_entropy(*leaves, t, ind), [x for x in leaves if x.requires_grad])
+    dh, dw = run(True, True)
+    assert torch.equal(run(True, False)[0], dh) and torch.equal(run(False, True)[0], dw)

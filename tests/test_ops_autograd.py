@@ -62,3 +62,22 @@ def test_weights_of_rows_that_are_not_whole_numbers_are_refused(dtype):
     """``attention_mask`` holds whole numbers: 0.5 would count as 0 and 1.9 as 1."""
     with pytest.raises(TypeError, match="attention_mask"):
         ops.linear_cross_entropy(z(3, 64), z(7, 64), torch.zeros(3, dtype=torch.long), None, torch.ones(3, dtype=dtype))
+
+
+def up(x, m):
+    return (x + m - 1) // m * m
+
+
+@pytest.mark.parametrize("M,d,V", [(32768, 384, 803), (131072, 4096, 1000), (131072, 4096, 256), (8192, 384, 803), (1 << 20, 384, 5000)])
+def test_scratch_of_the_head_loss(M, d, V):
+    """The backward asks for the score gradients of a piece (256 MB, or 256 columns where the rows are more than that), the slabs
+    of dh where sums over pieces or splits need them (512 MB, or one fp32 [M, d]) and at most 64 MB of slabs of dW; none of
+    the former where the product writes dh itself, or where dh is not asked for."""
+    size = ops._lib.lib().bd_linear_ce_workspace_bytes
+    rows = up(M, 256)
+    scores, dh, dw = max(256 << 20, 512 * rows), max(512 << 20, 4 * rows * d), 64 << 20
+    both, only_dw, only_dh = size(M, d, V, 1), size(M, d, V, 3), size(M, d, V, 4)
+    assert 0 < only_dw <= scores + dw and 0 < only_dh <= scores + dh and max(only_dw, only_dh) <= both <= scores + dh + dw
+    one_piece = 2 * rows * up(V, 256) <= 256 << 20
+    if one_piece and (-(-rows // 128) + 3) // 4 * -(-d // 128) > 128:      # (a quarter of the rows keeps half of the CUs busy: no splits)
+        assert only_dh <= scores and both <= scores + dw
