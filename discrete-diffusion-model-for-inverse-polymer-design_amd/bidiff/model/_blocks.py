@@ -127,9 +127,9 @@ def split_qkv(qkv, n_maps, dh, differential):
 
 def turn_positions(mha, qkv, positions, dh_padded, n_positions, inverse=False):
     """Rotary positions on the q and k parts of ``qkv`` [B, L, 3 * width] (or packed rows), in place. The head's own
-    values turn (a padded head's zeros behind them stay). The tables are kept on the module, shorter ones too: a
-    captured graph may still read one that a longer call replaced."""
-    tables = mha.__dict__.setdefault("_rotary_tables", [])
+    values turn (a padded head's zeros behind them stay). The tables are kept on the module by the base that they were made
+    with, shorter ones too: a captured graph may still read one that a longer call replaced."""
+    tables = mha.__dict__.setdefault("_rotary_tables", {}).setdefault(mha.rotary_base, [])
     table = next((x for x in tables if x.device == qkv.device and x.shape[0] >= n_positions), None)
     if table is None:
         table = ops.rotary_table(mha.head_dim, n_positions, base=mha.rotary_base, device=qkv.device)

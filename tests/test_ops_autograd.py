@@ -81,3 +81,23 @@ def test_scratch_of_the_head_loss(M, d, V):
     one_piece = 2 * rows * up(V, 256) <= 256 << 20
     if one_piece and (-(-rows // 128) + 3) // 4 * -(-d // 128) > 128:      # (a quarter of the rows keeps half of the CUs busy: no splits)
         assert only_dh <= scores and both <= scores + dw
+
+
+def turned_with(monkeypatch, mha, lengths):
+    """The tables that calls of these lengths turn with, and all that the module keeps."""
+    from bidiff.model import _blocks
+    handed = []
+    monkeypatch.setattr(_blocks.ops, "_rotary_launch", lambda pairs, table, *a: handed.append(table))
+    for n in lengths:
+        _blocks.turn_positions(mha, torch.zeros(1, n, 3 * mha.hidden_size, dtype=BF), None, mha.head_dim, n)
+    return handed, [t for tables in mha.__dict__["_rotary_tables"].values() for t in tables]
+
+
+def test_rotary_tables_follow_the_base(monkeypatch):
+    """A module whose base was changed (a longer context) turns by the new one, and by the old one again when it is put back."""
+    from bidiff.model.backbone import MultiHeadAttention
+    mha = MultiHeadAttention(64, 2, 0.0, rotary_base=10000.0)
+    for base in (10000.0, 500000.0, 10000.0):
+        mha.rotary_base = base
+        (table, again), _ = turned_with(monkeypatch, mha, (9, 5))
+        assert torch.equal(table[:9], ops.rotary_table(32, 9, base=base)) and again is table
