@@ -128,11 +128,13 @@ def split_qkv(qkv, n_maps, dh, differential):
 def turn_positions(mha, qkv, positions, dh_padded, n_positions, inverse=False):
     """Rotary positions on the q and k parts of ``qkv`` [B, L, 3 * width] (or packed rows), in place. The head's own
     values turn (a padded head's zeros behind them stay). The tables are kept on the module by the base that they were made
-    with, shorter ones too: a captured graph may still read one that a longer call replaced."""
+    with, shorter ones too: a captured graph may still read one that a longer call replaced. Each holds twice the positions
+    of the one before or more, so that a call that grows token by token makes few of them."""
     tables = mha.__dict__.setdefault("_rotary_tables", {}).setdefault(mha.rotary_base, [])
     table = next((x for x in tables if x.device == qkv.device and x.shape[0] >= n_positions), None)
     if table is None:
-        table = ops.rotary_table(mha.head_dim, n_positions, base=mha.rotary_base, device=qkv.device)
+        longest = max((x.shape[0] for x in tables if x.device == qkv.device), default=0)
+        table = ops.rotary_table(mha.head_dim, max(n_positions, 2 * longest), base=mha.rotary_base, device=qkv.device)
         tables.append(table)
     q, k, _ = split_qkv(qkv, mha.num_heads, dh_padded, False)
     ops._rotary_launch([(q, q), (k, k)], table, positions, False, inverse)

@@ -101,3 +101,14 @@ def test_rotary_tables_follow_the_base(monkeypatch):
         mha.rotary_base = base
         (table, again), _ = turned_with(monkeypatch, mha, (9, 5))
         assert torch.equal(table[:9], ops.rotary_table(32, 9, base=base)) and again is table
+
+
+def test_rotary_tables_of_growing_lengths(monkeypatch):
+    """A module that is called with one more token each time keeps a handful of tables, and those it has handed out stay."""
+    from bidiff.model.backbone import MultiHeadAttention
+    mha = MultiHeadAttention(64, 2, 0.0, rotary_base=10000.0)
+    handed, kept = turned_with(monkeypatch, mha, range(1, 1500))
+    assert all(t.shape[0] >= n for n, t in enumerate(handed, 1))
+    assert all(any(t is x for x in kept) for t in handed)          # a captured graph may still read any of them
+    assert sum(t.shape[0] for t in kept) <= 4 * 1500 and len(kept) <= 12
+    assert torch.equal(handed[-1][:1499], ops.rotary_table(32, 1499))
