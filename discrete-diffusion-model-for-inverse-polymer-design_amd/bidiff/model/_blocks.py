@@ -130,7 +130,7 @@ def turn_positions(mha, qkv, positions, dh_padded, n_positions, inverse=False):
     values turn (a padded head's zeros behind them stay). The tables are kept on the module by the base that they were made
     with, shorter ones too: a captured graph may still read one that a longer call replaced. Each holds twice the positions
     of the one before or more, so that a call that grows token by token makes few of them."""
-    tables = mha.__dict__.setdefault("_rotary_tables", {}).setdefault(mha.rotary_base, [])
+    tables = mha.__dict__.setdefault("_rotary_by_base", {}).setdefault(mha.rotary_base, [])
     table = next((x for x in tables if x.device == qkv.device and x.shape[0] >= n_positions), None)
     if table is None:
         longest = max((x.shape[0] for x in tables if x.device == qkv.device), default=0)

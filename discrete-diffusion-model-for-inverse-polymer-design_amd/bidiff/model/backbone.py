@@ -26,6 +26,7 @@ class MultiHeadAttention(nn.Module):
     times ``lambda_weight`` (one learned weight a pair), over both heads' values side by side. ``rotary_base``: queries and
     keys are turned by their positions (``bidiff.ops.rotary``, half layout) before they meet. Both off by default: the
     reference's attention."""
+    differential, rotary_base = False, None        # (of a module that was pickled whole before it had them)
 
     def __init__(self, hidden_size: int, num_heads: int, dropout: float = 0.1, differential: bool = False,
                  rotary_base: Optional[float] = None, depth: int = 0):
@@ -126,6 +127,7 @@ class DiffusionBackbone(nn.Module):
     attention maps are then not dropped in training, the other three dropout sites are), ``rotary_base`` turns queries and
     keys by their positions beside the learned position table. Such models train and sample through the per-layer kernels
     in bf16 (no single-launch, chosen-row, ragged or fp32 forward)."""
+    attention, rotary_base = "softmax", None       # (of a model that was pickled whole before it had them)
 
     def __init__(
         self,

@@ -73,6 +73,8 @@ class _Outputs(dict):
 
 
 class DiscreteMaskingDiffusion(nn.Module):
+    fused_head_loss = False        # (of a module that was pickled whole before it had it)
+
     def __init__(
         self,
         backbone: nn.Module,

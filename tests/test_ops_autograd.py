@@ -90,7 +90,7 @@ def turned_with(monkeypatch, mha, lengths):
     monkeypatch.setattr(_blocks.ops, "_rotary_launch", lambda pairs, table, *a: handed.append(table))
     for n in lengths:
         _blocks.turn_positions(mha, torch.zeros(1, n, 3 * mha.hidden_size, dtype=BF), None, mha.head_dim, n)
-    return handed, [t for tables in mha.__dict__["_rotary_tables"].values() for t in tables]
+    return handed, [t for tables in mha.__dict__["_rotary_by_base"].values() for t in tables]
 
 
 def test_rotary_tables_follow_the_base(monkeypatch):
@@ -112,3 +112,19 @@ def test_rotary_tables_of_growing_lengths(monkeypatch):
     assert all(any(t is x for x in kept) for t in handed)          # a captured graph may still read any of them
     assert sum(t.shape[0] for t in kept) <= 4 * 1500 and len(kept) <= 12
     assert torch.equal(handed[-1][:1499], ops.rotary_table(32, 1499))
+
+
+def test_models_pickled_before_the_options_existed():
+    """A module that was saved whole without the newer attributes (attention, rotary_base, fused_head_loss) works as what it was."""
+    from bidiff.model.backbone import DiffusionBackbone
+    from bidiff.model.diffusion import DiscreteMaskingDiffusion
+    bb = DiffusionBackbone(39, hidden_size=128, num_layers=1, num_heads=2, ffn_hidden_size=256, max_position_embeddings=16, num_diffusion_steps=5)
+    model = DiscreteMaskingDiffusion(bb, num_steps=5, mask_token_id=1, pad_token_id=0, bos_token_id=2, eos_token_id=3)
+    want = bb.config_dict()
+    for m in (bb, *(b.attn for b in bb.layers)):
+        for name in ("attention", "rotary_base", "differential"):
+            m.__dict__.pop(name, None)
+    model.__dict__.pop("fused_head_loss", None)
+    assert bb.plain_attention and not model.fused_head_loss
+    assert bb.layers[0].attn.rotary_base is None and not bb.layers[0].attn.differential
+    assert bb.config_dict() == want
