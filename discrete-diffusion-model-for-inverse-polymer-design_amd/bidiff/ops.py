@@ -5,7 +5,8 @@
 ``MultiHeadAttention``), and ``linear_cross_entropy`` is the masked cross entropy of the vocabulary head without its
 logits (beside ``training.autograd.masked_cross_entropy``). All run on the current stream of their operands' device, take
 their scratch memory from torch's allocator, repeat bit for bit, and may be captured into a HIP graph (packed rows:
-with ``max_seqlen`` given). Operands on a CPU raise ``RuntimeError``: there is no other execution path.
+with ``max_seqlen`` given). Operands on a CPU raise ``RuntimeError`` (there is no other execution path), operands with a
+forward-mode tangent ``NotImplementedError``.
 """
 import ctypes as C
 import functools
@@ -80,7 +81,8 @@ def _keeps_maps(Lk, D):
     (16 * head_dim bytes a row and head); up to there the backward walks the keys once more instead. Measured, all kernels of
     a step, maps kept / keys walked twice: 3 heads of 64, 256 x 128 tokens 140 / 122 us, 64 x 512 211 / 203, 42 x 768 262 / 272,
     16 x 2048 440 / 479; heads of 128, 32 x 512 263 / 243, 16 x 1024 447 / 458, 8 x 2048 736 / 813; heads of 32, 256 x 128
-    73 / 69, 128 x 256 92 / 90, 96 packed sequences of up to 509 267 / 282."""
+    73 / 69, 128 x 256 92 / 90, 96 packed sequences of up to 509 267 / 282. (At heads of 128 and 1024 keys, on the border, the
+    rule is 2 % on the wrong side.)"""
     return Lk > 8 * D
 
 
@@ -99,9 +101,11 @@ def rotary_table(dim: int, max_positions: int, base: float = 10000.0, scaling: O
     """Table of (cos, sin) for ``rotary``: fp32 [max_positions, dim / 2, 2], from angles evaluated in 64 bits.
 
     ``scaling`` stretches the positions for contexts longer than those trained on by ``factor``: None; ``"linear"``
-    (positions divided by it); ``"ntk"`` (the base raised so that the slowest pair is stretched by the factor and the
-    fastest not at all); ``"yarn"`` (pairs that turn at least ``beta_fast`` times within ``original_positions`` are kept,
-    those below ``beta_slow`` turns are stretched, a linear ramp over the pair's index between; cos and sin times 0.1 ln(factor) + 1)."""
+    (positions divided by it; Chen et al. 2023, "Extending Context Window of Large Language Models via Positional
+    Interpolation"); ``"ntk"`` (the base raised so that the slowest pair is stretched by the factor and the fastest not at
+    all); ``"yarn"`` (Peng et al. 2023, "YaRN: Efficient Context Window Extension of Large Language Models": pairs that turn at
+    least ``beta_fast`` times within ``original_positions`` are kept, those below ``beta_slow`` turns are stretched, a linear
+    ramp over the pair's index between; cos and sin times 0.1 ln(factor) + 1)."""
     if dim <= 0 or dim % 2:
         raise ValueError(f"rotary_table: dim must be positive and even, got {dim}")
     if max_positions <= 0 or not base > 0.0 or not factor > 0.0:
@@ -229,8 +233,9 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, posi
 
 def rotary_(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, positions: Optional[torch.Tensor] = None,
             interleaved: bool = False, inverse: bool = False):
-    """``rotary`` in place, for inference and for kernels' own buffers (no gradient is recorded; q and k must not share values).
-    ``inverse`` turns back."""
+    """``rotary`` in place, for inference and for kernels' own buffers (no gradient is recorded; q and k must not share values;
+    a graph that saved the old values raises in its backward pass, as after torch's in-place operations). ``inverse`` turns
+    back."""
     xs = [q] if k is None else [q, k]
     positions = _rotary_check(xs, table, positions)
     if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
@@ -389,7 +394,8 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     without the batch axis, ``cu_seqlens`` int [sequences + 1] (rows cu[b] .. cu[b + 1] - 1 belong to sequence b; offsets
     that do not fall; rows before the first and behind the last sequence come out zero), ``max_seqlen`` the longest (None: read
     back from the device; a longer sequence's rows from there on come out NaN, in the gradients too), ``key_mask``
-    [sequences, max_seqlen]. ``scale`` defaults to 1 / sqrt(D)."""
+    [sequences, max_seqlen]. ``scale`` defaults to 1 / sqrt(D). The backward pass leaves out what no operand needs: dq where q
+    is frozen, the keys' side where k and v are."""
     _same_device("differential_attention", q, k, v, lam, key_mask, cu_seqlens)
     _no_tangents("differential_attention", q, k, v, lam)
     packed = cu_seqlens is not None

@@ -2,13 +2,14 @@
 #pragma once
 #include <hip/hip_runtime.h>
 // kernel families the profiler keeps separate totals for (bd_prof_read_kind)
-enum { BD_PROF_GEMM = 0, BD_PROF_PANEL = 1, BD_PROF_FFN = 2, BD_PROF_ATTN_BLOCK = 3, BD_PROF_MEGA = 4,
+enum { BD_PROF_GEMM = 0,       // tiled GEMMs, and all launches of the vocabulary head's loss without logits (flops)
+       BD_PROF_PANEL = 1, BD_PROF_FFN = 2, BD_PROF_ATTN_BLOCK = 3, BD_PROF_MEGA = 4,
        BD_PROF_WGRAD = 5,      // weight-gradient GEMMs (flops)
-       BD_PROF_ATTN_FWD = 6,   // stand-alone attention forward (flops)
-       BD_PROF_ATTN_BWD = 7,   // attention backward, both kernels (flops)
+       BD_PROF_ATTN_FWD = 6,   // stand-alone attention forward, softmax or differential (flops)
+       BD_PROF_ATTN_BWD = 7,   // attention backward, both kernels, softmax or differential (flops)
        BD_PROF_LN = 8,         // LayerNorm forward / backward (bytes)
        BD_PROF_CE = 9,         // masked cross-entropy forward / backward (bytes)
-       BD_PROF_EMBED = 10,     // embedding sum / scatter, corruption, dropout, casts (bytes)
+       BD_PROF_EMBED = 10,     // embedding sum / scatter, rotary positions, corruption, dropout, casts (bytes)
        BD_PROF_OPT = 11,       // gradient norm, AdamW, Muon, weight-copy refresh (bytes)
        BD_PROF_SAMPLE = 12,    // reverse step and post-loop repairs (bytes)
        BD_PROF_KINDS = 13 };

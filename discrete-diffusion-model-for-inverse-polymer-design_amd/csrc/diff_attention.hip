@@ -361,8 +361,9 @@ __device__ __forceinline__ void da_unclaimed(const DaArgs& a, int tid, Fill fill
 // Forward. Waves work in pairs: wave 2 w + m holds map m of the 16 QB slots of query group w (NQG groups in a
 // workgroup). Split over keys (n_split > 1): each split leaves its unnormalised sums, maximum and normaliser.
 // Head size 128 (2 x 4096 tokens, 8 heads over 4: 391 us, 1.05 PFLOP/s): matrix cores busy 52 % of the cycles, vector units
-// 44 %: the exponentials of one wave of a SIMD run under the products of the other. Head sizes 32 and 64: bound by the
-// vector units (66 % and 56 % busy): about 4 instructions a score in the loop, the rest around it (many short sequences).
+// 44 %: the exponentials of one wave of a SIMD run under the products of the other. Head sizes 32 and 64: vector units 66 %
+// and 56 % busy, matrix cores 19 % and 11 %, so neither is full: about 4 vector instructions a score in the loop and those
+// around it (many short sequences), each waiting for the one before with four waves a SIMD to hide it.
 // =====================================================================================
 template <int D, int QB, int NQG, int OCC, bool TWO>
 __global__ __launch_bounds__(128 * NQG, OCC) void da_fwd_kernel(DaArgs a) {
@@ -716,7 +717,9 @@ __global__ __launch_bounds__(256) void da_join_few_kernel(DaArgs a) {
 // |dO||O| for all keys alike, as large as dS itself where attention is nearly uniform. dlam is always -sum_j P2 dP of the
 // walk: the fp32 maps hold the forward's bf16 weights (1.7e-3 of a row), which a weight per head, summed over rows that
 // cancel, does not bear (5.9e-3 of 36 x 739 rows' sum, now the 2^-8 of its own rounding; one fma a pair, 1 % of dq at
-// head size 32, 3 % at 128). Head size 128 as above: 440 us, 0.94 PFLOP/s, matrix cores busy 45 %, vector units 42 %.
+// head size 32, 3 % at 128). Head size 128 as above: 440 us, 0.94 PFLOP/s, matrix cores busy 45 %, vector units 42 %. At 128
+// keys of 64-wide heads the matrix cores are busy 10 % of the cycles and the vector units 36 %: it waits for its operands and
+// for dependent instructions (few tiles a workgroup).
 // =====================================================================================
 template <int D, int QB, int NW, int OCC, bool SHORT>
 __global__ __launch_bounds__(64 * NW, OCC) void da_bwd_dq_kernel(DaArgs a) {
@@ -1428,7 +1431,7 @@ extern "C" int bd_diff_attention_bwd(const bd_diff_attn_args* p, void* stream) {
   a.dq = (unsigned short*)p->dq; a.dk = (unsigned short*)p->dk; a.dv = (unsigned short*)p->dv;
   a.dlam = p->dlam; a.dlam_bf16 = p->dlam_dtype == BD_DTYPE_BF16;
   a.stats = (float*)p->workspace;
-  bd_prof_scope prof(stream, 28.0 * p->B * p->H * (double)p->Lq * p->Lk * p->head_dim, BD_PROF_ATTN_BWD);
+  bd_prof_scope prof(stream, (p->dk ? 28.0 : 12.0) * p->B * p->H * (double)p->Lq * p->Lk * p->head_dim, BD_PROF_ATTN_BWD);
   switch (p->head_dim) {
     case 32: return da_backward<32>(a, (hipStream_t)stream);
     case 64: return da_backward<64>(a, (hipStream_t)stream);

@@ -526,8 +526,8 @@ __global__ __launch_bounds__(256) void vl_dh_kernel(VlState st, const float* __r
 }
 
 // dW rows v0 .. v0 + rows from the slabs of their splits: 32 units of 8 values a workgroup, each added up by eight threads that
-// take every eighth slab, then in order. Bound by memory (803 x 384, 12 slabs) or latency (39 x 64, 256 slabs: 3.4 us, one
-// thread a unit 21)
+// take every eighth slab, then in order. Bound by memory (803 x 384, 10 slabs: 4.1 us; one thread a unit 4.6) or latency
+// (39 x 64, 64 slabs: 3.6 us; one thread a unit 16.7)
 __global__ __launch_bounds__(256) void vl_dw_kernel(VlState st, const float* __restrict__ slab, long long slab_stride, int n_slab,
                                                     const float* __restrict__ gout, void* __restrict__ dw, int dw_f32, int v0, int rows, int d) {
   __shared__ float part[7][32][9];
@@ -696,6 +696,8 @@ VlPlan vl_plan(long long M, int d, int V) {
   //   32768 x 384 -> 4096    58 / 64      82 / 80      76 / 66     74 / 90
   //   32768 x 384 -> 803     17 / 18      25 / 25      37 / 25     39 / 28
   //   8192 x 4096 -> 2048    88 / 63      96 / 64      73 / 83     82 / 66
+  // The rules below follow the column but for a few per cent: 3001 x 768 -> 32003 takes the larger tile for its scores (92,
+  // not 88), 32768 x 384 -> 803 sits on that rule's border (17 / 18 is noise).
   const long long tiles_z = (p.m_pad / 256) * ((V + 255) / 256), tiles_w = (long long)((V + 255) / 256) * ((d + 255) / 256);
   p.big_s = tiles_z >= 512;
   p.big_z = d >= 1024 && tiles_z >= 4096;

@@ -727,8 +727,9 @@ int bd_prof_read(long long* launches, double* total_ms, double* total_flops, int
 /* Same, for one kernel family: 0 tiled GEMM, 1 row-panel GEMM, 2 fused feed-forward block,
  * 3 fused attention block, 4 whole-forward kernel, 5 weight-gradient GEMM, 6 attention forward,
  * 7 attention backward; and, with algorithmic BYTES in place of flops, 8 LayerNorm forward / backward,
- * 9 masked cross-entropy, 10 embedding / corruption / dropout / casts, 11 optimizer, 12 reverse step and
- * repairs; -1 = all families together. */
+ * 9 masked cross-entropy, 10 embedding / corruption / dropout / casts / rotary positions, 11 optimizer, 12 reverse step
+ * and repairs; -1 = all families together. Differential attention counts in 6 and 7, the head's loss without logits (all of
+ * its launches) in 0. */
 int bd_prof_read_kind(int kind, long long* launches, double* total_ms, double* total_flops, int reset);
 
 /* The chosen-row forward for models on the per-layer kernels (d >= 512 or L > 128: no single-launch forward). Every
