@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void vl_gather_kernel(const unsigned short* __
                                                         const unsigned char* __restrict__ ind, const long long* __restrict__ attn,
                                                         const int* __restrict__ counts, const float* __restrict__ sums, VlState st,
                                                         int M, int d, int V) {
-  __shared__ int before[4], all[4], src[SCAN];
+  __shared__ int before[4], all[4], src[SCAN], here;
   __shared__ float wsum[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int groups = (M + SCAN - 1) / SCAN, grp = blockIdx.x;
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(256) void vl_gather_kernel(const unsigned short* __
       const long long t = targets[row];
       st.tgt[first + at] = t >= 0 && t < V ? (int)t : -1;      // outside the vocabulary: the row's loss is NaN
     }
-    if (lane == 0) before[0] = __popcll(live);
+    if (lane == 0) here = __popcll(live);                  // (a place of its own: the other waves may still read before[])
     if (lead && grp == 0 && lane == 0) {
       st.head[0] = total;
       ((float*)st.head)[1] = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256) void vl_gather_kernel(const unsigned short* __
   }
   __syncthreads();
   // (the row's 16-byte chunks are dealt to the workgroups of a group, grid.y)
-  const int n = before[0], per = d / 8, wide = (per + gridDim.y - 1) / gridDim.y, ch0 = wide * blockIdx.y, chn = min(wide, per - ch0);
+  const int n = here, per = d / 8, wide = (per + gridDim.y - 1) / gridDim.y, ch0 = wide * blockIdx.y, chn = min(wide, per - ch0);
   for (int i = tid; i < n * chn; i += 256) {
     const int r = i / chn, ch = ch0 + i - r * chn;
     *(u32x4*)(st.hc + (long long)(first + r) * d + 8 * ch) = *(const u32x4*)(hidden + (long long)src[r] * d + 8 * ch);

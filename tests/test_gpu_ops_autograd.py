@@ -196,3 +196,15 @@ def test_either_gradient_of_the_head_loss_alone(gpu_device, M, d, V, wdt):
         return torch.autograd.grad(ops.linear_cross_entropy(*leaves, t, ind), [x for x in leaves if x.requires_grad])
     dh, dw = run(True, True)
     assert torch.equal(run(True, False)[0], dh) and torch.equal(run(False, True)[0], dw)
+
+
+@pytest.mark.parametrize("M,d,live", [(40000, 576, 0.5), (40000, 64, 0.02), (9000, 1024, 0.9)])
+def test_rows_gathered_by_the_head_loss(gpu_device, M, d, live):
+    """The weighted rows reach the compact matrix whole and in order, whatever the timing of the waves that copy them: the loss
+    has the bits of the call that gets these rows alone, time after time."""
+    dev = gpu_device
+    g = torch.Generator(device=dev).manual_seed(41)
+    h, w = torch.randn(M, d, generator=g, device=dev).to(BF), (torch.randn(300, d, generator=g, device=dev) / d ** 0.5).to(BF)
+    t, ind = torch.randint(0, 300, (M,), generator=g, device=dev), torch.rand(M, generator=g, device=dev) < live
+    alone = ops.linear_cross_entropy(h[ind], w, t[ind])
+    assert all(torch.equal(ops.linear_cross_entropy(h, w, t, ind), alone) for _ in range(5))
