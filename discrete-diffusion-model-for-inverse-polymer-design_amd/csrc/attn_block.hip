@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   const float* xrow = p.x + row * D + 4 * (lane >> 5);
   f32x16 acc[NT / 2];
   load_rows(acc, xrow);
-  attn_phase<NT, DH, H>(ph, smem, acc);
+  attn_phase<NT, DH, H, true>(ph, smem, acc);
   if (tok < L) store_rows(acc, p.out + row * D + 4 * (lane >> 5));
 }
 

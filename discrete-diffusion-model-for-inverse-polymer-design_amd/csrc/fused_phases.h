@@ -468,7 +468,8 @@ struct AttnPhase {
   const float* wave_mask = nullptr;
 };
 
-template <int NT, int DH, int H>
+// ALONE: nothing but the caller's stores follows (see the end of the phase).
+template <int NT, int DH, int H, bool ALONE = false>
 __device__ __forceinline__ void attn_phase(const AttnPhase& p, unsigned char* smem, f32x16 (&acc)[NT / 2]) {
   constexpr int D = NT * 16;
   constexpr int NT32 = NT / 2;
@@ -776,8 +777,13 @@ __device__ __forceinline__ void attn_phase(const AttnPhase& p, unsigned char* sm
       ++u;
     }
   }
-  // the reads issued past the last unit
+  // the reads issued past the last unit. ALONE: their registers are in use until here, or the compiler moves the first
+  // accumulators into them while the reads are still on their way (it did); with a feed-forward phase behind, it does not.
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  if (ALONE) {
+#pragma unroll
+    for (int i = 0; i < LOOK; ++i) asm volatile("" : "+v"(wf[i]));
+  }
 
   // ---- + bias
   // (three tiles' worth of bias reads in flight at a time: left alone, the compiler issues all of them first and
