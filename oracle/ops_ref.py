@@ -29,6 +29,11 @@ def rotary(x, table, positions, interleaved, inverse=False):
 
 
 # ---------------------------------------------------------------- differential attention
+def mm(a, b):
+    """Batched product of contiguous operands (the library's batched products of transposed views have faulted a GPU)."""
+    return torch.matmul(a.contiguous(), b.contiguous())
+
+
 def _one(q, k, v, lam, seen, dout, scale, tol):
     """One sequence: q [Lq, 2H, D], k [Lk, 2Hkv, D], v [Lk, Hkv, E], lam [Lq, H], seen [Lk] bool. Results as float64;
     with ``tol`` also the error each may have when products take bf16 operands and sum in fp32."""
@@ -39,50 +44,50 @@ def _one(q, k, v, lam, seen, dout, scale, tol):
     vh = v.permute(1, 0, 2).repeat_interleave(share, 0)
     kh = torch.where(seen[:, None], kh, torch.zeros_like(kh))
     vh = torch.where(seen[:, None], vh, torch.zeros_like(vh))
-    s = (qh @ kh.transpose(-1, -2)) * scale
+    s = mm(qh, kh.transpose(-1, -2)) * scale
     s = torch.where(seen, s, torch.full_like(s, -math.inf))
     p = torch.softmax(s, -1) if bool(seen.any()) else torch.zeros_like(s)
     w = lam.t()[..., None]                                                   # [H, Lq, 1]
     pc = p[:, 0] - w * p[:, 1]
-    out = pc @ vh
+    out = mm(pc, vh)
     res = {"out": out.permute(1, 0, 2)}
     if tol:
         # a score's error: D products summed in fp32, the scaling, the exponent's arithmetic (a few steps of values
         # up to |s| log2 e); weights inherit it relatively, twice (numerator and normaliser)
-        es = ((qh.abs() @ kh.abs().transpose(-1, -2)) * scale).amax(-1, keepdim=True) * (D + 8) * F * 2 + 64 * F
+        es = (mm(qh.abs(), kh.abs().transpose(-1, -2)) * scale).amax(-1, keepdim=True) * (D + 8) * F * 2 + 64 * F
         pa = p[:, 0] + w.abs() * p[:, 1]
         ep = es.amax(1)
-        res["out_tol"] = (U * 1.01 * (pa @ vh.abs() + out.abs()) + ep * (pa @ vh.abs())).permute(1, 0, 2)
+        res["out_tol"] = (U * 1.01 * (mm(pa, vh.abs()) + out.abs()) + ep * mm(pa, vh.abs())).permute(1, 0, 2)
     if dout is None:
         return res
     do = dout.permute(1, 0, 2)
-    dp = do @ vh.transpose(-1, -2)
+    dp = mm(do, vh.transpose(-1, -2))
     delta = (p * dp[:, None]).sum(-1, keepdim=True)
     fac = torch.stack([torch.ones_like(w), -w], 1)
     ds = fac * p * (dp[:, None] - delta)
-    dq = (ds @ kh) * scale
-    dk = (ds.transpose(-1, -2) @ qh) * scale
-    dv = pc.transpose(-1, -2) @ do
+    dq = mm(ds, kh) * scale
+    dk = mm(ds.transpose(-1, -2), qh) * scale
+    dv = mm(pc.transpose(-1, -2), do)
     group = lambda x: x.view(Hkv, share, *x.shape[1:]).sum(1)  # noqa: E731
     res["dq"] = dq.permute(2, 0, 1, 3).reshape(q.shape)
     res["dk"] = group(dk).permute(2, 0, 1, 3).reshape(k.shape)
     res["dv"] = group(dv).permute(1, 0, 2)
     res["dlam"] = -delta[:, 1, :, 0].t()
     if tol:
-        pv = p @ vh.abs()[:, None]                                           # [H, 2, Lq, E]
+        pv = mm(p, vh.abs()[:, None])                                           # [H, 2, Lq, E]
         # delta from the forward's sums (weights rounded to bf16) or from fp32 products; dP: E products in fp32
-        edp = (do.abs() @ vh.abs().transpose(-1, -2)) * (E + 8) * F * 2
-        pdp = (p * (do.abs() @ vh.abs().transpose(-1, -2))[:, None]).sum(-1, keepdim=True)
+        edp = mm(do.abs(), vh.abs().transpose(-1, -2)) * (E + 8) * F * 2
+        pdp = (p * mm(do.abs(), vh.abs().transpose(-1, -2))[:, None]).sum(-1, keepdim=True)
         edelta = (do.abs()[:, None] * pv).sum(-1, keepdim=True) * (U * 1.01 + (E + 8) * F) + pdp * (es + 16 * F) + (p * edp[:, None]).sum(-1, keepdim=True)
         fa = fac.abs()
         eds = fa * (U * 1.01 * (ds / fac.where(fac != 0, torch.ones_like(fac))).abs() + p * (edelta + edp[:, None] + (dp[:, None] - delta).abs() * (es + 16 * F)))
         long_sum = lambda n: 1.0 + n * F  # noqa: E731
         # (the weight lam may join the bf16 value or the fp32 sum)
-        res["dq_tol"] = (((eds @ kh.abs()) * scale + U * 1.01 * dq.abs()) * long_sum(k.shape[0]) + (ds.abs() @ kh.abs()) * scale * k.shape[0] * F).permute(2, 0, 1, 3).reshape(q.shape)
-        dka = group(((eds.transpose(-1, -2) @ qh.abs()) + (ds.abs().transpose(-1, -2) @ qh.abs()) * Lq * share * F) * scale)
+        res["dq_tol"] = ((mm(eds, kh.abs()) * scale + U * 1.01 * dq.abs()) * long_sum(k.shape[0]) + mm(ds.abs(), kh.abs()) * scale * k.shape[0] * F).permute(2, 0, 1, 3).reshape(q.shape)
+        dka = group((mm(eds.transpose(-1, -2), qh.abs()) + mm(ds.abs().transpose(-1, -2), qh.abs()) * Lq * share * F) * scale)
         res["dk_tol"] = (dka + U * 1.01 * group(dk).abs()).permute(2, 0, 1, 3).reshape(k.shape)
         epc = U * 1.01 * pc.abs() + pa * (ep + 16 * F + Lq * share * F)
-        res["dv_tol"] = (group(epc.transpose(-1, -2) @ do.abs()) + U * 1.01 * group(dv).abs()).permute(1, 0, 2)
+        res["dv_tol"] = (group(mm(epc.transpose(-1, -2), do.abs())) + U * 1.01 * group(dv).abs()).permute(1, 0, 2)
         res["dlam_tol"] = edelta[:, 1, :, 0].t()
     return res
 
