@@ -394,7 +394,7 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     without the batch axis, ``cu_seqlens`` int [sequences + 1] (rows cu[b] .. cu[b + 1] - 1 belong to sequence b; offsets
     that do not fall; rows before the first and behind the last sequence come out zero), ``max_seqlen`` the longest (None: read
     back from the device; a longer sequence's rows from there on come out NaN, in the gradients too), ``key_mask``
-    [sequences, max_seqlen]. ``scale`` defaults to 1 / sqrt(D). The backward pass leaves out what no operand needs: dq where q
+    [sequences, max_seqlen]. ``scale`` (1e-30 to 1e30) defaults to 1 / sqrt(D). The backward pass leaves out what no operand needs: dq where q
     is frozen, the keys' side where k and v are."""
     _same_device("differential_attention", q, k, v, lam, key_mask, cu_seqlens)
     _no_tangents("differential_attention", q, k, v, lam)
@@ -426,8 +426,8 @@ def differential_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, la
     if lam_strides is None:
         raise ValueError(f"differential_attention: lam {tuple(lam.shape)} does not broadcast to {(*lead, H)}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError(f"differential_attention: scale must be positive and finite, got {scale}")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"differential_attention: scale must lie within 1e-30 and 1e30, got {scale}")
     longest = None
     if packed and max_seqlen is None:
         _lib.require_device(q, "differential_attention")

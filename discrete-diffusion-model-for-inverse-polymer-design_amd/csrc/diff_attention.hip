@@ -1270,7 +1270,8 @@ int da_check(const bd_diff_attn_args& p, const char* what, DaArgs& a) {
              "%s: too many rows or heads", what);
   BD_REQUIRE(!p.cu_seqlens || p.Lq == p.Lk, "%s: packed rows need Lq == Lk (the longest sequence)", what);
   BD_REQUIRE(!p.cu_seqlens || p.total_rows > 0, "%s: packed rows need total_rows", what);
-  BD_REQUIRE(p.scale > 0.f, "%s: scale must be positive", what);
+  // (2^8 over the scale is how far a score may pass the running maximum: it has to be finite)
+  BD_REQUIRE(p.scale >= 1e-30f && p.scale <= 1e30f, "%s: scale must lie within 1e-30 and 1e30", what);
   BD_REQUIRE(p.lam_dtype == BD_DTYPE_BF16 || p.lam_dtype == BD_DTYPE_F32, "%s: lam is neither bf16 nor fp32", what);
   const void* aligned[] = {p.q, p.k, p.v};
   for (const void* x : aligned) BD_REQUIRE(((uintptr_t)x & 15) == 0, "%s: q, k and v must be 16-byte aligned", what);

@@ -128,3 +128,17 @@ def test_models_pickled_before_the_options_existed():
     assert bb.plain_attention and not model.fused_head_loss
     assert bb.layers[0].attn.rotary_base is None and not bb.layers[0].attn.differential
     assert bb.config_dict() == want
+
+
+@pytest.mark.parametrize("scale", [1e-39, 9e-31, 2e30, 1e39, float("inf"), -0.1])
+def test_scales_out_of_range_are_refused(scale):
+    """Near the ends of fp32 the maximum's slack or the scaled scores are no numbers any more: refused in Python and at the C ABI."""
+    with pytest.raises(ValueError, match="scale"):
+        ops.differential_attention(z(2, 3, 4, 32), z(2, 5, 4, 32), z(2, 5, 2, 64), z(2), scale=scale)
+    import ctypes as C
+    from bidiff import _lib
+    a = _lib.DiffAttnArgs()
+    for n in ("q", "k", "v", "lam", "out", "workspace"):
+        setattr(a, n, 1 << 20)                # an aligned, made-up address that is never followed
+    a.B, a.Lq, a.Lk, a.H, a.Hkv, a.head_dim, a.scale, a.workspace_bytes = 2, 3, 5, 4, 2, 64, scale, 1 << 40
+    assert _lib.lib().bd_diff_attention_fwd(C.byref(a), None) == -1 and b"scale" in _lib.lib().bd_last_error()
